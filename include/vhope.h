@@ -468,6 +468,114 @@ int vh_residual_add_bwd(const float* grad_out, const void* branch, int32_t branc
                         int64_t workspace_bytes, int32_t batch, int64_t spatial, int32_t channels,
                         vh_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Selective state space operators (no counterpart in the reference): a short causal convolution
+ * and a selective scan over channels-last token rows, for whole sequences (forward, backward)
+ * and for single tokens of cached streams.
+ *
+ * Sequences.  With seq_offsets NULL there are `batch` sequences of `length` tokens; element
+ * (sequence s, token t, channel c) of a tensor is at base + s * batch_stride + t * token_stride
+ * + c (unit channel stride).  With seq_offsets (device, int32 [batch + 1]: 0 first, never
+ * decreasing, `length` last) the sequences lie one after another over `length` tokens in all and
+ * batch strides are ignored; sequences may be empty.  The offsets are read on the device: values
+ * outside [0, length] are clamped, and rows that no sequence covers are not written.
+ * reverse != 0 reads each sequence from its last token to its first (states then enter at the
+ * last token and leave at the first).  Outputs are contiguous, [tokens, channels].
+ * -------------------------------------------------------------------------------------*/
+
+/* Short causal convolution:  y_t = act(bias + sum_k weight[:, k] * x_{t - taps + 1 + k}),
+ * with the taps - 1 inputs before the first token taken from initial_state (zeros if NULL).
+ *   x: dtype, strided;  weight: fp32 [channels, taps], taps 2 to 8;  bias: fp32 [channels] or
+ *   NULL;  activation: 0 none, 1 silu;  initial_state / final_state: dtype [batch, taps - 1,
+ *   channels], oldest input first, or NULL;  y: dtype. */
+typedef struct {
+    const void* x;
+    int64_t x_batch_stride, x_token_stride;
+    const float* weight;
+    const float* bias;
+    const void* initial_state;
+    void* y;
+    void* final_state;
+    const int32_t* seq_offsets;
+    int64_t length;
+    int32_t dtype, activation, taps, batch, channels, reverse;
+} vh_short_conv_args;
+
+int vh_short_conv_fwd(const vh_short_conv_args* args, vh_stream_t stream);
+
+/* Its backward.  args: the forward's (y and final_state are not read).  grad_y: dtype,
+ * contiguous [tokens, channels];  grad_final: dtype [batch, taps - 1, channels] or NULL.  Writes
+ * grad_x (dtype [tokens, channels]), grad_weight (fp32 [channels, taps]), grad_bias (fp32
+ * [channels] or NULL) and grad_initial (dtype [batch, taps - 1, channels] or NULL).  Sums run in
+ * a fixed order. */
+int64_t vh_short_conv_bwd_workspace_bytes(const vh_short_conv_args* args);
+int vh_short_conv_bwd(const vh_short_conv_args* args, const void* grad_y, const void* grad_final, void* grad_x,
+                      float* grad_weight, float* grad_bias, void* grad_initial, void* workspace,
+                      int64_t workspace_bytes, vh_stream_t stream);
+
+/* One token of `batch` cached streams: x dtype [batch, channels] (x_batch_stride elements
+ * apart), state dtype [slots, taps - 1, channels].  slots_index: int32 [batch], the stream's slot
+ * (slot b for row b if NULL); a row whose slot is outside [0, slots) is skipped: y 0, no state
+ * written.  No two rows may name one slot.  state_out: as state, may be state itself. */
+int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t dtype, const float* weight, const float* bias,
+                       int32_t activation, const void* state, void* state_out, const int32_t* slots_index,
+                       int32_t slots, void* y, int32_t batch, int32_t channels, int32_t taps, vh_stream_t stream);
+
+/* Selective scan, per channel d and state n:
+ *     s_t = delta_t + delta_bias_d, through softplus when delta_softplus != 0
+ *     h_t = exp(s_t a[d, n]) h_{t-1} + s_t u_t b_t[n]
+ *     y_t = (sum_n c_t[n] h_t + d_skip_d u_t) * silu(z_t)
+ * u, delta, z (or NULL), b, c, y share dtype; b, c: [tokens, groups, states], unit state stride,
+ * channel d belongs to group d / (channels / groups); a: fp32 [channels, states]; d_skip,
+ * delta_bias: fp32 [channels] or NULL; states 4, 8, 16, 32 or 64; initial_state / final_state:
+ * fp32 [batch, channels, states] or NULL.  The state is held in fp32 throughout.
+ * checkpoints (or NULL): fp32 [vh_ssm_scan_checkpoint_slots, channels, states], the state before
+ * every 32nd token, which the backward starts from. */
+typedef struct {
+    const void *u, *delta, *z, *b, *c;
+    int64_t u_batch_stride, u_token_stride, delta_batch_stride, delta_token_stride;
+    int64_t z_batch_stride, z_token_stride;
+    int64_t b_batch_stride, b_token_stride, b_group_stride;
+    int64_t c_batch_stride, c_token_stride, c_group_stride;
+    const float *a, *d_skip, *delta_bias, *initial_state;
+    void* y;
+    float* final_state;
+    float* checkpoints;
+    const int32_t* seq_offsets;
+    int64_t length;
+    int32_t dtype, batch, channels, states, groups, delta_softplus, reverse;
+} vh_ssm_scan_args;
+
+int64_t vh_ssm_scan_checkpoint_slots(const vh_ssm_scan_args* args);
+int64_t vh_ssm_scan_fwd_workspace_bytes(const vh_ssm_scan_args* args);
+int vh_ssm_scan_fwd(const vh_ssm_scan_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
+
+/* Its backward.  args: the forward's, with the checkpoints it wrote (y and final_state are not
+ * read).  grad_y: dtype, contiguous [tokens, channels].  Outputs: grad_u, grad_delta, grad_z
+ * (dtype [tokens, channels]; grad_z when z is given), grad_b, grad_c (dtype [tokens, groups,
+ * states]), grad_a (fp32 [channels, states]), grad_d_skip, grad_delta_bias (fp32 [channels]; NULL
+ * when not wanted), grad_initial (fp32 [batch, channels, states] or NULL).  grad_final: fp32
+ * [batch, channels, states] or NULL.  Sums over channels, tokens and sequences run in a fixed
+ * order. */
+typedef struct {
+    vh_ssm_scan_args fwd;
+    const void* grad_y;
+    const float* grad_final;
+    void *grad_u, *grad_delta, *grad_z, *grad_b, *grad_c;
+    float *grad_a, *grad_d_skip, *grad_delta_bias, *grad_initial;
+} vh_ssm_scan_bwd_args;
+
+int64_t vh_ssm_scan_bwd_workspace_bytes(const vh_ssm_scan_bwd_args* args);
+int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
+
+/* One token of `batch` cached streams: u, delta, z dtype [batch, channels] and b, c dtype
+ * [batch, groups, states] (the batch strides of args; token strides are not used), state fp32
+ * [slots, channels, states].  args gives a, d_skip, delta_bias, delta_softplus, dtype, batch,
+ * channels, states, groups and y [batch, channels]; its other fields are not read.  slots_index,
+ * slots, state, state_out: as vh_short_conv_step. */
+int vh_ssm_scan_step(const vh_ssm_scan_args* args, const float* state, float* state_out, const int32_t* slots_index,
+                     int32_t slots, vh_stream_t stream);
+
 /* Measurement helper (no reference counterpart): launches `blocks` x 256 threads, each
  * running 32 * iters dependent-free FMAs; out needs blocks * 256 floats.  bench.py times it
  * to measure the device's FP32 (non-tensor) FMA peak. */

@@ -74,6 +74,32 @@ class VhDwconvArgs(ctypes.Structure):
                 ("pos_y", c_void_p), ("pos_ksize", c_int32)]
 
 
+class VhShortConvArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("x_batch_stride", c_int64), ("x_token_stride", c_int64), ("weight", c_void_p),
+                ("bias", c_void_p), ("initial_state", c_void_p), ("y", c_void_p), ("final_state", c_void_p),
+                ("seq_offsets", c_void_p), ("length", c_int64), ("dtype", c_int32), ("activation", c_int32),
+                ("taps", c_int32), ("batch", c_int32), ("channels", c_int32), ("reverse", c_int32)]
+
+
+class VhSsmScanArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("u", "delta", "z", "b", "c")]
+                + [(n, c_int64) for n in ("u_batch_stride", "u_token_stride", "delta_batch_stride",
+                                          "delta_token_stride", "z_batch_stride", "z_token_stride",
+                                          "b_batch_stride", "b_token_stride", "b_group_stride",
+                                          "c_batch_stride", "c_token_stride", "c_group_stride")]
+                + [(n, c_void_p) for n in ("a", "d_skip", "delta_bias", "initial_state", "y", "final_state",
+                                           "checkpoints", "seq_offsets")]
+                + [("length", c_int64)]
+                + [(n, c_int32) for n in ("dtype", "batch", "channels", "states", "groups", "delta_softplus",
+                                          "reverse")])
+
+
+class VhSsmScanBwdArgs(ctypes.Structure):
+    _fields_ = ([("fwd", VhSsmScanArgs)]
+                + [(n, c_void_p) for n in ("grad_y", "grad_final", "grad_u", "grad_delta", "grad_z", "grad_b",
+                                           "grad_c", "grad_a", "grad_d_skip", "grad_delta_bias", "grad_initial")])
+
+
 _lib = None
 _lock = threading.Lock()
 _inited = set()
@@ -174,6 +200,30 @@ def load() -> ctypes.CDLL:
             lib.vh_residual_add_bwd.restype = c_int32
             lib.vh_residual_add_bwd.argtypes = ([c_void_p, c_void_p, c_int32] + [c_void_p] * 5
                                                 + [c_int64, c_int32, c_int64, c_int32, c_void_p])
+            # selective state space operators
+            conv, scan, scan_bwd = (ctypes.POINTER(t) for t in (VhShortConvArgs, VhSsmScanArgs, VhSsmScanBwdArgs))
+            lib.vh_short_conv_fwd.restype = c_int32
+            lib.vh_short_conv_fwd.argtypes = [conv, c_void_p]
+            lib.vh_short_conv_bwd_workspace_bytes.restype = c_int64
+            lib.vh_short_conv_bwd_workspace_bytes.argtypes = [conv]
+            lib.vh_short_conv_bwd.restype = c_int32
+            lib.vh_short_conv_bwd.argtypes = [conv] + [c_void_p] * 7 + [c_int64, c_void_p]
+            lib.vh_short_conv_step.restype = c_int32
+            lib.vh_short_conv_step.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
+                                               c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32,
+                                               c_void_p]
+            lib.vh_ssm_scan_checkpoint_slots.restype = c_int64
+            lib.vh_ssm_scan_checkpoint_slots.argtypes = [scan]
+            lib.vh_ssm_scan_fwd_workspace_bytes.restype = c_int64
+            lib.vh_ssm_scan_fwd_workspace_bytes.argtypes = [scan]
+            lib.vh_ssm_scan_fwd.restype = c_int32
+            lib.vh_ssm_scan_fwd.argtypes = [scan, c_void_p, c_int64, c_void_p]
+            lib.vh_ssm_scan_bwd_workspace_bytes.restype = c_int64
+            lib.vh_ssm_scan_bwd_workspace_bytes.argtypes = [scan_bwd]
+            lib.vh_ssm_scan_bwd.restype = c_int32
+            lib.vh_ssm_scan_bwd.argtypes = [scan_bwd, c_void_p, c_int64, c_void_p]
+            lib.vh_ssm_scan_step.restype = c_int32
+            lib.vh_ssm_scan_step.argtypes = [scan, c_void_p, c_void_p, c_void_p, c_int32, c_void_p]
             _lib = lib
     return _lib
 

@@ -1,0 +1,204 @@
+// Shared pieces of the selective state space kernels (ssm_scan.cu, ssm_scan_bwd.cu, short_conv.cu).
+//
+// Sequences are channels-last token rows.  `Seqs` says where each one lies: equally long ones
+// follow a batch stride, packed ones start at seq_offsets[s].  Offsets come from the device, so
+// the host cannot check them; every kernel clamps them to [0, length], which keeps each access
+// inside the tensors whatever they hold.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace vh {
+namespace ssm {
+
+struct Seqs {
+    const int32_t* offsets;  // [count + 1] or null: `count` sequences of `length` tokens
+    int64_t length;          // tokens per sequence, or of all packed sequences together
+    int32_t count;
+    int32_t reverse;         // read each sequence from its last token to its first
+};
+
+// One sequence: its first row counted over all tokens (batch-major) and its length.
+struct Seq {
+    int64_t row;
+    int64_t len;
+};
+
+__device__ __forceinline__ Seq seq_at(const Seqs& q, int s) {
+    if (!q.offsets) return {(int64_t)s * q.length, q.length};
+    int64_t lo = q.offsets[s], hi = q.offsets[s + 1];
+    lo = lo < 0 ? 0 : (lo > q.length ? q.length : lo);
+    hi = hi < lo ? lo : (hi > q.length ? q.length : hi);
+    return {lo, hi - lo};
+}
+
+// Slots of `step` tokens: sequence s owns the slots from slot_base on, at least one and at least
+// ceil(len / step).  Packed sequences: floor(lo / step) + s, because consecutive starts then
+// differ by floor(hi / step) - floor(lo / step) + 1 >= ceil((hi - lo) / step); the total is at
+// most floor(length / step) + count.
+__host__ __device__ __forceinline__ int64_t slots_per_seq(int64_t len, int step) {
+    return len > 0 ? (len + step - 1) / step : 1;
+}
+__host__ __device__ __forceinline__ int64_t slot_total(bool packed, int64_t length, int32_t count, int step) {
+    return packed ? length / step + count : (int64_t)count * slots_per_seq(length, step);
+}
+__device__ __forceinline__ int64_t slot_base(const Seqs& q, int s, int64_t row, int step) {
+    return q.offsets ? row / step + s : (int64_t)s * slots_per_seq(q.length, step);
+}
+
+// The sequence that owns slot `slot` (binary search over the monotone slot bases).
+__device__ __forceinline__ int seq_of_slot(const Seqs& q, int64_t slot, int step) {
+    if (!q.offsets) return (int)(slot / slots_per_seq(q.length, step));
+    int lo = 0, hi = q.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        int64_t row = q.offsets[mid];
+        row = row < 0 ? 0 : (row > q.length ? q.length : row);
+        if (row / step + mid <= slot) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Token rows of one tensor: element (row r of sequence s, channel c).  Packed tensors ignore the
+// batch stride.
+struct Rows {
+    int64_t batch, token;  // strides in elements
+};
+__device__ __forceinline__ int64_t first_row(const Seqs& q, const Seq& e, int s, const Rows& r) {
+    const int64_t base = q.offsets ? e.row * r.token : (int64_t)s * r.batch;
+    return q.reverse && e.len > 0 ? base + (e.len - 1) * r.token : base;
+}
+__device__ __forceinline__ int64_t row_step(const Seqs& q, const Rows& r) { return q.reverse ? -r.token : r.token; }
+
+// V consecutive channels from c on; channels at or past `end` read as 0.  `vec`: the caller's
+// rule says that V-wide accesses are aligned and never straddle `end`.
+template <int V, typename T>
+__device__ __forceinline__ void load_v(const T* p, int c, int end, bool vec, float (&v)[V]) {
+    if (V > 1 && vec) {
+        if (c < end) {
+            if constexpr (V == 4) {
+                const float4 q = load4(p);
+                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+            } else {
+                struct alignas(sizeof(T) * V) Pack { T e[V]; };
+                const Pack q = *reinterpret_cast<const Pack*>(p);
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = to_f(q.e[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = 0.f;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = c + i < end ? to_f(p[i]) : 0.f;
+    }
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_v(T* p, int c, int end, bool vec, const float (&v)[V]) {
+    if (V > 1 && vec) {
+        if (c < end) {
+            if constexpr (V == 4) {
+                store4(p, make_float4(v[0], v[1], v[2], v[3]));
+            } else {
+                struct alignas(sizeof(T) * V) Pack { T e[V]; };
+                Pack q;
+#pragma unroll
+                for (int i = 0; i < V; ++i) q.e[i] = from_f<T>(v[i]);
+                *reinterpret_cast<Pack*>(p) = q;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (c + i < end) p[i] = from_f<T>(v[i]);
+    }
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 2^x on the FMA pipe.  x = i + f with i the nearest integer (added and taken off again with
+// 1.5 * 2^23, whose last mantissa bits then hold i) and |f| <= 1/2; 2^f = 1 + f q(f), q of degree 5
+// fitted for the relative error of 2^f by Lawson's iteration (2.0e-9); 2^i goes into the exponent.
+// Evaluated in fp32 it is off by 2.7e-8 root mean square and 0.9e-9 on average, against 3.8e-8
+// and -2e-8 for ex2.approx on [-0.1, 0] (one rounding: 1.8e-8): a state that remembers a
+// thousand tokens multiplies by a thousand decays, and there an average error adds up.
+// Past |x| = 126 (and for NaN) the hardware function: no scaling of the exponent there.
+constexpr float kRound = 12582912.f;
+__device__ __forceinline__ float exp2_fma(float x) {
+    constexpr float kQ[6] = {0.6931471824645996f,   0.24022647738456726f,  0.055503323674201965f,
+                                0.00961843691766262f, 0.0013398873852565885f, 0.00015353361959569156f};
+    const float t = x + kRound, f = x - (t - kRound);
+    float q = kQ[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) q = fmaf(q, f, kQ[i]);
+    const float y = __int_as_float(__float_as_int(fmaf(q, f, 1.f)) + (__float_as_int(t) << 23));
+    return fabsf(x) <= 126.f ? y : ex2(x);
+}
+
+__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + ex2(-kLog2e * x)); }
+
+// log(1 + exp(x)) without cancellation on either side: max(x, 0) + log1p(e), e = exp(-|x|) in
+// (0, 1], log1p(e) = e r(e) with r of degree 8 fitted for the relative error by Lawson's
+// iteration (3.0e-8).  The rounding of |x| log2(e), which e would carry as a relative error of
+// up to |x| 2^-24, is added back to first order.
+__device__ __forceinline__ float softplus(float x) {
+    const float m = -fabsf(x);
+    const float hi = m * kLog2e, lo = fmaf(m, kLog2e, -hi);
+    float e = ex2(hi);
+    e = fmaf(e, m > -80.f ? lo * kLn2 : 0.f, e);
+    constexpr float kR[9] = {0.9999999403953552f, -0.4999949336051941f,  0.3331909775733948f,
+                             -0.2484298199415207f, 0.19106006622314453f,  -0.13663244247436523f,
+                             0.07822594046592712f, -0.029505232349038124f, 0.005232692696154118f};
+    float r = kR[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) r = fmaf(r, e, kR[i]);
+    return fmaf(e, r, fmaxf(x, 0.f));
+}
+
+// A in the exponential's base: log2(e) A, kept finite so that a step of zero leaves the state as
+// it is (0 * inf would not).  NaN stays NaN.
+__device__ __forceinline__ float to_log2(float a) {
+    const float v = a * kLog2e;
+    constexpr float kMax = 3.4028234e38f;
+    return v < -kMax ? -kMax : (v > kMax ? kMax : v);
+}
+
+// Sum over lane groups with the values scattered: V values per lane enter, and after log2(LANES)
+// exchanges over lane distances DIST, 2 DIST, ... (largest first) each lane holds the sums of
+// V / LANES of them (one, summed over all lanes, when LANES > V).  The lane whose index among
+// the LANES is j keeps the values from j * V / LANES on.
+template <int V, int LANES, int DIST>
+__device__ __forceinline__ void reduce_scatter(float (&v)[V], int lane) {
+    if constexpr (LANES > 1) {
+        constexpr int kMask = (LANES / 2) * DIST;
+        if constexpr (V > 1) {
+            const bool upper = lane & kMask;
+            float keep[V / 2];
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float send = upper ? v[i] : v[i + V / 2];
+                keep[i] = (upper ? v[i + V / 2] : v[i]) + __shfl_xor_sync(0xffffffffu, send, kMask);
+            }
+            reduce_scatter<V / 2, LANES / 2, DIST>(keep, lane);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) v[i] = keep[i];
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], kMask);
+            reduce_scatter<1, LANES / 2, DIST>(v, lane);
+        }
+    }
+}
+
+}  // namespace ssm
+}  // namespace vh
