@@ -529,8 +529,8 @@ int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t dtype, con
  * channel d belongs to group d / (channels / groups); a: fp32 [channels, states]; d_skip,
  * delta_bias: fp32 [channels] or NULL; states 4, 8, 16, 32 or 64; initial_state / final_state:
  * fp32 [batch, channels, states] or NULL.  The state is held in fp32 throughout.
- * checkpoints (or NULL): fp32 [vh_ssm_scan_checkpoint_slots, channels, states], the state before
- * every 32nd token, which the backward starts from. */
+ * checkpoints (or NULL): vh_ssm_scan_checkpoint_bytes(args) bytes that receive the state before
+ * every 32nd token, which the backward starts from (in an order of the kernels' own). */
 typedef struct {
     const void *u, *delta, *z, *b, *c;
     int64_t u_batch_stride, u_token_stride, delta_batch_stride, delta_token_stride;
@@ -546,9 +546,8 @@ typedef struct {
     int32_t dtype, batch, channels, states, groups, delta_softplus, reverse;
 } vh_ssm_scan_args;
 
-int64_t vh_ssm_scan_checkpoint_slots(const vh_ssm_scan_args* args);
-int64_t vh_ssm_scan_fwd_workspace_bytes(const vh_ssm_scan_args* args);
-int vh_ssm_scan_fwd(const vh_ssm_scan_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
+int64_t vh_ssm_scan_checkpoint_bytes(const vh_ssm_scan_args* args);
+int vh_ssm_scan_fwd(const vh_ssm_scan_args* args, vh_stream_t stream);
 
 /* Its backward.  args: the forward's, with the checkpoints it wrote (y and final_state are not
  * read).  grad_y: dtype, contiguous [tokens, channels].  Outputs: grad_u, grad_delta, grad_z

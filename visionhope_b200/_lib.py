@@ -212,12 +212,10 @@ def load() -> ctypes.CDLL:
             lib.vh_short_conv_step.argtypes = [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
                                                c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32,
                                                c_void_p]
-            lib.vh_ssm_scan_checkpoint_slots.restype = c_int64
-            lib.vh_ssm_scan_checkpoint_slots.argtypes = [scan]
-            lib.vh_ssm_scan_fwd_workspace_bytes.restype = c_int64
-            lib.vh_ssm_scan_fwd_workspace_bytes.argtypes = [scan]
+            lib.vh_ssm_scan_checkpoint_bytes.restype = c_int64
+            lib.vh_ssm_scan_checkpoint_bytes.argtypes = [scan]
             lib.vh_ssm_scan_fwd.restype = c_int32
-            lib.vh_ssm_scan_fwd.argtypes = [scan, c_void_p, c_int64, c_void_p]
+            lib.vh_ssm_scan_fwd.argtypes = [scan, c_void_p]
             lib.vh_ssm_scan_bwd_workspace_bytes.restype = c_int64
             lib.vh_ssm_scan_bwd_workspace_bytes.argtypes = [scan_bwd]
             lib.vh_ssm_scan_bwd.restype = c_int32

@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace vh {
 namespace ssm {
@@ -127,22 +128,28 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// 2^x on the FMA pipe.  x = i + f with i the nearest integer (added and taken off again with
-// 1.5 * 2^23, whose last mantissa bits then hold i) and |f| <= 1/2; 2^f = 1 + f q(f), q of degree 5
-// fitted for the relative error of 2^f by Lawson's iteration (2.0e-9); 2^i goes into the exponent.
-// Evaluated in fp32 it is off by 2.7e-8 root mean square and 0.9e-9 on average, against 3.8e-8
-// and -2e-8 for ex2.approx on [-0.1, 0] (one rounding: 1.8e-8): a state that remembers a
-// thousand tokens multiplies by a thousand decays, and there an average error adds up.
-// Past |x| = 126 (and for NaN) the hardware function: no scaling of the exponent there.
+// 2^(s a) on the FMA pipe.  s a = i + f with i the nearest integer (rounded to by adding 1.5 *
+// 2^23, whose last mantissa bits then hold i) and |f| <= 1/2, f from one fused multiply-add; 2^f =
+// 1 + f q(f), q of degree 5 fitted for the relative error of 2^f by Lawson's iteration (2.0e-9);
+// 2^i goes into the exponent.  Evaluated in fp32 it is off by 2.7e-8 root mean square and 0.9e-9
+// on average, against 3.8e-8 and -2e-8 for ex2.approx on [-0.1, 0] (one rounding: 1.8e-8): a
+// state that remembers a thousand tokens multiplies by a thousand decays, and there an average
+// error adds up.  Past |s a| = 126 (and for NaN) the hardware function: no scaling of the
+// exponent there.
 constexpr float kRound = 12582912.f;
-__device__ __forceinline__ float exp2_fma(float x) {
-    constexpr float kQ[6] = {0.6931471824645996f,   0.24022647738456726f,  0.055503323674201965f,
-                                0.00961843691766262f, 0.0013398873852565885f, 0.00015353361959569156f};
-    const float t = x + kRound, f = x - (t - kRound);
-    float q = kQ[5];
+constexpr int kExp2Terms = 6;
+__device__ __forceinline__ float exp2_term(int i) {
+    constexpr float kQ[kExp2Terms] = {0.6931471824645996f,  0.24022647738456726f,  0.055503323674201965f,
+                                      0.00961843691766262f, 0.0013398873852565885f, 0.00015353361959569156f};
+    return kQ[i];
+}
+__device__ __forceinline__ float exp2_fma(float s, float a) {
+    const float t = __fmaf_rn(s, a, kRound), f = __fmaf_rn(s, a, __fsub_rn(kRound, t));
+    float q = exp2_term(kExp2Terms - 1);
 #pragma unroll
-    for (int i = 4; i >= 0; --i) q = fmaf(q, f, kQ[i]);
-    const float y = __int_as_float(__float_as_int(fmaf(q, f, 1.f)) + (__float_as_int(t) << 23));
+    for (int i = kExp2Terms - 2; i >= 0; --i) q = __fmaf_rn(q, f, exp2_term(i));
+    const float y = __int_as_float(__float_as_int(__fmaf_rn(q, f, 1.f)) + (__float_as_int(t) << 23));
+    const float x = s * a;
     return fabsf(x) <= 126.f ? y : ex2(x);
 }
 
@@ -152,19 +159,56 @@ __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f +
 // (0, 1], log1p(e) = e r(e) with r of degree 8 fitted for the relative error by Lawson's
 // iteration (3.0e-8).  The rounding of |x| log2(e), which e would carry as a relative error of
 // up to |x| 2^-24, is added back to first order.
+constexpr int kLog1pTerms = 9;
+__device__ __forceinline__ float log1p_term(int i) {
+    constexpr float kR[kLog1pTerms] = {0.9999999403953552f,   -0.4999949336051941f, 0.3331909775733948f,
+                                       -0.2484298199415207f,  0.19106006622314453f, -0.13663244247436523f,
+                                       0.07822594046592712f, -0.029505232349038124f, 0.005232692696154118f};
+    return kR[i];
+}
+__device__ __forceinline__ float exp_minus_abs(float x) {
+    const float m = -fabsf(x), hi = m * kLog2e, lo = fmaf(m, kLog2e, -hi);
+    const float e = ex2(hi);
+    return fmaf(e, m > -80.f ? lo * kLn2 : 0.f, e);
+}
 __device__ __forceinline__ float softplus(float x) {
-    const float m = -fabsf(x);
-    const float hi = m * kLog2e, lo = fmaf(m, kLog2e, -hi);
-    float e = ex2(hi);
-    e = fmaf(e, m > -80.f ? lo * kLn2 : 0.f, e);
-    constexpr float kR[9] = {0.9999999403953552f, -0.4999949336051941f,  0.3331909775733948f,
-                             -0.2484298199415207f, 0.19106006622314453f,  -0.13663244247436523f,
-                             0.07822594046592712f, -0.029505232349038124f, 0.005232692696154118f};
-    float r = kR[8];
+    const float e = exp_minus_abs(x);
+    float r = log1p_term(kLog1pTerms - 1);
 #pragma unroll
-    for (int i = 7; i >= 0; --i) r = fmaf(r, e, kR[i]);
+    for (int i = kLog1pTerms - 2; i >= 0; --i) r = fmaf(r, e, log1p_term(i));
     return fmaf(e, r, fmaxf(x, 0.f));
 }
+
+// Two of them, without the range check: |s a| <= 126.  The same bits as exp2_fma.
+__device__ __forceinline__ float2 exp2_fma2(float2 s, float2 a) {
+    const float2 t = ffma2(s, a, splat2(kRound)), f = ffma2(s, a, fsub2(splat2(kRound), t));
+    float2 q = splat2(exp2_term(kExp2Terms - 1));
+#pragma unroll
+    for (int i = kExp2Terms - 2; i >= 0; --i) q = ffma2(q, f, splat2(exp2_term(i)));
+    q = ffma2(q, f, splat2(1.f));
+    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+
+// softplus of n values, two at a time where there are two
+template <int N>
+__device__ __forceinline__ void softplus_n(float (&v)[N]) {
+    if constexpr (N == 1) {
+        v[0] = softplus(v[0]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            const float2 e = make_float2(exp_minus_abs(v[k]), exp_minus_abs(v[k + 1]));
+            float2 r = splat2(log1p_term(kLog1pTerms - 1));
+#pragma unroll
+            for (int i = kLog1pTerms - 2; i >= 0; --i) r = ffma2(r, e, splat2(log1p_term(i)));
+            r = ffma2(e, r, make_float2(fmaxf(v[k], 0.f), fmaxf(v[k + 1], 0.f)));
+            v[k] = r.x;
+            v[k + 1] = r.y;
+        }
+    }
+}
+__device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 
 // A in the exponential's base: log2(e) A, kept finite so that a step of zero leaves the state as
 // it is (0 * inf would not).  NaN stays NaN.

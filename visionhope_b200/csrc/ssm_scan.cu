@@ -1,122 +1,175 @@
 // Selective scan, forward and one-token step (vh_ssm_scan_fwd, vh_ssm_scan_step).
-#include <type_traits>
-
 #include "ssm_scan.cuh"
 
 namespace vh {
 namespace ssm {
 namespace {
 
-// The forward scan: one warp per (sequence, channel tile), tokens in order (layout: ssm_scan.cuh).
-template <typename T, int NL>
-__global__ void __launch_bounds__(32 * kWarps) scan_fwd_kernel(const ScanParams p, int64_t items) {
+constexpr int kWarps = 4;        // one warp a chain: warps per CTA, neighbouring channel tiles
+constexpr int kSplitWarps = 16;  // many warps a chain: warps per CTA, consecutive segments
+
+// Four staged tokens; Y: also y's partial sums (pairs of channels, over the thread's states).
+template <int NL, int MODE, bool Y>
+__device__ __forceinline__ void advance(const Stage<NL>& st, int ct, int j, const float2 (&a2)[8], float2 (&h)[8],
+                                        float (&acc)[16]) {
     using K = Tile<NL>;
-    constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE;
-    __shared__ __align__(16) float s_step[kWarps][kGroup * CW];
-    __shared__ __align__(16) float s_su[kWarps][kGroup * CW];
-    __shared__ __align__(16) float s_bc[kWarps][kGroup * 2 * N];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tiles = p.groups * p.tiles_per_group;
-    const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
-    if (item >= items) return;
-    const int s = (int)(item / tiles), tile = (int)(item % tiles);
-    const int group = tile / p.tiles_per_group;
-    const int cbase = group * p.per_group + (tile % p.tiles_per_group) * CW;
-    const int cend = (group + 1) * p.per_group;
-    const Seq seq = seq_at(p.seqs, s);
-    const LaneElems<NL> own(lane);
-    const int n0 = 4 * (lane / K::CL), c0 = cbase + 4 * (lane % K::CL);  // the thread's 4 x 4 block
-    const int ec = cbase + own.c0;                                      // its elements' first channel
-    float *step = s_step[warp], *su = s_su[warp], *bc = s_bc[warp];
-
-    const T* u = static_cast<const T*>(p.u) + first_row(p.seqs, seq, s, p.ur) + ec;
-    const T* dl = static_cast<const T*>(p.delta) + first_row(p.seqs, seq, s, p.dr) + ec;
-    const T* z = p.z ? static_cast<const T*>(p.z) + first_row(p.seqs, seq, s, p.zr) + ec : nullptr;
-    const T* b = static_cast<const T*>(p.b) + first_row(p.seqs, seq, s, p.br) + group * p.bg;
-    const T* c = static_cast<const T*>(p.c) + first_row(p.seqs, seq, s, p.cr) + group * p.cg;
-    const int64_t us = row_step(p.seqs, p.ur), ds = row_step(p.seqs, p.dr), zs = row_step(p.seqs, p.zr);
-    const int64_t bs = row_step(p.seqs, p.br), cs = row_step(p.seqs, p.cr);
-    const Rows yr{p.seqs.length * p.channels, p.channels};
-    T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + ec;
-    const int64_t ys = row_step(p.seqs, yr);
-
-    float a2[16], h[16];
-    load_block<N>(p.a, c0, cend, n0, a2);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) a2[i] = to_log2(a2[i]);
-    if (p.initial) load_block<N>(p.initial + (int64_t)s * p.channels * N, c0, cend, n0, h);
-    else
+    for (int r = 0; r < kGroup; ++r) {
+        float2 s[2], su[2], b[4], e[8];
+        lds22(st.step + r * K::CW + ct, s);
+        lds22(st.su + r * K::CW + ct, su);
+        lds_dup4(st.b(r, j), b);
+        decays<MODE>(s, a2, e);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) h[i] = 0.f;
-    float bias[CE], skip[CE];
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < CE; ++i) {
-        bias[i] = p.delta_bias && ec + i < cend ? p.delta_bias[ec + i] : 0.f;
-        skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
-    }
-    float* ck = p.checkpoints ? p.checkpoints + slot_base(p.seqs, s, seq.row, kCheckpoint) * p.channels * N : nullptr;
-
-    for (int64_t t = 0; t < seq.len; t += kGroup) {
-        const int cnt = seq.len - t < kGroup ? (int)(seq.len - t) : kGroup;
-        if (ck && t % kCheckpoint == 0) store_block<N>(ck + (t / kCheckpoint) * p.channels * N, c0, cend, n0, h);
-        float ue[TE][CE], ze[TE][CE];
-#pragma unroll
-        for (int e = 0; e < TE; ++e) {
-            const int r = own.t0 + e;
-            float de[CE], prod[CE];
-#pragma unroll
-            for (int i = 0; i < CE; ++i) ue[e][i] = ze[e][i] = de[i] = 0.f;
-            if (r < cnt) {
-                load_v<CE>(u + (t + r) * us, ec, cend, p.vec, ue[e]);
-                load_v<CE>(dl + (t + r) * ds, ec, cend, p.vec, de);
-                if (z) load_v<CE>(z + (t + r) * zs, ec, cend, p.vec, ze[e]);
-#pragma unroll
-                for (int i = 0; i < CE; ++i) {
-                    de[i] += bias[i];
-                    if (p.softplus) de[i] = softplus(de[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < CE; ++i) prod[i] = de[i] * ue[e][i];
-            sts_v<CE>(step + r * CW + own.c0, de);
-            sts_v<CE>(su + r * CW + own.c0, prod);
-        }
-        stage_bc<NL>(b + t * bs, c + t * cs, bs, cs, cnt, p.vec_bc, lane, bc);
-        __syncwarp();
-        float acc[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.f;
-#pragma unroll
-        for (int r = 0; r < kGroup; ++r) {
-            float sv[4], pv[4], bv[4], cv[4];
-            lds4(step + r * CW + 4 * (lane % K::CL), sv);
-            lds4(su + r * CW + 4 * (lane % K::CL), pv);
-            lds4(bc + r * 2 * N + n0, bv);
-            lds4(bc + r * 2 * N + N + n0, cv);
+            for (int p = 0; p < 2; ++p) h[2 * i + p] = ffma2(e[2 * i + p], h[2 * i + p], fmul2(su[p], b[i]));
+        if constexpr (Y) {
+            float2 c[4], y[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            lds_dup4(st.c(r, j), c);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    float& hh = h[4 * i + n];
-                    hh = fmaf(pv[i], bv[n], exp2_fma(sv[i] * a2[4 * i + n]) * hh);
-                    acc[4 * r + i] = fmaf(cv[n], hh, acc[4 * r + i]);
-                }
-        }
-        __syncwarp();
-        reduce_scatter<16, NL, K::CL>(acc, lane);
-#pragma unroll
-        for (int e = 0; e < TE; ++e) {
-            const int r = own.t0 + e;
-            float out[CE];
-#pragma unroll
-            for (int i = 0; i < CE; ++i) {
-                out[i] = fmaf(skip[i], ue[e][i], acc[e * CE + i]);
-                if (z) out[i] *= ze[e][i] * sigmoid(ze[e][i]);
-            }
-            if (r < cnt) store_v<CE>(y + (t + r) * ys, ec, cend, p.vec, out);
+                for (int p = 0; p < 2; ++p) y[p] = ffma2(c[i], h[2 * i + p], y[p]);
+            acc[4 * r] = y[0].x; acc[4 * r + 1] = y[0].y; acc[4 * r + 2] = y[1].x; acc[4 * r + 3] = y[1].y;
         }
     }
-    if (p.final_state) store_block<N>(p.final_state + (int64_t)s * p.channels * N, c0, cend, n0, h);
+}
+
+// The forward scan.  A chain is a channel tile of a sequence.
+// SPLIT = false: one warp walks a chain, four neighbouring chains a CTA.
+// SPLIT = true, for few chains: the sixteen warps of a CTA, and the CTAs of a cluster, take
+// consecutive segments of one chain.  Each warp first runs its segment from a zero state, without
+// outputs.  A segment maps the state before it to exp(a sum s) h + own state, so the states before
+// all segments follow from the sixteen own states and step sums of each CTA (512 threads, one
+// state each) and the totals of the CTAs before it, read from their shared memory.  Then each
+// warp runs its segment again from its true state.  Twice the exponentials, against the length
+// of a chain divided by up to 128.
+template <typename T, int NL, bool SPLIT>
+__global__ void __launch_bounds__(32 * (SPLIT ? kSplitWarps : kWarps), SPLIT ? 1 : 3)
+    scan_fwd_kernel(const ScanParams p, int64_t chains, int cluster) {
+    using K = Tile<NL>;
+    constexpr int CE = K::CE, TE = K::TE;
+    constexpr int W = SPLIT ? kSplitWarps : kWarps;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Stage<NL>* stages = reinterpret_cast<Stage<NL>*>(smem);
+    // split only: what leaves and enters the segments
+    float* states = reinterpret_cast<float*>(stages + 2 * W);
+    SplitSmem<NL, W>& sp = *reinterpret_cast<SplitSmem<NL, W>*>(states + 512 * W);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tiles = p.groups * p.tiles_per_group;
+    const int64_t chain = SPLIT ? blockIdx.x / cluster : (int64_t)blockIdx.x * W + warp;
+    if (!SPLIT && chain >= chains) return;
+    const int s = (int)(chain / tiles), tile = (int)(chain % tiles);
+    const Seq seq = seq_at(p.seqs, s);
+    Chain<T, NL> ch(p, seq, s, tile, lane);
+    const int j = lane / K::CL, ct = 4 * (lane % K::CL), c0 = ch.cbase + ct;  // the thread's 4 x 4 block
+    const int ec = ch.ec, cend = ch.cend;
+    Stage<NL>* st = stages + 2 * warp;
+    const Rows yr{p.seqs.length * p.channels, p.channels};
+    T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + ec;
+    const int64_t ys = row_step(p.seqs, yr);
+    float skip[CE];
+#pragma unroll
+    for (int i = 0; i < CE; ++i) skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
+    const float* initial = p.initial ? p.initial + (int64_t)s * p.channels * K::N : nullptr;
+    float2 a2[8], h[8];
+    float v[16];
+    const float top_a = load_rates<NL>(p, c0, cend, j, v);
+    pair_up(v, a2);
+
+    int64_t t0 = 0, t1 = seq.len;
+    if constexpr (SPLIT) {
+        if (warp == 0) store_lanes(sp.a2, lane, v);
+        const int rank = blockIdx.x % cluster;
+        const int seg = rank * W + warp, segs = cluster * W;
+        const int64_t size = max((seq.len + segs - 1) / segs + kGroup - 1, (int64_t)4 * kGroup) / kGroup * kGroup;
+        t0 = min(seq.len, seg * size);
+        t1 = min(seq.len, t0 + size);
+        float sum[CE];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < CE; ++i) sum[i] = 0.f;
+        if (t1 < seq.len) {  // what leaves the last segment is not needed
+            Chain<T, NL> at = ch;
+            at.move(t0);
+            typename Chain<T, NL>::Raw raw;
+            at.template load<false>(raw, t1 - t0);
+            int buf = 0;
+            for (int64_t t = t0; t < t1; t += kGroup, buf ^= 1) {
+                const float top = at.template stage<true>(raw, t1 - t, st[buf], sum);
+                __syncwarp();
+                at.move(kGroup);
+                if (t + kGroup < t1) at.template load<false>(raw, t1 - t - kGroup);
+                if (top * top_a <= 126.f) advance<NL, kMixed, false>(st[buf], ct, j, a2, h, v);
+                else advance<NL, kChecked, false>(st[buf], ct, j, a2, h, v);
+            }
+            __syncwarp();
+        }
+        pair_down(h, v);
+        store_lanes(states + 512 * warp, lane, v);
+        sum_tokens<NL>(sum, lane, ch.own_c, sp.sigma[warp]);
+        enter_segments<NL, W, false>(sp, [&](int w) { return states + 512 * w; }, initial, ch.cbase, cend, cluster, rank);
+        load_lanes(states + 512 * warp, lane, v);
+    } else if (initial) {
+        load_block<NL>(initial, c0, cend, j, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    }
+    pair_up(v, h);
+
+    float* ck = p.checkpoints
+                    ? p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512 : nullptr;
+    if (t0 < t1) {
+        float unused[CE];
+#pragma unroll
+        for (int i = 0; i < CE; ++i) unused[i] = 0.f;
+        ch.move(t0);
+        y += (t0 + ch.own_t) * ys;
+        typename Chain<T, NL>::Raw raw;
+        ch.template load<true>(raw, t1 - t0);
+        int buf = 0;
+        for (int64_t t = t0; t < t1; t += kGroup, buf ^= 1) {
+            if (ck && t % kCheckpoint == 0) {
+                pair_down(h, v);
+                store_lanes(ck + (t / kCheckpoint) * tiles * 512, lane, v);
+            }
+            const float top = ch.template stage<false>(raw, t1 - t, st[buf], unused);
+            float ue[TE][CE], ze[TE][CE];
+#pragma unroll
+            for (int e = 0; e < TE; ++e) {
+                raw.u[e].get(ue[e]);
+                if (ch.gated) raw.z[e].get(ze[e]);
+            }
+            __syncwarp();
+            ch.move(kGroup);
+            if (t + kGroup < t1) ch.template load<true>(raw, t1 - t - kGroup);
+            float acc[16];
+            if (top * top_a <= 126.f) advance<NL, kMixed, true>(st[buf], ct, j, a2, h, acc);
+            else advance<NL, kChecked, true>(st[buf], ct, j, a2, h, acc);
+            reduce_scatter<16, NL, K::CL>(acc, lane);
+#pragma unroll
+            for (int e = 0; e < TE; ++e) {
+                float out[CE];
+#pragma unroll
+                for (int i = 0; i < CE; ++i) {
+                    out[i] = fmaf(skip[i], ue[e][i], acc[e * CE + i]);
+                    if (ch.gated) out[i] *= ze[e][i] * sigmoid(ze[e][i]);
+                }
+                if (t + ch.own_t + e < t1) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
+            }
+            y += kGroup * ys;
+        }
+    }
+    // the last token's warp, or for an empty sequence the first one
+    const bool ends = seq.len > 0 ? t0 < t1 && t1 == seq.len : (!SPLIT || (warp == 0 && blockIdx.x % cluster == 0));
+    if (p.final_state && ends) {
+        pair_down(h, v);
+        store_block<NL>(p.final_state + (int64_t)s * p.channels * K::N, c0, cend, j, v);
+    }
+    if (SPLIT && cluster > 1) cluster_wait();
 }
 
 // One token per stream: a thread owns four states of one channel, N / 4 threads a channel.
@@ -147,7 +200,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanParams p, cons
         const float pu = st * uu;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            hv[n] = fmaf(pu, bv[n], exp2_fma(st * to_log2(av[n])) * hv[n]);
+            hv[n] = fmaf(pu, bv[n], exp2_fma(st, to_log2(av[n])) * hv[n]);
             part = fmaf(cv[n], hv[n], part);
         }
         *reinterpret_cast<float4*>(state_out + ((int64_t)slot * p.channels + c) * N + n0) =
@@ -166,6 +219,30 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanParams p, cons
 }
 
 bool stride_ok(int64_t v, int m) { return v % m == 0; }
+
+template <typename T, int NL>
+int launch_fwd(const ScanParams& p, int64_t chains, cudaStream_t st) {
+    // One warp a chain once there are two for each of the SM's four schedulers; fewer chains, and
+    // packed sequences, whose lengths the host does not know, are split.
+    const bool split = p.seqs.length > 4 * kGroup && (chains < 8 * sm_count() || p.seqs.offsets);
+    if (!split) {
+        const size_t smem = sizeof(Stage<NL>) * 2 * kWarps;
+        if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, false>), smem))
+            return fail(VH_E_DEVICE, "vh_ssm_scan_fwd: cannot reserve %zu bytes of shared memory", smem);
+        const int64_t blocks = (chains + kWarps - 1) / kWarps;
+        if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_fwd: too many channel tiles");
+        scan_fwd_kernel<T, NL, false><<<(int)blocks, 32 * kWarps, smem, st>>>(p, chains, 1);
+        return launch_status("selective scan");
+    }
+    const size_t smem = (sizeof(Stage<NL>) * 2 + 2048) * kSplitWarps + sizeof(SplitSmem<NL, kSplitWarps>);
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, true>), smem))
+        return fail(VH_E_DEVICE, "vh_ssm_scan_fwd: cannot reserve %zu bytes of shared memory", smem);
+    static std::atomic<int> known[64][9];
+    const int cluster = pick_cluster(scan_fwd_kernel<T, NL, true>, known, 32 * kSplitWarps, smem, chains,
+                                     p.seqs.length, 4 * kGroup);
+    return launch_cluster("selective scan", scan_fwd_kernel<T, NL, true>, chains * cluster, 32 * kSplitWarps, smem, cluster,
+                          st, p, chains, cluster);
+}
 
 }  // namespace
 
@@ -223,33 +300,36 @@ void fill_scan_params(const vh_ssm_scan_args* a, ScanParams* p) {
     p->vec_bc = w;
 }
 
+// The checkpoints: a warp's states for every slot of 32 tokens and channel tile.
+int64_t checkpoint_floats(const vh_ssm_scan_args* a) {
+    const int cw = 128 / (a->states / 4), per = a->channels / a->groups;
+    const int64_t tiles = (int64_t)a->groups * ((per + cw - 1) / cw);
+    return slot_total(a->seq_offsets != nullptr, a->length, a->batch, kCheckpoint) * tiles * 512;
+}
+
 }  // namespace ssm
 }  // namespace vh
 
 using namespace vh;
 using namespace vh::ssm;
 
-extern "C" int64_t vh_ssm_scan_checkpoint_slots(const vh_ssm_scan_args* a) {
-    if (!a || a->batch <= 0 || a->length < 0) return 0;
-    return slot_total(a->seq_offsets != nullptr, a->length, a->batch, kCheckpoint);
+extern "C" int64_t vh_ssm_scan_checkpoint_bytes(const vh_ssm_scan_args* a) {
+    if (!a || a->batch <= 0 || a->length < 0 || a->channels <= 0 || a->groups <= 0 || a->channels % a->groups ||
+        a->states < 4)
+        return 0;
+    return checkpoint_floats(a) * 4;
 }
 
-extern "C" int64_t vh_ssm_scan_fwd_workspace_bytes(const vh_ssm_scan_args*) { return 0; }
-
-extern "C" int vh_ssm_scan_fwd(const vh_ssm_scan_args* a, void*, int64_t, vh_stream_t stream) {
+extern "C" int vh_ssm_scan_fwd(const vh_ssm_scan_args* a, vh_stream_t stream) {
     clear_error();
     if (int rc = check_scan_args("vh_ssm_scan_fwd", a, false)) return rc;
     ScanParams p;
     fill_scan_params(a, &p);
-    const int64_t items = (int64_t)a->batch * p.groups * p.tiles_per_group;
-    const int64_t blocks = (items + kWarps - 1) / kWarps;
-    if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_fwd: too many channel tiles");
+    const int64_t chains = (int64_t)a->batch * p.groups * p.tiles_per_group;
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_states(a->states, [&](auto nl) {
-            scan_fwd_kernel<T, decltype(nl)::value>
-                <<<(int)blocks, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(p, items);
-            return launch_status("selective scan");
+            return launch_fwd<T, decltype(nl)::value>(p, chains, static_cast<cudaStream_t>(stream));
         });
     });
 }

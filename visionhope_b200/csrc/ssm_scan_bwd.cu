@@ -1,25 +1,23 @@
 // Selective scan, backward (vh_ssm_scan_bwd).
 //
-// With p_t = s_t u_t, i_t = sum_n c_t h_t + D u_t (the output before its gate) and
-// v_t = dy_t silu(z_t) (or dy_t):
-//     g_t = c_t v_t + exp(s_{t+1} a) g_{t+1}          (the gradient of h_t, last token first)
+// With p_t = s_t u_t, e_t = exp(s_t a), i_t = sum_n c_t h_t + D u_t (the output before its gate)
+// and v_t = dy_t silu(z_t) (or dy_t):
+//     g_t = c_t v_t + e_{t+1} g_{t+1}                 (the gradient of h_t, last token first)
 //     dc_t = sum_channels v_t h_t                     db_t = sum_channels p_t g_t
-//     q_t  = g_t exp(s_t a) h_{t-1}                   da = sum_t s_t q_t
+//     q_t  = e_t g_t h_{t-1}                          da = sum_t s_t q_t
 //     ds_t = sum_n a q_t + u_t sum_n b_t g_t          du_t = s_t sum_n b_t g_t + D v_t
 //     dz_t = dy_t i_t silu'(z_t)                      dD = sum_t v_t u_t
-// ds_t goes through softplus' derivative to delta_t and delta_bias.  The products e h_{t-1} and
-// the decays e = exp(s_t a) of a group of four tokens are computed once and kept in registers
-// between the two directions.
+// ds_t goes through softplus' derivative to delta_t and delta_bias.
 //
-// A warp owns a channel tile of a sequence (layout: ssm_scan.cuh) and walks its chunks of 32
+// A warp owns a channel tile (layout: ssm_scan.cuh) of a run of tokens and walks its chunks of 32
 // tokens from the last to the first.  The forward left the state before each chunk; the warp runs
-// it forward again once, leaving the state before each group of four in shared memory, and then
-// takes the groups in reverse, computing each again from its saved state.  Sums over channels
-// (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias) one per
-// sequence, and two small kernels add them in order.
-#include <algorithm>
-#include <type_traits>
-
+// the chunk forward once, leaving the state before each group of four in shared memory, and then
+// takes the groups in reverse: four tokens forward again with their decays and states in
+// registers, then back through them.  The states start from the forward's every 32 tokens, so
+// the first of these passes takes all its decays from the special-function unit; the second one's
+// carry the gradient along the whole sequence (see ssm_scan.cuh on the exponentials).  Sums over
+// channels (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias)
+// one per CTA, and small kernels add them in order.
 #include "ssm_scan.cuh"
 
 namespace vh {
@@ -27,6 +25,10 @@ namespace ssm {
 namespace {
 
 constexpr int kGroups = kCheckpoint / kGroup;  // groups in a chunk
+constexpr int kBwdWarps = 4;                   // one warp a chain: warps per CTA
+// many warps a chain: as many as the shared memory of a CTA holds
+template <int NL>
+constexpr int kBwdSplitWarps = NL >= 4 ? 8 : 4;
 
 struct BwdParams {
     ScanParams f;
@@ -35,297 +37,393 @@ struct BwdParams {
     void *du, *ddelta, *dz;
     float* dinitial;
     float* part_bc;  // [tiles][tokens][2][N]
-    float* part_a;   // [sequences][channels][N]
-    float* part_d;   // [sequences][2][channels]: dD, d delta_bias
+    float* part_a;   // [rows][tiles][512] in lane order; a row per sequence and CTA of its cluster
+    float* part_d;   // [rows][2][tiles][CW]: dD, d delta_bias
     int64_t tokens;
     int32_t vec;     // as f.vec, for dy and the outputs too
 };
 
 template <int NL>
-struct BwdSmem {
+struct BwdStage {
     using K = Tile<NL>;
-    float h[kGroups][32 * 16];
-    float step[kGroup * K::CW], su[kGroup * K::CW], v[kGroup * K::CW];
-    float bc[kGroup * 2 * K::N];
-    float y[kGroup * K::CW], ds[kGroup * K::CW], gb[kGroup * K::CW];
+    float h[kGroups][512];        // the states before the groups of a chunk
+    float past[kGroup - 1][512];  // before the second to fourth token of the group at hand
+    Stage<NL> s;
+    float v[kGroup * K::CW], y[kGroup * K::CW], ds[kGroup * K::CW], gb[kGroup * K::CW];
+};
+template <int NL, int W>
+struct BwdSplitSmem {
+    SplitSmem<NL, W> s;
+    float dd[2][W][Tile<NL>::CW];
 };
 
-// Sums four values (channels c of one token) over the state lanes into row[c of the tile].
+// Values in shared memory are read again after this, instead of being kept in registers.
+__device__ __forceinline__ void reload() { asm volatile("" ::: "memory"); }
+
+// Sums four values (channels of one token) over the state lanes into row[channel of the tile].
 template <int NL>
-__device__ __forceinline__ void sum_states(float (&v)[4], int lane, float* row) {
+__device__ __forceinline__ void sum_states(const float2 (&p)[2], int lane, float* row) {
     using K = Tile<NL>;
+    float v[4] = {p[0].x, p[0].y, p[1].x, p[1].y};
     reduce_scatter<4, NL, K::CL>(v, lane);
-    constexpr int kKeep = NL >= 4 ? 1 : 4 / NL;
+    constexpr int kKeep = NL >= 4 ? 1 : 4 / NL, kSame = NL >= 4 ? NL / 4 : 1;
     const int j = lane / K::CL, k = lane % K::CL;
-    const int first = j * 4 / NL;
-    if (NL <= 4 || j % (NL / 4 > 0 ? NL / 4 : 1) == 0) {
+    if (j % kSame == 0) {
 #pragma unroll
-        for (int i = 0; i < kKeep; ++i) row[4 * k + first + i] = v[i];
+        for (int i = 0; i < kKeep; ++i) row[4 * k + j * 4 / NL + i] = v[i];
     }
 }
 
-template <typename T, int NL>
-__global__ void __launch_bounds__(32 * kWarps, 2) scan_bwd_kernel(const BwdParams bp, int64_t items) {
+template <typename T, int NL, bool SPLIT>
+__global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps), SPLIT ? 1 : 2)
+    scan_bwd_kernel(const BwdParams bp, int64_t chains, int cluster) {
     using K = Tile<NL>;
     constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL;
+    constexpr int W = SPLIT ? kBwdSplitWarps<NL> : kBwdWarps;
     extern __shared__ __align__(16) unsigned char smem[];
+    BwdStage<NL>* stages = reinterpret_cast<BwdStage<NL>*>(smem);
+    BwdSplitSmem<NL, W>& sp = *reinterpret_cast<BwdSplitSmem<NL, W>*>(stages + W);
     const ScanParams& p = bp.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tiles = p.groups * p.tiles_per_group;
-    const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
-    if (item >= items) return;
-    BwdSmem<NL>& sm = reinterpret_cast<BwdSmem<NL>*>(smem)[warp];
-    const int s = (int)(item / tiles), tile = (int)(item % tiles);
-    const int group = tile / p.tiles_per_group;
-    const int cbase = group * p.per_group + (tile % p.tiles_per_group) * CW;
-    const int cend = (group + 1) * p.per_group;
+    const int64_t chain = SPLIT ? blockIdx.x / cluster : (int64_t)blockIdx.x * W + warp;
+    if (!SPLIT && chain >= chains) return;
+    BwdStage<NL>& sm = stages[warp];
+    const int s = (int)(chain / tiles), tile = (int)(chain % tiles);
+    const int rank = SPLIT ? blockIdx.x % cluster : 0;
     const Seq seq = seq_at(p.seqs, s);
-    const LaneElems<NL> own(lane);
-    const int n0 = 4 * (lane / CL), ct = 4 * (lane % CL), c0 = cbase + ct;
-    const int ec = cbase + own.c0;
-
-    const T* u = static_cast<const T*>(p.u) + first_row(p.seqs, seq, s, p.ur) + ec;
-    const T* dl = static_cast<const T*>(p.delta) + first_row(p.seqs, seq, s, p.dr) + ec;
-    const T* z = p.z ? static_cast<const T*>(p.z) + first_row(p.seqs, seq, s, p.zr) + ec : nullptr;
-    const T* b = static_cast<const T*>(p.b) + first_row(p.seqs, seq, s, p.br) + group * p.bg;
-    const T* c = static_cast<const T*>(p.c) + first_row(p.seqs, seq, s, p.cr) + group * p.cg;
-    const int64_t us = row_step(p.seqs, p.ur), ds = row_step(p.seqs, p.dr), zs = row_step(p.seqs, p.zr);
-    const int64_t bs = row_step(p.seqs, p.br), cs = row_step(p.seqs, p.cr);
+    Chain<T, NL> chn(p, seq, s, tile, lane);
+    const int j = lane / CL, ct = 4 * (lane % CL), c0 = chn.cbase + ct;
+    const int ec = chn.ec, cend = chn.cend, own_t = chn.own_t, own_c = chn.own_c;
     const Rows yr{p.seqs.length * p.channels, p.channels};
     const int64_t y0 = first_row(p.seqs, seq, s, yr) + ec, ys = row_step(p.seqs, yr);
     const T* dy = static_cast<const T*>(bp.dy) + y0;
+    const bool gated = p.z != nullptr;
+    float2 a2[8], g[8], da[8];
+    float v16[16];
+    const float top_a = load_rates<NL>(p, c0, cend, j, v16);
+    pair_up(v16, a2);
+    const float* dfinal = bp.dfinal ? bp.dfinal + (int64_t)s * p.channels * N : nullptr;
+
+    struct Raw {
+        typename Chain<T, NL>::Raw r;
+        Pack<T, CE> dy[TE];
+    };
+    // dy's rows lie as y's; it moves with the chain's view, which stands at token `pos`
+    const T* dyr = dy + (chn.left > 0 ? 0 : -(ec - (cend - (bp.vec ? CE : 1)))) + own_t * ys;
+    int64_t pos = 0;
+    auto move = [&](int64_t to) {
+        chn.move(to - pos);
+        dyr += (to - pos) * ys;
+        pos = to;
+    };
+    auto load = [&](Raw& r, int64_t count) {
+        chn.template load<true>(r.r, count);
+#pragma unroll
+        for (int e = 0; e < TE; ++e) {
+            const int64_t by = count >= kGroup ? e : min((int64_t)e, count - 1 - own_t);
+            r.dy[e].load(dyr + by * ys, chn.left, bp.vec);
+        }
+    };
+    // s, s u, B, C and v of a group
+    auto stage = [&](const Raw& r, int64_t count, float (&sum)[CE]) {
+        const float top = chn.template stage<true>(r.r, count, sm.s, sum);
+#pragma unroll
+        for (int e = 0; e < TE; ++e) {
+            float ve[CE], ze[CE];
+            r.dy[e].get(ve);
+            if (gated) {
+                r.r.z[e].get(ze);
+#pragma unroll
+                for (int i = 0; i < CE; ++i) ve[i] *= ze[i] * sigmoid(ze[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < CE; ++i)
+                ve[i] = own_t + e < count && (bp.vec ? chn.left > 0 : i < chn.left) ? ve[i] : 0.f;
+            sts_v<CE>(sm.v + (own_t + e) * CW + own_c, ve);
+        }
+        return top;
+    };
+
+    int64_t t0 = 0, t1 = seq.len;
+    if constexpr (SPLIT) {
+        if (warp == 0) store_lanes(sp.s.a2, lane, v16);
+        const int seg = rank * W + warp, segs = cluster * W;
+        const int64_t size = ((seq.len + segs - 1) / segs + kCheckpoint - 1) / kCheckpoint * kCheckpoint;
+        t0 = min(seq.len, seg * size);
+        t1 = min(seq.len, t0 + size);
+        // The own gradient of a segment, that of the state before it when nothing enters from the
+        // right: sum_t (e_{t0} ... e_t) c_t v_t, in one pass forward.
+        float2 prod[8], own[8];
+        float sum[CE];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { prod[i] = make_float2(1.f, 1.f); own[i] = make_float2(0.f, 0.f); }
+#pragma unroll
+        for (int i = 0; i < CE; ++i) sum[i] = 0.f;
+        if (t0 > 0 && t0 < t1) {  // what leaves the first segment comes from its second pass
+            move(t0);
+            Raw raw;
+            load(raw, t1 - t0);
+            for (int64_t t = t0; t < t1; t += kGroup) {
+                const float top = stage(raw, t1 - t, sum);
+                __syncwarp();
+                move(t + kGroup);
+                if (t + kGroup < t1) load(raw, t1 - t - kGroup);
+                auto pass = [&](auto mode) {
+#pragma unroll
+                    for (int r = 0; r < kGroup; ++r) {
+                        float2 sv[2], vv[2], c[4], e[8];
+                        lds22(sm.s.step + r * CW + ct, sv);
+                        lds22(sm.v + r * CW + ct, vv);
+                        lds_dup4(sm.s.c(r, j), c);
+                        decays<decltype(mode)::value>(sv, a2, e);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                prod[2 * i + q] = fmul2(prod[2 * i + q], e[2 * i + q]);
+                                own[2 * i + q] = ffma2(prod[2 * i + q], fmul2(c[i], vv[q]), own[2 * i + q]);
+                            }
+                    }
+                };
+                if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
+            else pass(std::integral_constant<int, kChecked>{});
+                __syncwarp();
+            }
+        }
+        pair_down(own, v16);
+        store_lanes(sm.h[0], lane, v16);
+        sum_tokens<NL>(sum, lane, own_c, sp.s.sigma[warp]);
+        enter_segments<NL, W, true>(sp.s, [&](int w) { return stages[w].h[0]; }, dfinal, chn.cbase, cend, cluster, rank);
+        load_lanes(sm.h[0], lane, v16);
+    } else if (dfinal) {
+        load_block<NL>(dfinal, c0, cend, j, v16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v16[i] = 0.f;
+    }
+    pair_up(v16, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) da[i] = make_float2(0.f, 0.f);
+
     T* du = static_cast<T*>(bp.du) + y0;
     T* dd = static_cast<T*>(bp.ddelta) + y0;
     T* dz = bp.dz ? static_cast<T*>(bp.dz) + y0 : nullptr;
     const Rows tr{p.seqs.length, 1};
     float* pbc = bp.part_bc + ((int64_t)tile * bp.tokens + first_row(p.seqs, seq, s, tr)) * 2 * N;
     const int64_t ps = row_step(p.seqs, tr) * 2 * N;
-    const float* ck = p.checkpoints + slot_base(p.seqs, s, seq.row, kCheckpoint) * p.channels * N;
-
-    float a2[16], g[16], da[16];
-    load_block<N>(p.a, c0, cend, n0, a2);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        a2[i] = to_log2(a2[i]);
-        g[i] = da[i] = 0.f;
-    }
-    if (bp.dfinal) load_block<N>(bp.dfinal + (int64_t)s * p.channels * N, c0, cend, n0, g);
-    float bias[CE], skip[CE], dskip[CE], dbias[CE];
+    const float* ck = p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512;
+    float skip[CE], dskip[CE], dbias[CE];
 #pragma unroll
     for (int i = 0; i < CE; ++i) {
-        bias[i] = p.delta_bias && ec + i < cend ? p.delta_bias[ec + i] : 0.f;
         skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
         dskip[i] = dbias[i] = 0.f;
     }
 
-    const int64_t chunks = (seq.len + kCheckpoint - 1) / kCheckpoint;
-    for (int64_t ch = chunks - 1; ch >= 0; --ch) {
+    const int64_t first = t0 / kCheckpoint, last = (t1 + kCheckpoint - 1) / kCheckpoint;
+    for (int64_t ch = last - 1; ch >= first && t0 < t1; --ch) {
         const int64_t tc = ch * kCheckpoint;
-        const int len = seq.len - tc < kCheckpoint ? (int)(seq.len - tc) : kCheckpoint;
-        const int groups = (len + kGroup - 1) / kGroup;
-        float h[16];
-        load_block<N>(ck + ch * p.channels * N, c0, cend, n0, h);
-
+        const int64_t te = min(t1, tc + kCheckpoint);
+        const int groups = (int)((te - tc + kGroup - 1) / kGroup);
+        float unused[CE];
+#pragma unroll
+        for (int i = 0; i < CE; ++i) unused[i] = 0.f;
+        float2 h[8];
+        load_lanes(ck + ch * tiles * 512, lane, v16);
+        pair_up(v16, h);
         // forward over all groups but the last, whose state is not needed beyond its start
-        for (int gi = 0; gi < groups; ++gi) {
+        {
+            move(tc);
+            typename Chain<T, NL>::Raw raw;
+            if (groups > 1) chn.template load<false>(raw, te - tc);
+            for (int gi = 0; gi < groups; ++gi) {
+                pair_down(h, v16);
+                store_lanes(sm.h[gi], lane, v16);
+                if (gi + 1 == groups) break;
+                chn.template stage<false>(raw, kGroup, sm.s, unused);
+                __syncwarp();
+                move(tc + (gi + 1) * kGroup);
+                if (gi + 2 < groups) chn.template load<false>(raw, kGroup);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4*>(&sm.h[gi][(i * 32 + lane) * 4]) =
-                    make_float4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
-            if (gi + 1 == groups) break;
-            const int64_t t = tc + gi * kGroup;
+                for (int r = 0; r < kGroup; ++r) {
+                    float2 sv[2], pv[2], b[4], e[8];
+                    lds22(sm.s.step + r * CW + ct, sv);
+                    lds22(sm.s.su + r * CW + ct, pv);
+                    lds_dup4(sm.s.b(r, j), b);
+                    decays<kHardware>(sv, a2, e);
 #pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                const int r = own.t0 + e;
-                float ue[CE], de[CE];
-                load_v<CE>(u + (t + r) * us, ec, cend, p.vec, ue);
-                load_v<CE>(dl + (t + r) * ds, ec, cend, p.vec, de);
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int i = 0; i < CE; ++i) {
-                    de[i] += bias[i];
-                    if (p.softplus) de[i] = softplus(de[i]);
-                    ue[i] *= de[i];
+                        for (int q = 0; q < 2; ++q) h[2 * i + q] = ffma2(e[2 * i + q], h[2 * i + q], fmul2(pv[q], b[i]));
                 }
-                sts_v<CE>(sm.step + r * CW + own.c0, de);
-                sts_v<CE>(sm.su + r * CW + own.c0, ue);
+                __syncwarp();
             }
-            stage_bc<NL>(b + t * bs, c + t * cs, bs, cs, kGroup, p.vec_bc, lane, sm.bc);
-            __syncwarp();
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) {
-                float sv[4], pv[4], bv[4];
-                lds4(sm.step + r * CW + ct, sv);
-                lds4(sm.su + r * CW + ct, pv);
-                lds4(sm.bc + r * 2 * N + n0, bv);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        float& hh = h[4 * i + n];
-                        hh = fmaf(pv[i], bv[n], exp2_fma(sv[i] * a2[4 * i + n]) * hh);
-                    }
-            }
-            __syncwarp();
         }
-
+        Raw raw;
+        load(raw, te - pos);  // the last group: the forward pass moved there
         for (int gi = groups - 1; gi >= 0; --gi) {
             const int64_t t = tc + gi * kGroup;
-            const int cnt = len - gi * kGroup < kGroup ? len - gi * kGroup : kGroup;
-            float ue[TE][CE], ze[TE][CE], re[TE][CE], ye[TE][CE];  // u, z, delta + bias, dy
-#pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                const int r = own.t0 + e;
-                float de[CE], pe[CE], ve[CE];
-#pragma unroll
-                for (int i = 0; i < CE; ++i) ue[e][i] = ze[e][i] = re[e][i] = ye[e][i] = de[i] = 0.f;
-                if (r < cnt) {
-                    load_v<CE>(u + (t + r) * us, ec, cend, p.vec, ue[e]);
-                    load_v<CE>(dl + (t + r) * ds, ec, cend, p.vec, re[e]);
-                    if (z) load_v<CE>(z + (t + r) * zs, ec, cend, p.vec, ze[e]);
-                    load_v<CE>(dy + (t + r) * ys, ec, cend, bp.vec, ye[e]);
-#pragma unroll
-                    for (int i = 0; i < CE; ++i) {
-                        re[e][i] += bias[i];
-                        de[i] = p.softplus ? softplus(re[e][i]) : re[e][i];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < CE; ++i) {
-                    pe[i] = de[i] * ue[e][i];
-                    ve[i] = z ? ye[e][i] * (ze[e][i] * sigmoid(ze[e][i])) : ye[e][i];
-                }
-                sts_v<CE>(sm.step + r * CW + own.c0, de);
-                sts_v<CE>(sm.su + r * CW + own.c0, pe);
-                sts_v<CE>(sm.v + r * CW + own.c0, ve);
-            }
-            stage_bc<NL>(b + t * bs, c + t * cs, bs, cs, cnt, p.vec_bc, lane, sm.bc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float q[4];
-                lds4(&sm.h[gi][(i * 32 + lane) * 4], q);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) h[4 * i + n] = q[n];
-            }
+            const float top = stage(raw, te - t, unused);
+            const Raw now = raw;
             __syncwarp();
-            float e[kGroup][16], eh[kGroup][16];  // decays, and decays times the state before
-            float dcs[kGroup][4];
-#pragma unroll
-            for (int r = 0; r < kGroup; ++r) {
-                float sv[4], pv[4], vv[4], bv[4], cv[4], acc[4];
-                lds4(sm.step + r * CW + ct, sv);
-                lds4(sm.su + r * CW + ct, pv);
-                lds4(sm.v + r * CW + ct, vv);
-                lds4(sm.bc + r * 2 * N + n0, bv);
-                lds4(sm.bc + r * 2 * N + N + n0, cv);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) dcs[r][n] = acc[n] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        float& hh = h[4 * i + n];
-                        e[r][4 * i + n] = exp2_fma(sv[i] * a2[4 * i + n]);
-                        eh[r][4 * i + n] = e[r][4 * i + n] * hh;
-                        hh = fmaf(pv[i], bv[n], eh[r][4 * i + n]);
-                        acc[i] = fmaf(cv[n], hh, acc[i]);
-                        dcs[r][n] = fmaf(vv[i], hh, dcs[r][n]);
-                    }
-                if (z) sum_states<NL>(acc, lane, sm.y + r * CW);
+            if (gi > 0) {
+                move(t - kGroup);
+                load(raw, kGroup);
             }
+            auto pass = [&](auto mode) {
+                float2 e[kGroup][8];
+                float dcs[kGroup][4];
+                load_lanes(sm.h[gi], lane, v16);
+                pair_up(v16, h);
 #pragma unroll
-            for (int r = kGroup - 1; r >= 0; --r) {
-                float sv[4], pv[4], vv[4], bv[4], cv[4], dsum[4], gsum[4], bcs[8];
-                lds4(sm.step + r * CW + ct, sv);
-                lds4(sm.su + r * CW + ct, pv);
-                lds4(sm.v + r * CW + ct, vv);
-                lds4(sm.bc + r * 2 * N + n0, bv);
-                lds4(sm.bc + r * 2 * N + N + n0, cv);
+                for (int r = 0; r < kGroup; ++r) {
+                    reload();
+                    float2 sv[2], pv[2], vv[2], b[4], c[4], acc[2], dc[4];
+                    lds22(sm.s.step + r * CW + ct, sv);
+                    lds22(sm.s.su + r * CW + ct, pv);
+                    lds22(sm.v + r * CW + ct, vv);
+                    lds_dup4(sm.s.b(r, j), b);
+                    lds_dup4(sm.s.c(r, j), c);
+                    decays<decltype(mode)::value>(sv, a2, e[r]);
+                    acc[0] = acc[1] = make_float2(0.f, 0.f);
+                    if (r > 0) {
+                        pair_down(h, v16);
+                        store_lanes(sm.past[r - 1], lane, v16);
+                    }
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    dsum[n] = gsum[n] = bcs[n] = 0.f;
-                    bcs[4 + n] = dcs[r][n];
+                    for (int i = 0; i < 4; ++i) {
+                        dc[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            float2& hh = h[2 * i + q];
+                            hh = ffma2(e[r][2 * i + q], hh, fmul2(pv[q], b[i]));
+                            acc[q] = ffma2(c[i], hh, acc[q]);
+                            dc[i] = ffma2(vv[q], hh, dc[i]);
+                        }
+                        dcs[r][i] = dc[i].x + dc[i].y;
+                    }
+                    if (gated) sum_states<NL>(acc, lane, sm.y + r * CW);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int r = kGroup - 1; r >= 0; --r) {
+                    reload();
+                    float2 sv[2], pv[2], vv[2], b[4], c[4], dsum[2], gsum[2], db[4];
+                    float bcs[8];
+                    lds22(sm.s.step + r * CW + ct, sv);
+                    lds22(sm.s.su + r * CW + ct, pv);
+                    lds22(sm.v + r * CW + ct, vv);
+                    lds_dup4(sm.s.b(r, j), b);
+                    lds_dup4(sm.s.c(r, j), c);
+                    dsum[0] = dsum[1] = gsum[0] = gsum[1] = make_float2(0.f, 0.f);
+                    load_lanes(r > 0 ? sm.past[r - 1] : sm.h[gi], lane, v16);
+                    pair_up(v16, h);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int k = 4 * i + n;
-                        g[k] = fmaf(cv[n], vv[i], g[k]);
-                        const float q = g[k] * eh[r][k];
-                        da[k] = fmaf(sv[i], q, da[k]);
-                        dsum[i] = fmaf(a2[k], q, dsum[i]);
-                        gsum[i] = fmaf(bv[n], g[k], gsum[i]);
-                        bcs[n] = fmaf(pv[i], g[k], bcs[n]);
-                        g[k] *= e[r][k];
+                    for (int i = 0; i < 4; ++i) {
+                        db[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int k = 2 * i + q;
+                            g[k] = ffma2(c[i], vv[q], g[k]);
+                            gsum[q] = ffma2(b[i], g[k], gsum[q]);
+                            db[i] = ffma2(pv[q], g[k], db[i]);
+                            g[k] = fmul2(g[k], e[r][k]);
+                            const float2 w = fmul2(g[k], h[k]);
+                            da[k] = ffma2(sv[q], w, da[k]);
+                            dsum[q] = ffma2(a2[k], w, dsum[q]);
+                        }
+                        bcs[i] = db[i].x + db[i].y;
+                        bcs[4 + i] = dcs[r][i];
                     }
-                sum_states<NL>(dsum, lane, sm.ds + r * CW);
-                sum_states<NL>(gsum, lane, sm.gb + r * CW);
-                // db and dc of the thread's four states over the channel lanes
-                reduce_scatter<8, CL, 1>(bcs, lane);
-                if (r < cnt) {
-                    constexpr int kKeep = CL >= 8 ? 1 : 8 / CL;
-                    const int k = lane % CL, first = k * 8 / CL;
-                    if (CL <= 8 || k % (CL / 8 > 0 ? CL / 8 : 1) == 0) {
+                    sum_states<NL>(dsum, lane, sm.ds + r * CW);
+                    sum_states<NL>(gsum, lane, sm.gb + r * CW);
+                    // db and dc of the thread's four states over the channel lanes
+                    reduce_scatter<8, CL, 1>(bcs, lane);
+                    constexpr int kKeep = CL >= 8 ? 1 : 8 / CL, kSame = CL >= 8 ? CL / 8 : 1;
+                    const int k = lane % CL;
+                    if (t + r < te && k % kSame == 0) {
 #pragma unroll
                         for (int i = 0; i < kKeep; ++i) {
-                            const int w = first + i;  // 0-3: db, 4-7: dc
-                            pbc[(t + r) * ps + (w / 4) * N + n0 + w % 4] = bcs[i];
+                            const int w = k * 8 / CL + i;  // 0-3: db, 4-7: dc of the lane's states
+                            pbc[(t + r) * ps + (w / 4) * N + j + NL * (w % 4)] = bcs[i];
                         }
                     }
                 }
-            }
+            };
+            if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
+            else pass(std::integral_constant<int, kChecked>{});
             __syncwarp();
 #pragma unroll
             for (int x = 0; x < TE; ++x) {
-                const int r = own.t0 + x;
-                float yo[CE], dso[CE], gbo[CE], duo[CE], ddo[CE], dzo[CE];
-                if (z) lds_v<CE>(sm.y + r * CW + own.c0, yo);
-                lds_v<CE>(sm.ds + r * CW + own.c0, dso);
-                lds_v<CE>(sm.gb + r * CW + own.c0, gbo);
-                if (r < cnt) {
+                const int r = own_t + x;
+                const int64_t row = t + r;
+                float yo[CE], dso[CE], gbo[CE], ste[CE], duo[CE], ddo[CE], dzo[CE], ue[CE], re[CE], ye[CE], ze[CE];
+                now.r.u[x].get(ue);
+                now.r.d[x].get(re);
+                now.dy[x].get(ye);
+                if (gated) now.r.z[x].get(ze);
+                if (gated) lds_v<CE>(sm.y + r * CW + own_c, yo);
+                lds_v<CE>(sm.ds + r * CW + own_c, dso);
+                lds_v<CE>(sm.gb + r * CW + own_c, gbo);
+                lds_v<CE>(sm.s.step + r * CW + own_c, ste);
+                if (row < te) {
+                    const int64_t off = row * ys;
 #pragma unroll
                     for (int i = 0; i < CE; ++i) {
-                        float v = ye[x][i];
-                        if (z) {
-                            const float sg = sigmoid(ze[x][i]);
-                            dzo[i] = ye[x][i] * fmaf(skip[i], ue[x][i], yo[i]) * (sg * (1.f + ze[x][i] * (1.f - sg)));
-                            v *= ze[x][i] * sg;
+                        float v = ye[i];
+                        if (gated) {
+                            const float sg = sigmoid(ze[i]);
+                            dzo[i] = ye[i] * fmaf(skip[i], ue[i], yo[i]) * (sg * (1.f + ze[i] * (1.f - sg)));
+                            v *= ze[i] * sg;
                         }
-                        const float st = p.softplus ? softplus(re[x][i]) : re[x][i];
-                        duo[i] = fmaf(st, gbo[i], skip[i] * v);
-                        ddo[i] = fmaf(ue[x][i], gbo[i], kLn2 * dso[i]);
-                        if (p.softplus) ddo[i] *= sigmoid(re[x][i]);
-                        dskip[i] = fmaf(v, ue[x][i], dskip[i]);
+                        duo[i] = fmaf(ste[i], gbo[i], skip[i] * v);
+                        ddo[i] = fmaf(ue[i], gbo[i], kLn2 * dso[i]);
+                        if (p.softplus) ddo[i] *= sigmoid(re[i] + chn.bias[i]);
+                        dskip[i] = fmaf(v, ue[i], dskip[i]);
                         dbias[i] += ddo[i];
                     }
-                    store_v<CE>(du + (t + r) * ys, ec, cend, bp.vec, duo);
-                    store_v<CE>(dd + (t + r) * ys, ec, cend, bp.vec, ddo);
-                    if (dz) store_v<CE>(dz + (t + r) * ys, ec, cend, bp.vec, dzo);
+                    store_v<CE>(du + off, ec, cend, bp.vec, duo);
+                    store_v<CE>(dd + off, ec, cend, bp.vec, ddo);
+                    if (dz) store_v<CE>(dz + off, ec, cend, bp.vec, dzo);
                 }
             }
             __syncwarp();
         }
     }
-    if (bp.dinitial) store_block<N>(bp.dinitial + (int64_t)s * p.channels * N, c0, cend, n0, g);
-    store_block<N>(bp.part_a + (int64_t)s * p.channels * N, c0, cend, n0, da);
-    // dD and d delta_bias over the lanes that share channels: those of one channel lane whose
-    // elements differ in the token (lane distances CL * (lanes per token) and up)
-    constexpr int kLanesPerToken = NL <= 4 ? 1 : NL / 4;
+    // the gradient of what enters the chain: the first segment's warp holds it (an empty
+    // sequence's first warp passes the final state's on)
+    const bool begins = !SPLIT || (warp == 0 && rank == 0);
+    if (bp.dinitial && begins) {
+        pair_down(g, v16);
+        store_block<NL>(bp.dinitial + (int64_t)s * p.channels * N, c0, cend, j, v16);
+    }
+    pair_down(da, v16);
+    const int64_t row = (int64_t)s * cluster + rank;
+    float* pa = bp.part_a + (row * tiles + tile) * 512;
+    float* pd = bp.part_d + (row * 2 * tiles + tile) * CW;
+    if constexpr (SPLIT) {
+        __syncthreads();
+        store_lanes(sm.h[0], lane, v16);
+        sum_tokens<NL>(dskip, lane, own_c, sp.dd[0][warp]);
+        sum_tokens<NL>(dbias, lane, own_c, sp.dd[1][warp]);
+        __syncthreads();
+        for (int x = threadIdx.x; x < 512 + 2 * CW; x += 32 * W) {
+            float sum = 0.f;
+            if (x < 512) {
 #pragma unroll
-    for (int o = 16; o >= CL * kLanesPerToken; o >>= 1)
+                for (int w = 0; w < W; ++w) sum += stages[w].h[0][x];
+                pa[x] = sum;
+            } else {
+                const int k = (x - 512) / CW, c = (x - 512) % CW;
 #pragma unroll
-        for (int i = 0; i < CE; ++i) {
-            dskip[i] += __shfl_xor_sync(0xffffffffu, dskip[i], o);
-            dbias[i] += __shfl_xor_sync(0xffffffffu, dbias[i], o);
-        }
-    if (lane < CL * kLanesPerToken) {
-        float* pd = bp.part_d + (int64_t)s * 2 * p.channels;
-#pragma unroll
-        for (int i = 0; i < CE; ++i)
-            if (ec + i < cend) {
-                pd[ec + i] = dskip[i];
-                pd[p.channels + ec + i] = dbias[i];
+                for (int w = 0; w < W; ++w) sum += sp.dd[k][w][c];
+                pd[(int64_t)k * tiles * CW + c] = sum;
             }
+        }
+        if (cluster > 1) cluster_wait();
+    } else {
+        store_lanes(pa, lane, v16);
+        sum_tokens<NL>(dskip, lane, own_c, pd);
+        sum_tokens<NL>(dbias, lane, own_c, pd + (int64_t)tiles * CW);
     }
 }
 
@@ -345,37 +443,83 @@ __global__ void __launch_bounds__(256) sum_bc_kernel(const float* __restrict__ p
     out[(t * groups + gr) * n + w % n] = from_f<T>(sum);
 }
 
-// out[i] = sum over `rows` of part[r][i], in order: 8 outputs by 32 row lanes per CTA.
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ part, int64_t rows, int64_t stride,
-                                                       int64_t count, float* __restrict__ out) {
+// da, dD and d delta_bias: the partials' rows added in order, 8 outputs by 32 row lanes per CTA.
+template <int NL>
+__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ pa, const float* __restrict__ pd, int64_t rows,
+                                                       int tiles, int per_group, int tiles_per_group, float* __restrict__ da,
+                                                       float* __restrict__ dd, float* __restrict__ dbias) {
+    constexpr int CW = Tile<NL>::CW, N = 4 * NL;
     __shared__ float red[32][9];
     const int x = threadIdx.x % 8, r = threadIdx.x / 8;
-    const int64_t i = (int64_t)blockIdx.x * 8 + x;
+    const int64_t i = (int64_t)blockIdx.x * 8 + x, na = (int64_t)tiles * 512, nd = (int64_t)tiles * CW;
+    if ((int64_t)blockIdx.x * 8 >= na + 2 * nd) return;
+    const float* src = i < na ? pa + i : pd + (i - na);
+    const int64_t stride = i < na ? na : 2 * nd;
     float sum = 0.f;
-    if (i < count)
-        for (int64_t k = r; k < rows; k += 32) sum += part[k * stride + i];
+    if (i < na + 2 * nd)
+        for (int64_t k = r; k < rows; k += 32) sum += src[k * stride];
     red[r][x] = sum;
     __syncthreads();
     for (int o = 16; o > 0; o >>= 1) {
         if (r < o) red[r][x] += red[r + o][x];
         __syncthreads();
     }
-    if (r == 0 && i < count) out[i] = red[0][x];
+    if (r != 0 || i >= na + 2 * nd) return;
+    int tile, c, n = 0;
+    if (i < na) {
+        tile = (int)(i / 512);
+        element<NL>((int)(i % 512), c, n);
+    } else {
+        tile = (int)((i - na) % nd / CW);
+        c = (int)((i - na) % CW);
+    }
+    const int at = (tile % tiles_per_group) * CW + c;
+    if (at >= per_group) return;
+    const int ch = tile / tiles_per_group * per_group + at;
+    if (i < na) da[(int64_t)ch * N + n] = red[0][x];
+    else if (i < na + nd) { if (dd) dd[ch] = red[0][x]; }
+    else if (dbias) dbias[ch] = red[0][x];
 }
 
 struct Layout {
     int64_t tokens, bc, a, d, total;  // floats
 };
+// Room for the largest cluster, whichever the launch takes.
 Layout layout_of(const vh_ssm_scan_args* a) {
     Layout l;
     l.tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
     const int cw = 128 / (a->states / 4), per = a->channels / a->groups;
     const int64_t tiles = (int64_t)a->groups * ((per + cw - 1) / cw);
+    const int64_t rows = (int64_t)a->batch * (a->batch * tiles * 2 <= 256 ? 8 : 1);
     l.bc = tiles * l.tokens * 2 * a->states;
-    l.a = (int64_t)a->batch * a->channels * a->states;
-    l.d = (int64_t)a->batch * 2 * a->channels;
+    l.a = rows * tiles * 512;
+    l.d = rows * 2 * tiles * cw;
     l.total = l.bc + l.a + l.d;
     return l;
+}
+
+template <typename T, int NL>
+int launch_bwd(const BwdParams& p, int64_t chains, int* cluster, cudaStream_t st) {
+    // as the forward: one warp a chain only where they fill the schedulers
+    *cluster = 1;
+    const bool split = p.f.seqs.length > kCheckpoint && (chains < 8 * sm_count() || p.f.seqs.offsets);
+    if (!split) {
+        const size_t smem = sizeof(BwdStage<NL>) * kBwdWarps;
+        if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, false>), smem))
+            return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
+        const int64_t blocks = (chains + kBwdWarps - 1) / kBwdWarps;
+        if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
+        scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, chains, 1);
+        return launch_status("selective scan backward");
+    }
+    const size_t smem = sizeof(BwdStage<NL>) * kBwdSplitWarps<NL> + sizeof(BwdSplitSmem<NL, kBwdSplitWarps<NL>>);
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), smem))
+        return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
+    static std::atomic<int> known[64][9];
+    *cluster = pick_cluster(scan_bwd_kernel<T, NL, true>, known, 32 * kBwdSplitWarps<NL>, smem, chains, p.f.seqs.length,
+                            kCheckpoint);
+    return launch_cluster("selective scan backward", scan_bwd_kernel<T, NL, true>, chains * *cluster, 32 * kBwdSplitWarps<NL>,
+                          smem, *cluster, st, p, chains, *cluster);
 }
 
 int check_bwd(const char* what, const vh_ssm_scan_bwd_args* a) {
@@ -404,6 +548,7 @@ using namespace vh;
 using namespace vh::ssm;
 
 extern "C" int64_t vh_ssm_scan_bwd_workspace_bytes(const vh_ssm_scan_bwd_args* a) {
+    clear_error();
     if (check_bwd("vh_ssm_scan_bwd_workspace_bytes", a)) return 0;
     return layout_of(&a->fwd).total * 4;
 }
@@ -430,39 +575,27 @@ extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, i
     p.vec = p.f.vec && aligned(a->grad_y, 4 * es) && aligned(a->grad_u, 4 * es) && aligned(a->grad_delta, 4 * es) &&
             (!p.dz || aligned(p.dz, 4 * es));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t items = (int64_t)f->batch * p.f.groups * p.f.tiles_per_group;
-    const int64_t blocks = (items + kWarps - 1) / kWarps;
-    if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
+    const int64_t chains = (int64_t)f->batch * p.f.groups * p.f.tiles_per_group;
+    const int tiles = p.f.groups * p.f.tiles_per_group;
     return with_dtype(f->dtype, [&](auto t) {
         using T = decltype(t);
         int rc = with_states(f->states, [&](auto nl) {
             constexpr int NL = decltype(nl)::value;
-            const size_t smem = sizeof(BwdSmem<NL>) * kWarps;
-            const void* fn = reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL>);
-            if (!ensure_smem_attr(fn, smem))
-                return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
-            scan_bwd_kernel<T, NL><<<(int)blocks, 32 * kWarps, smem, st>>>(p, items);
-            return launch_status("selective scan backward");
+            int cluster = 1;
+            if (int e = launch_bwd<T, NL>(p, chains, &cluster, st)) return e;
+            const int64_t outs = (int64_t)tiles * (512 + 2 * Tile<NL>::CW);
+            sum_rows_kernel<NL><<<(int)((outs + 7) / 8), 256, 0, st>>>(
+                p.part_a, p.part_d, (int64_t)f->batch * cluster, tiles, p.f.per_group, p.f.tiles_per_group, a->grad_a,
+                a->grad_d_skip, a->grad_delta_bias);
+            return launch_status("selective scan backward: parameters");
         });
         if (rc) return rc;
         const int64_t outs = l.tokens * f->groups * 2 * f->states;
-        if (outs > 0) {
-            const int64_t grid = (outs + 255) / 256;
-            if (grid > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many tokens");
-            sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(p.part_bc, static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c),
-                                                        l.tokens, f->groups, p.f.tiles_per_group, f->states);
-            if ((rc = launch_status("selective scan backward: b, c"))) return rc;
-        }
-        auto rows = [&](const float* part, int64_t stride, int64_t count, float* out) {
-            sum_rows_kernel<<<(int)((count + 7) / 8), 256, 0, st>>>(part, f->batch, stride, count, out);
-            return launch_status("selective scan backward: parameters");
-        };
-        const int64_t dn = (int64_t)f->channels * f->states;
-        if ((rc = rows(p.part_a, dn, dn, a->grad_a))) return rc;
-        if (a->grad_d_skip && (rc = rows(p.part_d, 2 * f->channels, f->channels, a->grad_d_skip))) return rc;
-        if (a->grad_delta_bias &&
-            (rc = rows(p.part_d + f->channels, 2 * f->channels, f->channels, a->grad_delta_bias)))
-            return rc;
-        return 0;
+        if (outs == 0) return 0;
+        const int64_t grid = (outs + 255) / 256;
+        if (grid > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many tokens");
+        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(p.part_bc, static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c),
+                                                    l.tokens, f->groups, p.f.tiles_per_group, f->states);
+        return launch_status("selective scan backward: b, c");
     });
 }

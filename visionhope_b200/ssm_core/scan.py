@@ -75,12 +75,9 @@ class _Call:
         lib, a = _lib.load(), self.args
         ck = None
         if want_checkpoints:
-            slots = int(lib.vh_ssm_scan_checkpoint_slots(ctypes.byref(a)))
-            ck = torch.empty((slots,) + self.state_shape[1:], dtype=torch.float32, device=dev)
+            ck = _args.workspace(lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)), dev)
         a.y, a.final_state, a.checkpoints = y.data_ptr(), _lib.ptr(final), _lib.ptr(ck)
-        nbytes = lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a))
-        ws = _args.workspace(nbytes, dev) if nbytes else None
-        _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), _lib.ptr(ws), nbytes, _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
+        _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
         return y, final, ck
 
     def backward(self, dy, dfinal, ck, want_initial):
