@@ -547,7 +547,8 @@ typedef struct {
 } vh_ssm_scan_args;
 
 int64_t vh_ssm_scan_checkpoint_bytes(const vh_ssm_scan_args* args);
-int vh_ssm_scan_fwd(const vh_ssm_scan_args* args, vh_stream_t stream);
+int64_t vh_ssm_scan_fwd_workspace_bytes(const vh_ssm_scan_args* args);
+int vh_ssm_scan_fwd(const vh_ssm_scan_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
 
 /* Its backward.  args: the forward's, with the checkpoints it wrote (y and final_state are not
  * read).  grad_y: dtype, contiguous [tokens, channels].  Outputs: grad_u, grad_delta, grad_z

@@ -141,7 +141,7 @@ def test_scan_entry_points_refuse(change, code, text):
 
     lib, (p, keep) = _lib.load(), _fake()
     a = _scan_args(_lib, p, **change)
-    assert lib.vh_ssm_scan_fwd(ctypes.byref(a), None) == code
+    assert lib.vh_ssm_scan_fwd(ctypes.byref(a), p, 1 << 40, None) == code
     assert text in _err(lib)
     if "length" not in change:
         assert lib.vh_ssm_scan_step(ctypes.byref(a), p, p, None, 4, None) == code

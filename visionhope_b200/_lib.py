@@ -215,7 +215,9 @@ def load() -> ctypes.CDLL:
             lib.vh_ssm_scan_checkpoint_bytes.restype = c_int64
             lib.vh_ssm_scan_checkpoint_bytes.argtypes = [scan]
             lib.vh_ssm_scan_fwd.restype = c_int32
-            lib.vh_ssm_scan_fwd.argtypes = [scan, c_void_p]
+            lib.vh_ssm_scan_fwd.argtypes = [scan, c_void_p, c_int64, c_void_p]
+            lib.vh_ssm_scan_fwd_workspace_bytes.restype = c_int64
+            lib.vh_ssm_scan_fwd_workspace_bytes.argtypes = [scan]
             lib.vh_ssm_scan_bwd_workspace_bytes.restype = c_int64
             lib.vh_ssm_scan_bwd_workspace_bytes.argtypes = [scan_bwd]
             lib.vh_ssm_scan_bwd.restype = c_int32

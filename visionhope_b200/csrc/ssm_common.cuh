@@ -166,18 +166,23 @@ __device__ __forceinline__ float log1p_term(int i) {
                                        0.07822594046592712f, -0.029505232349038124f, 0.005232692696154118f};
     return kR[i];
 }
-__device__ __forceinline__ float exp_minus_abs(float x) {
-    const float m = -fabsf(x), hi = m * kLog2e, lo = fmaf(m, kLog2e, -hi);
-    const float e = ex2(hi);
-    return fmaf(e, m > -80.f ? lo * kLn2 : 0.f, e);
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ float softplus(float x) {
-    const float e = exp_minus_abs(x);
-    float r = log1p_term(kLog1pTerms - 1);
+__device__ __forceinline__ float2 softplus2(float2 x) {
+    // exp(-104) is 0 here: past it the result is max(x, 0)
+    const float2 m = make_float2(fmaxf(-fabsf(x.x), -104.f), fmaxf(-fabsf(x.y), -104.f));
+    const float2 hi = fmul2(m, splat2(kLog2e)), lo = ffma2(m, splat2(kLog2e), fmul2(hi, splat2(-1.f)));
+    float2 e = make_float2(ex2(hi.x), ex2(hi.y));
+    e = ffma2(e, fmul2(lo, splat2(kLn2)), e);
+    float2 r = splat2(log1p_term(kLog1pTerms - 1));
 #pragma unroll
-    for (int i = kLog1pTerms - 2; i >= 0; --i) r = fmaf(r, e, log1p_term(i));
-    return fmaf(e, r, fmaxf(x, 0.f));
+    for (int i = kLog1pTerms - 2; i >= 0; --i) r = ffma2(r, e, splat2(log1p_term(i)));
+    return ffma2(e, r, make_float2(max_nan(x.x, 0.f), max_nan(x.y, 0.f)));
 }
+__device__ __forceinline__ float softplus(float x) { return softplus2(make_float2(x, x)).x; }
 
 // Two of them, without the range check: |s a| <= 126.  The same bits as exp2_fma.
 __device__ __forceinline__ float2 exp2_fma2(float2 s, float2 a) {
@@ -198,11 +203,7 @@ __device__ __forceinline__ void softplus_n(float (&v)[N]) {
     } else {
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
-            const float2 e = make_float2(exp_minus_abs(v[k]), exp_minus_abs(v[k + 1]));
-            float2 r = splat2(log1p_term(kLog1pTerms - 1));
-#pragma unroll
-            for (int i = kLog1pTerms - 2; i >= 0; --i) r = ffma2(r, e, splat2(log1p_term(i)));
-            r = ffma2(e, r, make_float2(fmaxf(v[k], 0.f), fmaxf(v[k + 1], 0.f)));
+            const float2 r = softplus2(make_float2(v[k], v[k + 1]));
             v[k] = r.x;
             v[k + 1] = r.y;
         }

@@ -5,13 +5,12 @@ namespace vh {
 namespace ssm {
 namespace {
 
-constexpr int kWarps = 4;        // one warp a chain: warps per CTA, neighbouring channel tiles
-constexpr int kSplitWarps = 16;  // many warps a chain: warps per CTA, consecutive segments
+constexpr int kWarps = 4;  // warps per CTA: neighbouring channel tiles
 
-// Four staged tokens; Y: also y's partial sums (pairs of channels, over the thread's states).
+// Four staged tokens; Y: also y's partial sums over the thread's states, left in `part`.
 template <int NL, int MODE, bool Y>
 __device__ __forceinline__ void advance(const Stage<NL>& st, int ct, int j, const float2 (&a2)[8], float2 (&h)[8],
-                                        float (&acc)[16]) {
+                                        float* part) {
     using K = Tile<NL>;
 #pragma unroll
     for (int r = 0; r < kGroup; ++r) {
@@ -31,145 +30,192 @@ __device__ __forceinline__ void advance(const Stage<NL>& st, int ct, int j, cons
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int p = 0; p < 2; ++p) y[p] = ffma2(c[i], h[2 * i + p], y[p]);
-            acc[4 * r] = y[0].x; acc[4 * r + 1] = y[0].y; acc[4 * r + 2] = y[1].x; acc[4 * r + 3] = y[1].y;
+            put_part<NL>(part + 128 * r, j, ct, y);
         }
     }
 }
 
-// The forward scan.  A chain is a channel tile of a sequence.
-// SPLIT = false: one warp walks a chain, four neighbouring chains a CTA.
-// SPLIT = true, for few chains: the sixteen warps of a CTA, and the CTAs of a cluster, take
-// consecutive segments of one chain.  Each warp first runs its segment from a zero state, without
-// outputs.  A segment maps the state before it to exp(a sum s) h + own state, so the states before
-// all segments follow from the sixteen own states and step sums of each CTA (512 threads, one
-// state each) and the totals of the CTAs before it, read from their shared memory.  Then each
-// warp runs its segment again from its true state.  Twice the exponentials, against the length
-// of a chain divided by up to 128.
-template <typename T, int NL, bool SPLIT>
-__global__ void __launch_bounds__(32 * (SPLIT ? kSplitWarps : kWarps), SPLIT ? 1 : 3)
-    scan_fwd_kernel(const ScanParams p, int64_t chains, int cluster) {
+// The forward scan: a warp runs a channel tile of a sequence, or of a segment of one.
+// OWN: the first of the three kernels of a chain in segments, without outputs: the segment's own
+// state and sum of steps.
+template <typename T, int NL, bool OWN>
+__global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanParams p, const Segments g, int64_t items) {
     using K = Tile<NL>;
     constexpr int CE = K::CE, TE = K::TE;
-    constexpr int W = SPLIT ? kSplitWarps : kWarps;
-    extern __shared__ __align__(16) unsigned char smem[];
-    Stage<NL>* stages = reinterpret_cast<Stage<NL>*>(smem);
-    // split only: what leaves and enters the segments
-    float* states = reinterpret_cast<float*>(stages + 2 * W);
-    SplitSmem<NL, W>& sp = *reinterpret_cast<SplitSmem<NL, W>*>(states + 512 * W);
+    __shared__ __align__(16) Stage<NL> stages[kWarps][2];
+    __shared__ __align__(16) float parts[kWarps][OWN ? 4 : 512];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
+    if (OWN) launch_dependents();
+    Unit w;
+    if (item >= items || !unit_at(p, g, item, w)) return;
     const int tiles = p.groups * p.tiles_per_group;
-    const int64_t chain = SPLIT ? blockIdx.x / cluster : (int64_t)blockIdx.x * W + warp;
-    if (!SPLIT && chain >= chains) return;
-    const int s = (int)(chain / tiles), tile = (int)(chain % tiles);
-    const Seq seq = seq_at(p.seqs, s);
-    Chain<T, NL> ch(p, seq, s, tile, lane);
+    Chain<T, NL> ch(p, w.seq, w.s, w.tile, lane);
     const int j = lane / K::CL, ct = 4 * (lane % K::CL), c0 = ch.cbase + ct;  // the thread's 4 x 4 block
     const int ec = ch.ec, cend = ch.cend;
-    Stage<NL>* st = stages + 2 * warp;
+    Stage<NL>* st = stages[warp];
+    float* part = parts[warp];
+    const int64_t unit = w.slot * tiles + w.tile;
+    float2 a2[8], h[8];
+    float v[16], sum[CE];
+    const float top_a = load_rates<NL>(p, c0, cend, j, v);
+    pair_up(v, a2);
+    typename Chain<T, NL>::Raw raw;
+    ch.move(w.t0);
+    // the last segment's own state is not needed
+    const bool some = w.t0 < w.t1 && (!OWN || w.t1 < w.seq.len);
+    if (some) ch.template load<!OWN>(raw, w.t1 - w.t0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < CE; ++i) sum[i] = 0.f;
+
+    if constexpr (OWN) {
+        pair_up(v, h);
+        int buf = 0;
+        for (int64_t t = w.t0; some && t < w.t1; t += kGroup, buf ^= 1) {
+            const float top = ch.template stage<true>(raw, w.t1 - t, st[buf], sum);
+            __syncwarp();
+            ch.move(kGroup);
+            if (t + kGroup < w.t1) ch.template load<false>(raw, w.t1 - t - kGroup);
+            if (top * top_a <= 126.f) advance<NL, kMixed, false>(st[buf], ct, j, a2, h, nullptr);
+            else advance<NL, kChecked, false>(st[buf], ct, j, a2, h, nullptr);
+        }
+        pair_down(h, v);
+        store_lanes(g.state + unit * 512, lane, v);
+        sum_tokens<NL>(sum, lane, ch.own_c, g.sigma + unit * K::CW);
+        return;
+    }
+
     const Rows yr{p.seqs.length * p.channels, p.channels};
-    T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + ec;
     const int64_t ys = row_step(p.seqs, yr);
+    T* y = static_cast<T*>(p.y) + first_row(p.seqs, w.seq, w.s, yr) + ec + (w.t0 + ch.own_t) * ys;
     float skip[CE];
 #pragma unroll
     for (int i = 0; i < CE; ++i) skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
-    const float* initial = p.initial ? p.initial + (int64_t)s * p.channels * K::N : nullptr;
-    float2 a2[8], h[8];
-    float v[16];
-    const float top_a = load_rates<NL>(p, c0, cend, j, v);
-    pair_up(v, a2);
-
-    int64_t t0 = 0, t1 = seq.len;
-    if constexpr (SPLIT) {
-        if (warp == 0) store_lanes(sp.a2, lane, v);
-        const int rank = blockIdx.x % cluster;
-        const int seg = rank * W + warp, segs = cluster * W;
-        const int64_t size = max((seq.len + segs - 1) / segs + kGroup - 1, (int64_t)4 * kGroup) / kGroup * kGroup;
-        t0 = min(seq.len, seg * size);
-        t1 = min(seq.len, t0 + size);
-        float sum[CE];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int i = 0; i < CE; ++i) sum[i] = 0.f;
-        if (t1 < seq.len) {  // what leaves the last segment is not needed
-            Chain<T, NL> at = ch;
-            at.move(t0);
-            typename Chain<T, NL>::Raw raw;
-            at.template load<false>(raw, t1 - t0);
-            int buf = 0;
-            for (int64_t t = t0; t < t1; t += kGroup, buf ^= 1) {
-                const float top = at.template stage<true>(raw, t1 - t, st[buf], sum);
-                __syncwarp();
-                at.move(kGroup);
-                if (t + kGroup < t1) at.template load<false>(raw, t1 - t - kGroup);
-                if (top * top_a <= 126.f) advance<NL, kMixed, false>(st[buf], ct, j, a2, h, v);
-                else advance<NL, kChecked, false>(st[buf], ct, j, a2, h, v);
-            }
-            __syncwarp();
-        }
-        pair_down(h, v);
-        store_lanes(states + 512 * warp, lane, v);
-        sum_tokens<NL>(sum, lane, ch.own_c, sp.sigma[warp]);
-        enter_segments<NL, W, false>(sp, [&](int w) { return states + 512 * w; }, initial, ch.cbase, cend, cluster, rank);
-        load_lanes(states + 512 * warp, lane, v);
-    } else if (initial) {
-        load_block<NL>(initial, c0, cend, j, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    if (g.state) {
+        wait_for_previous();
+        load_lanes(g.state + unit * 512, lane, v);
+    } else if (p.initial) {
+        load_block<NL>(p.initial + (int64_t)w.s * p.channels * K::N, c0, cend, j, v);
     }
     pair_up(v, h);
+    float* ck = p.checkpoints ? p.checkpoints + (slot_base(p.seqs, w.s, w.seq.row, kCheckpoint) * tiles + w.tile) * 512
+                              : nullptr;
+    int buf = 0;
+    for (int64_t t = w.t0; t < w.t1; t += kGroup, buf ^= 1) {
+        if (ck && t % kCheckpoint == 0) {
+            pair_down(h, v);
+            store_lanes(ck + (t / kCheckpoint) * tiles * 512, lane, v);
+        }
+        const float top = ch.template stage<false>(raw, w.t1 - t, st[buf], sum);
+        float ue[TE][CE], ze[TE][CE];
+#pragma unroll
+        for (int e = 0; e < TE; ++e) {
+            raw.u[e].get(ue[e]);
+            if (ch.gated) raw.z[e].get(ze[e]);
+        }
+        __syncwarp();
+        ch.move(kGroup);
+        if (t + kGroup < w.t1) ch.template load<true>(raw, w.t1 - t - kGroup);
+        if (top * top_a <= 126.f) advance<NL, kMixed, true>(st[buf], ct, j, a2, h, part);
+        else advance<NL, kChecked, true>(st[buf], ct, j, a2, h, part);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < TE; ++e) {
+            float out[CE];
+            sum_parts<NL>(part + 128 * (ch.own_t + e), ch.own_c, out);
+#pragma unroll
+            for (int i = 0; i < CE; ++i) {
+                out[i] = fmaf(skip[i], ue[e][i], out[i]);
+                if (ch.gated) out[i] *= ze[e][i] * sigmoid(ze[e][i]);
+            }
+            if (t + ch.own_t + e < w.t1) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
+        }
+        y += kGroup * ys;
+    }
+    if (p.final_state && w.t1 == w.seq.len) {
+        pair_down(h, v);
+        store_block<NL>(p.final_state + (int64_t)w.s * p.channels * K::N, c0, cend, j, v);
+    }
+}
 
-    float* ck = p.checkpoints
-                    ? p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512 : nullptr;
-    if (t0 < t1) {
-        float unused[CE];
+// What enters every segment of a chain: a thread holds four states (one of four channels) and one
+// of RUNS runs of segments.  It composes its run, the CTA chains the runs, and it walks its run
+// again.  A CTA has 128 / PARTS of a chain's 128 such fours.
+template <int NL, int RUNS, int PARTS>
+__global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(const ScanParams p, const Segments g,
+                                                                            const float* __restrict__ first, int right) {
+    constexpr int kWide = 128 / PARTS;
+    __shared__ float4 s_dec[RUNS][kWide], s_add[RUNS][kWide];
+    constexpr int CW = Tile<NL>::CW, N = 4 * NL;
+    launch_dependents();
+    const int tiles = p.groups * p.tiles_per_group;
+    const int64_t chain = blockIdx.x / PARTS;
+    const int tile = (int)(chain % tiles), s = (int)(chain / tiles);
+    const int run = threadIdx.x / kWide, lane = threadIdx.x % kWide;
+    const int x = 4 * ((blockIdx.x % PARTS) * kWide + lane);
+    int c, n;
+    element<NL>(x, c, n);
+    const int ch = tile / p.tiles_per_group * p.per_group + (tile % p.tiles_per_group) * CW + c;
+    const int left = p.per_group - ((tile % p.tiles_per_group) * CW + c);
+    float a2[4], carry[4];
 #pragma unroll
-        for (int i = 0; i < CE; ++i) unused[i] = 0.f;
-        ch.move(t0);
-        y += (t0 + ch.own_t) * ys;
-        typename Chain<T, NL>::Raw raw;
-        ch.template load<true>(raw, t1 - t0);
-        int buf = 0;
-        for (int64_t t = t0; t < t1; t += kGroup, buf ^= 1) {
-            if (ck && t % kCheckpoint == 0) {
-                pair_down(h, v);
-                store_lanes(ck + (t / kCheckpoint) * tiles * 512, lane, v);
+    for (int i = 0; i < 4; ++i) {
+        a2[i] = i < left ? to_log2(p.a[(int64_t)(ch + i) * N + n]) : 0.f;
+        carry[i] = first && i < left ? first[((int64_t)s * p.channels + ch + i) * N + n] : 0.f;
+    }
+    const Seq seq = seq_at(p.seqs, s);
+    const int segs = (int)slots_per_seq(seq.len, g.size), each = (segs + RUNS - 1) / RUNS;
+    const int k0 = min(segs, run * each), k1 = min(segs, k0 + each);
+    const int64_t base = slot_base(p.seqs, s, seq.row, g.size);
+    // segment k of the walk: its states and its sums of steps
+    const int64_t unit0 = (base + (right ? segs - 1 : 0)) * tiles + tile, by = right ? -tiles : tiles;
+    float* state = g.state + unit0 * 512 + x;
+    const float* sigma = g.sigma + unit0 * CW + c;
+    wait_for_previous();
+    if constexpr (RUNS > 1) {
+        float dec[4] = {1.f, 1.f, 1.f, 1.f}, add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int k = k0; k < k1; ++k) {
+            float own[4], sg[4];
+            lds4(state + k * by * 512, own);
+            lds4(sigma + k * by * CW, sg);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float d = exp2_fma(sg[i], a2[i]);
+                add[i] = fmaf(d, add[i], own[i]);
+                dec[i] *= d;
             }
-            const float top = ch.template stage<false>(raw, t1 - t, st[buf], unused);
-            float ue[TE][CE], ze[TE][CE];
-#pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                raw.u[e].get(ue[e]);
-                if (ch.gated) raw.z[e].get(ze[e]);
-            }
-            __syncwarp();
-            ch.move(kGroup);
-            if (t + kGroup < t1) ch.template load<true>(raw, t1 - t - kGroup);
-            float acc[16];
-            if (top * top_a <= 126.f) advance<NL, kMixed, true>(st[buf], ct, j, a2, h, acc);
-            else advance<NL, kChecked, true>(st[buf], ct, j, a2, h, acc);
-            reduce_scatter<16, NL, K::CL>(acc, lane);
-#pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                float out[CE];
-#pragma unroll
-                for (int i = 0; i < CE; ++i) {
-                    out[i] = fmaf(skip[i], ue[e][i], acc[e * CE + i]);
-                    if (ch.gated) out[i] *= ze[e][i] * sigmoid(ze[e][i]);
-                }
-                if (t + ch.own_t + e < t1) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
-            }
-            y += kGroup * ys;
+        }
+        s_dec[run][lane] = make_float4(dec[0], dec[1], dec[2], dec[3]);
+        s_add[run][lane] = make_float4(add[0], add[1], add[2], add[3]);
+        __syncthreads();
+        for (int r = 0; r < run; ++r) {
+            const float4 d = s_dec[r][lane], e = s_add[r][lane];
+            carry[0] = fmaf(d.x, carry[0], e.x);
+            carry[1] = fmaf(d.y, carry[1], e.y);
+            carry[2] = fmaf(d.z, carry[2], e.z);
+            carry[3] = fmaf(d.w, carry[3], e.w);
         }
     }
-    // the last token's warp, or for an empty sequence the first one
-    const bool ends = seq.len > 0 ? t0 < t1 && t1 == seq.len : (!SPLIT || (warp == 0 && blockIdx.x % cluster == 0));
-    if (p.final_state && ends) {
-        pair_down(h, v);
-        store_block<NL>(p.final_state + (int64_t)s * p.channels * K::N, c0, cend, j, v);
+    // four segments' loads at a time: the stores between them would hold the loads back
+    for (int k = k0; k < k1; k += 4) {
+        float own[4][4], sg[4][4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const int64_t at = min(k + m, k1 - 1) * by;
+            lds4(state + at * 512, own[m]);
+            lds4(sigma + at * CW, sg[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            if (k + m < k1)
+                *reinterpret_cast<float4*>(state + (k + m) * by * 512) = make_float4(carry[0], carry[1], carry[2], carry[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) carry[i] = fmaf(exp2_fma(sg[m][i], a2[i]), carry[i], own[m][i]);
+        }
     }
-    if (SPLIT && cluster > 1) cluster_wait();
 }
 
 // One token per stream: a thread owns four states of one channel, N / 4 threads a channel.
@@ -220,28 +266,25 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanParams p, cons
 
 bool stride_ok(int64_t v, int m) { return v % m == 0; }
 
+// Warps that a B200 holds of the forward kernel (four CTAs of four an SM).
+int64_t fwd_warps() { return (int64_t)16 * sm_count(); }
+
+int fwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, fwd_warps() / 4, fwd_warps(), kGroup); }
+
 template <typename T, int NL>
-int launch_fwd(const ScanParams& p, int64_t chains, cudaStream_t st) {
-    // One warp a chain once there are two for each of the SM's four schedulers; fewer chains, and
-    // packed sequences, whose lengths the host does not know, are split.
-    const bool split = p.seqs.length > 4 * kGroup && (chains < 8 * sm_count() || p.seqs.offsets);
-    if (!split) {
-        const size_t smem = sizeof(Stage<NL>) * 2 * kWarps;
-        if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, false>), smem))
-            return fail(VH_E_DEVICE, "vh_ssm_scan_fwd: cannot reserve %zu bytes of shared memory", smem);
-        const int64_t blocks = (chains + kWarps - 1) / kWarps;
-        if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_fwd: too many channel tiles");
-        scan_fwd_kernel<T, NL, false><<<(int)blocks, 32 * kWarps, smem, st>>>(p, chains, 1);
+int launch_fwd(const ScanParams& p, const Segments& g, cudaStream_t st) {
+    const int64_t tiles = (int64_t)p.groups * p.tiles_per_group;
+    const int64_t items = (g.state ? g.slots : (int64_t)p.seqs.count) * tiles;
+    const int64_t blocks = (items + kWarps - 1) / kWarps;
+    if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_fwd: too many channel tiles");
+    if (!g.state) {
+        scan_fwd_kernel<T, NL, false><<<(int)blocks, 32 * kWarps, 0, st>>>(p, g, items);
         return launch_status("selective scan");
     }
-    const size_t smem = (sizeof(Stage<NL>) * 2 + 2048) * kSplitWarps + sizeof(SplitSmem<NL, kSplitWarps>);
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, true>), smem))
-        return fail(VH_E_DEVICE, "vh_ssm_scan_fwd: cannot reserve %zu bytes of shared memory", smem);
-    static std::atomic<int> known[64][9];
-    const int cluster = pick_cluster(scan_fwd_kernel<T, NL, true>, known, 32 * kSplitWarps, smem, chains,
-                                     p.seqs.length, 4 * kGroup);
-    return launch_cluster("selective scan", scan_fwd_kernel<T, NL, true>, chains * cluster, 32 * kSplitWarps, smem, cluster,
-                          st, p, chains, cluster);
+    scan_fwd_kernel<T, NL, true><<<(int)blocks, 32 * kWarps, 0, st>>>(p, g, items);
+    if (int rc = launch_status("selective scan: own states")) return rc;
+    if (int rc = enter_segments(p, 4 * NL, g, p.initial, false, st)) return rc;
+    return launch_after("selective scan", scan_fwd_kernel<T, NL, false>, blocks, 32 * kWarps, 0, st, p, g, items);
 }
 
 }  // namespace
@@ -300,11 +343,61 @@ void fill_scan_params(const vh_ssm_scan_args* a, ScanParams* p) {
     p->vec_bc = w;
 }
 
+int64_t tile_count(const vh_ssm_scan_args* a) {
+    const int cw = 128 / (a->states / 4), per = a->channels / a->groups;
+    return (int64_t)a->groups * ((per + cw - 1) / cw);
+}
+
 // The checkpoints: a warp's states for every slot of 32 tokens and channel tile.
 int64_t checkpoint_floats(const vh_ssm_scan_args* a) {
-    const int cw = 128 / (a->states / 4), per = a->channels / a->groups;
-    const int64_t tiles = (int64_t)a->groups * ((per + cw - 1) / cw);
-    return slot_total(a->seq_offsets != nullptr, a->length, a->batch, kCheckpoint) * tiles * 512;
+    return slot_total(a->seq_offsets != nullptr, a->length, a->batch, kCheckpoint) * tile_count(a) * 512;
+}
+
+int segment_size(const vh_ssm_scan_args* a, int64_t enough, int64_t warps, int step) {
+    const int64_t tiles = tile_count(a), tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
+    // The host does not know the lengths of packed sequences: any of them may hold most tokens, so
+    // they are always cut, and twice as fine, because a sequence's last segment is a short one.
+    if (a->seq_offsets) warps *= 2;
+    else if (a->batch * tiles >= enough) return 0;
+    int64_t size = (tokens * tiles + warps - 1) / warps;
+    size = std::max<int64_t>((size + step - 1) / step * step, kCheckpoint);
+    if (!a->seq_offsets) {
+        // segments of one length: a rounded-up number of them must not exceed the warps again
+        while (a->batch * tiles * ((a->length + size - 1) / size) > warps) size += step;
+        const int64_t segs = (a->length + size - 1) / size;
+        size = std::max<int64_t>((((a->length + segs - 1) / segs) + step - 1) / step * step, kCheckpoint);
+    }
+    return size < a->length ? (int)size : 0;
+}
+
+int64_t segment_bytes(const vh_ssm_scan_args* a, int size) {
+    if (size == 0) return 0;
+    const int64_t units = slot_total(a->seq_offsets != nullptr, a->length, a->batch, size) * tile_count(a);
+    return units * (512 + 128 / (a->states / 4)) * 4;
+}
+
+void place_segments(const vh_ssm_scan_args* a, int size, void* workspace, Segments* g) {
+    *g = Segments{};
+    if (size == 0) return;
+    g->size = size;
+    g->slots = slot_total(a->seq_offsets != nullptr, a->length, a->batch, size);
+    g->state = static_cast<float*>(workspace);
+    g->sigma = g->state + g->slots * tile_count(a) * 512;
+}
+
+int enter_segments(const ScanParams& p, int states, const Segments& g, const float* first, bool right, cudaStream_t st) {
+    // Long chains, of which there are few, are cut into runs; a packed sequence may hold most of the
+    // slots.
+    const int64_t chains = (int64_t)p.seqs.count * p.groups * p.tiles_per_group;
+    const int64_t segs = p.seqs.offsets ? std::min<int64_t>(g.slots, 4 * (g.slots / p.seqs.count + 1)) : g.slots / p.seqs.count;
+    return with_states(states, [&](auto nl) {
+        constexpr int NL = decltype(nl)::value;
+        const char* what = "selective scan: entering states";
+        if (segs <= 8) return launch_after(what, enter_segments_kernel<NL, 1, 1>, chains, 128, 0, st, p, g, first, (int)right);
+        if (segs <= 32 || chains > 2 * sm_count())
+            return launch_after(what, enter_segments_kernel<NL, 4, 1>, chains, 512, 0, st, p, g, first, (int)right);
+        return launch_after(what, enter_segments_kernel<NL, 16, 4>, chains * 4, 512, 0, st, p, g, first, (int)right);
+    });
 }
 
 }  // namespace ssm
@@ -320,16 +413,28 @@ extern "C" int64_t vh_ssm_scan_checkpoint_bytes(const vh_ssm_scan_args* a) {
     return checkpoint_floats(a) * 4;
 }
 
-extern "C" int vh_ssm_scan_fwd(const vh_ssm_scan_args* a, vh_stream_t stream) {
+extern "C" int64_t vh_ssm_scan_fwd_workspace_bytes(const vh_ssm_scan_args* a) {
+    clear_error();
+    if (check_scan_args("vh_ssm_scan_fwd_workspace_bytes", a, false)) return 0;
+    return segment_bytes(a, fwd_segment_size(a));
+}
+
+extern "C" int vh_ssm_scan_fwd(const vh_ssm_scan_args* a, void* workspace, int64_t workspace_bytes, vh_stream_t stream) {
     clear_error();
     if (int rc = check_scan_args("vh_ssm_scan_fwd", a, false)) return rc;
+    const int size = fwd_segment_size(a);
+    const int64_t need = segment_bytes(a, size);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return fail(VH_E_ARG, "vh_ssm_scan_fwd: workspace too small");
+    if (need > 0 && !aligned(workspace, 16))
+        return fail(VH_E_ALIGN, "vh_ssm_scan_fwd: the workspace must be 16-byte aligned");
     ScanParams p;
+    Segments g;
     fill_scan_params(a, &p);
-    const int64_t chains = (int64_t)a->batch * p.groups * p.tiles_per_group;
+    place_segments(a, size, workspace, &g);
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_states(a->states, [&](auto nl) {
-            return launch_fwd<T, decltype(nl)::value>(p, chains, static_cast<cudaStream_t>(stream));
+            return launch_fwd<T, decltype(nl)::value>(p, g, static_cast<cudaStream_t>(stream));
         });
     });
 }

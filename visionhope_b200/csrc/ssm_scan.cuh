@@ -27,7 +27,6 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
 #include "abi_util.h"
@@ -79,16 +78,40 @@ struct LaneElems {
 };
 
 // V elements as they lie in memory, loaded ahead of their use.  `left`: how many of them exist
-// (vec: the pointer is aligned and all do).
+// (vec: the pointer is aligned and all do).  The loads are volatile, so that they are issued where
+// they stand, a group ahead of their use: left to the compiler they moved next to it, and the
+// forward waited for memory in 4 of 10 cycles (64 x 256 tokens of two images: 279 us, now 191).
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
     T e[V];
     __device__ __forceinline__ void load(const T* p, int left, bool vec) {
         if (vec) {
-            *this = *reinterpret_cast<const Pack*>(p);
+            if constexpr (sizeof(Pack) == 16) {
+                uint4 r;
+                asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+                *reinterpret_cast<uint4*>(e) = r;
+            } else if constexpr (sizeof(Pack) == 8) {
+                uint2 r;
+                asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+                *reinterpret_cast<uint2*>(e) = r;
+            } else if constexpr (sizeof(Pack) == 4) {
+                uint32_t r;
+                asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
+                *reinterpret_cast<uint32_t*>(e) = r;
+            } else {
+                *this = *reinterpret_cast<const Pack*>(p);
+            }
         } else {
+            // element by element; missing ones repeat the last
 #pragma unroll
-            for (int i = 0; i < V; ++i) e[i] = i < left ? p[i] : from_f<T>(0.f);
+            for (int i = 0; i < V; ++i) {
+                const T* q = p + max(min(i, left - 1), 0);
+                if constexpr (sizeof(T) == 4) {
+                    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&e[i])) : "l"(q));
+                } else {
+                    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&e[i])) : "l"(q));
+                }
+            }
         }
     }
     __device__ __forceinline__ void get(float (&v)[V]) const {
@@ -105,11 +128,10 @@ __device__ __forceinline__ void lds22(const float* p, float2 (&v)[2]) {
     const float4 q = *reinterpret_cast<const float4*>(p);
     v[0] = make_float2(q.x, q.y); v[1] = make_float2(q.z, q.w);
 }
-// four values that each fill both halves of a pair
+// four values, each for both halves of a pair
 __device__ __forceinline__ void lds_dup4(const float* p, float2 (&v)[4]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = make_float2(a.x, a.y); v[1] = make_float2(a.z, a.w);
-    v[2] = make_float2(b.x, b.y); v[3] = make_float2(b.z, b.w);
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = splat2(a.x); v[1] = splat2(a.y); v[2] = splat2(a.z); v[3] = splat2(a.w);
 }
 template <int CE>
 __device__ __forceinline__ void sts_v(float* p, const float (&v)[CE]) {
@@ -174,45 +196,42 @@ __device__ __forceinline__ void decays(const float2 (&s)[2], const float2 (&a2)[
         }
 }
 
-// ---- thread-block clusters -------------------------------------------------------------------
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// p of this CTA's shared memory, in the CTA of `rank`
-__device__ __forceinline__ float ld_cluster(const float* p, uint32_t rank) {
-    const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(p));
-    uint32_t there;
-    float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
-    return v;
-}
-
-// Shared memory of a group of tokens.  A row of B or C holds every value twice, for the packed
-// arithmetic; its stride keeps the rows' stores in different banks.
+// Shared memory of a group of tokens.  A row of B or C lies as [state lane][4 states]; its stride
+// keeps the rows' stores in different banks.
 template <int NL>
 struct Stage {
     using K = Tile<NL>;
-    static constexpr int kRow = 2 * K::N + 8;
+    static constexpr int kRow = K::N + 4;
     float step[kGroup * K::CW], su[kGroup * K::CW], bc[kGroup * 2 * kRow];
     // the four values of state lane j at token r
-    __device__ __forceinline__ const float* b(int r, int j) const { return bc + 2 * r * kRow + 8 * j; }
-    __device__ __forceinline__ const float* c(int r, int j) const { return bc + (2 * r + 1) * kRow + 8 * j; }
+    __device__ __forceinline__ const float* b(int r, int j) const { return bc + 2 * r * kRow + 4 * j; }
+    __device__ __forceinline__ const float* c(int r, int j) const { return bc + (2 * r + 1) * kRow + 4 * j; }
 };
 
-// Larger of the two, NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-// ... over the warp, of values that are not negative
+// The largest over the warp, of values that are not negative
 __device__ __forceinline__ float warp_max_nan(float v) {
     return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+// Sums over the state lanes through shared memory: every lane leaves its four channels of token r,
+// and the lane that owns an element adds the NL parts.  (Four stores and loads a group against 12
+// shuffles, each with two selections and an addition.)  rows: 512 floats.
+template <int NL>
+__device__ __forceinline__ void put_part(float* rows, int j, int ct, const float2 (&v)[2]) {
+    *reinterpret_cast<float4*>(rows + j * Tile<NL>::CW + ct) = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+}
+// ... of one token: NL rows of CW
+template <int NL>
+__device__ __forceinline__ void sum_parts(const float* rows, int own_c, float (&v)[Tile<NL>::CE]) {
+    using K = Tile<NL>;
+    lds_v<K::CE>(rows + own_c, v);
+#pragma unroll
+    for (int k = 1; k < NL; ++k) {
+        float w[K::CE];
+        lds_v<K::CE>(rows + k * K::CW + own_c, w);
+#pragma unroll
+        for (int i = 0; i < K::CE; ++i) v[i] += w[i];
+    }
 }
 
 // A warp's place in its chain: for each sequence the address of the lane's elements in the group
@@ -334,7 +353,7 @@ struct Chain {
                 r.bc[i].get(v);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    *reinterpret_cast<float2*>(row + 2 * (((n + k) % NL) * 4 + (n + k) / NL)) = splat2(v[k]);
+                    row[((n + k) % NL) * 4 + (n + k) / NL] = v[k];
             }
         }
         return warp_max_nan(top);
@@ -363,16 +382,18 @@ __device__ __forceinline__ float load_rates(const ScanParams& p, int c0, int cen
     return warp_max_nan(top);
 }
 
-// ---- one chain over many warps ------------------------------------------------------------------
-// The W warps of a CTA, and the CTAs of a cluster, take consecutive segments of one chain.  A
-// segment maps the state that enters it to exp(a sum s) h + its own state, so what enters every
-// segment follows from the own states and the step sums.  REV: entering from the right (the
-// gradient's way).
-template <int NL, int W>
-struct SplitSmem {
-    float sigma[W][Tile<NL>::CW];       // a segment's sum of steps per channel
-    float a2[512];
-    float total[512], total_sigma[Tile<NL>::CW];  // of all the CTA's segments
+// ---- a chain in segments ----------------------------------------------------------------------
+// With few chains, consecutive segments of `size` tokens of a chain go to warps of their own.  A
+// segment maps the state that enters it to exp(a sum s) h + its own state (what leaves it when
+// nothing enters), so a first kernel finds every segment's own state and sum of steps, a second one
+// what enters each segment, and a third one runs the segments.  The gradient goes through the
+// same, from the right.  Segment k of sequence s is slot slot_base(s) + k; a slot without tokens
+// maps every state to itself.
+struct Segments {
+    float* state;  // [slot][tile][512]: own states, then what enters, in lane order; null: whole chains
+    float* sigma;  // [slot][tile][CW]: sums of steps
+    int64_t slots;
+    int32_t size;
 };
 
 // The channel of the tile and the state of element x of the lane order.
@@ -383,63 +404,36 @@ __device__ __forceinline__ void element(int x, int& c, int& n) {
     n = l / Tile<NL>::CL + NL * (x / 128);
 }
 
-// state(w): 512 floats of warp w, in: its segment's own state, out: what enters it.
-// first: what enters the chain, [channels][N] of the sequence, or null.  Ends with a barrier of
-// the CTA; with a cluster it leaves one cluster barrier to be waited for before the CTA ends
-// (its totals are read until then).
-template <int NL, int W, bool REV, typename State>
-__device__ __forceinline__ void enter_segments(SplitSmem<NL, W>& sp, State&& state, const float* first, int cbase, int cend, int cluster,
-                                               int rank) {
-    constexpr int PER = 512 / (32 * W);
-    constexpr int N = 4 * NL;
-    __syncthreads();
-    float dec[PER][W], add[PER][W], carry[PER];
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int x = threadIdx.x + 32 * W * k;
-        int c, n;
-        element<NL>(x, c, n);
-        float run = 0.f, sig = 0.f;
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            const int w = REV ? W - 1 - i : i;
-            const float sw = sp.sigma[w][c];
-            dec[k][i] = exp2_fma(sw, sp.a2[x]);
-            add[k][i] = state(w)[x];
-            run = fmaf(dec[k][i], run, add[k][i]);
-            sig += sw;
-        }
-        carry[k] = first && cbase + c < cend ? first[(int64_t)(cbase + c) * N + n] : 0.f;
-        if (cluster > 1) {
-            sp.total[x] = run;
-            if (n == 0) sp.total_sigma[c] = sig;
-        }
+// What a warp works on: tokens t0 .. t1 - 1 of a chain.
+struct Unit {
+    Seq seq;
+    int64_t slot, t0, t1;
+    int s, tile;
+};
+// Unit `item` of slots (or sequences) x tiles; false when its slot belongs to no sequence.
+__device__ __forceinline__ bool unit_at(const ScanParams& p, const Segments& g, int64_t item, Unit& u) {
+    const int tiles = p.groups * p.tiles_per_group;
+    u.slot = item / tiles;
+    u.tile = (int)(item % tiles);
+    if (!g.state) {
+        u.s = (int)u.slot;
+        u.seq = seq_at(p.seqs, u.s);
+        u.t0 = 0;
+        u.t1 = u.seq.len;
+        return true;
     }
-    if (cluster > 1) {
-        cluster_arrive();
-        cluster_wait();
-#pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int x = threadIdx.x + 32 * W * k;
-            int c, n;
-            element<NL>(x, c, n);
-            const int steps = REV ? cluster - 1 - rank : rank;
-            for (int i = 0; i < steps; ++i) {
-                const int r = REV ? cluster - 1 - i : i;
-                carry[k] = fmaf(exp2_fma(ld_cluster(&sp.total_sigma[c], r), sp.a2[x]), carry[k], ld_cluster(&sp.total[x], r));
-            }
-        }
-        cluster_arrive();
-    }
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            state(REV ? W - 1 - i : i)[threadIdx.x + 32 * W * k] = carry[k];
-            carry[k] = fmaf(dec[k][i], carry[k], add[k][i]);
-        }
-    __syncthreads();
+    u.s = seq_of_slot(p.seqs, u.slot, g.size);
+    u.seq = seq_at(p.seqs, u.s);
+    const int64_t k = u.slot - slot_base(p.seqs, u.s, u.seq.row, g.size);
+    u.t0 = min(u.seq.len, k * g.size);
+    u.t1 = min(u.seq.len, u.t0 + g.size);
+    return k == 0 || (k > 0 && u.t0 < u.t1);
 }
+
+// Programmatic dependent launch: the next kernel of the stream may start now / wait here for the
+// previous one's results.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Sums v (per element channel) over the lanes that hold the same channels at other tokens, and
 // leaves the tile's row of them at out.
@@ -460,50 +454,26 @@ __device__ __forceinline__ void sum_tokens(float (&v)[Tile<NL>::CE], int lane, i
 int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token);
 void fill_scan_params(const vh_ssm_scan_args* a, ScanParams* p);
 int64_t checkpoint_floats(const vh_ssm_scan_args* a);
+int64_t tile_count(const vh_ssm_scan_args* a);
 
-// The largest cluster of split-kernel CTAs with which all `chains` run at once while a segment
-// keeps `least` tokens (1: no cluster).  The occupancy of each cluster size is asked once per
-// device and kept in known[device][size] (+ 1).
-template <typename Kernel>
-int pick_cluster(Kernel kernel, std::atomic<int> (&known)[64][9], int threads, size_t smem, int64_t chains,
-                 int64_t length, int least) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
-    int best = 1;
-    for (int size = 2; size <= 8; ++size) {
-        if (chains * size > sm_count() || (int64_t)least * (threads / 32) * size > length) break;
-        int n = known[dev][size].load(std::memory_order_relaxed);
-        if (n == 0) {
-            cudaLaunchAttribute at[1];
-            at[0].id = cudaLaunchAttributeClusterDimension;
-            at[0].val.clusterDim = {(unsigned)size, 1, 1};
-            cudaLaunchConfig_t cfg{};
-            cfg.gridDim = dim3(size);
-            cfg.blockDim = dim3(threads);
-            cfg.dynamicSmemBytes = smem;
-            cfg.attrs = at;
-            cfg.numAttrs = 1;
-            int got = 0;
-            if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) {
-                cudaGetLastError();
-                got = 0;
-            }
-            n = got + 1;
-            known[dev][size].store(n, std::memory_order_relaxed);
-        }
-        if (n - 1 >= chains) best = size;
-    }
-    return best;
-}
+// The segment size that gives `warps` warps a segment each (0: whole chains, when there are
+// `enough` of them or they are short): a multiple of `step` tokens.
+int segment_size(const vh_ssm_scan_args* a, int64_t enough, int64_t warps, int step);
+// Bytes of the segments' states and sums (0 without segments), and their places in a workspace.
+int64_t segment_bytes(const vh_ssm_scan_args* a, int size);
+void place_segments(const vh_ssm_scan_args* a, int size, void* workspace, Segments* g);
+// What enters every segment, from their own states.  first: what enters each chain, [sequence]
+// [channels][N], or null.  right: segments follow each other from the last to the first.
+int enter_segments(const ScanParams& p, int states, const Segments& g, const float* first, bool right, cudaStream_t st);
 
-// Launches `kernel` with clusters of `cluster` CTAs.
+// Launches `kernel` behind the previous kernel of the stream, which it may overlap up to its
+// wait_for_previous().
 template <typename... P, typename... A>
-int launch_cluster(const char* what, void (*kernel)(P...), int64_t blocks, int threads, size_t smem, int cluster,
-                   cudaStream_t st, A... args) {
+int launch_after(const char* what, void (*kernel)(P...), int64_t blocks, int threads, size_t smem, cudaStream_t st, A... args) {
     if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "%s: too many channel tiles", what);
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(threads);

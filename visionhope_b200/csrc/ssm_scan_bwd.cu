@@ -25,10 +25,7 @@ namespace ssm {
 namespace {
 
 constexpr int kGroups = kCheckpoint / kGroup;  // groups in a chunk
-constexpr int kBwdWarps = 4;                   // one warp a chain: warps per CTA
-// many warps a chain: as many as the shared memory of a CTA holds
-template <int NL>
-constexpr int kBwdSplitWarps = NL >= 4 ? 8 : 4;
+constexpr int kBwdWarps = 4;                   // warps per CTA: neighbouring channel tiles
 
 struct BwdParams {
     ScanParams f;
@@ -36,62 +33,85 @@ struct BwdParams {
     const float* dfinal;
     void *du, *ddelta, *dz;
     float* dinitial;
-    float* part_bc;  // [tiles][tokens][2][N]
-    float* part_a;   // [rows][tiles][512] in lane order; a row per sequence and CTA of its cluster
+    float* part_bc;  // [tiles][tokens][db, dc][state lane][4 states]
+    float* part_a;   // [rows][tiles][512] in lane order; a row per sequence or segment
     float* part_d;   // [rows][2][tiles][CW]: dD, d delta_bias
     int64_t tokens;
     int32_t vec;     // as f.vec, for dy and the outputs too
 };
 
+// Shared memory of a warp.  A token's sums over lanes (ds, sum b g, db and dc) take the place of
+// the state before it, once that is read.
 template <int NL>
 struct BwdStage {
     using K = Tile<NL>;
     float h[kGroups][512];        // the states before the groups of a chunk
     float past[kGroup - 1][512];  // before the second to fourth token of the group at hand
     Stage<NL> s;
-    float v[kGroup * K::CW], y[kGroup * K::CW], ds[kGroup * K::CW], gb[kGroup * K::CW];
-};
-template <int NL, int W>
-struct BwdSplitSmem {
-    SplitSmem<NL, W> s;
-    float dd[2][W][Tile<NL>::CW];
+    float v[kGroup * K::CW], y[512];
 };
 
 // Values in shared memory are read again after this, instead of being kept in registers.
 __device__ __forceinline__ void reload() { asm volatile("" ::: "memory"); }
 
-// Sums four values (channels of one token) over the state lanes into row[channel of the tile].
+// db and dc of one token over the channel lanes: every lane leaves its four states of both, and
+// output w = [db, dc][state lane][4 states] adds the CL parts.  A row is turned by its lane, so
+// that neither side meets bank conflicts.  part: 256 floats.
 template <int NL>
-__device__ __forceinline__ void sum_states(const float2 (&p)[2], int lane, float* row) {
-    using K = Tile<NL>;
-    float v[4] = {p[0].x, p[0].y, p[1].x, p[1].y};
-    reduce_scatter<4, NL, K::CL>(v, lane);
-    constexpr int kKeep = NL >= 4 ? 1 : 4 / NL, kSame = NL >= 4 ? NL / 4 : 1;
-    const int j = lane / K::CL, k = lane % K::CL;
-    if (j % kSame == 0) {
+__device__ __forceinline__ void put_bc(float* part, int j, int k, const float (&db)[4], const float (&dc)[4]) {
+    constexpr int R = 8 * NL;
+    float* row = part + k * R;
+    const int turn = 4 * k % R;
+    *reinterpret_cast<float4*>(row + ((4 * j) ^ turn)) = make_float4(db[0], db[1], db[2], db[3]);
+    *reinterpret_cast<float4*>(row + ((R / 2 + 4 * j) ^ turn)) = make_float4(dc[0], dc[1], dc[2], dc[3]);
+}
+// ... summed and stored in that order
+template <int NL>
+__device__ __forceinline__ void sum_bc(const float* part, int lane, bool live, float* out) {
+    constexpr int R = 8 * NL, CL = Tile<NL>::CL;
+    constexpr int kSplit = R < 32 ? 32 / R : 1;  // lanes an output: each takes some of the parts
 #pragma unroll
-        for (int i = 0; i < kKeep; ++i) row[4 * k + j * 4 / NL + i] = v[i];
+    for (int m = 0; m < (R + 31) / 32; ++m) {
+        const int w = R < 32 ? lane % R : lane + 32 * m, k0 = R < 32 ? lane / R * (CL / kSplit) : 0;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < CL / kSplit; ++i) {
+            const int k = k0 + i;
+            sum += part[k * R + (w ^ (4 * k % R))];
+        }
+#pragma unroll
+        for (int o = 16; o >= R; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (live && (R >= 32 || lane < R)) out[w] = sum;
     }
 }
 
-template <typename T, int NL, bool SPLIT>
-__global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps), SPLIT ? 1 : 2)
-    scan_bwd_kernel(const BwdParams bp, int64_t chains, int cluster) {
+// OWN: the first of the three kernels of a chain in segments: the segment's own gradient, that of
+// the state before it when nothing enters from the right, and its sum of steps.
+template <typename T, int NL, bool OWN>
+__global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
     using K = Tile<NL>;
     constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL;
-    constexpr int W = SPLIT ? kBwdSplitWarps<NL> : kBwdWarps;
     extern __shared__ __align__(16) unsigned char smem[];
-    BwdStage<NL>* stages = reinterpret_cast<BwdStage<NL>*>(smem);
-    BwdSplitSmem<NL, W>& sp = *reinterpret_cast<BwdSplitSmem<NL, W>*>(stages + W);
     const ScanParams& p = bp.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    BwdStage<NL>& sm = reinterpret_cast<BwdStage<NL>*>(smem)[warp];
+    const int64_t item = (int64_t)blockIdx.x * kBwdWarps + warp;
+    if (OWN) launch_dependents();
+    Unit w;
+    if (item >= items) return;
     const int tiles = p.groups * p.tiles_per_group;
-    const int64_t chain = SPLIT ? blockIdx.x / cluster : (int64_t)blockIdx.x * W + warp;
-    if (!SPLIT && chain >= chains) return;
-    BwdStage<NL>& sm = stages[warp];
-    const int s = (int)(chain / tiles), tile = (int)(chain % tiles);
-    const int rank = SPLIT ? blockIdx.x % cluster : 0;
-    const Seq seq = seq_at(p.seqs, s);
+    const int64_t unit = item;
+    if (!unit_at(p, seg, item, w)) {  // a row of zeros
+        if (!OWN) {
+            for (int x = lane; x < 512; x += 32) bp.part_a[unit * 512 + x] = 0.f;
+            for (int x = lane; x < CW; x += 32)
+                bp.part_d[(w.slot * 2 * tiles + w.tile) * CW + x] = bp.part_d[((w.slot * 2 + 1) * tiles + w.tile) * CW + x] = 0.f;
+        }
+        return;
+    }
+    const Seq seq = w.seq;
+    const int s = w.s, tile = w.tile;
+    const int64_t t0 = w.t0, t1 = w.t1;
     Chain<T, NL> chn(p, seq, s, tile, lane);
     const int j = lane / CL, ct = 4 * (lane % CL), c0 = chn.cbase + ct;
     const int ec = chn.ec, cend = chn.cend, own_t = chn.own_t, own_c = chn.own_c;
@@ -145,22 +165,15 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
         return top;
     };
 
-    int64_t t0 = 0, t1 = seq.len;
-    if constexpr (SPLIT) {
-        if (warp == 0) store_lanes(sp.s.a2, lane, v16);
-        const int seg = rank * W + warp, segs = cluster * W;
-        const int64_t size = ((seq.len + segs - 1) / segs + kCheckpoint - 1) / kCheckpoint * kCheckpoint;
-        t0 = min(seq.len, seg * size);
-        t1 = min(seq.len, t0 + size);
-        // The own gradient of a segment, that of the state before it when nothing enters from the
-        // right: sum_t (e_{t0} ... e_t) c_t v_t, in one pass forward.
+    if constexpr (OWN) {
+        // sum_t (e_{t0} ... e_t) c_t v_t, in one pass forward
         float2 prod[8], own[8];
         float sum[CE];
 #pragma unroll
         for (int i = 0; i < 8; ++i) { prod[i] = make_float2(1.f, 1.f); own[i] = make_float2(0.f, 0.f); }
 #pragma unroll
         for (int i = 0; i < CE; ++i) sum[i] = 0.f;
-        if (t0 > 0 && t0 < t1) {  // what leaves the first segment comes from its second pass
+        if (t0 > 0 && t0 < t1) {  // the first segment's own gradient is not needed
             move(t0);
             Raw raw;
             load(raw, t1 - t0);
@@ -192,10 +205,13 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
             }
         }
         pair_down(own, v16);
-        store_lanes(sm.h[0], lane, v16);
-        sum_tokens<NL>(sum, lane, own_c, sp.s.sigma[warp]);
-        enter_segments<NL, W, true>(sp.s, [&](int w) { return stages[w].h[0]; }, dfinal, chn.cbase, cend, cluster, rank);
-        load_lanes(sm.h[0], lane, v16);
+        store_lanes(seg.state + unit * 512, lane, v16);
+        sum_tokens<NL>(sum, lane, own_c, seg.sigma + unit * CW);
+        return;
+    }
+    if (seg.state) {
+        wait_for_previous();
+        load_lanes(seg.state + unit * 512, lane, v16);
     } else if (dfinal) {
         load_block<NL>(dfinal, c0, cend, j, v16);
     } else {
@@ -302,13 +318,13 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
                         }
                         dcs[r][i] = dc[i].x + dc[i].y;
                     }
-                    if (gated) sum_states<NL>(acc, lane, sm.y + r * CW);
+                    if (gated) put_part<NL>(sm.y + 128 * r, j, ct, acc);
                 }
 #pragma unroll
                 for (int r = kGroup - 1; r >= 0; --r) {
                     reload();
                     float2 sv[2], pv[2], vv[2], b[4], c[4], dsum[2], gsum[2], db[4];
-                    float bcs[8];
+                    float dbs[4];
                     lds22(sm.s.step + r * CW + ct, sv);
                     lds22(sm.s.su + r * CW + ct, pv);
                     lds22(sm.v + r * CW + ct, vv);
@@ -331,22 +347,15 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
                             da[k] = ffma2(sv[q], w, da[k]);
                             dsum[q] = ffma2(a2[k], w, dsum[q]);
                         }
-                        bcs[i] = db[i].x + db[i].y;
-                        bcs[4 + i] = dcs[r][i];
+                        dbs[i] = db[i].x + db[i].y;
                     }
-                    sum_states<NL>(dsum, lane, sm.ds + r * CW);
-                    sum_states<NL>(gsum, lane, sm.gb + r * CW);
-                    // db and dc of the thread's four states over the channel lanes
-                    reduce_scatter<8, CL, 1>(bcs, lane);
-                    constexpr int kKeep = CL >= 8 ? 1 : 8 / CL, kSame = CL >= 8 ? CL / 8 : 1;
-                    const int k = lane % CL;
-                    if (t + r < te && k % kSame == 0) {
-#pragma unroll
-                        for (int i = 0; i < kKeep; ++i) {
-                            const int w = k * 8 / CL + i;  // 0-3: db, 4-7: dc of the lane's states
-                            pbc[(t + r) * ps + (w / 4) * N + j + NL * (w % 4)] = bcs[i];
-                        }
-                    }
+                    __syncwarp();  // every lane has read the state that the sums replace
+                    float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
+                    put_part<NL>(sums, j, ct, dsum);
+                    put_part<NL>(sums + 128, j, ct, gsum);
+                    put_bc<NL>(sums + 256, j, lane % CL, dbs, dcs[r]);
+                    __syncwarp();
+                    sum_bc<NL>(sums + 256, lane, t + r < te, pbc + (t + r) * ps);
                 }
             };
             if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
@@ -361,9 +370,10 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
                 now.r.d[x].get(re);
                 now.dy[x].get(ye);
                 if (gated) now.r.z[x].get(ze);
-                if (gated) lds_v<CE>(sm.y + r * CW + own_c, yo);
-                lds_v<CE>(sm.ds + r * CW + own_c, dso);
-                lds_v<CE>(sm.gb + r * CW + own_c, gbo);
+                const float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
+                if (gated) sum_parts<NL>(sm.y + 128 * r, own_c, yo);
+                sum_parts<NL>(sums, own_c, dso);
+                sum_parts<NL>(sums + 128, own_c, gbo);
                 lds_v<CE>(sm.s.step + r * CW + own_c, ste);
                 if (row < te) {
                     const int64_t off = row * ys;
@@ -389,58 +399,38 @@ __global__ void __launch_bounds__(32 * (SPLIT ? kBwdSplitWarps<NL> : kBwdWarps),
             __syncwarp();
         }
     }
-    // the gradient of what enters the chain: the first segment's warp holds it (an empty
-    // sequence's first warp passes the final state's on)
-    const bool begins = !SPLIT || (warp == 0 && rank == 0);
-    if (bp.dinitial && begins) {
+    if (bp.dinitial && t0 == 0) {
         pair_down(g, v16);
         store_block<NL>(bp.dinitial + (int64_t)s * p.channels * N, c0, cend, j, v16);
     }
     pair_down(da, v16);
-    const int64_t row = (int64_t)s * cluster + rank;
-    float* pa = bp.part_a + (row * tiles + tile) * 512;
-    float* pd = bp.part_d + (row * 2 * tiles + tile) * CW;
-    if constexpr (SPLIT) {
-        __syncthreads();
-        store_lanes(sm.h[0], lane, v16);
-        sum_tokens<NL>(dskip, lane, own_c, sp.dd[0][warp]);
-        sum_tokens<NL>(dbias, lane, own_c, sp.dd[1][warp]);
-        __syncthreads();
-        for (int x = threadIdx.x; x < 512 + 2 * CW; x += 32 * W) {
-            float sum = 0.f;
-            if (x < 512) {
-#pragma unroll
-                for (int w = 0; w < W; ++w) sum += stages[w].h[0][x];
-                pa[x] = sum;
-            } else {
-                const int k = (x - 512) / CW, c = (x - 512) % CW;
-#pragma unroll
-                for (int w = 0; w < W; ++w) sum += sp.dd[k][w][c];
-                pd[(int64_t)k * tiles * CW + c] = sum;
-            }
-        }
-        if (cluster > 1) cluster_wait();
-    } else {
-        store_lanes(pa, lane, v16);
-        sum_tokens<NL>(dskip, lane, own_c, pd);
-        sum_tokens<NL>(dbias, lane, own_c, pd + (int64_t)tiles * CW);
-    }
+    store_lanes(bp.part_a + unit * 512, lane, v16);
+    sum_tokens<NL>(dskip, lane, own_c, bp.part_d + (w.slot * 2 * tiles + tile) * CW);
+    sum_tokens<NL>(dbias, lane, own_c, bp.part_d + ((w.slot * 2 + 1) * tiles + tile) * CW);
 }
 
-// db and dc: the channel tiles' partials of each group added in order.
+// db and dc: the channel tiles' partials of each group added in order.  A thread adds four states
+// of one state lane j (j, j + N / 4, ...).
 template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const float* __restrict__ part, T* __restrict__ db, T* __restrict__ dc,
+__global__ void __launch_bounds__(256) sum_bc_kernel(const float4* __restrict__ part, T* __restrict__ db, T* __restrict__ dc,
                                                      int64_t tokens, int groups, int tiles, int n) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [token][group][2][N]
-    if (i >= tokens * groups * 2 * n) return;
-    const int w = (int)(i % (2 * n));
-    const int64_t tg = i / (2 * n);
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [token][group][db, dc][state lane]
+    const int per = n / 2;
+    if (i >= tokens * groups * per) return;
+    const int w = (int)(i % per), nl = n / 4;
+    const int64_t tg = i / per;
     const int64_t t = tg / groups;
     const int gr = (int)(tg % groups);
-    float sum = 0.f;
-    for (int k = 0; k < tiles; ++k) sum += part[((int64_t)(gr * tiles + k) * tokens + t) * 2 * n + w];
-    T* out = w < n ? db : dc;
-    out[(t * groups + gr) * n + w % n] = from_f<T>(sum);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < tiles; ++k) {
+        const float4 v = part[((int64_t)(gr * tiles + k) * tokens + t) * per + w];
+        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    T* out = (w < nl ? db : dc) + (t * groups + gr) * n + w % nl;
+    out[0] = from_f<T>(sum.x);
+    out[nl] = from_f<T>(sum.y);
+    out[2 * nl] = from_f<T>(sum.z);
+    out[3 * nl] = from_f<T>(sum.w);
 }
 
 // da, dD and d delta_bias: the partials' rows added in order, 8 outputs by 32 row lanes per CTA.
@@ -482,44 +472,43 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
 }
 
 struct Layout {
-    int64_t tokens, bc, a, d, total;  // floats
+    int64_t tokens, rows, bc, a, d, total;  // floats
 };
-// Room for the largest cluster, whichever the launch takes.
-Layout layout_of(const vh_ssm_scan_args* a) {
+// Warps that a B200 holds of the backward kernel (two CTAs of four an SM).
+int64_t bwd_warps() { return (int64_t)8 * sm_count(); }
+
+int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps() / 2, bwd_warps(), kCheckpoint); }
+
+Layout layout_of(const vh_ssm_scan_args* a, int size) {
     Layout l;
-    l.tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
-    const int cw = 128 / (a->states / 4), per = a->channels / a->groups;
-    const int64_t tiles = (int64_t)a->groups * ((per + cw - 1) / cw);
-    const int64_t rows = (int64_t)a->batch * (a->batch * tiles * 2 <= 256 ? 8 : 1);
+    const bool packed = a->seq_offsets != nullptr;
+    l.tokens = packed ? a->length : (int64_t)a->batch * a->length;
+    const int64_t tiles = tile_count(a);
+    l.rows = size ? slot_total(packed, a->length, a->batch, size) : a->batch;
     l.bc = tiles * l.tokens * 2 * a->states;
-    l.a = rows * tiles * 512;
-    l.d = rows * 2 * tiles * cw;
-    l.total = l.bc + l.a + l.d;
+    l.a = l.rows * tiles * 512;
+    l.d = l.rows * 2 * tiles * (128 / (a->states / 4));
+    l.total = l.bc + l.a + l.d + segment_bytes(a, size) / 4;
     return l;
 }
 
 template <typename T, int NL>
-int launch_bwd(const BwdParams& p, int64_t chains, int* cluster, cudaStream_t st) {
-    // as the forward: one warp a chain only where they fill the schedulers
-    *cluster = 1;
-    const bool split = p.f.seqs.length > kCheckpoint && (chains < 8 * sm_count() || p.f.seqs.offsets);
-    if (!split) {
-        const size_t smem = sizeof(BwdStage<NL>) * kBwdWarps;
-        if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, false>), smem))
-            return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
-        const int64_t blocks = (chains + kBwdWarps - 1) / kBwdWarps;
-        if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
-        scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, chains, 1);
+int launch_bwd(const BwdParams& p, const Segments& g, cudaStream_t st) {
+    const size_t smem = sizeof(BwdStage<NL>) * kBwdWarps;
+    const int64_t items = (g.state ? g.slots : (int64_t)p.f.seqs.count) * p.f.groups * p.f.tiles_per_group;
+    const int64_t blocks = (items + kBwdWarps - 1) / kBwdWarps;
+    if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, false>), smem) ||
+        !ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), smem))
+        return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
+    if (!g.state) {
+        scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, g, items);
         return launch_status("selective scan backward");
     }
-    const size_t smem = sizeof(BwdStage<NL>) * kBwdSplitWarps<NL> + sizeof(BwdSplitSmem<NL, kBwdSplitWarps<NL>>);
-    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), smem))
-        return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
-    static std::atomic<int> known[64][9];
-    *cluster = pick_cluster(scan_bwd_kernel<T, NL, true>, known, 32 * kBwdSplitWarps<NL>, smem, chains, p.f.seqs.length,
-                            kCheckpoint);
-    return launch_cluster("selective scan backward", scan_bwd_kernel<T, NL, true>, chains * *cluster, 32 * kBwdSplitWarps<NL>,
-                          smem, *cluster, st, p, chains, *cluster);
+    scan_bwd_kernel<T, NL, true><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, g, items);
+    if (int rc = launch_status("selective scan backward: own gradients")) return rc;
+    if (int rc = enter_segments(p.f, 4 * NL, g, p.dfinal, true, st)) return rc;
+    return launch_after("selective scan backward", scan_bwd_kernel<T, NL, false>, blocks, 32 * kBwdWarps, smem, st, p, g, items);
 }
 
 int check_bwd(const char* what, const vh_ssm_scan_bwd_args* a) {
@@ -550,7 +539,7 @@ using namespace vh::ssm;
 extern "C" int64_t vh_ssm_scan_bwd_workspace_bytes(const vh_ssm_scan_bwd_args* a) {
     clear_error();
     if (check_bwd("vh_ssm_scan_bwd_workspace_bytes", a)) return 0;
-    return layout_of(&a->fwd).total * 4;
+    return layout_of(&a->fwd, bwd_segment_size(&a->fwd)).total * 4;
 }
 
 extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, int64_t workspace_bytes,
@@ -558,7 +547,8 @@ extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, i
     clear_error();
     if (int rc = check_bwd("vh_ssm_scan_bwd", a)) return rc;
     const vh_ssm_scan_args* f = &a->fwd;
-    const Layout l = layout_of(f);
+    const int size = bwd_segment_size(f);
+    const Layout l = layout_of(f, size);
     if (!workspace || workspace_bytes < l.total * 4) return fail(VH_E_ARG, "vh_ssm_scan_bwd: workspace too small");
     if (!aligned(workspace, 16)) return fail(VH_E_ALIGN, "vh_ssm_scan_bwd: the workspace must be 16-byte aligned");
     BwdParams p{};
@@ -571,30 +561,30 @@ extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, i
     p.part_a = static_cast<float*>(workspace);
     p.part_bc = p.part_a + l.a;
     p.part_d = p.part_bc + l.bc;
+    Segments g;
+    place_segments(f, size, static_cast<float*>(workspace) + l.a + l.bc + l.d, &g);
     p.tokens = l.tokens;
     p.vec = p.f.vec && aligned(a->grad_y, 4 * es) && aligned(a->grad_u, 4 * es) && aligned(a->grad_delta, 4 * es) &&
             (!p.dz || aligned(p.dz, 4 * es));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t chains = (int64_t)f->batch * p.f.groups * p.f.tiles_per_group;
     const int tiles = p.f.groups * p.f.tiles_per_group;
     return with_dtype(f->dtype, [&](auto t) {
         using T = decltype(t);
         int rc = with_states(f->states, [&](auto nl) {
             constexpr int NL = decltype(nl)::value;
-            int cluster = 1;
-            if (int e = launch_bwd<T, NL>(p, chains, &cluster, st)) return e;
+            if (int e = launch_bwd<T, NL>(p, g, st)) return e;
             const int64_t outs = (int64_t)tiles * (512 + 2 * Tile<NL>::CW);
             sum_rows_kernel<NL><<<(int)((outs + 7) / 8), 256, 0, st>>>(
-                p.part_a, p.part_d, (int64_t)f->batch * cluster, tiles, p.f.per_group, p.f.tiles_per_group, a->grad_a,
+                p.part_a, p.part_d, l.rows, tiles, p.f.per_group, p.f.tiles_per_group, a->grad_a,
                 a->grad_d_skip, a->grad_delta_bias);
             return launch_status("selective scan backward: parameters");
         });
         if (rc) return rc;
-        const int64_t outs = l.tokens * f->groups * 2 * f->states;
+        const int64_t outs = l.tokens * f->groups * f->states / 2;
         if (outs == 0) return 0;
         const int64_t grid = (outs + 255) / 256;
         if (grid > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many tokens");
-        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(p.part_bc, static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c),
+        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(reinterpret_cast<const float4*>(p.part_bc), static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c),
                                                     l.tokens, f->groups, p.f.tiles_per_group, f->states);
         return launch_status("selective scan backward: b, c");
     });

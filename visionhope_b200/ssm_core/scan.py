@@ -77,7 +77,9 @@ class _Call:
         if want_checkpoints:
             ck = _args.workspace(lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)), dev)
         a.y, a.final_state, a.checkpoints = y.data_ptr(), _lib.ptr(final), _lib.ptr(ck)
-        _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
+        nbytes = lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a))
+        ws = _args.workspace(nbytes, dev) if nbytes else None
+        _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), _lib.ptr(ws), nbytes, _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
         return y, final, ck
 
     def backward(self, dy, dfinal, ck, want_initial):
