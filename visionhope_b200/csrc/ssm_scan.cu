@@ -7,6 +7,16 @@ namespace {
 
 constexpr int kWarps = 4;  // warps per CTA: neighbouring channel tiles
 
+constexpr int kAhead = 2;  // groups fetched ahead
+
+// Shared memory of a warp.
+template <typename T, int NL>
+struct FwdSmem {
+    Stage<NL> st[2];
+    float part[512];
+    typename Chain<T, NL>::Raw raw[kAhead + 1];
+};
+
 // Four staged tokens; Y: also y's partial sums over the thread's states, left in `part`.
 template <int NL, int MODE, bool Y>
 __device__ __forceinline__ void advance(const Stage<NL>& st, int ct, int j, const float2 (&a2)[8], float2 (&h)[8],
@@ -42,8 +52,7 @@ template <typename T, int NL, bool OWN>
 __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanParams p, const Segments g, int64_t items) {
     using K = Tile<NL>;
     constexpr int CE = K::CE, TE = K::TE;
-    __shared__ __align__(16) Stage<NL> stages[kWarps][2];
-    __shared__ __align__(16) float parts[kWarps][OWN ? 4 : 512];
+    extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
     if (OWN) launch_dependents();
@@ -53,18 +62,29 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     Chain<T, NL> ch(p, w.seq, w.s, w.tile, lane);
     const int j = lane / K::CL, ct = 4 * (lane % K::CL), c0 = ch.cbase + ct;  // the thread's 4 x 4 block
     const int ec = ch.ec, cend = ch.cend;
-    Stage<NL>* st = stages[warp];
-    float* part = parts[warp];
+    FwdSmem<T, NL>& sm = reinterpret_cast<FwdSmem<T, NL>*>(smem)[warp];
     const int64_t unit = w.slot * tiles + w.tile;
     float2 a2[8], h[8];
     float v[16], sum[CE];
     const float top_a = load_rates<NL>(p, c0, cend, j, v);
     pair_up(v, a2);
-    typename Chain<T, NL>::Raw raw;
     ch.move(w.t0);
     // the last segment's own state is not needed
     const bool some = w.t0 < w.t1 && (!OWN || w.t1 < w.seq.len);
-    if (some) ch.template load<!OWN>(raw, w.t1 - w.t0);
+    // the first kAhead groups; every group is a commit of its own, empty past the end
+    int64_t ahead = w.t0;
+    int slot = 0, next = 0;  // of the group at hand and the one fetched next
+    auto fetch_next = [&]() {
+        if (some && ahead < w.t1) {
+            ch.template load<!OWN>(sm.raw[next], w.t1 - ahead);
+            ch.move(kGroup);
+            ahead += kGroup;
+        }
+        cp_async_commit();
+        next = next == kAhead ? 0 : next + 1;
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) fetch_next();
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.f;
 #pragma unroll
@@ -74,12 +94,13 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
         pair_up(v, h);
         int buf = 0;
         for (int64_t t = w.t0; some && t < w.t1; t += kGroup, buf ^= 1) {
-            const float top = ch.template stage<true>(raw, w.t1 - t, st[buf], sum);
+            cp_async_wait<kAhead - 1>();
+            const float top = ch.template stage<true>(sm.raw[slot], w.t1 - t, sm.st[buf], sum);
+            slot = slot == kAhead ? 0 : slot + 1;
             __syncwarp();
-            ch.move(kGroup);
-            if (t + kGroup < w.t1) ch.template load<false>(raw, w.t1 - t - kGroup);
-            if (top * top_a <= 126.f) advance<NL, kMixed, false>(st[buf], ct, j, a2, h, nullptr);
-            else advance<NL, kChecked, false>(st[buf], ct, j, a2, h, nullptr);
+            fetch_next();
+            if (top * top_a <= 126.f) advance<NL, kMixed, false>(sm.st[buf], ct, j, a2, h, nullptr);
+            else advance<NL, kChecked, false>(sm.st[buf], ct, j, a2, h, nullptr);
         }
         pair_down(h, v);
         store_lanes(g.state + unit * 512, lane, v);
@@ -108,23 +129,25 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
             pair_down(h, v);
             store_lanes(ck + (t / kCheckpoint) * tiles * 512, lane, v);
         }
-        const float top = ch.template stage<false>(raw, w.t1 - t, st[buf], sum);
+        cp_async_wait<kAhead - 1>();
+        const typename Chain<T, NL>::Raw& raw = sm.raw[slot];
+        const float top = ch.template stage<false>(raw, w.t1 - t, sm.st[buf], sum);
         float ue[TE][CE], ze[TE][CE];
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
-            raw.u[e].get(ue[e]);
-            if (ch.gated) raw.z[e].get(ze[e]);
+            raw.u[e][lane].get(ue[e]);
+            if (ch.gated) raw.z[e][lane].get(ze[e]);
         }
+        slot = slot == kAhead ? 0 : slot + 1;
         __syncwarp();
-        ch.move(kGroup);
-        if (t + kGroup < w.t1) ch.template load<true>(raw, w.t1 - t - kGroup);
-        if (top * top_a <= 126.f) advance<NL, kMixed, true>(st[buf], ct, j, a2, h, part);
-        else advance<NL, kChecked, true>(st[buf], ct, j, a2, h, part);
+        fetch_next();
+        if (top * top_a <= 126.f) advance<NL, kMixed, true>(sm.st[buf], ct, j, a2, h, sm.part);
+        else advance<NL, kChecked, true>(sm.st[buf], ct, j, a2, h, sm.part);
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             float out[CE];
-            sum_parts<NL>(part + 128 * (ch.own_t + e), ch.own_c, out);
+            sum_parts<NL>(sm.part + 128 * (ch.own_t + e), ch.own_c, out);
 #pragma unroll
             for (int i = 0; i < CE; ++i) {
                 out[i] = fmaf(skip[i], ue[e][i], out[i]);
@@ -277,14 +300,18 @@ int launch_fwd(const ScanParams& p, const Segments& g, cudaStream_t st) {
     const int64_t items = (g.state ? g.slots : (int64_t)p.seqs.count) * tiles;
     const int64_t blocks = (items + kWarps - 1) / kWarps;
     if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_fwd: too many channel tiles");
+    const size_t smem = sizeof(FwdSmem<T, NL>) * kWarps;
+    if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, false>), smem) ||
+        !ensure_smem_attr(reinterpret_cast<const void*>(&scan_fwd_kernel<T, NL, true>), smem))
+        return fail(VH_E_DEVICE, "vh_ssm_scan_fwd: cannot reserve %zu bytes of shared memory", smem);
     if (!g.state) {
-        scan_fwd_kernel<T, NL, false><<<(int)blocks, 32 * kWarps, 0, st>>>(p, g, items);
+        scan_fwd_kernel<T, NL, false><<<(int)blocks, 32 * kWarps, smem, st>>>(p, g, items);
         return launch_status("selective scan");
     }
-    scan_fwd_kernel<T, NL, true><<<(int)blocks, 32 * kWarps, 0, st>>>(p, g, items);
+    scan_fwd_kernel<T, NL, true><<<(int)blocks, 32 * kWarps, smem, st>>>(p, g, items);
     if (int rc = launch_status("selective scan: own states")) return rc;
     if (int rc = enter_segments(p, 4 * NL, g, p.initial, false, st)) return rc;
-    return launch_after("selective scan", scan_fwd_kernel<T, NL, false>, blocks, 32 * kWarps, 0, st, p, g, items);
+    return launch_after("selective scan", scan_fwd_kernel<T, NL, false>, blocks, 32 * kWarps, smem, st, p, g, items);
 }
 
 }  // namespace

@@ -77,41 +77,18 @@ struct LaneElems {
     }
 };
 
-// V elements as they lie in memory, loaded ahead of their use.  `left`: how many of them exist
-// (vec: the pointer is aligned and all do).  The loads are volatile, so that they are issued where
-// they stand, a group ahead of their use: left to the compiler they moved next to it, and the
-// forward waited for memory in 4 of 10 cycles (64 x 256 tokens of two images: 279 us, now 191).
+// V elements as they lie in memory.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Pack {
     T e[V];
+    // `left`: how many of them exist (vec: the pointer is aligned and all do); missing ones repeat
+    // the last
     __device__ __forceinline__ void load(const T* p, int left, bool vec) {
         if (vec) {
-            if constexpr (sizeof(Pack) == 16) {
-                uint4 r;
-                asm volatile("ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-                *reinterpret_cast<uint4*>(e) = r;
-            } else if constexpr (sizeof(Pack) == 8) {
-                uint2 r;
-                asm volatile("ld.global.nc.v2.b32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-                *reinterpret_cast<uint2*>(e) = r;
-            } else if constexpr (sizeof(Pack) == 4) {
-                uint32_t r;
-                asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(r) : "l"(p));
-                *reinterpret_cast<uint32_t*>(e) = r;
-            } else {
-                *this = *reinterpret_cast<const Pack*>(p);
-            }
+            *this = *reinterpret_cast<const Pack*>(p);
         } else {
-            // element by element; missing ones repeat the last
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const T* q = p + max(min(i, left - 1), 0);
-                if constexpr (sizeof(T) == 4) {
-                    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&e[i])) : "l"(q));
-                } else {
-                    asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&e[i])) : "l"(q));
-                }
-            }
+            for (int i = 0; i < V; ++i) e[i] = p[max(min(i, left - 1), 0)];
         }
     }
     __device__ __forceinline__ void get(float (&v)[V]) const {
@@ -119,6 +96,21 @@ struct alignas(sizeof(T) * V) Pack {
         for (int i = 0; i < V; ++i) v[i] = to_f(e[i]);
     }
 };
+// The same into shared memory, asynchronously where the copy is one of 4, 8 or 16 bytes.  Issued a
+// group or two ahead of its use it takes no registers; plain loads ahead of their use do, and were
+// moved next to it by the compiler (the forward then waited for memory in 4 of 10 cycles).
+template <typename T, int V>
+__device__ __forceinline__ void fetch(Pack<T, V>* dst, const T* p, int left, bool vec) {
+    if constexpr (sizeof(T) * V >= 4) {
+        if (vec) {
+            cp_async<sizeof(T) * V>(dst, p);
+            return;
+        }
+    }
+    Pack<T, V> r;
+    r.load(p, left, vec);
+    *dst = r;
+}
 
 __device__ __forceinline__ void lds4(const float* p, float (&v)[4]) {
     const float4 q = *reinterpret_cast<const float4*>(p);
@@ -286,36 +278,26 @@ struct Chain {
         for (int i = 0; i < Q; ++i) bc[i] += n * bcs;
     }
 
+    // A group's values as loaded; every lane reads back only what it fetched.
     struct Raw {
-        Pack<T, CE> u[TE], d[TE], z[TE];
-        Pack<T, 4> bc[Q];
+        Pack<T, CE> u[TE][32], d[TE][32], z[TE][32];
+        Pack<T, 4> bc[Q][32];
     };
-    // The loads of the group at hand, of which the first `count` (or more) tokens exist.
+    // Fetches the group at hand, of which the first `count` (or more) tokens exist.
     template <bool GATE>
     __device__ __forceinline__ void load(Raw& r, int64_t count) const {
-        if (count >= kGroup) {
+        const int last = count >= kGroup ? kGroup - 1 : (int)count - 1;
 #pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                r.u[e].load(u + e * us, left, vec);
-                r.d[e].load(dl + e * ds, left, vec);
-                if (GATE && gated) r.z[e].load(z + e * zs, left, vec);
-            }
+        for (int e = 0; e < TE; ++e) {
+            const int64_t by = min(e, last - own_t);
+            fetch(&r.u[e][lane], u + by * us, left, vec);
+            fetch(&r.d[e][lane], dl + by * ds, left, vec);
+            if (GATE && gated) fetch(&r.z[e][lane], z + by * zs, left, vec);
+        }
 #pragma unroll
-            for (int i = 0; i < Q; ++i) r.bc[i].load(bc[i], 4, vec_bc);
-        } else {
-            const int last = (int)count - 1;
-#pragma unroll
-            for (int e = 0; e < TE; ++e) {
-                const int64_t by = min(e, last - own_t);
-                r.u[e].load(u + by * us, left, vec);
-                r.d[e].load(dl + by * ds, left, vec);
-                if (GATE && gated) r.z[e].load(z + by * zs, left, vec);
-            }
-#pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const int t = min(lane + 32 * i, kQuads - 1) / (2 * NL);
-                r.bc[i].load(bc[i] + min(0, last - t) * bcs, 4, vec_bc);
-            }
+        for (int i = 0; i < Q; ++i) {
+            const int t = min(lane + 32 * i, kQuads - 1) / (2 * NL);
+            fetch(&r.bc[i][lane], bc[i] + min(0, last - t) * bcs, 4, vec_bc);
         }
     }
     // s, s u, B and C of a loaded group into shared memory.  SUM: adds s to sum.  Returns the
@@ -326,8 +308,8 @@ struct Chain {
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             float uv[CE], sv[CE];
-            r.u[e].get(uv);
-            r.d[e].get(sv);
+            r.u[e][lane].get(uv);
+            r.d[e][lane].get(sv);
             const bool live = own_t + e < count;
 #pragma unroll
             for (int i = 0; i < CE; ++i) sv[i] += bias[i];
@@ -350,7 +332,7 @@ struct Chain {
                 const int n = 4 * (at % NL);
                 float* row = st.bc + (at / NL) * Stage<NL>::kRow;
                 float v[4];
-                r.bc[i].get(v);
+                r.bc[i][lane].get(v);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     row[((n + k) % NL) * 4 + (n + k) / NL] = v[k];

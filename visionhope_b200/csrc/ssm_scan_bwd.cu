@@ -25,7 +25,9 @@ namespace ssm {
 namespace {
 
 constexpr int kGroups = kCheckpoint / kGroup;  // groups in a chunk
-constexpr int kBwdWarps = 4;                   // warps per CTA: neighbouring channel tiles
+// Warps per CTA (neighbouring channel tiles): what the shared memory of half an SM holds.
+template <typename T>
+constexpr int kBwdWarps = sizeof(T) == 4 ? 3 : 4;
 
 struct BwdParams {
     ScanParams f;
@@ -42,9 +44,15 @@ struct BwdParams {
 
 // Shared memory of a warp.  A token's sums over lanes (ds, sum b g, db and dc) take the place of
 // the state before it, once that is read.
-template <int NL>
+template <typename T, int NL>
+struct BwdRaw {
+    typename Chain<T, NL>::Raw r;
+    Pack<T, Tile<NL>::CE> dy[Tile<NL>::TE][32];
+};
+template <typename T, int NL>
 struct BwdStage {
     using K = Tile<NL>;
+    BwdRaw<T, NL> raw;            // the next group, as loaded
     float h[kGroups][512];        // the states before the groups of a chunk
     float past[kGroup - 1][512];  // before the second to fourth token of the group at hand
     Stage<NL> s;
@@ -88,14 +96,14 @@ __device__ __forceinline__ void sum_bc(const float* part, int lane, bool live, f
 // OWN: the first of the three kernels of a chain in segments: the segment's own gradient, that of
 // the state before it when nothing enters from the right, and its sum of steps.
 template <typename T, int NL, bool OWN>
-__global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
+__global__ void __launch_bounds__(32 * kBwdWarps<T>, 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
     using K = Tile<NL>;
     constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL;
     extern __shared__ __align__(16) unsigned char smem[];
     const ScanParams& p = bp.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    BwdStage<NL>& sm = reinterpret_cast<BwdStage<NL>*>(smem)[warp];
-    const int64_t item = (int64_t)blockIdx.x * kBwdWarps + warp;
+    BwdStage<T, NL>& sm = reinterpret_cast<BwdStage<T, NL>*>(smem)[warp];
+    const int64_t item = (int64_t)blockIdx.x * kBwdWarps<T> + warp;
     if (OWN) launch_dependents();
     Unit w;
     if (item >= items) return;
@@ -125,35 +133,36 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
     pair_up(v16, a2);
     const float* dfinal = bp.dfinal ? bp.dfinal + (int64_t)s * p.channels * N : nullptr;
 
-    struct Raw {
-        typename Chain<T, NL>::Raw r;
-        Pack<T, CE> dy[TE];
-    };
     // dy's rows lie as y's; it moves with the chain's view, which stands at token `pos`
     const T* dyr = dy + (chn.left > 0 ? 0 : -(ec - (cend - (bp.vec ? CE : 1)))) + own_t * ys;
     int64_t pos = 0;
-    auto move = [&](int64_t to) {
-        chn.move(to - pos);
-        dyr += (to - pos) * ys;
-        pos = to;
-    };
-    auto load = [&](Raw& r, int64_t count) {
-        chn.template load<true>(r.r, count);
+    // Fetches the group at `t` (of `count` tokens or more) behind the one at hand: a lane reads
+    // back only what it fetched, and has read the group at hand by then.
+    auto fetch_at = [&](int64_t t, int64_t count, bool all) {
+        chn.move(t - pos);
+        dyr += (t - pos) * ys;
+        pos = t;
+        if (all) {
+            chn.template load<true>(sm.raw.r, count);
 #pragma unroll
-        for (int e = 0; e < TE; ++e) {
-            const int64_t by = count >= kGroup ? e : min((int64_t)e, count - 1 - own_t);
-            r.dy[e].load(dyr + by * ys, chn.left, bp.vec);
+            for (int e = 0; e < TE; ++e) {
+                const int64_t by = count >= kGroup ? e : min((int64_t)e, count - 1 - own_t);
+                fetch(&sm.raw.dy[e][lane], dyr + by * ys, chn.left, (bool)bp.vec);
+            }
+        } else {
+            chn.template load<false>(sm.raw.r, count);
         }
+        cp_async_commit();
     };
-    // s, s u, B, C and v of a group
-    auto stage = [&](const Raw& r, int64_t count, float (&sum)[CE]) {
-        const float top = chn.template stage<true>(r.r, count, sm.s, sum);
+    // s, s u, B, C and v of the fetched group
+    auto stage = [&](int64_t count, float (&sum)[CE]) {
+        const float top = chn.template stage<true>(sm.raw.r, count, sm.s, sum);
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             float ve[CE], ze[CE];
-            r.dy[e].get(ve);
+            sm.raw.dy[e][lane].get(ve);
             if (gated) {
-                r.r.z[e].get(ze);
+                sm.raw.r.z[e][lane].get(ze);
 #pragma unroll
                 for (int i = 0; i < CE; ++i) ve[i] *= ze[i] * sigmoid(ze[i]);
             }
@@ -174,14 +183,12 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
 #pragma unroll
         for (int i = 0; i < CE; ++i) sum[i] = 0.f;
         if (t0 > 0 && t0 < t1) {  // the first segment's own gradient is not needed
-            move(t0);
-            Raw raw;
-            load(raw, t1 - t0);
+            fetch_at(t0, t1 - t0, true);
             for (int64_t t = t0; t < t1; t += kGroup) {
-                const float top = stage(raw, t1 - t, sum);
+                cp_async_wait<0>();
+                const float top = stage(t1 - t, sum);
                 __syncwarp();
-                move(t + kGroup);
-                if (t + kGroup < t1) load(raw, t1 - t - kGroup);
+                if (t + kGroup < t1) fetch_at(t + kGroup, t1 - t - kGroup, true);
                 auto pass = [&](auto mode) {
 #pragma unroll
                     for (int r = 0; r < kGroup; ++r) {
@@ -237,6 +244,10 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
     }
 
     const int64_t first = t0 / kCheckpoint, last = (t1 + kCheckpoint - 1) / kCheckpoint;
+    if (t0 < t1) {  // the last chunk's first group
+        const int64_t tc = (last - 1) * kCheckpoint;
+        fetch_at(tc, t1 - tc, t1 - tc <= kGroup);
+    }
     for (int64_t ch = last - 1; ch >= first && t0 < t1; --ch) {
         const int64_t tc = ch * kCheckpoint;
         const int64_t te = min(t1, tc + kCheckpoint);
@@ -249,17 +260,15 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
         pair_up(v16, h);
         // forward over all groups but the last, whose state is not needed beyond its start
         {
-            move(tc);
-            typename Chain<T, NL>::Raw raw;
-            if (groups > 1) chn.template load<false>(raw, te - tc);
             for (int gi = 0; gi < groups; ++gi) {
                 pair_down(h, v16);
                 store_lanes(sm.h[gi], lane, v16);
                 if (gi + 1 == groups) break;
-                chn.template stage<false>(raw, kGroup, sm.s, unused);
+                cp_async_wait<0>();
+                chn.template stage<false>(sm.raw.r, kGroup, sm.s, unused);
                 __syncwarp();
-                move(tc + (gi + 1) * kGroup);
-                if (gi + 2 < groups) chn.template load<false>(raw, kGroup);
+                const int64_t next = tc + (gi + 1) * kGroup;  // of the last group all, for the way back
+                fetch_at(next, te - next, gi + 2 == groups);
 #pragma unroll
                 for (int r = 0; r < kGroup; ++r) {
                     float2 sv[2], pv[2], b[4], e[8];
@@ -275,17 +284,21 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
                 __syncwarp();
             }
         }
-        Raw raw;
-        load(raw, te - pos);  // the last group: the forward pass moved there
         for (int gi = groups - 1; gi >= 0; --gi) {
             const int64_t t = tc + gi * kGroup;
-            const float top = stage(raw, te - t, unused);
-            const Raw now = raw;
-            __syncwarp();
-            if (gi > 0) {
-                move(t - kGroup);
-                load(raw, kGroup);
+            cp_async_wait<0>();
+            const float top = stage(te - t, unused);
+            Pack<T, CE> nu[TE], nd[TE], nz[TE], ndy[TE];
+#pragma unroll
+            for (int x = 0; x < TE; ++x) {
+                nu[x] = sm.raw.r.u[x][lane];
+                nd[x] = sm.raw.r.d[x][lane];
+                ndy[x] = sm.raw.dy[x][lane];
+                if (gated) nz[x] = sm.raw.r.z[x][lane];
             }
+            __syncwarp();
+            if (gi > 0) fetch_at(t - kGroup, kGroup, true);
+            else if (ch > first) fetch_at(tc - kCheckpoint, kGroup, false);
             auto pass = [&](auto mode) {
                 float2 e[kGroup][8];
                 float dcs[kGroup][4];
@@ -366,10 +379,10 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 2) scan_bwd_kernel(const BwdPa
                 const int r = own_t + x;
                 const int64_t row = t + r;
                 float yo[CE], dso[CE], gbo[CE], ste[CE], duo[CE], ddo[CE], dzo[CE], ue[CE], re[CE], ye[CE], ze[CE];
-                now.r.u[x].get(ue);
-                now.r.d[x].get(re);
-                now.dy[x].get(ye);
-                if (gated) now.r.z[x].get(ze);
+                nu[x].get(ue);
+                nd[x].get(re);
+                ndy[x].get(ye);
+                if (gated) nz[x].get(ze);
                 const float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
                 if (gated) sum_parts<NL>(sm.y + 128 * r, own_c, yo);
                 sum_parts<NL>(sums, own_c, dso);
@@ -474,10 +487,10 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
 struct Layout {
     int64_t tokens, rows, bc, a, d, total;  // floats
 };
-// Warps that a B200 holds of the backward kernel (two CTAs of four an SM).
-int64_t bwd_warps() { return (int64_t)8 * sm_count(); }
+// Warps that a B200 holds of the backward kernel (two CTAs of three or four an SM).
+int64_t bwd_warps(const vh_ssm_scan_args* a) { return (int64_t)(a->dtype == VH_F32 ? 6 : 8) * sm_count(); }
 
-int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps() / 2, bwd_warps(), kCheckpoint); }
+int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) / 2, bwd_warps(a), kCheckpoint); }
 
 Layout layout_of(const vh_ssm_scan_args* a, int size) {
     Layout l;
@@ -494,21 +507,22 @@ Layout layout_of(const vh_ssm_scan_args* a, int size) {
 
 template <typename T, int NL>
 int launch_bwd(const BwdParams& p, const Segments& g, cudaStream_t st) {
-    const size_t smem = sizeof(BwdStage<NL>) * kBwdWarps;
+    constexpr int W = kBwdWarps<T>;
+    const size_t smem = sizeof(BwdStage<T, NL>) * W;
     const int64_t items = (g.state ? g.slots : (int64_t)p.f.seqs.count) * p.f.groups * p.f.tiles_per_group;
-    const int64_t blocks = (items + kBwdWarps - 1) / kBwdWarps;
+    const int64_t blocks = (items + W - 1) / W;
     if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
     if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, false>), smem) ||
         !ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), smem))
         return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
     if (!g.state) {
-        scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, g, items);
+        scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * W, smem, st>>>(p, g, items);
         return launch_status("selective scan backward");
     }
-    scan_bwd_kernel<T, NL, true><<<(int)blocks, 32 * kBwdWarps, smem, st>>>(p, g, items);
+    scan_bwd_kernel<T, NL, true><<<(int)blocks, 32 * W, smem, st>>>(p, g, items);
     if (int rc = launch_status("selective scan backward: own gradients")) return rc;
     if (int rc = enter_segments(p.f, 4 * NL, g, p.dfinal, true, st)) return rc;
-    return launch_after("selective scan backward", scan_bwd_kernel<T, NL, false>, blocks, 32 * kBwdWarps, smem, st, p, g, items);
+    return launch_after("selective scan backward", scan_bwd_kernel<T, NL, false>, blocks, 32 * W, smem, st, p, g, items);
 }
 
 int check_bwd(const char* what, const vh_ssm_scan_bwd_args* a) {
