@@ -102,6 +102,24 @@ def test_struct_layouts_match_the_header():
         assert offsets == [getattr(cls, f).offset for f in fields]
 
 
+def test_packed_structs_match_their_mirrors():
+    from visionhope_b200 import _lib
+    from visionhope_b200.ssm_core import conv, scan
+
+    def packed(cls):
+        """(offset, size) of every value that ``struct`` packs, from the mirror's fields."""
+        return [(getattr(cls, f[0]).offset, ctypes.sizeof(f[1])) for f in cls._fields_]
+
+    def values(fmt, count, size):
+        ones = [fmt.unpack(bytes(i) + b"\xff" + bytes(size - i - 1)) for i in range(size)]
+        return [(min(i for i in range(size) if ones[i][k]), sum(1 for i in range(size) if ones[i][k])) for k in range(count)]
+
+    for cls, fmt in ((_lib.VhShortConvArgs, conv._ARGS), (_lib.VhSsmScanArgs, scan._ARGS)):
+        assert fmt.size == ctypes.sizeof(cls)
+        assert values(fmt, len(cls._fields_), fmt.size) == packed(cls)
+    assert scan._ARGS.size + scan._GRADS.size == ctypes.sizeof(_lib.VhSsmScanBwdArgs)
+
+
 @pytest.mark.parametrize("change,code,text", [
     (dict(x=None), -1, "null"), (dict(dtype=7), -3, "dtype"), (dict(taps=1), -2, "taps"), (dict(taps=9), -2, "taps"),
     (dict(activation=2), -1, "activation"), (dict(batch=0), -2, "positive"), (dict(channels=-4), -2, "positive"),

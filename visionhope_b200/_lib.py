@@ -201,7 +201,8 @@ def load() -> ctypes.CDLL:
             lib.vh_residual_add_bwd.argtypes = ([c_void_p, c_void_p, c_int32] + [c_void_p] * 5
                                                 + [c_int64, c_int32, c_int64, c_int32, c_void_p])
             # selective state space operators
-            conv, scan, scan_bwd = (ctypes.POINTER(t) for t in (VhShortConvArgs, VhSsmScanArgs, VhSsmScanBwdArgs))
+            # argument structs: a packed bytes object or a reference to the mirror above
+            conv = scan = scan_bwd = c_void_p
             lib.vh_short_conv_fwd.restype = c_int32
             lib.vh_short_conv_fwd.argtypes = [conv, c_void_p]
             lib.vh_short_conv_bwd_workspace_bytes.restype = c_int64
@@ -258,7 +259,8 @@ def ensure_device(t: torch.Tensor) -> None:
 
 
 def stream_handle(device=None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = device.index if isinstance(device, torch.device) else device
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def ptr(t: torch.Tensor | None):

@@ -50,13 +50,16 @@ struct BwdRaw {
     Pack<T, Tile<NL>::CE> dy[Tile<NL>::TE][32];
 };
 template <typename T, int NL>
-struct BwdStage {
-    using K = Tile<NL>;
-    BwdRaw<T, NL> raw;            // the next group, as loaded
+struct OwnStage {
+    BwdRaw<T, NL> raw;  // the next group, as loaded
+    Stage<NL> s;
+    float v[kGroup * Tile<NL>::CW];
+};
+template <typename T, int NL>
+struct BwdStage : OwnStage<T, NL> {
     float h[kGroups][512];        // the states before the groups of a chunk
     float past[kGroup - 1][512];  // before the second to fourth token of the group at hand
-    Stage<NL> s;
-    float v[kGroup * K::CW], y[512];
+    float y[512];
 };
 
 // Values in shared memory are read again after this, instead of being kept in registers.
@@ -96,13 +99,14 @@ __device__ __forceinline__ void sum_bc(const float* part, int lane, bool live, f
 // OWN: the first of the three kernels of a chain in segments: the segment's own gradient, that of
 // the state before it when nothing enters from the right, and its sum of steps.
 template <typename T, int NL, bool OWN>
-__global__ void __launch_bounds__(32 * kBwdWarps<T>, 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
+__global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
     using K = Tile<NL>;
     constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL;
     extern __shared__ __align__(16) unsigned char smem[];
     const ScanParams& p = bp.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    BwdStage<T, NL>& sm = reinterpret_cast<BwdStage<T, NL>*>(smem)[warp];
+    using Smem = std::conditional_t<OWN, OwnStage<T, NL>, BwdStage<T, NL>>;
+    Smem& sm = reinterpret_cast<Smem*>(smem)[warp];
     const int64_t item = (int64_t)blockIdx.x * kBwdWarps<T> + warp;
     if (OWN) launch_dependents();
     Unit w;
@@ -214,8 +218,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, 2) scan_bwd_kernel(const Bw
         pair_down(own, v16);
         store_lanes(seg.state + unit * 512, lane, v16);
         sum_tokens<NL>(sum, lane, own_c, seg.sigma + unit * CW);
-        return;
-    }
+    } else {
     if (seg.state) {
         wait_for_previous();
         load_lanes(seg.state + unit * 512, lane, v16);
@@ -420,6 +423,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, 2) scan_bwd_kernel(const Bw
     store_lanes(bp.part_a + unit * 512, lane, v16);
     sum_tokens<NL>(dskip, lane, own_c, bp.part_d + (w.slot * 2 * tiles + tile) * CW);
     sum_tokens<NL>(dbias, lane, own_c, bp.part_d + ((w.slot * 2 + 1) * tiles + tile) * CW);
+    }
 }
 
 // db and dc: the channel tiles' partials of each group added in order.  A thread adds four states
@@ -508,18 +512,18 @@ Layout layout_of(const vh_ssm_scan_args* a, int size) {
 template <typename T, int NL>
 int launch_bwd(const BwdParams& p, const Segments& g, cudaStream_t st) {
     constexpr int W = kBwdWarps<T>;
-    const size_t smem = sizeof(BwdStage<T, NL>) * W;
+    const size_t smem = sizeof(BwdStage<T, NL>) * W, own = sizeof(OwnStage<T, NL>) * W;
     const int64_t items = (g.state ? g.slots : (int64_t)p.f.seqs.count) * p.f.groups * p.f.tiles_per_group;
     const int64_t blocks = (items + W - 1) / W;
     if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many channel tiles");
     if (!ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, false>), smem) ||
-        !ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), smem))
+        !ensure_smem_attr(reinterpret_cast<const void*>(&scan_bwd_kernel<T, NL, true>), own))
         return fail(VH_E_DEVICE, "vh_ssm_scan_bwd: cannot reserve %zu bytes of shared memory", smem);
     if (!g.state) {
         scan_bwd_kernel<T, NL, false><<<(int)blocks, 32 * W, smem, st>>>(p, g, items);
         return launch_status("selective scan backward");
     }
-    scan_bwd_kernel<T, NL, true><<<(int)blocks, 32 * W, smem, st>>>(p, g, items);
+    scan_bwd_kernel<T, NL, true><<<(int)blocks, 32 * W, own, st>>>(p, g, items);
     if (int rc = launch_status("selective scan backward: own gradients")) return rc;
     if (int rc = enter_segments(p.f, 4 * NL, g, p.dfinal, true, st)) return rc;
     return launch_after("selective scan backward", scan_bwd_kernel<T, NL, false>, blocks, 32 * W, smem, st, p, g, items);

@@ -1,12 +1,14 @@
 """Short causal convolution over token rows (``vh_short_conv_fwd``, ``_bwd``, ``_step``)."""
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
 from . import _args
+from ._args import ptr
 
 _ACTIVATIONS = {None: 0, "silu": 1}
+_ARGS = struct.Struct("QqqQQQQQQqiiiiii")  # vh_short_conv_args
 
 
 def _activation(activation):
@@ -19,50 +21,54 @@ def _activation(activation):
 def _taps(weight, channels):
     if weight.dim() != 2 or weight.shape[0] != channels:
         raise ValueError(f"weight must be [{channels}, taps], got {tuple(weight.shape)}")
-    if not 2 <= weight.shape[1] <= 8:
-        raise ValueError(f"short_conv takes 2 to 8 taps, got {weight.shape[1]}")
-    return weight.shape[1]
+    k = weight.shape[1]
+    if not 2 <= k <= 8:
+        raise ValueError(f"short_conv takes 2 to 8 taps, got {k}")
+    return k
 
 
 class _Call:
-    """One call's checked arguments: the C struct, and the tensors that it points to."""
+    """One call's checked arguments; ``args`` packs them with the output pointers."""
+
+    __slots__ = ("x", "weight", "bias", "initial", "offsets", "state_shape", "head", "tail")
 
     def __init__(self, x, weight, bias, activation, initial, offsets, reverse):
         count, length, offsets = _args.sequences(x, offsets, "x")
-        d = x.shape[-1]
+        shape, device, dtype = x.shape, x.device, x.dtype
+        d = shape[-1]
         k = _taps(weight, d)
-        x = _args.rows(x, tuple(x.shape), "x", x)
-        weight = _args.fp32(weight, (d, k), "weight", x.device)
-        bias = _args.fp32(bias, (d,), "bias", x.device)
-        initial = _args.state(initial, (count, k - 1, d), "initial_state", x.dtype, x.device)
-        if initial is not None and initial.requires_grad:
-            initial = initial.detach()
-        self.kept = x, weight, bias, initial, offsets
+        self.x = x = _args.rows(x, shape, "x", dtype, device)
+        self.weight = weight = _args.fp32(weight, (d, k), "weight", device)
+        self.bias = bias = _args.fp32(bias, (d,), "bias", device)
         self.state_shape = count, k - 1, d
-        self.args = _lib.VhShortConvArgs(
-            x.data_ptr(), x.stride(0), x.stride(-2), weight.data_ptr(), _lib.ptr(bias), _lib.ptr(initial), None, None,
-            _lib.ptr(offsets), length, _lib.DTYPES[x.dtype], activation, k, count, d, int(bool(reverse)))
+        self.initial = initial = _args.state(initial, self.state_shape, "initial_state", dtype, device)
+        self.offsets = offsets
+        stride = x.stride()
+        self.head = (x.data_ptr(), stride[0], stride[-2], weight.data_ptr(), ptr(bias), ptr(initial))
+        self.tail = (ptr(offsets), length, _lib.DTYPES[dtype], activation, k, count, d, 1 if reverse else 0)
+
+    def args(self, y=0, final=0):
+        return _ARGS.pack(*self.head, y, final, *self.tail)
 
     def forward(self, want_final):
-        x, initial = self.kept[0], self.kept[3]
+        x = self.x
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         final = torch.empty(self.state_shape, dtype=x.dtype, device=x.device) if want_final else None
         if y.numel() == 0:  # no tokens: every state leaves as it entered
             if final is not None:
-                final.copy_(initial) if initial is not None else final.zero_()
+                final.copy_(self.initial.detach()) if self.initial is not None else final.zero_()
             return y, final
-        self.args.y, self.args.final_state = y.data_ptr(), _lib.ptr(final)
-        _lib.check(_lib.load().vh_short_conv_fwd(ctypes.byref(self.args), _lib.stream_handle(x.device)),
+        _lib.check(_lib.load().vh_short_conv_fwd(self.args(y.data_ptr(), ptr(final)), _lib.stream_handle(x.device)),
                    "vh_short_conv_fwd")
         return y, final
 
-    def backward(self, dy, dfinal, want_bias, want_initial):
-        x, weight = self.kept[:2]
-        dev, d, k = x.device, weight.shape[0], weight.shape[1]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dw = torch.empty((d, k), dtype=torch.float32, device=dev)
-        db = torch.empty((d,), dtype=torch.float32, device=dev) if want_bias else None
-        di = torch.empty(self.state_shape, dtype=x.dtype, device=dev) if want_initial else None
+    def backward(self, dy, dfinal, want_initial):
+        x, weight = self.x, self.weight
+        dev, dtype = x.device, x.dtype
+        dx = torch.empty(x.shape, dtype=dtype, device=dev)
+        dw = torch.empty(weight.shape, dtype=torch.float32, device=dev)
+        db = None if self.bias is None else torch.empty(self.bias.shape, dtype=torch.float32, device=dev)
+        di = torch.empty(self.state_shape, dtype=dtype, device=dev) if want_initial else None
         if x.numel() == 0:
             dw.zero_()
             if db is not None:
@@ -70,11 +76,10 @@ class _Call:
             if di is not None:
                 di.copy_(dfinal) if dfinal is not None else di.zero_()
             return dx, dw, db, di
-        lib = _lib.load()
-        ws = _args.workspace(lib.vh_short_conv_bwd_workspace_bytes(ctypes.byref(self.args)), dev)
-        _lib.check(lib.vh_short_conv_bwd(
-            ctypes.byref(self.args), dy.data_ptr(), _lib.ptr(dfinal), dx.data_ptr(), dw.data_ptr(), _lib.ptr(db),
-            _lib.ptr(di), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)), "vh_short_conv_bwd")
+        lib, args = _lib.load(), self.args()
+        ws = _args.workspace(lib.vh_short_conv_bwd_workspace_bytes(args), dev)
+        _lib.check(lib.vh_short_conv_bwd(args, dy.data_ptr(), ptr(dfinal), dx.data_ptr(), dw.data_ptr(), ptr(db), ptr(di),
+                                         ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)), "vh_short_conv_bwd")
         return dx, dw, db, di
 
 
@@ -85,7 +90,7 @@ class _ShortConvFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, initial, activation, want_final, offsets, reverse):
         call = _Call(x, weight, bias, activation, initial, offsets, reverse)
         y, final = call.forward(want_final)
-        ctx.save_for_backward(x, weight, bias, initial, call.kept[4])
+        ctx.save_for_backward(x, weight, bias, initial, call.offsets)
         ctx.options = activation, reverse
         ctx.set_materialize_grads(False)
         return (y, final) if want_final else y
@@ -93,16 +98,22 @@ class _ShortConvFunction(torch.autograd.Function):
     @staticmethod
     @_lib.on_input_device
     def backward(ctx, dy, dfinal=None):
-        x, weight, bias, initial, offsets = ctx.saved_tensors
-        activation, reverse = ctx.options
         if dy is None and dfinal is None:
             return (None,) * 8
+        x, weight, bias, initial, offsets = ctx.saved_tensors
+        activation, reverse = ctx.options
         call = _Call(x, weight, bias, activation, initial, offsets, reverse)
         dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _args.grad_rows(dy)
         dfinal = None if dfinal is None else _args.grad_rows(dfinal)
-        dx, dw, db, di = call.backward(dy, dfinal, bias is not None,
-                                       initial is not None and ctx.needs_input_grad[3])
-        return (dx, dw.to(weight.dtype), None if db is None else db.to(bias.dtype), di, None, None, None, None)
+        dx, dw, db, di = call.backward(dy, dfinal, initial is not None and ctx.needs_input_grad[3])
+        return dx, _args.grad_like(dw, weight), _args.grad_like(db, bias), di, None, None, None, None
+
+
+def _needs_grad(*tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 @_lib.on_input_device
@@ -119,36 +130,37 @@ def short_conv(x, weight, bias=None, *, activation=None, initial_state=None, ret
     or (y, final_state) with ``return_final_state``, the last taps - 1 inputs.  Differentiable in
     x, weight, bias and initial_state, through y and the final state."""
     act = _activation(activation)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, initial_state)):
+    if torch.is_grad_enabled() and _needs_grad(x, weight, bias, initial_state):
         return _ShortConvFunction.apply(x, weight, bias, initial_state, act, bool(return_final_state), seq_offsets,
                                         bool(reverse))
     y, final = _Call(x, weight, bias, act, initial_state, seq_offsets, reverse).forward(return_final_state)
     return (y, final) if return_final_state else y
 
 
-@torch.no_grad()
 @_lib.on_input_device
 def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None, state_out=None):
     """One token of ``B`` cached streams: x [B, C], state [slots, taps - 1, C] of x's dtype, whose
     rows move up by one with x as the newest (in place, or into ``state_out``).  slots: int32 or
     int64 [B], each stream's row of the state (row b without it); a stream whose slot lies outside
-    the state is skipped and its y is 0; no two streams may name one slot.  Returns y [B, C]."""
+    the state is skipped and its y is 0; no two streams may name one slot.  Returns y [B, C].  Not
+    differentiable."""
     act = _activation(activation)
     _lib.ensure_device(x)
-    code = _lib.dtype_code(x.dtype)
+    device, dtype = x.device, x.dtype
+    code = _lib.dtype_code(dtype)
     if x.dim() != 2:
         raise ValueError(f"x must be [batch, channels], got {tuple(x.shape)}")
-    b, d = x.shape
+    b, d = shape = x.shape
     k = _taps(weight, d)
-    x = _args.rows(x, (b, d), "x", x)
-    weight = _args.fp32(weight, (d, k), "weight", x.device)
-    bias = _args.fp32(bias, (d,), "bias", x.device)
-    slots = _args.slot_index(slots, b, x.device)
-    state, state_out = _args.cache(state, state_out, (k - 1, d), b, slots, x.dtype, x.device)
-    y = torch.empty((b, d), dtype=x.dtype, device=x.device)
-    if y.numel() == 0:
+    x = _args.rows(x, shape, "x", dtype, device)
+    weight = _args.fp32(weight, (d, k), "weight", device)
+    bias = _args.fp32(bias, (d,), "bias", device)
+    slots = _args.slot_index(slots, b, device)
+    state, state_out = _args.cache(state, state_out, (k - 1, d), b, slots, dtype, device)
+    y = torch.empty(shape, dtype=dtype, device=device)
+    if b * d == 0:
         return y
     _lib.check(_lib.load().vh_short_conv_step(
-        x.data_ptr(), x.stride(0), code, weight.data_ptr(), _lib.ptr(bias), act, state.data_ptr(), state_out.data_ptr(),
-        _lib.ptr(slots), state.shape[0], y.data_ptr(), b, d, k, _lib.stream_handle(x.device)), "vh_short_conv_step")
+        x.data_ptr(), x.stride(0), code, weight.data_ptr(), ptr(bias), act, state.data_ptr(), state_out.data_ptr(),
+        ptr(slots), state.shape[0], y.data_ptr(), b, d, k, _lib.stream_handle(device)), "vh_short_conv_step")
     return y

@@ -1,92 +1,104 @@
 """Selective scan over token rows (``vh_ssm_scan_fwd``, ``_bwd``, ``_step``)."""
-import ctypes
+import struct
 
 import torch
 
 from .. import _lib
 from . import _args
+from ._args import ptr
+from .conv import _needs_grad
 
 STATES = (4, 8, 16, 32, 64)
+_ARGS = struct.Struct("5Q12q8Qq7i4x")  # vh_ssm_scan_args
+_GRADS = struct.Struct("11Q")          # the rest of vh_ssm_scan_bwd_args
+_NONE = (0, 0, 0)
 
 
-def _grouped(t, lead, n, name, like):
-    """B or C as [..., groups, states] rows; a tensor without a group dim has one group."""
-    if t.dim() == len(lead) + 1:
-        t = t.unsqueeze(-2)
-    if t.dim() != len(lead) + 2 or tuple(t.shape[:-2]) != lead or t.shape[-1] != n:
-        raise ValueError(f"{name} must be [{', '.join(map(str, lead))}, (groups,) {n}], got {tuple(t.shape)}")
-    return _args.rows(t, tuple(t.shape), name, like)
+def _grouped(t, lead, n, name, dtype, device):
+    """B or C as [..., groups, states] rows, and (groups, batch, token and group strides); a tensor
+    without a group dim has one group."""
+    shape, ranks = t.shape, len(lead) + 1
+    if len(shape) not in (ranks, ranks + 1) or shape[:ranks - 1] != lead or shape[-1] != n:
+        raise ValueError(f"{name} must be [{', '.join(map(str, lead))}, (groups,) {n}], got {tuple(shape)}")
+    t = _args.rows(t, shape, name, dtype, device)
+    stride = t.stride()
+    if len(shape) == ranks:
+        return t, 1, (stride[0], stride[-2], 0)
+    return t, shape[-2], (stride[0], stride[-3], stride[-2])
 
 
 class _Call:
-    """One call's checked arguments: the C struct, and the tensors that it points to."""
+    """One call's checked arguments; ``args`` packs them with the output pointers."""
+
+    __slots__ = ("u", "delta", "A", "B", "C", "D", "z", "bias", "initial", "offsets", "state_shape", "head", "tail")
 
     def __init__(self, u, delta, A, B, C, D, z, delta_bias, softplus, initial, offsets, reverse, one_token=False):
         if one_token:
             _lib.ensure_device(u)
-            _lib.dtype_code(u.dtype)
             if u.dim() != 2:
                 raise ValueError(f"u must be [batch, channels], got {tuple(u.shape)}")
             count, length = u.shape[0], 1
         else:
             count, length, offsets = _args.sequences(u, offsets, "u")
-        shape, d = tuple(u.shape), u.shape[-1]
+        shape, device, dtype = u.shape, u.device, u.dtype
+        code = _lib.dtype_code(dtype)
+        d, lead = shape[-1], shape[:-1]
         if A.dim() != 2 or A.shape[0] != d:
             raise ValueError(f"A must be [{d}, states], got {tuple(A.shape)}")
         n = A.shape[1]
         if n not in STATES:
             raise ValueError(f"ssm_scan takes {', '.join(map(str, STATES))} states, got {n}")
-        dev = u.device
-        u = _args.rows(u, shape, "u", u)
-        delta = _args.rows(delta, shape, "delta", u)
-        z = _args.rows(z, shape, "z", u)
-        B, C = _grouped(B, shape[:-1], n, "B", u), _grouped(C, shape[:-1], n, "C", u)
-        groups = B.shape[-2]
-        if C.shape[-2] != groups or groups == 0 or d % groups:
-            raise ValueError(f"B and C must have the same number of groups, a divisor of {d}; got {groups} and "
-                             f"{C.shape[-2]}")
-        A = _args.fp32(A, (d, n), "A", dev)
-        D = _args.fp32(D, (d,), "D", dev)
-        delta_bias = _args.fp32(delta_bias, (d,), "delta_bias", dev)
-        initial = _args.state(initial, (count, d, n), "initial_state", torch.float32, dev)
-        if initial is not None and initial.requires_grad:
-            initial = initial.detach()
-        self.kept = u, delta, A, B, C, D, z, delta_bias, initial, offsets
+        self.u = u = _args.rows(u, shape, "u", dtype, device)
+        self.delta = delta = _args.rows(delta, shape, "delta", dtype, device)
+        self.z = z = _args.rows(z, shape, "z", dtype, device)
+        self.B, groups, bs = _grouped(B, lead, n, "B", dtype, device)
+        self.C, cgroups, cs = _grouped(C, lead, n, "C", dtype, device)
+        if cgroups != groups or groups == 0 or d % groups:
+            raise ValueError(f"B and C must have the same number of groups, a divisor of {d}; got {groups} and {cgroups}")
+        self.A = A = _args.fp32(A, (d, n), "A", device)
+        self.D = D = _args.fp32(D, (d,), "D", device)
+        self.bias = bias = _args.fp32(delta_bias, (d,), "delta_bias", device)
         self.state_shape = count, d, n
-        ut = u.stride(-2)
-        self.args = _lib.VhSsmScanArgs(
-            u.data_ptr(), delta.data_ptr(), _lib.ptr(z), B.data_ptr(), C.data_ptr(),
-            u.stride(0), ut, delta.stride(0), delta.stride(-2),
-            0 if z is None else z.stride(0), 0 if z is None else z.stride(-2),
-            B.stride(0), 0 if one_token else B.stride(-3), B.stride(-2) if groups > 1 else 0,
-            C.stride(0), 0 if one_token else C.stride(-3), C.stride(-2) if groups > 1 else 0,
-            A.data_ptr(), _lib.ptr(D), _lib.ptr(delta_bias), _lib.ptr(initial), None, None, None, _lib.ptr(offsets),
-            length, _lib.DTYPES[u.dtype], count, d, n, groups, int(bool(softplus)), int(bool(reverse)))
+        self.initial = _args.state(initial, self.state_shape, "initial_state", torch.float32, device)
+        self.offsets = offsets
+        us, ds = u.stride(), delta.stride()
+        zs = _NONE if z is None else z.stride()
+        self.head = (u.data_ptr(), delta.data_ptr(), ptr(z), self.B.data_ptr(), self.C.data_ptr(),
+                     us[0], us[-2], ds[0], ds[-2], zs[0], zs[-2], *bs, *cs,
+                     A.data_ptr(), ptr(D), ptr(bias), ptr(self.initial))
+        self.tail = (ptr(offsets), length, code, count, d, n, groups, 1 if softplus else 0, 1 if reverse else 0)
+
+    def args(self, y=0, final=0, checkpoints=0):
+        return _ARGS.pack(*self.head, y, final, checkpoints, *self.tail)
 
     def forward(self, want_final, want_checkpoints=False):
-        u, initial = self.kept[0], self.kept[8]
+        u, initial = self.u, self.initial
         dev = u.device
         y = torch.empty(u.shape, dtype=u.dtype, device=dev)
         final = torch.empty(self.state_shape, dtype=torch.float32, device=dev) if want_final else None
         if y.numel() == 0:  # no tokens: every state leaves as it entered
             if final is not None:
-                final.copy_(initial) if initial is not None else final.zero_()
+                final.copy_(initial.detach()) if initial is not None else final.zero_()
             return y, final, None
-        lib, a = _lib.load(), self.args
+        lib = _lib.load()
+        args = self.args(y.data_ptr(), ptr(final))
+        nbytes = lib.vh_ssm_scan_fwd_workspace_bytes(args)
+        ws = _args.workspace(nbytes, dev) if nbytes else None
         ck = None
         if want_checkpoints:
-            ck = _args.workspace(lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)), dev)
-        a.y, a.final_state, a.checkpoints = y.data_ptr(), _lib.ptr(final), _lib.ptr(ck)
-        nbytes = lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a))
-        ws = _args.workspace(nbytes, dev) if nbytes else None
-        _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), _lib.ptr(ws), nbytes, _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
+            ck = _args.workspace(lib.vh_ssm_scan_checkpoint_bytes(args), dev)
+            args = self.args(y.data_ptr(), ptr(final), ck.data_ptr())
+        _lib.check(lib.vh_ssm_scan_fwd(args, ptr(ws), nbytes, _lib.stream_handle(dev)), "vh_ssm_scan_fwd")
         return y, final, ck
 
     def backward(self, dy, dfinal, ck, want_initial):
-        u, delta, A, B, C, D, z, delta_bias, _, _ = self.kept
-        dev = u.device
-        like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-        du, dd, dz, dB, dC, dA, dD, dbias = (like(t) for t in (u, delta, z, B, C, A, D, delta_bias))
+        u, dev, dtype = self.u, self.u.device, self.u.dtype
+
+        def like(t, kind):
+            return None if t is None else torch.empty(t.shape, dtype=kind, device=dev)
+
+        du, dd, dz, dB, dC = (like(t, dtype) for t in (u, self.delta, self.z, self.B, self.C))
+        dA, dD, dbias = (like(t, torch.float32) for t in (self.A, self.D, self.bias))
         di = torch.empty(self.state_shape, dtype=torch.float32, device=dev) if want_initial else None
         if u.numel() == 0:
             for t in (dA, dD, dbias):
@@ -96,13 +108,11 @@ class _Call:
                 di.copy_(dfinal) if dfinal is not None else di.zero_()
             return du, dd, dA, dB, dC, dD, dz, dbias, di
         lib = _lib.load()
-        self.args.checkpoints = ck.data_ptr()
-        args = _lib.VhSsmScanBwdArgs(self.args, dy.data_ptr(), _lib.ptr(dfinal), du.data_ptr(), dd.data_ptr(),
-                                     _lib.ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _lib.ptr(dD),
-                                     _lib.ptr(dbias), _lib.ptr(di))
-        ws = _args.workspace(lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(args)), dev)
-        _lib.check(lib.vh_ssm_scan_bwd(ctypes.byref(args), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)),
-                   "vh_ssm_scan_bwd")
+        args = self.args(checkpoints=ck.data_ptr()) + _GRADS.pack(
+            dy.data_ptr(), ptr(dfinal), du.data_ptr(), dd.data_ptr(), ptr(dz), dB.data_ptr(), dC.data_ptr(),
+            dA.data_ptr(), ptr(dD), ptr(dbias), ptr(di))
+        ws = _args.workspace(lib.vh_ssm_scan_bwd_workspace_bytes(args), dev)
+        _lib.check(lib.vh_ssm_scan_bwd(args, ws.data_ptr(), ws.numel(), _lib.stream_handle(dev)), "vh_ssm_scan_bwd")
         return du, dd, dA, dB, dC, dD, dz, dbias, di
 
 
@@ -113,7 +123,7 @@ class _SsmScanFunction(torch.autograd.Function):
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, initial, softplus, want_final, offsets, reverse):
         call = _Call(u, delta, A, B, C, D, z, delta_bias, softplus, initial, offsets, reverse)
         y, final, ck = call.forward(want_final, want_checkpoints=True)
-        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, initial, call.kept[9], ck)
+        ctx.save_for_backward(u, delta, A, B, C, D, z, delta_bias, initial, call.offsets, ck)
         ctx.options = softplus, reverse
         ctx.set_materialize_grads(False)
         return (y, final) if want_final else y
@@ -121,17 +131,16 @@ class _SsmScanFunction(torch.autograd.Function):
     @staticmethod
     @_lib.on_input_device
     def backward(ctx, dy, dfinal=None):
+        if dy is None and dfinal is None:
+            return (None,) * 13
         *inputs, offsets, ck = ctx.saved_tensors
         u, delta, A, B, C, D, z, delta_bias, initial = inputs
         softplus, reverse = ctx.options
-        if dy is None and dfinal is None:
-            return (None,) * 13
         call = _Call(u, delta, A, B, C, D, z, delta_bias, softplus, initial, offsets, reverse)
         dy = torch.zeros(u.shape, dtype=u.dtype, device=u.device) if dy is None else _args.grad_rows(dy)
         dfinal = None if dfinal is None else _args.grad_rows(dfinal)
         grads = call.backward(dy, dfinal, ck, initial is not None and ctx.needs_input_grad[8])
-        grads = [None if g is None else g.view(t.shape).to(t.dtype) for g, t in zip(grads, inputs)]
-        return (*grads, None, None, None, None)
+        return (*map(_args.grad_like, grads, inputs), None, None, None, None)
 
 
 @_lib.on_input_device
@@ -152,7 +161,7 @@ def ssm_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softpl
     final_state) with ``return_final_state``.  Differentiable in every tensor, through y and the
     final state; the sums of the backward run in a fixed order."""
     tensors = (u, delta, A, B, C, D, z, delta_bias, initial_state)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and _needs_grad(*tensors):
         return _SsmScanFunction.apply(*tensors, bool(delta_softplus), bool(return_final_state), seq_offsets,
                                       bool(reverse))
     call = _Call(*tensors[:8], delta_softplus, initial_state, seq_offsets, reverse)
@@ -160,23 +169,20 @@ def ssm_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softpl
     return (y, final) if return_final_state else y
 
 
-@torch.no_grad()
 @_lib.on_input_device
 def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, delta_softplus=False, slots=None,
                   state_out=None):
     """One token of ``B`` cached streams: u, delta, z [B, C]; B, C [B, (groups,) states]; state fp32
     [slots, C, states], advanced in place (or into ``state_out``).  slots: as
-    :func:`short_conv_step`.  Returns y [B, C]."""
+    :func:`short_conv_step`.  Returns y [B, C].  Not differentiable."""
     call = _Call(u, delta, A, B, C, D, z, delta_bias, delta_softplus, None, None, False, one_token=True)
-    u = call.kept[0]
+    device = u.device
     b, d, n = call.state_shape
-    slots = _args.slot_index(slots, b, u.device)
-    state, state_out = _args.cache(state, state_out, (d, n), b, slots, torch.float32, u.device)
-    y = torch.empty((b, d), dtype=u.dtype, device=u.device)
-    if y.numel() == 0:
+    slots = _args.slot_index(slots, b, device)
+    state, state_out = _args.cache(state, state_out, (d, n), b, slots, torch.float32, device)
+    y = torch.empty(u.shape, dtype=u.dtype, device=device)
+    if b * d == 0:
         return y
-    call.args.y = y.data_ptr()
-    _lib.check(_lib.load().vh_ssm_scan_step(ctypes.byref(call.args), state.data_ptr(), state_out.data_ptr(),
-                                            _lib.ptr(slots), state.shape[0], _lib.stream_handle(u.device)),
-               "vh_ssm_scan_step")
+    _lib.check(_lib.load().vh_ssm_scan_step(call.args(y.data_ptr()), state.data_ptr(), state_out.data_ptr(),
+                                            ptr(slots), state.shape[0], _lib.stream_handle(device)), "vh_ssm_scan_step")
     return y
