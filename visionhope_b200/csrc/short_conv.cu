@@ -3,9 +3,12 @@
 //
 //   c_t = bias + sum_k w_k x_{t-K+1+k},   y_t = c_t or silu(c_t)
 //
-// A thread owns V neighbouring channels and walks a run of tokens of one sequence with the last K
-// inputs in registers, so each input is read once, plus K - 1 rows of halo per run.  There is no
-// reuse beyond the window and 2 K flops per element: the kernels are bounded by HBM.
+// A thread owns V neighbouring channels (16 bytes of them in the forward) and walks runs of tokens
+// with the last K inputs in registers, so each input is read once, plus K - 1 rows of halo per run.
+// There is no reuse beyond the window and 2 K flops per element: the kernels are bounded by HBM, and
+// what counts is bytes in flight.  A thread therefore loads four tokens while it computes the four
+// before them, and runs are as long as one wave of threads allows, so that weights, halo and the
+// search for the sequence are paid once for many tokens.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,8 +19,7 @@ namespace vh {
 namespace ssm {
 namespace {
 
-constexpr int kFwdRun = 16;   // tokens a thread walks in the forward
-constexpr int kBwdRun = 32;   // and in the backward (its halo is K - 1 rows on both sides)
+constexpr int kBlock = 4;     // tokens loaded at a time
 constexpr int kThreads = 256;
 
 struct ConvParams {
@@ -28,83 +30,149 @@ struct ConvParams {
     void* y;
     void* final_state;
     Seqs seqs;
-    int32_t channels, silu, vec;
+    int32_t channels, silu, run;  // run: tokens a thread walks
     // backward
     const void *dy, *dfinal;
     void *dx, *dinitial;
     float* partial;  // [blocks][K + 1][channels]
 };
 
+// V channels as pairs (V = 1: the second half is unused).
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
+
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& q, float2 (&v)[kPairs<V>]) {
+    float f[V];
+    q.get(f);
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) v[i] = make_float2(f[2 * i], V > 1 ? f[V > 1 ? 2 * i + 1 : 0] : 0.f);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float2 (&v)[kPairs<V>]) {
+    Pack<T, V> q;
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i % 2 ? v[i / 2].y : v[i / 2].x;
+    q.set(f);
+    *reinterpret_cast<Pack<T, V>*>(p) = q;
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+
 template <int V, int K>
 struct Weights {
-    float w[K][V], b[V];
+    float2 w[K][kPairs<V>], b[kPairs<V>];
     __device__ __forceinline__ void load(const ConvParams& p, int c) {
+        float v[V * K];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
+        for (int i = 0; i < V * K; ++i) v[i] = p.w[(int64_t)c * K + i];
 #pragma unroll
-            for (int k = 0; k < K; ++k) w[k][v] = c + v < p.channels ? p.w[(int64_t)(c + v) * K + k] : 0.f;
-            b[v] = p.bias && c + v < p.channels ? p.bias[c + v] : 0.f;
+        for (int i = 0; i < kPairs<V>; ++i) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) w[k][i] = make_float2(v[2 * i * K + k], V > 1 ? v[(V > 1 ? 2 * i + 1 : 0) * K + k] : 0.f);
+            b[i] = p.bias ? make_float2(p.bias[c + 2 * i], V > 1 ? p.bias[c + (V > 1 ? 2 * i + 1 : 0)] : 0.f)
+                          : make_float2(0.f, 0.f);
         }
+    }
+    // c_t of the window whose newest input is win[K - 1]
+    __device__ __forceinline__ float2 at(const float2 (&win)[K][kPairs<V>], int i) const {
+        float2 a = b[i];
+#pragma unroll
+        for (int k = 0; k < K; ++k) a = ffma2(w[k][i], win[k][i], a);
+        return a;
     }
 };
 
-// Input j of a sequence, j >= -(K - 1): tokens, and before them the initial state.
-template <typename T, int V, int K>
-__device__ __forceinline__ void input_at(const ConvParams& p, const T* x, int64_t step, int s, int c, int64_t j,
-                                         float (&v)[V]) {
-    if (j >= 0) {
-        load_v<V>(x + j * step, c, p.channels, p.vec, v);
-    } else if (p.initial) {
-        load_v<V>(static_cast<const T*>(p.initial) + ((int64_t)s * (K - 1) + (j + K - 1)) * p.channels + c, c,
-                  p.channels, p.vec, v);
-    } else {
+template <int K, int P>
+__device__ __forceinline__ void shift(float2 (&win)[K][P]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = 0.f;
+    for (int k = 0; k + 1 < K; ++k)
+#pragma unroll
+        for (int i = 0; i < P; ++i) win[k][i] = win[k + 1][i];
+}
+
+// The inputs before token j0 of a sequence into win[1 .. K - 1]: tokens, and before them the initial
+// state.
+template <typename T, int V, int K>
+__device__ __forceinline__ void enter(const ConvParams& p, const T* x, int64_t step, int s, int c, int64_t j0,
+                                      float2 (&win)[K][kPairs<V>]) {
+#pragma unroll
+    for (int k = 1; k < K; ++k) {
+        const int64_t j = j0 - K + k;
+        if (j >= 0) unpack<T, V>(load<T, V>(x + j * step), win[k]);
+        else if (p.initial)
+            unpack<T, V>(load<T, V>(static_cast<const T*>(p.initial) + ((int64_t)s * (K - 1) + (j + K - 1)) * p.channels + c),
+                         win[k]);
+        else
+#pragma unroll
+            for (int i = 0; i < kPairs<V>; ++i) win[k][i] = make_float2(0.f, 0.f);
     }
 }
 
+// A block: `cblock` channel groups by kThreads / cblock runs, over channels and slots.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvParams p, int64_t items, int32_t cgroups) {
-    const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    if (item >= items) return;
-    const int64_t slot = item / cgroups;
-    const int c = (int)(item % cgroups) * V;
-    const int s = seq_of_slot(p.seqs, slot, kFwdRun);
-    const Seq seq = seq_at(p.seqs, s);
-    const int64_t j0 = (slot - slot_base(p.seqs, s, seq.row, kFwdRun)) * kFwdRun;
-    if (j0 < 0 || (j0 > 0 && j0 >= seq.len)) return;  // a slot that no sequence, or not this one, needs
-    const int64_t j1 = min(j0 + kFwdRun, seq.len);
-    const T* x = static_cast<const T*>(p.x) + first_row(p.seqs, seq, s, p.xr) + c;
-    const int64_t xs = row_step(p.seqs, p.xr);
-    const Rows yr{p.seqs.length * p.channels, p.channels};
-    T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + c;
-    const int64_t ys = row_step(p.seqs, yr);
+__global__ void __launch_bounds__(kThreads, 2)
+    conv_fwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
+    constexpr int P = kPairs<V>;
+    const int lanes = kThreads / cblock;
+    const int ri = threadIdx.x / cblock;
+    const int c = (blockIdx.x * cblock + threadIdx.x % cblock) * V;
+    if (ri >= lanes || c >= p.channels) return;
     Weights<V, K> wt;
     wt.load(p, c);
-    float win[K][V];  // the last K inputs, newest last
+    const int64_t xs = row_step(p.seqs, p.xr);
+    const Rows yr{p.seqs.length * p.channels, p.channels};
+    const int64_t ys = row_step(p.seqs, yr);
+    for (int64_t slot = (int64_t)blockIdx.y * lanes + ri; slot < slots; slot += (int64_t)gridDim.y * lanes) {
+        const int s = seq_of_slot(p.seqs, slot, p.run);
+        const Seq seq = seq_at(p.seqs, s);
+        const int64_t j0 = (slot - slot_base(p.seqs, s, seq.row, p.run)) * p.run;
+        if (j0 < 0 || (j0 > 0 && j0 >= seq.len)) continue;  // a slot that no sequence, or not this one, needs
+        const int count = (int)min((int64_t)p.run, seq.len - j0);
+        const T* x = static_cast<const T*>(p.x) + first_row(p.seqs, seq, s, p.xr) + c;
+        T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + c + j0 * ys;
+        const T* xj = x + j0 * xs;
+        float2 win[K][P];
+        auto step = [&](const Pack<T, V>& in, int t) {
+            shift(win);
+            unpack<T, V>(in, win[K - 1]);
+            float2 out[P];
 #pragma unroll
-    for (int k = 1; k < K; ++k) input_at<T, V, K>(p, x, xs, s, c, j0 - K + k, win[k]);
-    for (int64_t j = j0; j < j1; ++j) {
+            for (int q = 0; q < P; ++q) {
+                const float2 a = wt.at(win, q);
+                out[q] = p.silu ? fmul2(a, sigmoid2(a)) : a;
+            }
+            store<T, V>(y + t * ys, out);
+        };
+        int t = 0;
+        if (count >= 2 * kBlock) {
+            // a block is loaded while the one before it is computed
+            Pack<T, V> in[2][kBlock];
+            auto fill = [&](Pack<T, V> (&to)[kBlock], int from) {
 #pragma unroll
-        for (int k = 0; k + 1 < K; ++k)
+                for (int i = 0; i < kBlock; ++i) to[i] = load<T, V>(xj + (from + i) * xs);
+            };
+            fill(in[0], 0);
+            enter<T, V, K>(p, x, xs, s, c, j0, win);
+            for (; t + 2 * kBlock <= count; t += 2 * kBlock) {
+                fill(in[1], t + kBlock);
 #pragma unroll
-            for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
-        load_v<V>(x + j * xs, c, p.channels, p.vec, win[K - 1]);
-        float out[V];
+                for (int i = 0; i < kBlock; ++i) step(in[0][i], t + i);
+                if (t + 4 * kBlock <= count) fill(in[0], t + 2 * kBlock);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float a = wt.b[v];
-#pragma unroll
-            for (int k = 0; k < K; ++k) a = fmaf(wt.w[k][v], win[k][v], a);
-            out[v] = p.silu ? a * sigmoid(a) : a;
+                for (int i = 0; i < kBlock; ++i) step(in[1][i], t + kBlock + i);
+            }
+        } else {
+            enter<T, V, K>(p, x, xs, s, c, j0, win);
         }
-        store_v<V>(y + j * ys, c, p.channels, p.vec, out);
-    }
-    if (p.final_state && j1 == seq.len) {
-        // the last K - 1 inputs, which are the initial state's where the sequence is shorter
-        T* f = static_cast<T*>(p.final_state) + (int64_t)s * (K - 1) * p.channels + c;
+        for (; t < count; ++t) step(load<T, V>(xj + t * xs), t);
+        if (p.final_state && j0 + count == seq.len) {
+            // the last K - 1 inputs, which are the initial state's where the sequence is shorter
+            T* f = static_cast<T*>(p.final_state) + (int64_t)s * (K - 1) * p.channels + c;
 #pragma unroll
-        for (int k = 1; k < K; ++k) store_v<V>(f + (k - 1) * p.channels, c, p.channels, p.vec, win[k]);
+            for (int k = 1; k < K; ++k) store<T, V>(f + (k - 1) * p.channels, win[k]);
+        }
     }
 }
 
@@ -117,98 +185,133 @@ __global__ void __launch_bounds__(kThreads) conv_fwd_kernel(const ConvParams p, 
 // their runs in registers, the block in shared memory, and a second kernel over the blocks, all in
 // a fixed order.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
-    // A block: `cblock` channel groups by kThreads / cblock runs.
-    extern __shared__ float red[];
+__global__ void __launch_bounds__(kThreads, 2) conv_bwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
+    constexpr int P = kPairs<V>;
+    __shared__ float red[kThreads];
     const int lanes = kThreads / cblock;
     const int ci = threadIdx.x % cblock, ri = threadIdx.x / cblock;
-    const int cg = blockIdx.x * cblock + ci;
-    const int c = cg * V;
+    const int c = (blockIdx.x * cblock + ci) * V;
     const bool live = ri < lanes && c < p.channels;
-    float dw[K][V], db[V];
+    const float2 zero = make_float2(0.f, 0.f);
+    float2 dw[K][P], db[P];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        db[v] = 0.f;
+    for (int q = 0; q < P; ++q) {
+        db[q] = zero;
 #pragma unroll
-        for (int k = 0; k < K; ++k) dw[k][v] = 0.f;
+        for (int k = 0; k < K; ++k) dw[k][q] = zero;
     }
     if (live) {
         Weights<V, K> wt;
         wt.load(p, c);
+        const int64_t xs = row_step(p.seqs, p.xr);
         const Rows yr{p.seqs.length * p.channels, p.channels};
+        const int64_t ys = row_step(p.seqs, yr);
         for (int64_t slot = (int64_t)blockIdx.y * lanes + ri; slot < slots; slot += (int64_t)gridDim.y * lanes) {
-            const int s = seq_of_slot(p.seqs, slot, kBwdRun);
+            const int s = seq_of_slot(p.seqs, slot, p.run);
             const Seq seq = seq_at(p.seqs, s);
-            const int64_t j0 = (slot - slot_base(p.seqs, s, seq.row, kBwdRun)) * kBwdRun;
+            const int64_t j0 = (slot - slot_base(p.seqs, s, seq.row, p.run)) * p.run;
             if (j0 < 0 || (j0 > 0 && j0 >= seq.len)) continue;
-            const int64_t j1 = min(j0 + kBwdRun, seq.len);
             const T* x = static_cast<const T*>(p.x) + first_row(p.seqs, seq, s, p.xr) + c;
-            const int64_t xs = row_step(p.seqs, p.xr);
-            const int64_t y0 = first_row(p.seqs, seq, s, yr), ys = row_step(p.seqs, yr);
-            const T* dy = static_cast<const T*>(p.dy) + y0 + c;
-            T* dx = static_cast<T*>(p.dx) + y0 + c;
+            const int64_t y0 = first_row(p.seqs, seq, s, yr);
+            const T* dy = static_cast<const T*>(p.dy) + y0 + c + j0 * ys;
+            T* dx = static_cast<T*>(p.dx) + y0 + c + j0 * ys;
             const T* df = p.dfinal ? static_cast<const T*>(p.dfinal) + (int64_t)s * (K - 1) * p.channels + c : nullptr;
-            T* di = p.dinitial ? static_cast<T*>(p.dinitial) + (int64_t)s * (K - 1) * p.channels + c : nullptr;
-            float win[K][V], dc[K][V];
-#pragma unroll
-            for (int k = 1; k < K; ++k) input_at<T, V, K>(p, x, xs, s, c, j0 - K + k, win[k]);
+            T* di = p.dinitial && j0 == 0 ? static_cast<T*>(p.dinitial) + (int64_t)s * (K - 1) * p.channels + c : nullptr;
+            // tokens counted from j0: [0, count) are the run's, [count, ends) belong to the next one
+            const int count = (int)min((int64_t)p.run, seq.len - j0);
+            const int ends = (int)min((int64_t)(count + K - 1), seq.len - j0);
+            const int64_t kept0 = j0 - (seq.len - (K - 1));  // place of token 0 in the final state
+            const T* xj = x + j0 * xs;
+            float2 win[K][P], dc[K][P];
+            enter<T, V, K>(p, x, xs, s, c, j0, win);
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int v = 0; v < V; ++v) dc[k][v] = 0.f;
-            for (int64_t i = j0; i < j1 + K - 1; ++i) {
+                for (int q = 0; q < P; ++q) dc[k][q] = zero;
+            // INNER: the token is the run's and so is the one that it completes
+            auto step = [&](const Pack<T, V>& xin, const Pack<T, V>& gin, int t, auto inner) {
+                constexpr bool kInner = decltype(inner)::value;
+                shift(win);
+                shift(dc);
+                if (kInner || t < ends) {
+                    float2 g[P];
+                    unpack<T, V>(xin, win[K - 1]);
+                    unpack<T, V>(gin, g);
 #pragma unroll
-                for (int k = 0; k + 1 < K; ++k)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        win[k][v] = win[k + 1][v];
-                        dc[k][v] = dc[k + 1][v];
-                    }
-                if (i < seq.len) {
-                    float g[V];
-                    load_v<V>(x + i * xs, c, p.channels, p.vec, win[K - 1]);
-                    load_v<V>(dy + i * ys, c, p.channels, p.vec, g);
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
+                    for (int q = 0; q < P; ++q) {
                         if (p.silu) {
-                            float a = wt.b[v];
-#pragma unroll
-                            for (int k = 0; k < K; ++k) a = fmaf(wt.w[k][v], win[k][v], a);
-                            const float sg = sigmoid(a);
-                            g[v] *= sg * (1.f + a * (1.f - sg));
+                            // silu'(a) = sg (1 + a (1 - sg))
+                            const float2 a = wt.at(win, q), sg = sigmoid2(a);
+                            const float2 r = ffma2(a, fsub2(splat2(1.f), sg), splat2(1.f));
+                            g[q] = fmul2(g[q], fmul2(sg, r));
                         }
-                        dc[K - 1][v] = g[v];
-                        if (i < j1) {
-                            db[v] += g[v];
-#pragma unroll
-                            for (int k = 0; k < K; ++k) dw[k][v] = fmaf(g[v], win[k][v], dw[k][v]);
-                        }
+                        dc[K - 1][q] = g[q];
                     }
+                    if (kInner || t < count)
+#pragma unroll
+                        for (int q = 0; q < P; ++q) {
+                            db[q] = fadd2(db[q], g[q]);
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dw[k][q] = ffma2(g[q], win[k][q], dw[k][q]);
+                        }
                 } else {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) dc[K - 1][v] = 0.f;
+                    for (int q = 0; q < P; ++q) dc[K - 1][q] = zero;
                 }
-                const int64_t j = i - (K - 1);
-                if (j >= j0 || (j < 0 && di)) {
-                    float out[V];
+                const int j = t - (K - 1);
+                if (kInner || j >= 0 || di) {
+                    float2 out[P];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        out[v] = 0.f;
+                    for (int q = 0; q < P; ++q) {
                         // dc[m] is dc_{j+m}: tap K - 1 - m
+                        out[q] = fmul2(wt.w[K - 1][q], dc[0][q]);
 #pragma unroll
-                        for (int m = 0; m < K; ++m) out[v] = fmaf(wt.w[K - 1 - m][v], dc[m][v], out[v]);
+                        for (int m = 1; m < K; ++m) out[q] = ffma2(wt.w[K - 1 - m][q], dc[m][q], out[q]);
                     }
-                    const int64_t kept = j - (seq.len - (K - 1));  // place of input j in the final state
-                    if (df && kept >= 0) {
-                        float f[V];
-                        load_v<V>(df + kept * p.channels, c, p.channels, p.vec, f);
+                    if (!kInner && df && kept0 + j >= 0) {
+                        float2 f[P];
+                        unpack<T, V>(load<T, V>(df + (kept0 + j) * p.channels), f);
 #pragma unroll
-                        for (int v = 0; v < V; ++v) out[v] += f[v];
+                        for (int q = 0; q < P; ++q) out[q] = fadd2(out[q], f[q]);
                     }
-                    if (j >= 0) store_v<V>(dx + j * ys, c, p.channels, p.vec, out);
-                    else store_v<V>(di + (j + K - 1) * p.channels, c, p.channels, p.vec, out);
+                    if (kInner || j >= 0) store<T, V>(dx + j * ys, out);
+                    else store<T, V>(di + (j + K - 1) * p.channels, out);
+                }
+            };
+            auto edge = [&](int from, int to) {
+                for (int t = from; t < to; ++t) {
+                    const int at = min(t, ends - 1);
+                    Pack<T, V> a{}, b{};
+                    if (ends > 0) {
+                        a = load<T, V>(xj + at * xs);
+                        b = load<T, V>(dy + at * ys);
+                    }
+                    step(a, b, t, std::false_type{});
+                }
+            };
+            const int total = count + K - 1;
+            int t = min(K - 1, total);
+            edge(0, t);
+            if (t + 2 * kBlock <= count) {  // what these complete is the run's, and not in the final state
+                Pack<T, V> xin[2][kBlock], gin[2][kBlock];
+                auto fill = [&](Pack<T, V> (&a)[kBlock], Pack<T, V> (&b)[kBlock], int from) {
+#pragma unroll
+                    for (int i = 0; i < kBlock; ++i) {
+                        a[i] = load<T, V>(xj + (from + i) * xs);
+                        b[i] = load<T, V>(dy + (from + i) * ys);
+                    }
+                };
+                fill(xin[0], gin[0], t);
+                for (; t + 2 * kBlock <= count; t += 2 * kBlock) {
+                    fill(xin[1], gin[1], t + kBlock);
+#pragma unroll
+                    for (int i = 0; i < kBlock; ++i) step(xin[0][i], gin[0][i], t + i, std::true_type{});
+                    if (t + 4 * kBlock <= count) fill(xin[0], gin[0], t + 2 * kBlock);
+#pragma unroll
+                    for (int i = 0; i < kBlock; ++i) step(xin[1][i], gin[1][i], t + kBlock + i, std::true_type{});
                 }
             }
+            edge(t, total);
         }
     }
     // the block's sums: one value of every thread at a time, added over the runs in order
@@ -216,9 +319,10 @@ __global__ void __launch_bounds__(kThreads) conv_bwd_kernel(const ConvParams p, 
     for (int k = 0; k <= K; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            red[threadIdx.x] = k < K ? dw[k < K ? k : 0][v] : db[v];
+            const float2 a = k < K ? dw[k < K ? k : 0][v / 2] : db[v / 2];
+            red[threadIdx.x] = v % 2 ? a.y : a.x;
             __syncthreads();
-            if (ri == 0 && live && c + v < p.channels) {
+            if (ri == 0 && live) {
                 float sum = 0.f;
                 for (int r = 0; r < lanes; ++r) sum += red[r * cblock + ci];
                 p.partial[((int64_t)blockIdx.y * (K + 1) + k) * p.channels + c + v] = sum;
@@ -249,33 +353,36 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const T* __restrict
                                                              const T* state, T* state_out,
                                                              const int32_t* __restrict__ index, int32_t slots,
                                                              T* __restrict__ y, int64_t items, int32_t cgroups,
-                                                             int32_t channels, int32_t silu, int32_t vec) {
+                                                             int32_t channels, int32_t silu) {
+    constexpr int P = kPairs<V>;
     const int64_t item = (int64_t)blockIdx.x * kThreads + threadIdx.x;
     if (item >= items) return;
     const int s = (int)(item / cgroups), c = (int)(item % cgroups) * V;
     const int slot = index ? index[s] : s;
-    float out[V];
+    float2 out[P];
     if (slot < 0 || slot >= slots) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = 0.f;
-        store_v<V>(y + (int64_t)s * channels + c, c, channels, vec, out);
+        for (int q = 0; q < P; ++q) out[q] = make_float2(0.f, 0.f);
+        store<T, V>(y + (int64_t)s * channels + c, out);
         return;
     }
-    float win[K][V];
+    ConvParams p{};
+    p.w = w; p.bias = bias;
+    Weights<V, K> wt;
+    wt.load(p, c);
     const int64_t at = (int64_t)slot * (K - 1) * channels + c;
+    float2 win[K][P];
 #pragma unroll
-    for (int k = 0; k + 1 < K; ++k) load_v<V>(state + at + (int64_t)k * channels, c, channels, vec, win[k]);
-    load_v<V>(x + s * x_stride + c, c, channels, vec, win[K - 1]);
+    for (int k = 0; k + 1 < K; ++k) unpack<T, V>(load<T, V>(state + at + (int64_t)k * channels), win[k]);
+    unpack<T, V>(load<T, V>(x + s * x_stride + c), win[K - 1]);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float a = bias && c + v < channels ? bias[c + v] : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) a = fmaf(c + v < channels ? w[(int64_t)(c + v) * K + k] : 0.f, win[k][v], a);
-        out[v] = silu ? a * sigmoid(a) : a;
+    for (int q = 0; q < P; ++q) {
+        const float2 a = wt.at(win, q);
+        out[q] = silu ? fmul2(a, sigmoid2(a)) : a;
     }
-    store_v<V>(y + (int64_t)s * channels + c, c, channels, vec, out);
+    store<T, V>(y + (int64_t)s * channels + c, out);
 #pragma unroll
-    for (int k = 1; k < K; ++k) store_v<V>(state_out + at + (int64_t)(k - 1) * channels, c, channels, vec, win[k]);
+    for (int k = 1; k < K; ++k) store<T, V>(state_out + at + (int64_t)(k - 1) * channels, win[k]);
 }
 
 template <typename F>
@@ -296,9 +403,15 @@ int with_taps(int taps, F&& f) {
         default: return f(std::integral_constant<int, 8>{});
     }
 }
-template <typename F>
-int with_width(bool vec, F&& f) {
-    return vec ? f(std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 1>{});
+// V channels at a time: `bytes` (16, 8 or 0, one channel) is what every row's start is a multiple
+// of; MOST bytes an access.
+template <typename T, int MOST, typename F>
+int with_width(int bytes, F&& f) {
+    if constexpr (MOST >= 16) {
+        if (bytes == 16) return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
+    }
+    if (bytes >= 8) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{});
+    return f(std::integral_constant<int, 1>{});
 }
 
 int check_conv(const char* what, const vh_short_conv_args* a) {
@@ -318,13 +431,17 @@ int check_conv(const char* what, const vh_short_conv_args* a) {
     return 0;
 }
 
-// Four channels at a time wherever every row starts on a boundary of four elements.
-bool conv_vec(const vh_short_conv_args* a, std::initializer_list<const void*> more) {
-    const size_t es = 4 * dtype_size(a->dtype);
-    bool v = a->channels % 4 == 0 && a->x_batch_stride % 4 == 0 && a->x_token_stride % 4 == 0;
-    for (const void* t : {a->x, a->initial_state}) v = v && (!t || aligned(t, es));
-    for (const void* t : more) v = v && (!t || aligned(t, es));
-    return v;
+// The widest access, in bytes, that every row's start and the channel count are multiples of.
+int conv_bytes(const vh_short_conv_args* a, std::initializer_list<const void*> more) {
+    const int64_t es = (int64_t)dtype_size(a->dtype);
+    for (int bytes : {16, 8}) {
+        bool v = a->channels * es % bytes == 0 && a->x_token_stride * es % bytes == 0 &&
+                 (a->seq_offsets || a->x_batch_stride * es % bytes == 0);
+        for (const void* t : {a->x, a->initial_state}) v = v && (!t || aligned(t, bytes));
+        for (const void* t : more) v = v && (!t || aligned(t, bytes));
+        if (v) return bytes;
+    }
+    return 0;
 }
 
 ConvParams conv_params(const vh_short_conv_args* a) {
@@ -336,20 +453,36 @@ ConvParams conv_params(const vh_short_conv_args* a) {
     return p;
 }
 
-struct BwdPlan {
+// A launch: blocks of `cblock` channel groups by runs; gy blocks share the slots.  Two blocks fit
+// an SM, and a run is as long as one wave of them needs to cover all tokens (8 at least).
+struct Plan {
     int64_t slots;
-    int cgroups, cblock, gx, gy;
+    int cblock, gx, gy, run;
 };
-BwdPlan bwd_plan(const vh_short_conv_args* a, int width) {
-    BwdPlan b;
-    b.slots = slot_total(a->seq_offsets != nullptr, a->length, a->batch, kBwdRun);
-    b.cgroups = (a->channels + width - 1) / width;
-    b.cblock = std::min(b.cgroups, 64);
-    b.gx = (b.cgroups + b.cblock - 1) / b.cblock;
-    const int lanes = kThreads / b.cblock;
-    const int64_t want = (b.slots + lanes - 1) / lanes;
-    b.gy = (int)std::max<int64_t>(1, std::min<int64_t>(want, (8 * 148 + b.gx - 1) / b.gx));
+Plan plan(const vh_short_conv_args* a, int width) {
+    Plan b;
+    const bool packed = a->seq_offsets != nullptr;
+    const int cgroups = (a->channels + width - 1) / width;
+    b.cblock = std::min(cgroups, 16);  // 16 neighbouring groups fill the memory's lines
+    b.gx = (cgroups + b.cblock - 1) / b.cblock;
+    const int64_t lanes = kThreads / b.cblock;
+    const int64_t fit = std::max<int64_t>(1, 2 * sm_count() / b.gx);
+    const int64_t tokens = packed ? a->length : a->length * a->batch;
+    const int64_t want = (tokens + fit * lanes - 1) / (fit * lanes);
+    b.run = (int)std::min<int64_t>(std::max<int64_t>((want + 7) / 8 * 8, 8), 1 << 20);
+    if (!packed) {  // equal shares of every sequence
+        const int64_t runs = slots_per_seq(a->length, b.run);
+        b.run = (int)std::max<int64_t>(((a->length + runs - 1) / runs + 7) / 8 * 8, 8);
+    }
+    b.slots = slot_total(packed, a->length, a->batch, b.run);
+    b.gy = (int)std::max<int64_t>(1, std::min<int64_t>((b.slots + lanes - 1) / lanes, 2 * fit));
     return b;
+}
+// The backward's sums over blocks hold as many rows as the largest of its launches has blocks.
+int64_t bwd_rows(const vh_short_conv_args* a) {
+    int64_t rows = 0;
+    for (int width : {1, 2, 4}) rows = std::max<int64_t>(rows, plan(a, width).gy);
+    return rows;
 }
 
 }  // namespace
@@ -363,18 +496,16 @@ extern "C" int vh_short_conv_fwd(const vh_short_conv_args* a, vh_stream_t stream
     clear_error();
     if (int rc = check_conv("vh_short_conv_fwd", a)) return rc;
     ConvParams p = conv_params(a);
-    p.vec = conv_vec(a, {a->y, a->final_state});
+    const int bytes = conv_bytes(a, {a->y, a->final_state});
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width(p.vec, [&](auto width) {
+        return with_width<T, 16>(bytes, [&](auto width) {
             constexpr int V = decltype(width)::value;
-            const int cgroups = (a->channels + V - 1) / V;
-            const int64_t items = slot_total(a->seq_offsets != nullptr, a->length, a->batch, kFwdRun) * cgroups;
-            const int64_t blocks = (items + kThreads - 1) / kThreads;
-            if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_short_conv_fwd: too many elements");
+            const Plan b = plan(a, V);
+            p.run = b.run;
             return with_taps(a->taps, [&](auto taps) {
                 conv_fwd_kernel<T, V, decltype(taps)::value>
-                    <<<(int)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, items, cgroups);
+                    <<<dim3(b.gx, b.gy), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, b.slots, b.cblock);
                 return launch_status("short convolution");
             });
         });
@@ -383,8 +514,7 @@ extern "C" int vh_short_conv_fwd(const vh_short_conv_args* a, vh_stream_t stream
 
 extern "C" int64_t vh_short_conv_bwd_workspace_bytes(const vh_short_conv_args* a) {
     if (!a || a->batch <= 0 || a->channels <= 0 || a->length < 0 || a->taps < 2 || a->taps > 8) return 0;
-    const int64_t rows = std::max(bwd_plan(a, 4).gy, bwd_plan(a, 1).gy);
-    return rows * (a->taps + 1) * a->channels * 4;
+    return bwd_rows(a) * (a->taps + 1) * a->channels * 4;
 }
 
 extern "C" int vh_short_conv_bwd(const vh_short_conv_args* a, const void* grad_y, const void* grad_final, void* grad_x,
@@ -406,20 +536,20 @@ extern "C" int vh_short_conv_bwd(const vh_short_conv_args* a, const void* grad_y
     if (workspace_bytes < vh_short_conv_bwd_workspace_bytes(a) || !aligned(workspace, 4))
         return fail(VH_E_ARG, "vh_short_conv_bwd: workspace too small");
     ConvParams p = conv_params(a);
-    p.vec = conv_vec(a, {grad_y, grad_final, grad_x, grad_initial});
+    const int bytes = conv_bytes(a, {grad_y, grad_final, grad_x, grad_initial});
     p.dy = grad_y; p.dfinal = grad_final; p.dx = grad_x; p.dinitial = grad_initial;
     p.partial = static_cast<float*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int blocks = 0;
     const int rc = with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width(p.vec, [&](auto width) {
+        return with_width<T, 8>(bytes, [&](auto width) {
             constexpr int V = decltype(width)::value;
-            const BwdPlan b = bwd_plan(a, V);
+            const Plan b = plan(a, V);
+            p.run = b.run;
             blocks = b.gy;
             return with_taps(a->taps, [&](auto taps) {
-                conv_bwd_kernel<T, V, decltype(taps)::value>
-                    <<<dim3(b.gx, b.gy), kThreads, kThreads * sizeof(float), st>>>(p, b.slots, b.cblock);
+                conv_bwd_kernel<T, V, decltype(taps)::value><<<dim3(b.gx, b.gy), kThreads, 0, st>>>(p, b.slots, b.cblock);
                 return launch_status("short convolution backward");
             });
         });
@@ -445,10 +575,10 @@ extern "C" int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t
         return fail(VH_E_ALIGN, "vh_short_conv_step: misaligned pointers");
     if (slots <= 0 || (!slots_index && slots < batch))
         return fail(VH_E_SHAPE, "vh_short_conv_step: %d slots for %d streams", slots, batch);
-    const bool vec = conv_vec(&a, {state, (const void*)state_out, (const void*)y});
+    const int bytes = conv_bytes(&a, {state, (const void*)state_out, (const void*)y});
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width(vec, [&](auto width) {
+        return with_width<T, 8>(bytes, [&](auto width) {
             constexpr int V = decltype(width)::value;
             const int cgroups = (channels + V - 1) / V;
             const int64_t items = (int64_t)batch * cgroups;
@@ -458,7 +588,7 @@ extern "C" int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t
                 conv_step_kernel<T, V, decltype(k)::value><<<(int)blocks, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
                     static_cast<const T*>(x), x_batch_stride, weight, bias, static_cast<const T*>(state),
                     static_cast<T*>(state_out), slots_index, slots, static_cast<T*>(y), items, cgroups, channels,
-                    activation, vec);
+                    activation);
                 return launch_status("short convolution step");
             });
         });

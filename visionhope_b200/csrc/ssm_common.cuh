@@ -9,6 +9,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "f32x2.cuh"
 
@@ -119,6 +121,77 @@ __device__ __forceinline__ void store_v(T* p, int c, int end, bool vec, const fl
     }
 }
 
+// V elements as they lie in memory, in whole words (separate 16-bit values would take a register
+// each).
+__device__ __forceinline__ float2 halves(uint32_t w, __nv_bfloat16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 halves(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ uint32_t join(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t join(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T, int V>
+struct Pack {
+    static constexpr int kBytes = sizeof(T) * V;
+    using Word = std::conditional_t<kBytes == 2, uint16_t, std::conditional_t<kBytes == 4, uint32_t,
+                 std::conditional_t<kBytes == 8, uint2, uint4>>>;
+    static_assert(kBytes == 2 || kBytes == 4 || kBytes == 8 || kBytes == 16, "one access");
+    Word w;
+    __device__ __forceinline__ uint32_t word(int i) const {
+        if constexpr (kBytes <= 4) return w;
+        else if constexpr (kBytes == 8) return i == 0 ? w.x : w.y;
+        else return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+    }
+    __device__ __forceinline__ void set_word(int i, uint32_t v) {
+        if constexpr (kBytes <= 4) w = (Word)v;
+        else if constexpr (kBytes == 8) { if (i == 0) w.x = v; else w.y = v; }
+        else { if (i == 0) w.x = v; else if (i == 1) w.y = v; else if (i == 2) w.z = v; else w.w = v; }
+    }
+    __device__ __forceinline__ void get(float (&v)[V]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = __uint_as_float(word(i));
+        } else if constexpr (V == 1) {
+            v[0] = halves(w, T{}).x;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 f = halves(word(i), T{});
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float (&v)[V]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) set_word(i, __float_as_uint(v[i]));
+        } else if constexpr (V == 1) {
+            set_word(0, join(v[0], 0.f, T{}));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) set_word(i, join(v[2 * i], v[2 * i + 1], T{}));
+        }
+    }
+    // `left`: how many of them exist (vec: the pointer is aligned and all do); missing ones repeat
+    // the last
+    __device__ __forceinline__ void load(const T* p, int left, bool vec) {
+        if (vec) {
+            *this = *reinterpret_cast<const Pack*>(p);
+        } else {
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = to_f(p[max(min(i, left - 1), 0)]);
+            set(v);  // exact: they came from T
+        }
+    }
+};
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -154,6 +227,16 @@ __device__ __forceinline__ float exp2_fma(float s, float a) {
 }
 
 __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + ex2(-kLog2e * x)); }
+// Two of them with one reciprocal, 1 / a = b / (a b): three operations of the special-function unit
+// in place of four.  exp(-x) is held to 2^60, so that a b is finite: below x = -41 the result is
+// 2^-60.
+__device__ __forceinline__ float2 sigmoid2(float2 x) {
+    const float2 m = fmul2(x, splat2(-kLog2e));
+    constexpr float kMost = 1.152921504606846976e18f;
+    const float2 d = fadd2(make_float2(fminf(ex2(m.x), kMost), fminf(ex2(m.y), kMost)), splat2(1.f));
+    const float r = __fdividef(1.f, d.x * d.y);
+    return make_float2(r * d.y, r * d.x);
+}
 
 // log(1 + exp(x)) without cancellation on either side: max(x, 0) + log1p(e), e = exp(-|x|) in
 // (0, 1], log1p(e) = e r(e) with r of degree 8 fitted for the relative error by Lawson's

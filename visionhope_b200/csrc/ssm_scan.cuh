@@ -77,25 +77,6 @@ struct LaneElems {
     }
 };
 
-// V elements as they lie in memory.
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
-    T e[V];
-    // `left`: how many of them exist (vec: the pointer is aligned and all do); missing ones repeat
-    // the last
-    __device__ __forceinline__ void load(const T* p, int left, bool vec) {
-        if (vec) {
-            *this = *reinterpret_cast<const Pack*>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) e[i] = p[max(min(i, left - 1), 0)];
-        }
-    }
-    __device__ __forceinline__ void get(float (&v)[V]) const {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = to_f(e[i]);
-    }
-};
 // The same into shared memory, asynchronously where the copy is one of 4, 8 or 16 bytes.  Issued a
 // group or two ahead of its use it takes no registers; plain loads ahead of their use do, and were
 // moved next to it by the compiler (the forward then waited for memory in 4 of 10 cycles).
