@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kBlock = 4;     // tokens loaded at a time
 constexpr int kThreads = 256;
+constexpr int kFwdBlocks = 3, kBwdBlocks = 2;  // blocks an SM holds
 
 struct ConvParams {
     const void* x;
@@ -112,7 +113,7 @@ __device__ __forceinline__ void enter(const ConvParams& p, const T* x, int64_t s
 
 // A block: `cblock` channel groups by kThreads / cblock runs, over channels and slots.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, kFwdBlocks)
     conv_fwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
     constexpr int P = kPairs<V>;
     const int lanes = kThreads / cblock;
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 // their runs in registers, the block in shared memory, and a second kernel over the blocks, all in
 // a fixed order.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads, 2) conv_bwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
+__global__ void __launch_bounds__(kThreads, kBwdBlocks) conv_bwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
     constexpr int P = kPairs<V>;
     __shared__ float red[kThreads];
     const int lanes = kThreads / cblock;
@@ -453,20 +454,20 @@ ConvParams conv_params(const vh_short_conv_args* a) {
     return p;
 }
 
-// A launch: blocks of `cblock` channel groups by runs; gy blocks share the slots.  Two blocks fit
-// an SM, and a run is as long as one wave of them needs to cover all tokens (8 at least).
+// A launch: blocks of `cblock` channel groups by runs; gy blocks share the slots.  A run
+// is as long as one wave of per_sm blocks an SM needs to cover all tokens (8 at least).
 struct Plan {
     int64_t slots;
     int cblock, gx, gy, run;
 };
-Plan plan(const vh_short_conv_args* a, int width) {
+Plan plan(const vh_short_conv_args* a, int width, int per_sm) {
     Plan b;
     const bool packed = a->seq_offsets != nullptr;
     const int cgroups = (a->channels + width - 1) / width;
     b.cblock = std::min(cgroups, 16);  // 16 neighbouring groups fill the memory's lines
     b.gx = (cgroups + b.cblock - 1) / b.cblock;
     const int64_t lanes = kThreads / b.cblock;
-    const int64_t fit = std::max<int64_t>(1, 2 * sm_count() / b.gx);
+    const int64_t fit = std::max<int64_t>(1, (int64_t)per_sm * sm_count() / b.gx);
     const int64_t tokens = packed ? a->length : a->length * a->batch;
     const int64_t want = (tokens + fit * lanes - 1) / (fit * lanes);
     b.run = (int)std::min<int64_t>(std::max<int64_t>((want + 7) / 8 * 8, 8), 1 << 20);
@@ -481,7 +482,7 @@ Plan plan(const vh_short_conv_args* a, int width) {
 // The backward's sums over blocks hold as many rows as the largest of its launches has blocks.
 int64_t bwd_rows(const vh_short_conv_args* a) {
     int64_t rows = 0;
-    for (int width : {1, 2, 4}) rows = std::max<int64_t>(rows, plan(a, width).gy);
+    for (int width : {1, 2, 4}) rows = std::max<int64_t>(rows, plan(a, width, kBwdBlocks).gy);
     return rows;
 }
 
@@ -499,9 +500,9 @@ extern "C" int vh_short_conv_fwd(const vh_short_conv_args* a, vh_stream_t stream
     const int bytes = conv_bytes(a, {a->y, a->final_state});
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width<T, 16>(bytes, [&](auto width) {
+        return with_width<T, 8>(bytes, [&](auto width) {
             constexpr int V = decltype(width)::value;
-            const Plan b = plan(a, V);
+            const Plan b = plan(a, V, kFwdBlocks);
             p.run = b.run;
             return with_taps(a->taps, [&](auto taps) {
                 conv_fwd_kernel<T, V, decltype(taps)::value>
@@ -545,7 +546,7 @@ extern "C" int vh_short_conv_bwd(const vh_short_conv_args* a, const void* grad_y
         using T = decltype(t);
         return with_width<T, 8>(bytes, [&](auto width) {
             constexpr int V = decltype(width)::value;
-            const Plan b = plan(a, V);
+            const Plan b = plan(a, V, kBwdBlocks);
             p.run = b.run;
             blocks = b.gy;
             return with_taps(a->taps, [&](auto taps) {

@@ -241,49 +241,82 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
     }
 }
 
-// One token per stream: a thread owns four states of one channel, N / 4 threads a channel.
+// One token per stream.  NL = N / 4 lanes share NL channels: a lane loads u, delta and z of its own
+// channel and finishes its y, and holds four states of all NL channels; s and s u of a channel
+// come from its lane, y's sums go back there.  A block keeps its channels' rates over several
+// streams where registers allow.
 template <typename T, int NL>
-__global__ void __launch_bounds__(256) scan_step_kernel(const ScanParams p, const float* state,
-                                                        float* state_out,
-                                                        const int32_t* __restrict__ index, int32_t slots, int64_t rows) {
+__global__ void __launch_bounds__(256, NL <= 4 ? 4 : 1) scan_step_kernel(const ScanParams p, const float* state, float* state_out,
+                                                        const int32_t* __restrict__ index, int32_t slots) {
     constexpr int N = 4 * NL;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = i / NL;  // (stream, channel); whole groups of NL lanes are in or out together
-    const int n0 = 4 * (int)(i % NL);
-    const bool live = row < rows;
-    const int s = live ? (int)(row / p.channels) : 0, c = live ? (int)(row % p.channels) : 0;
-    const int slot = !live ? -1 : (index ? index[s] : s);
-    const bool known = slot >= 0 && slot < slots;
-    float part = 0.f, uu = 0.f, zz = 0.f;
-    if (known) {
-        const int g = c / p.per_group;
-        uu = to_f(static_cast<const T*>(p.u)[s * p.ur.batch + c]);
-        float st = to_f(static_cast<const T*>(p.delta)[s * p.dr.batch + c]) + (p.delta_bias ? p.delta_bias[c] : 0.f);
-        if (p.z) zz = to_f(static_cast<const T*>(p.z)[s * p.zr.batch + c]);
+    constexpr bool kKeep = NL <= 4;
+    const int c = blockIdx.x * 256 + threadIdx.x, lane = threadIdx.x & 31;
+    const int j = lane % NL, first = c - j;
+    const bool live = c < p.channels;
+    const int group = min(c, p.channels - 1) / p.per_group;
+    const float bias = live && p.delta_bias ? p.delta_bias[c] : 0.f, skip = live && p.d_skip ? p.d_skip[c] : 0.f;
+    float a2[kKeep ? NL : 1][4];
+    auto rates = [&](int i, float (&v)[4]) {
+        lds4(p.a + (int64_t)min(first + i, p.channels - 1) * N + 4 * j, v);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[n] = to_log2(v[n]);
+    };
+    if constexpr (kKeep)
+#pragma unroll
+        for (int i = 0; i < NL; ++i) rates(i, a2[i]);
+    for (int s = blockIdx.y; s < p.seqs.count; s += gridDim.y) {
+        const int slot = index ? index[s] : s;
+        if (slot < 0 || slot >= slots) {  // the same for the whole block
+            if (live) static_cast<T*>(p.y)[(int64_t)s * p.channels + c] = from_f<T>(0.f);
+            continue;
+        }
+        const int64_t at = (int64_t)slot * p.channels * N + 4 * j;
+        float h[NL][4];
+#pragma unroll
+        for (int i = 0; i < NL; ++i) lds4(state + at + (int64_t)min(first + i, p.channels - 1) * N, h[i]);
+        float uu = 0.f, st = 0.f, zz = 0.f;
+        if (live) {
+            uu = to_f(static_cast<const T*>(p.u)[s * p.ur.batch + c]);
+            st = to_f(static_cast<const T*>(p.delta)[s * p.dr.batch + c]) + bias;
+            if (p.z) zz = to_f(static_cast<const T*>(p.z)[s * p.zr.batch + c]);
+        }
         if (p.softplus) st = softplus(st);
-        float av[4], hv[4], bv[4], cv[4];
-        lds4(p.a + (int64_t)c * N + n0, av);
-        lds4(state + ((int64_t)slot * p.channels + c) * N + n0, hv);
-        load_v<4>(static_cast<const T*>(p.b) + s * p.br.batch + g * p.bg + n0, 0, 4, p.vec_bc, bv);
-        load_v<4>(static_cast<const T*>(p.c) + s * p.cr.batch + g * p.cg + n0, 0, 4, p.vec_bc, cv);
         const float pu = st * uu;
+        const T *pb = static_cast<const T*>(p.b) + s * p.br.batch, *pc = static_cast<const T*>(p.c) + s * p.cr.batch;
+        float y[NL], bv[4], cv[4];
+        int held = -1;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            hv[n] = fmaf(pu, bv[n], exp2_fma(st, to_log2(av[n])) * hv[n]);
-            part = fmaf(cv[n], hv[n], part);
+        for (int i = 0; i < NL; ++i) {
+            const float si = __shfl_sync(0xffffffffu, st, i, NL), pi = __shfl_sync(0xffffffffu, pu, i, NL);
+            const int gi = p.groups == 1 ? 0 : __shfl_sync(0xffffffffu, group, i, NL);
+            if (gi != held) {  // a group of lanes may straddle two groups of B and C
+                load_v<4>(pb + gi * p.bg + 4 * j, 0, 4, p.vec_bc, bv);
+                load_v<4>(pc + gi * p.cg + 4 * j, 0, 4, p.vec_bc, cv);
+                held = gi;
+            }
+            float av[4];
+            if constexpr (kKeep) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) av[n] = a2[i][n];
+            } else {
+                rates(i, av);
+            }
+            y[i] = 0.f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                h[i][n] = fmaf(exp2_fma(si, av[n]), h[i][n], pi * bv[n]);
+                y[i] = fmaf(cv[n], h[i][n], y[i]);
+            }
+            if (first + i < p.channels)
+                *reinterpret_cast<float4*>(state_out + at + (int64_t)(first + i) * N) =
+                    make_float4(h[i][0], h[i][1], h[i][2], h[i][3]);
         }
-        *reinterpret_cast<float4*>(state_out + ((int64_t)slot * p.channels + c) * N + n0) =
-            make_float4(hv[0], hv[1], hv[2], hv[3]);
-    }
-#pragma unroll
-    for (int o = NL / 2; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    if (live && n0 == 0) {
-        float out = 0.f;
-        if (known) {
-            out = fmaf(p.d_skip ? p.d_skip[c] : 0.f, uu, part);
+        reduce_scatter<NL, NL, 1>(y, lane);
+        if (live) {
+            float out = fmaf(skip, uu, y[0]);
             if (p.z) out *= zz * sigmoid(zz);
+            static_cast<T*>(p.y)[(int64_t)s * p.channels + c] = from_f<T>(out);
         }
-        static_cast<T*>(p.y)[(int64_t)s * p.channels + c] = from_f<T>(out);
     }
 }
 
@@ -477,14 +510,14 @@ extern "C" int vh_ssm_scan_step(const vh_ssm_scan_args* a, const float* state, f
         return fail(VH_E_SHAPE, "vh_ssm_scan_step: %d slots for %d streams", slots, a->batch);
     ScanParams p;
     fill_scan_params(a, &p);
-    const int64_t rows = (int64_t)a->batch * a->channels;
-    const int64_t blocks = (rows * (a->states / 4) + 255) / 256;
-    if (blocks > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_step: too many channels");
+    // streams share a block once there are four blocks an SM
+    const int gx = (a->channels + 255) / 256;
+    const int gy = std::min<int>(a->batch, std::max(1, 4 * sm_count() / gx));
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
         return with_states(a->states, [&](auto nl) {
-            scan_step_kernel<T, decltype(nl)::value><<<(int)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                p, state, state_out, slots_index, slots, rows);
+            scan_step_kernel<T, decltype(nl)::value><<<dim3(gx, gy), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+                p, state, state_out, slots_index, slots);
             return launch_status("selective scan step");
         });
     });
