@@ -38,23 +38,11 @@ struct ConvParams {
     float* partial;  // [blocks][K + 1][channels]
 };
 
-// V channels as pairs (V = 1: the second half is unused).
-template <int V>
-constexpr int kPairs = (V + 1) / 2;
-
-template <typename T, int V>
-__device__ __forceinline__ void unpack(const Pack<T, V>& q, float2 (&v)[kPairs<V>]) {
-    float f[V];
-    q.get(f);
-#pragma unroll
-    for (int i = 0; i < kPairs<V>; ++i) v[i] = make_float2(f[2 * i], V > 1 ? f[V > 1 ? 2 * i + 1 : 0] : 0.f);
-}
 template <typename T, int V>
 __device__ __forceinline__ void store(T* p, const float2 (&v)[kPairs<V>]) {
     Pack<T, V> q;
     float f[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i % 2 ? v[i / 2].y : v[i / 2].x;
+    from_pairs<V>(v, f);
     q.set(f);
     *reinterpret_cast<Pack<T, V>*>(p) = q;
 }

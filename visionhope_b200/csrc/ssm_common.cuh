@@ -192,6 +192,26 @@ struct Pack {
     }
 };
 
+// V values as pairs for the packed arithmetic (V = 1: the second half repeats the first).
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
+template <int V>
+__device__ __forceinline__ void to_pairs(const float (&f)[V], float2 (&v)[kPairs<V>]) {
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) v[i] = make_float2(f[2 * i], f[V > 1 ? 2 * i + 1 : 0]);
+}
+template <int V>
+__device__ __forceinline__ void from_pairs(const float2 (&v)[kPairs<V>], float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i % 2 ? v[i / 2].y : v[i / 2].x;
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& q, float2 (&v)[kPairs<V>]) {
+    float f[V];
+    q.get(f);
+    to_pairs<V>(f, v);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -278,20 +298,6 @@ __device__ __forceinline__ float2 exp2_fma2(float2 s, float2 a) {
                        __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
 }
 
-// softplus of n values, two at a time where there are two
-template <int N>
-__device__ __forceinline__ void softplus_n(float (&v)[N]) {
-    if constexpr (N == 1) {
-        v[0] = softplus(v[0]);
-    } else {
-#pragma unroll
-        for (int k = 0; k < N; k += 2) {
-            const float2 r = softplus2(make_float2(v[k], v[k + 1]));
-            v[k] = r.x;
-            v[k + 1] = r.y;
-        }
-    }
-}
 __device__ __forceinline__ float2 ex2_2(float2 x) { return make_float2(ex2(x.x), ex2(x.y)); }
 
 // A in the exponential's base: log2(e) A, kept finite so that a step of zero leaves the state as

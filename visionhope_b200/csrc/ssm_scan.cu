@@ -65,7 +65,9 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     FwdSmem<T, NL>& sm = reinterpret_cast<FwdSmem<T, NL>*>(smem)[warp];
     const int64_t unit = w.slot * tiles + w.tile;
     float2 a2[8], h[8];
-    float v[16], sum[CE];
+    constexpr int P = kPairs<CE>;
+    float v[16];
+    float2 sum[P];
     const float top_a = load_rates<NL>(p, c0, cend, j, v);
     pair_up(v, a2);
     ch.move(w.t0);
@@ -88,14 +90,14 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < CE; ++i) sum[i] = 0.f;
+    for (int i = 0; i < P; ++i) sum[i] = make_float2(0.f, 0.f);
 
     if constexpr (OWN) {
         pair_up(v, h);
         int buf = 0;
         for (int64_t t = w.t0; some && t < w.t1; t += kGroup, buf ^= 1) {
             cp_async_wait<kAhead - 1>();
-            const float top = ch.template stage<true>(sm.raw[slot], w.t1 - t, sm.st[buf], sum);
+            const float top = ch.template stage<true, true>(sm.raw[slot], w.t1 - t, sm.st[buf], sum);
             slot = slot == kAhead ? 0 : slot + 1;
             __syncwarp();
             fetch_next();
@@ -111,9 +113,8 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     const Rows yr{p.seqs.length * p.channels, p.channels};
     const int64_t ys = row_step(p.seqs, yr);
     T* y = static_cast<T*>(p.y) + first_row(p.seqs, w.seq, w.s, yr) + ec + (w.t0 + ch.own_t) * ys;
-    float skip[CE];
-#pragma unroll
-    for (int i = 0; i < CE; ++i) skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
+    float2 skip[P];
+    ch.load_params(p.d_skip, skip);
     if (g.state) {
         wait_for_previous();
         load_lanes(g.state + unit * 512, lane, v);
@@ -131,12 +132,12 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
         }
         cp_async_wait<kAhead - 1>();
         const typename Chain<T, NL>::Raw& raw = sm.raw[slot];
-        const float top = ch.template stage<false>(raw, w.t1 - t, sm.st[buf], sum);
-        float ue[TE][CE], ze[TE][CE];
+        const float top = ch.template stage<false, true>(raw, w.t1 - t, sm.st[buf], sum);
+        Pack<T, CE> nu[TE], nz[TE];
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
-            raw.u[e][lane].get(ue[e]);
-            if (ch.gated) raw.z[e][lane].get(ze[e]);
+            nu[e] = raw.u[e][lane];
+            if (ch.gated) nz[e] = raw.z[e][lane];
         }
         slot = slot == kAhead ? 0 : slot + 1;
         __syncwarp();
@@ -146,13 +147,18 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
         __syncwarp();
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
-            float out[CE];
-            sum_parts<NL>(sm.part + 128 * (ch.own_t + e), ch.own_c, out);
+            float2 y2[P], u2[P];
+            sum_parts<NL>(sm.part + 128 * (ch.own_t + e), ch.own_c, y2);
+            unpack<T, CE>(nu[e], u2);
 #pragma unroll
-            for (int i = 0; i < CE; ++i) {
-                out[i] = fmaf(skip[i], ue[e][i], out[i]);
-                if (ch.gated) out[i] *= ze[e][i] * sigmoid(ze[e][i]);
+            for (int i = 0; i < P; ++i) y2[i] = ffma2(skip[i], u2[i], y2[i]);
+            if (ch.gated) {
+                unpack<T, CE>(nz[e], u2);
+#pragma unroll
+                for (int i = 0; i < P; ++i) y2[i] = fmul2(y2[i], fmul2(u2[i], sigmoid2(u2[i])));
             }
+            float out[CE];
+            from_pairs<CE>(y2, out);
             if (t + ch.own_t + e < w.t1) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
         }
         y += kGroup * ys;

@@ -195,15 +195,18 @@ __device__ __forceinline__ void put_part(float* rows, int j, int ct, const float
 }
 // ... of one token: NL rows of CW
 template <int NL>
-__device__ __forceinline__ void sum_parts(const float* rows, int own_c, float (&v)[Tile<NL>::CE]) {
+__device__ __forceinline__ void sum_parts(const float* rows, int own_c, float2 (&v)[kPairs<Tile<NL>::CE>]) {
     using K = Tile<NL>;
-    lds_v<K::CE>(rows + own_c, v);
+    float f[K::CE];
+    lds_v<K::CE>(rows + own_c, f);
+    to_pairs<K::CE>(f, v);
 #pragma unroll
     for (int k = 1; k < NL; ++k) {
-        float w[K::CE];
-        lds_v<K::CE>(rows + k * K::CW + own_c, w);
+        float2 w[kPairs<K::CE>];
+        lds_v<K::CE>(rows + k * K::CW + own_c, f);
+        to_pairs<K::CE>(f, w);
 #pragma unroll
-        for (int i = 0; i < K::CE; ++i) v[i] += w[i];
+        for (int i = 0; i < kPairs<K::CE>; ++i) v[i] = fadd2(v[i], w[i]);
     }
 }
 
@@ -220,8 +223,8 @@ struct Chain {
     const T *u, *dl, *z, *bc[Q];
     int64_t us, ds, zs, bcs;  // bcs: of the tensor (B or C) that the lane reads
     int cbase, cend, ec, lane, own_t, own_c, left;
-    bool vec, vec_bc, softplus, gated;
-    float bias[CE];
+    bool vec, vec_bc, softplus, gated, whole;  // whole: every channel of the tile exists
+    float2 bias[kPairs<CE>];
 
     __device__ __forceinline__ Chain(const ScanParams& p, const Seq& seq, int s, int tile, int lane_) {
         const LaneElems<NL> own(lane_);
@@ -232,6 +235,7 @@ struct Chain {
         ec = cbase + own_c;
         left = cend - ec;
         vec = p.vec; vec_bc = p.vec_bc; softplus = p.softplus; gated = p.z != nullptr;
+        whole = cbase + K::CW <= cend;
         const int at = left > 0 ? ec : cend - (vec ? CE : 1);
         us = row_step(p.seqs, p.ur); ds = row_step(p.seqs, p.dr); zs = row_step(p.seqs, p.zr);
         u = static_cast<const T*>(p.u) + first_row(p.seqs, seq, s, p.ur) + at + own_t * us;
@@ -247,8 +251,14 @@ struct Chain {
             const int q = min(lane + 32 * i, kQuads - 1);
             bc[i] = base + (q / (2 * NL)) * bcs + 4 * (q % NL);
         }
+        load_params(p.delta_bias, bias);
+    }
+    // one fp32 value per element channel; 0 for a null pointer and past the end
+    __device__ __forceinline__ void load_params(const float* src, float2 (&v)[kPairs<CE>]) const {
+        float f[CE];
 #pragma unroll
-        for (int i = 0; i < CE; ++i) bias[i] = p.delta_bias && i < left ? p.delta_bias[ec + i] : 0.f;
+        for (int i = 0; i < CE; ++i) f[i] = src && i < left ? src[ec + i] : 0.f;
+        to_pairs<CE>(f, v);
     }
     // n tokens on (or back)
     __device__ __forceinline__ void move(int64_t n) {
@@ -281,30 +291,45 @@ struct Chain {
             fetch(&r.bc[i][lane], bc[i] + min(0, last - t) * bcs, 4, vec_bc);
         }
     }
-    // s, s u, B and C of a loaded group into shared memory.  SUM: adds s to sum.  Returns the
+    // Zeros in place of values that do not exist: tokens from `count` on, channels past the end.
+    __device__ __forceinline__ void keep_real(int e, int64_t count, float2 (&v)[kPairs<CE>]) const {
+        if (whole && count >= kGroup) return;  // the same for the whole warp
+        const bool live = own_t + e < count;
+#pragma unroll
+        for (int i = 0; i < kPairs<CE>; ++i) {
+            v[i].x = live && 2 * i < left ? v[i].x : 0.f;
+            v[i].y = live && 2 * i + 1 < left ? v[i].y : 0.f;
+        }
+    }
+    // s, s u, B and C of a loaded group into shared memory.  SUM: adds s to sum.  TOP: returns the
     // largest |s| of the warp.
-    template <bool SUM>
-    __device__ __forceinline__ float stage(const Raw& r, int64_t count, Stage<NL>& st, float (&sum)[CE]) const {
+    template <bool SUM, bool TOP>
+    __device__ __forceinline__ float stage(const Raw& r, int64_t count, Stage<NL>& st, float2 (&sum)[kPairs<CE>]) const {
+        constexpr int P = kPairs<CE>;
         float top = 0.f;
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
-            float uv[CE], sv[CE];
-            r.u[e][lane].get(uv);
-            r.d[e][lane].get(sv);
-            const bool live = own_t + e < count;
+            float2 u2[P], s2[P];
+            unpack<T, CE>(r.u[e][lane], u2);
+            unpack<T, CE>(r.d[e][lane], s2);
 #pragma unroll
-            for (int i = 0; i < CE; ++i) sv[i] += bias[i];
-            if (softplus) softplus_n<CE>(sv);
-#pragma unroll
-            for (int i = 0; i < CE; ++i) {
-                const bool ok = live && (vec ? left > 0 : i < left);
-                sv[i] = ok ? sv[i] : 0.f;
-                uv[i] = ok ? sv[i] * uv[i] : 0.f;
-                if (SUM) sum[i] += sv[i];
-                top = max_nan(top, fabsf(sv[i]));
+            for (int i = 0; i < P; ++i) {
+                s2[i] = fadd2(s2[i], bias[i]);
+                if (softplus) s2[i] = softplus2(s2[i]);
+                u2[i] = fmul2(u2[i], s2[i]);
             }
-            sts_v<CE>(st.step + (own_t + e) * K::CW + own_c, sv);
-            sts_v<CE>(st.su + (own_t + e) * K::CW + own_c, uv);
+            keep_real(e, count, s2);
+            keep_real(e, count, u2);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                if (SUM) sum[i] = fadd2(sum[i], s2[i]);
+                if (TOP) top = max_nan(top, max_nan(fabsf(s2[i].x), fabsf(s2[i].y)));
+            }
+            float f[CE];
+            from_pairs<CE>(s2, f);
+            sts_v<CE>(st.step + (own_t + e) * K::CW + own_c, f);
+            from_pairs<CE>(u2, f);
+            sts_v<CE>(st.su + (own_t + e) * K::CW + own_c, f);
         }
 #pragma unroll
         for (int i = 0; i < Q; ++i) {
@@ -319,7 +344,7 @@ struct Chain {
                     row[((n + k) % NL) * 4 + (n + k) / NL] = v[k];
             }
         }
-        return warp_max_nan(top);
+        return TOP ? warp_max_nan(top) : 0.f;
     }
 };
 
@@ -401,9 +426,11 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // Sums v (per element channel) over the lanes that hold the same channels at other tokens, and
 // leaves the tile's row of them at out.
 template <int NL>
-__device__ __forceinline__ void sum_tokens(float (&v)[Tile<NL>::CE], int lane, int own_c, float* out) {
+__device__ __forceinline__ void sum_tokens(const float2 (&p)[kPairs<Tile<NL>::CE>], int lane, int own_c, float* out) {
     using K = Tile<NL>;
     constexpr int kLanesPerToken = NL <= 4 ? 1 : NL / 4;
+    float v[K::CE];
+    from_pairs<K::CE>(p, v);
 #pragma unroll
     for (int o = 16; o >= K::CL * kLanesPerToken; o >>= 1)
 #pragma unroll

@@ -101,7 +101,7 @@ __device__ __forceinline__ void sum_bc(const float* part, int lane, bool live, f
 template <typename T, int NL, bool OWN>
 __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kernel(const BwdParams bp, const Segments seg, int64_t items) {
     using K = Tile<NL>;
-    constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL;
+    constexpr int N = K::N, CW = K::CW, CE = K::CE, TE = K::TE, CL = K::CL, P = kPairs<CE>;
     extern __shared__ __align__(16) unsigned char smem[];
     const ScanParams& p = bp.f;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -159,21 +159,21 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
         cp_async_commit();
     };
     // s, s u, B, C and v of the fetched group
-    auto stage = [&](int64_t count, float (&sum)[CE]) {
-        const float top = chn.template stage<true>(sm.raw.r, count, sm.s, sum);
+    auto stage = [&](int64_t count, float2 (&sum)[P]) {
+        const float top = chn.template stage<OWN, true>(sm.raw.r, count, sm.s, sum);
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
-            float ve[CE], ze[CE];
-            sm.raw.dy[e][lane].get(ve);
+            float2 v2[P], z2[P];
+            unpack<T, CE>(sm.raw.dy[e][lane], v2);
             if (gated) {
-                sm.raw.r.z[e][lane].get(ze);
+                unpack<T, CE>(sm.raw.r.z[e][lane], z2);
 #pragma unroll
-                for (int i = 0; i < CE; ++i) ve[i] *= ze[i] * sigmoid(ze[i]);
+                for (int i = 0; i < P; ++i) v2[i] = fmul2(v2[i], fmul2(z2[i], sigmoid2(z2[i])));
             }
-#pragma unroll
-            for (int i = 0; i < CE; ++i)
-                ve[i] = own_t + e < count && (bp.vec ? chn.left > 0 : i < chn.left) ? ve[i] : 0.f;
-            sts_v<CE>(sm.v + (own_t + e) * CW + own_c, ve);
+            chn.keep_real(e, count, v2);
+            float f[CE];
+            from_pairs<CE>(v2, f);
+            sts_v<CE>(sm.v + (own_t + e) * CW + own_c, f);
         }
         return top;
     };
@@ -181,11 +181,11 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     if constexpr (OWN) {
         // sum_t (e_{t0} ... e_t) c_t v_t, in one pass forward
         float2 prod[8], own[8];
-        float sum[CE];
+        float2 sum[P];
 #pragma unroll
         for (int i = 0; i < 8; ++i) { prod[i] = make_float2(1.f, 1.f); own[i] = make_float2(0.f, 0.f); }
 #pragma unroll
-        for (int i = 0; i < CE; ++i) sum[i] = 0.f;
+        for (int i = 0; i < P; ++i) sum[i] = make_float2(0.f, 0.f);
         if (t0 > 0 && t0 < t1) {  // the first segment's own gradient is not needed
             fetch_at(t0, t1 - t0, true);
             for (int64_t t = t0; t < t1; t += kGroup) {
@@ -239,12 +239,10 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     float* pbc = bp.part_bc + ((int64_t)tile * bp.tokens + first_row(p.seqs, seq, s, tr)) * 2 * N;
     const int64_t ps = row_step(p.seqs, tr) * 2 * N;
     const float* ck = p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512;
-    float skip[CE], dskip[CE], dbias[CE];
+    float2 skip[P], dskip[P], dbias[P], unused[P];
+    chn.load_params(p.d_skip, skip);
 #pragma unroll
-    for (int i = 0; i < CE; ++i) {
-        skip[i] = p.d_skip && ec + i < cend ? p.d_skip[ec + i] : 0.f;
-        dskip[i] = dbias[i] = 0.f;
-    }
+    for (int i = 0; i < P; ++i) dskip[i] = dbias[i] = unused[i] = make_float2(0.f, 0.f);
 
     const int64_t first = t0 / kCheckpoint, last = (t1 + kCheckpoint - 1) / kCheckpoint;
     if (t0 < t1) {  // the last chunk's first group
@@ -255,9 +253,6 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
         const int64_t tc = ch * kCheckpoint;
         const int64_t te = min(t1, tc + kCheckpoint);
         const int groups = (int)((te - tc + kGroup - 1) / kGroup);
-        float unused[CE];
-#pragma unroll
-        for (int i = 0; i < CE; ++i) unused[i] = 0.f;
         float2 h[8];
         load_lanes(ck + ch * tiles * 512, lane, v16);
         pair_up(v16, h);
@@ -268,7 +263,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                 store_lanes(sm.h[gi], lane, v16);
                 if (gi + 1 == groups) break;
                 cp_async_wait<0>();
-                chn.template stage<false>(sm.raw.r, kGroup, sm.s, unused);
+                chn.template stage<false, false>(sm.raw.r, kGroup, sm.s, unused);
                 __syncwarp();
                 const int64_t next = tc + (gi + 1) * kGroup;  // of the last group all, for the way back
                 fetch_at(next, te - next, gi + 2 == groups);
@@ -381,31 +376,44 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
             for (int x = 0; x < TE; ++x) {
                 const int r = own_t + x;
                 const int64_t row = t + r;
-                float yo[CE], dso[CE], gbo[CE], ste[CE], duo[CE], ddo[CE], dzo[CE], ue[CE], re[CE], ye[CE], ze[CE];
-                nu[x].get(ue);
-                nd[x].get(re);
-                ndy[x].get(ye);
-                if (gated) nz[x].get(ze);
+                float2 yo[P], dso[P], gbo[P], st2[P], du2[P], dd2[P], dz2[P], u2[P], r2[P], v2[P], z2[P];
+                float f[CE];
+                unpack<T, CE>(nu[x], u2);
+                unpack<T, CE>(nd[x], r2);
+                unpack<T, CE>(ndy[x], v2);
                 const float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
-                if (gated) sum_parts<NL>(sm.y + 128 * r, own_c, yo);
                 sum_parts<NL>(sums, own_c, dso);
                 sum_parts<NL>(sums + 128, own_c, gbo);
-                lds_v<CE>(sm.s.step + r * CW + own_c, ste);
+                lds_v<CE>(sm.s.step + r * CW + own_c, f);
+                to_pairs<CE>(f, st2);
+                if (gated) {
+                    sum_parts<NL>(sm.y + 128 * r, own_c, yo);
+                    unpack<T, CE>(nz[x], z2);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        // silu'(z) = sg (1 + z (1 - sg))
+                        const float2 sg = sigmoid2(z2[i]), one = splat2(1.f);
+                        const float2 slope = fmul2(sg, ffma2(z2[i], fsub2(one, sg), one));
+                        dz2[i] = fmul2(fmul2(v2[i], ffma2(skip[i], u2[i], yo[i])), slope);
+                        v2[i] = fmul2(v2[i], fmul2(z2[i], sg));
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    du2[i] = ffma2(st2[i], gbo[i], fmul2(skip[i], v2[i]));
+                    dd2[i] = ffma2(u2[i], gbo[i], fmul2(splat2(kLn2), dso[i]));
+                    if (p.softplus) dd2[i] = fmul2(dd2[i], sigmoid2(fadd2(r2[i], chn.bias[i])));
+                }
                 if (row < te) {
                     const int64_t off = row * ys;
+                    float duo[CE], ddo[CE], dzo[CE];
+                    from_pairs<CE>(du2, duo);
+                    from_pairs<CE>(dd2, ddo);
+                    from_pairs<CE>(dz2, dzo);
 #pragma unroll
-                    for (int i = 0; i < CE; ++i) {
-                        float v = ye[i];
-                        if (gated) {
-                            const float sg = sigmoid(ze[i]);
-                            dzo[i] = ye[i] * fmaf(skip[i], ue[i], yo[i]) * (sg * (1.f + ze[i] * (1.f - sg)));
-                            v *= ze[i] * sg;
-                        }
-                        duo[i] = fmaf(ste[i], gbo[i], skip[i] * v);
-                        ddo[i] = fmaf(ue[i], gbo[i], kLn2 * dso[i]);
-                        if (p.softplus) ddo[i] *= sigmoid(re[i] + chn.bias[i]);
-                        dskip[i] = fmaf(v, ue[i], dskip[i]);
-                        dbias[i] += ddo[i];
+                    for (int i = 0; i < P; ++i) {
+                        dskip[i] = ffma2(v2[i], u2[i], dskip[i]);
+                        dbias[i] = fadd2(dbias[i], dd2[i]);
                     }
                     store_v<CE>(du + off, ec, cend, bp.vec, duo);
                     store_v<CE>(dd + off, ec, cend, bp.vec, ddo);
