@@ -502,7 +502,7 @@ struct Layout {
 // Warps that a B200 holds of the backward kernel (two CTAs of three or four an SM).
 int64_t bwd_warps(const vh_ssm_scan_args* a) { return (int64_t)(a->dtype == VH_F32 ? 6 : 8) * sm_count(); }
 
-int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) / 2, bwd_warps(a), kCheckpoint); }
+int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) / 2, 4 * bwd_warps(a), kCheckpoint); }
 
 Layout layout_of(const vh_ssm_scan_args* a, int size) {
     Layout l;
