@@ -76,23 +76,34 @@ __device__ __forceinline__ void put_bc(float* part, int j, int k, const float (&
     *reinterpret_cast<float4*>(row + ((4 * j) ^ turn)) = make_float4(db[0], db[1], db[2], db[3]);
     *reinterpret_cast<float4*>(row + ((R / 2 + 4 * j) ^ turn)) = make_float4(dc[0], dc[1], dc[2], dc[3]);
 }
-// ... summed and stored in that order
-template <int NL>
-__device__ __forceinline__ void sum_bc(const float* part, int lane, bool live, float* out) {
-    constexpr int R = 8 * NL, CL = Tile<NL>::CL;
-    constexpr int kSplit = R < 32 ? 32 / R : 1;  // lanes an output: each takes some of the parts
+// ... of the four tokens of a group, summed four outputs at a time and stored in that order.
+// part(r): token r's parts; out: the group's first row, `ps` floats a token.
+template <int NL, typename Part>
+__device__ __forceinline__ void sum_bc(Part&& part, int lane, int64_t count, float* out, int64_t ps) {
+    constexpr int R = 8 * NL, CL = Tile<NL>::CL, kQuads = kGroup * R / 4;
+    constexpr int kSplit = kQuads < 32 ? 32 / kQuads : 1;  // lanes a quad: each takes some of the parts
 #pragma unroll
-    for (int m = 0; m < (R + 31) / 32; ++m) {
-        const int w = R < 32 ? lane % R : lane + 32 * m, k0 = R < 32 ? lane / R * (CL / kSplit) : 0;
-        float sum = 0.f;
+    for (int m = 0; m < (kQuads + 31) / 32; ++m) {
+        const int q = lane % kQuads + 32 * m, r = q / (R / 4), w = 4 * (q % (R / 4));
+        const int k0 = kSplit > 1 ? lane / kQuads * (CL / kSplit) : 0;
+        const float* rows = part(r);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int i = 0; i < CL / kSplit; ++i) {
-            const int k = k0 + i;
-            sum += part[k * R + (w ^ (4 * k % R))];
+            float2 v[2];
+            lds22(rows + (k0 + i) * R + (w ^ (4 * (k0 + i) % R)), v);
+            sum[0] = fadd2(sum[0], v[0]);
+            sum[1] = fadd2(sum[1], v[1]);
         }
 #pragma unroll
-        for (int o = 16; o >= R; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (live && (R >= 32 || lane < R)) out[w] = sum;
+        for (int o = 16; o >= kQuads; o >>= 1) {
+            sum[0].x += __shfl_xor_sync(0xffffffffu, sum[0].x, o);
+            sum[0].y += __shfl_xor_sync(0xffffffffu, sum[0].y, o);
+            sum[1].x += __shfl_xor_sync(0xffffffffu, sum[1].x, o);
+            sum[1].y += __shfl_xor_sync(0xffffffffu, sum[1].y, o);
+        }
+        if (r < count && (kSplit == 1 || lane < kQuads))
+            *reinterpret_cast<float4*>(out + r * ps + w) = make_float4(sum[0].x, sum[0].y, sum[1].x, sum[1].y);
     }
 }
 
@@ -365,13 +376,13 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                     put_part<NL>(sums, j, ct, dsum);
                     put_part<NL>(sums + 128, j, ct, gsum);
                     put_bc<NL>(sums + 256, j, lane % CL, dbs, dcs[r]);
-                    __syncwarp();
-                    sum_bc<NL>(sums + 256, lane, t + r < te, pbc + (t + r) * ps);
                 }
             };
             if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
             else pass(std::integral_constant<int, kChecked>{});
             __syncwarp();
+            auto sums_of = [&](int r) { return r > 0 ? sm.past[r - 1] : sm.h[gi]; };
+            sum_bc<NL>([&](int r) { return sums_of(r) + 256; }, lane, te - t, pbc + t * ps, ps);
 #pragma unroll
             for (int x = 0; x < TE; ++x) {
                 const int r = own_t + x;
@@ -381,7 +392,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                 unpack<T, CE>(nu[x], u2);
                 unpack<T, CE>(nd[x], r2);
                 unpack<T, CE>(ndy[x], v2);
-                const float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
+                const float* sums = sums_of(r);
                 sum_parts<NL>(sums, own_c, dso);
                 sum_parts<NL>(sums + 128, own_c, gbo);
                 lds_v<CE>(sm.s.step + r * CW + own_c, f);
