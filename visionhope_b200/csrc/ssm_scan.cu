@@ -68,19 +68,20 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     constexpr int P = kPairs<CE>;
     float v[16];
     float2 sum[P];
-    const float top_a = load_rates<NL>(p, c0, cend, j, v);
+    const float most = mixed_limit(load_rates<NL>(p, c0, cend, j, v));
     pair_up(v, a2);
     ch.move(w.t0);
     // the last segment's own state is not needed
     const bool some = w.t0 < w.t1 && (!OWN || w.t1 < w.seq.len);
     // the first kAhead groups; every group is a commit of its own, empty past the end
-    int64_t ahead = w.t0;
-    int slot = 0, next = 0;  // of the group at hand and the one fetched next
+    const int tokens = (int)(w.t1 - w.t0);
+    int ahead = some ? tokens : 0;  // tokens still to fetch
+    int slot = 0, next = 0;         // of the group at hand and the one fetched next
     auto fetch_next = [&]() {
-        if (some && ahead < w.t1) {
-            ch.template load<!OWN>(sm.raw[next], w.t1 - ahead);
-            ch.move(kGroup);
-            ahead += kGroup;
+        if (ahead > 0) {
+            ch.template load<!OWN>(sm.raw[next], ahead);
+            ch.advance();
+            ahead -= kGroup;
         }
         cp_async_commit();
         next = next == kAhead ? 0 : next + 1;
@@ -95,13 +96,13 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     if constexpr (OWN) {
         pair_up(v, h);
         int buf = 0;
-        for (int64_t t = w.t0; some && t < w.t1; t += kGroup, buf ^= 1) {
+        for (int left = some ? tokens : 0; left > 0; left -= kGroup, buf ^= 1) {
             cp_async_wait<kAhead - 1>();
-            const float top = ch.template stage<true, true>(sm.raw[slot], w.t1 - t, sm.st[buf], sum);
+            const bool fast = ch.template stage<true, true>(sm.raw[slot], left, sm.st[buf], sum, most);
             slot = slot == kAhead ? 0 : slot + 1;
             __syncwarp();
             fetch_next();
-            if (top * top_a <= 126.f) advance<NL, kMixed, false>(sm.st[buf], ct, j, a2, h, nullptr);
+            if (fast) advance<NL, kMixed, false>(sm.st[buf], ct, j, a2, h, nullptr);
             else advance<NL, kChecked, false>(sm.st[buf], ct, j, a2, h, nullptr);
         }
         pair_down(h, v);
@@ -125,14 +126,21 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     float* ck = p.checkpoints ? p.checkpoints + (slot_base(p.seqs, w.s, w.seq.row, kCheckpoint) * tiles + w.tile) * 512
                               : nullptr;
     int buf = 0;
-    for (int64_t t = w.t0; t < w.t1; t += kGroup, buf ^= 1) {
-        if (ck && t % kCheckpoint == 0) {
-            pair_down(h, v);
-            store_lanes(ck + (t / kCheckpoint) * tiles * 512, lane, v);
+    if (ck) ck += (w.t0 + kCheckpoint - 1) / kCheckpoint * tiles * 512;
+    int until = (int)((kCheckpoint - w.t0 % kCheckpoint) % kCheckpoint);  // tokens to the next saved state
+    for (int left = tokens; left > 0; left -= kGroup, buf ^= 1) {
+        if (ck) {
+            if (until == 0) {
+                pair_down(h, v);
+                store_lanes(ck, lane, v);
+                ck += (int64_t)tiles * 512;
+                until = kCheckpoint;
+            }
+            until -= kGroup;
         }
         cp_async_wait<kAhead - 1>();
         const typename Chain<T, NL>::Raw& raw = sm.raw[slot];
-        const float top = ch.template stage<false, true>(raw, w.t1 - t, sm.st[buf], sum);
+        const bool fast = ch.template stage<false, true>(raw, left, sm.st[buf], sum, most);
         Pack<T, CE> nu[TE], nz[TE];
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
@@ -142,7 +150,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
         slot = slot == kAhead ? 0 : slot + 1;
         __syncwarp();
         fetch_next();
-        if (top * top_a <= 126.f) advance<NL, kMixed, true>(sm.st[buf], ct, j, a2, h, sm.part);
+        if (fast) advance<NL, kMixed, true>(sm.st[buf], ct, j, a2, h, sm.part);
         else advance<NL, kChecked, true>(sm.st[buf], ct, j, a2, h, sm.part);
         __syncwarp();
 #pragma unroll
@@ -159,7 +167,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
             }
             float out[CE];
             from_pairs<CE>(y2, out);
-            if (t + ch.own_t + e < w.t1) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
+            if (ch.own_t + e < left) store_v<CE>(y + e * ys, ec, cend, p.vec, out);
         }
         y += kGroup * ys;
     }

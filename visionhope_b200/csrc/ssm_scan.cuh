@@ -222,6 +222,7 @@ struct Chain {
     static constexpr int kQuads = kGroup * 2 * NL;
     const T *u, *dl, *z, *bc[Q];
     int64_t us, ds, zs, bcs;  // bcs: of the tensor (B or C) that the lane reads
+    int64_t ug, dg, zg, bcg;  // of a group
     int cbase, cend, ec, lane, own_t, own_c, left;
     bool vec, vec_bc, softplus, gated, whole;  // whole: every channel of the tile exists
     float2 bias[kPairs<CE>];
@@ -252,6 +253,7 @@ struct Chain {
             bc[i] = base + (q / (2 * NL)) * bcs + 4 * (q % NL);
         }
         load_params(p.delta_bias, bias);
+        ug = kGroup * us; dg = kGroup * ds; zg = kGroup * zs; bcg = kGroup * bcs;
     }
     // one fp32 value per element channel; 0 for a null pointer and past the end
     __device__ __forceinline__ void load_params(const float* src, float2 (&v)[kPairs<CE>]) const {
@@ -259,6 +261,14 @@ struct Chain {
 #pragma unroll
         for (int i = 0; i < CE; ++i) f[i] = src && i < left ? src[ec + i] : 0.f;
         to_pairs<CE>(f, v);
+    }
+    // a group on
+    __device__ __forceinline__ void advance() {
+        u += ug;
+        dl += dg;
+        if (gated) z += zg;
+#pragma unroll
+        for (int i = 0; i < Q; ++i) bc[i] += bcg;
     }
     // n tokens on (or back)
     __device__ __forceinline__ void move(int64_t n) {
@@ -276,8 +286,19 @@ struct Chain {
     };
     // Fetches the group at hand, of which the first `count` (or more) tokens exist.
     template <bool GATE>
-    __device__ __forceinline__ void load(Raw& r, int64_t count) const {
-        const int last = count >= kGroup ? kGroup - 1 : (int)count - 1;
+    __device__ __forceinline__ void load(Raw& r, int count) const {
+        if (count >= kGroup) {
+#pragma unroll
+            for (int e = 0; e < TE; ++e) {
+                fetch(&r.u[e][lane], u + e * us, left, vec);
+                fetch(&r.d[e][lane], dl + e * ds, left, vec);
+                if (GATE && gated) fetch(&r.z[e][lane], z + e * zs, left, vec);
+            }
+#pragma unroll
+            for (int i = 0; i < Q; ++i) fetch(&r.bc[i][lane], bc[i], 4, vec_bc);
+            return;
+        }
+        const int last = count - 1;
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             const int64_t by = min(e, last - own_t);
@@ -292,7 +313,7 @@ struct Chain {
         }
     }
     // Zeros in place of values that do not exist: tokens from `count` on, channels past the end.
-    __device__ __forceinline__ void keep_real(int e, int64_t count, float2 (&v)[kPairs<CE>]) const {
+    __device__ __forceinline__ void keep_real(int e, int count, float2 (&v)[kPairs<CE>]) const {
         if (whole && count >= kGroup) return;  // the same for the whole warp
         const bool live = own_t + e < count;
 #pragma unroll
@@ -301,10 +322,11 @@ struct Chain {
             v[i].y = live && 2 * i + 1 < left ? v[i].y : 0.f;
         }
     }
-    // s, s u, B and C of a loaded group into shared memory.  SUM: adds s to sum.  TOP: returns the
-    // largest |s| of the warp.
+    // s, s u, B and C of a loaded group into shared memory.  SUM: adds s to sum.  TOP: returns
+    // whether every |s| of the warp is at most `most` (false with a NaN among them).
     template <bool SUM, bool TOP>
-    __device__ __forceinline__ float stage(const Raw& r, int64_t count, Stage<NL>& st, float2 (&sum)[kPairs<CE>]) const {
+    __device__ __forceinline__ bool stage(const Raw& r, int count, Stage<NL>& st, float2 (&sum)[kPairs<CE>],
+                                          float most = 0.f) const {
         constexpr int P = kPairs<CE>;
         float top = 0.f;
 #pragma unroll
@@ -344,7 +366,7 @@ struct Chain {
                     row[((n + k) % NL) * 4 + (n + k) / NL] = v[k];
             }
         }
-        return TOP ? warp_max_nan(top) : 0.f;
+        return TOP && __all_sync(0xffffffffu, top <= most);
     }
 };
 
@@ -357,7 +379,7 @@ __device__ __forceinline__ void pair_down(const float2 (&p)[8], float (&v)[16]) 
     for (int i = 0; i < 8; ++i) { v[2 * i] = p[i].x; v[2 * i + 1] = p[i].y; }
 }
 
-// log2(e) A of the thread's block; returns the warp's largest of the states whose decays run on
+// log2(e) A of the thread's block; returns the warp's largest |.| of the states whose decays run on
 // the FMA pipe (see decays).
 template <int NL>
 __device__ __forceinline__ float load_rates(const ScanParams& p, int c0, int cend, int j, float (&v)[16]) {
@@ -369,6 +391,9 @@ __device__ __forceinline__ float load_rates(const ScanParams& p, int c0, int cen
     for (int i = 0; i < 4; ++i) top = max_nan(top, fabsf(v[i]));
     return warp_max_nan(top);
 }
+
+// The largest |s| that kMixed takes with such a rate (none for NaN; an infinite one never).
+__device__ __forceinline__ float mixed_limit(float top) { return top < 1e-30f ? 3e38f : 126.f / top; }
 
 // ---- a chain in segments ----------------------------------------------------------------------
 // With few chains, consecutive segments of `size` tokens of a chain go to warps of their own.  A

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     const bool gated = p.z != nullptr;
     float2 a2[8], g[8], da[8];
     float v16[16];
-    const float top_a = load_rates<NL>(p, c0, cend, j, v16);
+    const float most = mixed_limit(load_rates<NL>(p, c0, cend, j, v16));
     pair_up(v16, a2);
     const float* dfinal = bp.dfinal ? bp.dfinal + (int64_t)s * p.channels * N : nullptr;
 
@@ -153,7 +153,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     int64_t pos = 0;
     // Fetches the group at `t` (of `count` tokens or more) behind the one at hand: a lane reads
     // back only what it fetched, and has read the group at hand by then.
-    auto fetch_at = [&](int64_t t, int64_t count, bool all) {
+    auto fetch_at = [&](int64_t t, int64_t tokens, bool all) {
+        const int count = (int)min(tokens, (int64_t)kGroup);
         chn.move(t - pos);
         dyr += (t - pos) * ys;
         pos = t;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
             chn.template load<true>(sm.raw.r, count);
 #pragma unroll
             for (int e = 0; e < TE; ++e) {
-                const int64_t by = count >= kGroup ? e : min((int64_t)e, count - 1 - own_t);
+                const int64_t by = count >= kGroup ? e : min(e, count - 1 - own_t);
                 fetch(&sm.raw.dy[e][lane], dyr + by * ys, chn.left, (bool)bp.vec);
             }
         } else {
@@ -170,8 +171,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
         cp_async_commit();
     };
     // s, s u, B, C and v of the fetched group
-    auto stage = [&](int64_t count, float2 (&sum)[P]) {
-        const float top = chn.template stage<OWN, true>(sm.raw.r, count, sm.s, sum);
+    auto stage = [&](int64_t tokens, float2 (&sum)[P]) {
+        const int count = (int)min(tokens, (int64_t)kGroup);
+        const bool fast = chn.template stage<OWN, true>(sm.raw.r, count, sm.s, sum, most);
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             float2 v2[P], z2[P];
@@ -186,7 +188,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
             from_pairs<CE>(v2, f);
             sts_v<CE>(sm.v + (own_t + e) * CW + own_c, f);
         }
-        return top;
+        return fast;
     };
 
     if constexpr (OWN) {
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
             fetch_at(t0, t1 - t0, true);
             for (int64_t t = t0; t < t1; t += kGroup) {
                 cp_async_wait<0>();
-                const float top = stage(t1 - t, sum);
+                const bool fast = stage(t1 - t, sum);
                 __syncwarp();
                 if (t + kGroup < t1) fetch_at(t + kGroup, t1 - t - kGroup, true);
                 auto pass = [&](auto mode) {
@@ -221,7 +223,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                             }
                     }
                 };
-                if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
+                if (fast) pass(std::integral_constant<int, kMixed>{});
             else pass(std::integral_constant<int, kChecked>{});
                 __syncwarp();
             }
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
         for (int gi = groups - 1; gi >= 0; --gi) {
             const int64_t t = tc + gi * kGroup;
             cp_async_wait<0>();
-            const float top = stage(te - t, unused);
+            const bool fast = stage(te - t, unused);
             Pack<T, CE> nu[TE], nd[TE], nz[TE], ndy[TE];
 #pragma unroll
             for (int x = 0; x < TE; ++x) {
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                     put_bc<NL>(sums + 256, j, lane % CL, dbs, dcs[r]);
                 }
             };
-            if (top * top_a <= 126.f) pass(std::integral_constant<int, kMixed>{});
+            if (fast) pass(std::integral_constant<int, kMixed>{});
             else pass(std::integral_constant<int, kChecked>{});
             __syncwarp();
             auto sums_of = [&](int r) { return r > 0 ? sm.past[r - 1] : sm.h[gi]; };
