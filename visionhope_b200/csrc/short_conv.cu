@@ -6,8 +6,8 @@
 // A thread owns V neighbouring channels (16 bytes of them in the forward) and walks runs of tokens
 // with the last K inputs in registers, so each input is read once, plus K - 1 rows of halo per run.
 // There is no reuse beyond the window and 2 K flops per element: the kernels are bounded by HBM, and
-// what counts is bytes in flight.  A thread therefore loads four tokens while it computes the four
-// before them, and runs are as long as one wave of threads allows, so that weights, halo and the
+// what counts is bytes in flight.  A thread therefore fetches its tokens into shared memory of its own
+// two blocks of four ahead (asynchronous copies take no registers), and runs are as long as one wave of threads allows, so that weights, halo and the
 // search for the sequence are paid once for many tokens.
 #include <algorithm>
 #include <type_traits>
@@ -19,7 +19,8 @@ namespace vh {
 namespace ssm {
 namespace {
 
-constexpr int kBlock = 4;     // tokens loaded at a time
+constexpr int kBlock = 4;     // tokens fetched at a time
+constexpr int kRing = 3;      // blocks held: the one at hand and two ahead
 constexpr int kThreads = 256;
 constexpr int kFwdBlocks = 3, kBwdBlocks = 2;  // blocks an SM holds
 
@@ -99,6 +100,28 @@ __device__ __forceinline__ void enter(const ConvParams& p, const T* x, int64_t s
     }
 }
 
+// A thread's ring of fetched rows: row i of block b lies kThreads apart from its neighbours, and the
+// thread reads only what it fetched.
+template <typename T, int V>
+struct Ring {
+    Pack<T, V>* own;
+    __device__ __forceinline__ explicit Ring(void* smem) : own(static_cast<Pack<T, V>*>(smem) + threadIdx.x) {}
+    __device__ __forceinline__ Pack<T, V>& at(int slot, int i) const { return own[(slot * kBlock + i) * kThreads]; }
+    // rows from .. from + 3, none past `last`
+    __device__ __forceinline__ void fill(int slot, const T* p, int64_t step, int from, int last) const {
+        if (from + kBlock - 1 <= last) {
+            const T* q = p + from * step;
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) fetch(&at(slot, i), q + i * step, V, true);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i)
+                if (from + i <= last) fetch(&at(slot, i), p + (from + i) * step, V, true);
+        }
+    }
+};
+__device__ __forceinline__ int next_slot(int slot) { return slot + 1 == kRing ? 0 : slot + 1; }
+
 // A block: `cblock` channel groups by kThreads / cblock runs, over channels and slots.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads, kFwdBlocks)
@@ -108,6 +131,8 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
     const int ri = threadIdx.x / cblock;
     const int c = (blockIdx.x * cblock + threadIdx.x % cblock) * V;
     if (ri >= lanes || c >= p.channels) return;
+    extern __shared__ __align__(16) unsigned char smem[];
+    const Ring<T, V> ring(smem);
     Weights<V, K> wt;
     wt.load(p, c);
     const int64_t xs = row_step(p.seqs, p.xr);
@@ -134,28 +159,29 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
             }
             store<T, V>(y + t * ys, out);
         };
-        int t = 0;
-        if (count >= 2 * kBlock) {
-            // a block is loaded while the one before it is computed
-            Pack<T, V> in[2][kBlock];
-            auto fill = [&](Pack<T, V> (&to)[kBlock], int from) {
 #pragma unroll
-                for (int i = 0; i < kBlock; ++i) to[i] = load<T, V>(xj + (from + i) * xs);
-            };
-            fill(in[0], 0);
-            enter<T, V, K>(p, x, xs, s, c, j0, win);
-            for (; t + 2 * kBlock <= count; t += 2 * kBlock) {
-                fill(in[1], t + kBlock);
-#pragma unroll
-                for (int i = 0; i < kBlock; ++i) step(in[0][i], t + i);
-                if (t + 4 * kBlock <= count) fill(in[0], t + 2 * kBlock);
-#pragma unroll
-                for (int i = 0; i < kBlock; ++i) step(in[1][i], t + kBlock + i);
-            }
-        } else {
-            enter<T, V, K>(p, x, xs, s, c, j0, win);
+        for (int b = 0; b + 1 < kRing; ++b) {
+            ring.fill(b, xj, xs, b * kBlock, count - 1);
+            cp_async_commit();
         }
-        for (; t < count; ++t) step(load<T, V>(xj + t * xs), t);
+        enter<T, V, K>(p, x, xs, s, c, j0, win);
+        for (int t = 0, slot = 0; t < count; t += kBlock, slot = next_slot(slot)) {
+            cp_async_wait<kRing - 2>();
+            Pack<T, V> in[kBlock];
+#pragma unroll
+            for (int i = 0; i < kBlock; ++i) in[i] = ring.at(slot, i);
+            ring.fill(slot == 0 ? kRing - 1 : slot - 1, xj, xs, t + (kRing - 1) * kBlock, count - 1);
+            cp_async_commit();
+            if (t + kBlock <= count) {
+#pragma unroll
+                for (int i = 0; i < kBlock; ++i) step(in[i], t + i);
+            } else {
+#pragma unroll
+                for (int i = 0; i + 1 < kBlock; ++i)
+                    if (t + i < count) step(in[i], t + i);
+            }
+        }
+        cp_async_wait<0>();
         if (p.final_state && j0 + count == seq.len) {
             // the last K - 1 inputs, which are the initial state's where the sequence is shorter
             T* f = static_cast<T*>(p.final_state) + (int64_t)s * (K - 1) * p.channels + c;
@@ -176,7 +202,8 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads, kBwdBlocks) conv_bwd_kernel(const ConvParams p, int64_t slots, int32_t cblock) {
     constexpr int P = kPairs<V>;
-    __shared__ float red[kThreads];
+    extern __shared__ __align__(16) unsigned char smem[];
+    const Ring<T, V> rx(smem), rg(static_cast<Pack<T, V>*>(static_cast<void*>(smem)) + kRing * kBlock * kThreads);
     const int lanes = kThreads / cblock;
     const int ci = threadIdx.x % cblock, ri = threadIdx.x / cblock;
     const int c = (blockIdx.x * cblock + ci) * V;
@@ -267,43 +294,41 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) conv_bwd_kernel(const Co
                     else store<T, V>(di + (j + K - 1) * p.channels, out);
                 }
             };
-            auto edge = [&](int from, int to) {
-                for (int t = from; t < to; ++t) {
-                    const int at = min(t, ends - 1);
-                    Pack<T, V> a{}, b{};
-                    if (ends > 0) {
-                        a = load<T, V>(xj + at * xs);
-                        b = load<T, V>(dy + at * ys);
-                    }
-                    step(a, b, t, std::false_type{});
-                }
-            };
+            // token t's x and dy from block slot; past `ends` nothing was fetched, and nothing is used
             const int total = count + K - 1;
-            int t = min(K - 1, total);
-            edge(0, t);
-            if (t + 2 * kBlock <= count) {  // what these complete is the run's, and not in the final state
-                Pack<T, V> xin[2][kBlock], gin[2][kBlock];
-                auto fill = [&](Pack<T, V> (&a)[kBlock], Pack<T, V> (&b)[kBlock], int from) {
 #pragma unroll
-                    for (int i = 0; i < kBlock; ++i) {
-                        a[i] = load<T, V>(xj + (from + i) * xs);
-                        b[i] = load<T, V>(dy + (from + i) * ys);
-                    }
-                };
-                fill(xin[0], gin[0], t);
-                for (; t + 2 * kBlock <= count; t += 2 * kBlock) {
-                    fill(xin[1], gin[1], t + kBlock);
+            for (int b = 0; b + 1 < kRing; ++b) {
+                rx.fill(b, xj, xs, b * kBlock, ends - 1);
+                rg.fill(b, dy, ys, b * kBlock, ends - 1);
+                cp_async_commit();
+            }
+            for (int t = 0, slot = 0; t < total; t += kBlock, slot = next_slot(slot)) {
+                cp_async_wait<kRing - 2>();
+                Pack<T, V> xin[kBlock], gin[kBlock];
 #pragma unroll
-                    for (int i = 0; i < kBlock; ++i) step(xin[0][i], gin[0][i], t + i, std::true_type{});
-                    if (t + 4 * kBlock <= count) fill(xin[0], gin[0], t + 2 * kBlock);
+                for (int i = 0; i < kBlock; ++i) {
+                    xin[i] = rx.at(slot, i);
+                    gin[i] = rg.at(slot, i);
+                }
+                const int free = slot == 0 ? kRing - 1 : slot - 1;
+                rx.fill(free, xj, xs, t + (kRing - 1) * kBlock, ends - 1);
+                rg.fill(free, dy, ys, t + (kRing - 1) * kBlock, ends - 1);
+                cp_async_commit();
+                if (t >= K - 1 && t + kBlock <= count) {  // what these complete is the run's, and not in the final state
 #pragma unroll
-                    for (int i = 0; i < kBlock; ++i) step(xin[1][i], gin[1][i], t + kBlock + i, std::true_type{});
+                    for (int i = 0; i < kBlock; ++i) step(xin[i], gin[i], t + i, std::true_type{});
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kBlock; ++i)
+                        if (t + i < total) step(xin[i], gin[i], t + i, std::false_type{});
                 }
             }
-            edge(t, total);
+            cp_async_wait<0>();
         }
     }
     // the block's sums: one value of every thread at a time, added over the runs in order
+    __syncthreads();  // the rings are no longer read
+    float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int k = 0; k <= K; ++k)
 #pragma unroll
@@ -493,8 +518,12 @@ extern "C" int vh_short_conv_fwd(const vh_short_conv_args* a, vh_stream_t stream
             const Plan b = plan(a, V, kFwdBlocks);
             p.run = b.run;
             return with_taps(a->taps, [&](auto taps) {
-                conv_fwd_kernel<T, V, decltype(taps)::value>
-                    <<<dim3(b.gx, b.gy), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p, b.slots, b.cblock);
+                constexpr int K = decltype(taps)::value;
+                constexpr size_t smem = sizeof(Pack<T, V>) * kRing * kBlock * kThreads;
+                if (!ensure_smem_attr(reinterpret_cast<const void*>(&conv_fwd_kernel<T, V, K>), smem))
+                    return fail(VH_E_DEVICE, "vh_short_conv_fwd: cannot reserve %zu bytes of shared memory", smem);
+                conv_fwd_kernel<T, V, K><<<dim3(b.gx, b.gy), kThreads, smem, static_cast<cudaStream_t>(stream)>>>(
+                    p, b.slots, b.cblock);
                 return launch_status("short convolution");
             });
         });
@@ -538,7 +567,11 @@ extern "C" int vh_short_conv_bwd(const vh_short_conv_args* a, const void* grad_y
             p.run = b.run;
             blocks = b.gy;
             return with_taps(a->taps, [&](auto taps) {
-                conv_bwd_kernel<T, V, decltype(taps)::value><<<dim3(b.gx, b.gy), kThreads, 0, st>>>(p, b.slots, b.cblock);
+                constexpr int K = decltype(taps)::value;
+                constexpr size_t smem = std::max(sizeof(Pack<T, V>) * 2 * kRing * kBlock, sizeof(float)) * kThreads;
+                if (!ensure_smem_attr(reinterpret_cast<const void*>(&conv_bwd_kernel<T, V, K>), smem))
+                    return fail(VH_E_DEVICE, "vh_short_conv_bwd: cannot reserve %zu bytes of shared memory", smem);
+                conv_bwd_kernel<T, V, K><<<dim3(b.gx, b.gy), kThreads, smem, st>>>(p, b.slots, b.cblock);
                 return launch_status("short convolution backward");
             });
         });

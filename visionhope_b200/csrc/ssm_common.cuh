@@ -192,6 +192,22 @@ struct Pack {
     }
 };
 
+// A Pack into shared memory, asynchronously where the copy is one of 4, 8 or 16 bytes.  Issued a
+// group or two ahead of its use it takes no registers; plain loads ahead of their use do, and were
+// moved next to it by the compiler (the forward then waited for memory in 4 of 10 cycles).
+template <typename T, int V>
+__device__ __forceinline__ void fetch(Pack<T, V>* dst, const T* p, int left, bool vec) {
+    if constexpr (sizeof(T) * V >= 4) {
+        if (vec) {
+            cp_async<sizeof(T) * V>(dst, p);
+            return;
+        }
+    }
+    Pack<T, V> r;
+    r.load(p, left, vec);
+    *dst = r;
+}
+
 // V values as pairs for the packed arithmetic (V = 1: the second half repeats the first).
 template <int V>
 constexpr int kPairs = (V + 1) / 2;
