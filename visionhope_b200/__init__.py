@@ -10,8 +10,10 @@ replacements of the reference modules that own its kernels:
                                              query_normalization}.py
 
 The reference's own ``models/srnl.py``, ``models/operator.py`` and ``models/block.py`` run
-unchanged on top of them.  ``visionhope_b200.backbone`` (with ``mixer``) is a separate
-caller harness that drives the kernels end to end for the whole-model benchmark.
+unchanged on top of them.  ``visionhope_b200.ssm_core`` adds the selective
+state space operators (short causal convolution, selective scan, their one-token steps) and
+``visionhope_b200.ssm_mixer`` a layer that runs them.  ``visionhope_b200.backbone`` (with ``mixer``)
+is a separate caller harness that drives the kernels end to end for the whole-model benchmark.
 """
 from ._lib import load as load_library, version  # noqa: F401
 

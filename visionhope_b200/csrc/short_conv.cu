@@ -483,10 +483,10 @@ Plan plan(const vh_short_conv_args* a, int width, int per_sm) {
     const int64_t fit = std::max<int64_t>(1, (int64_t)per_sm * sm_count() / b.gx);
     const int64_t tokens = packed ? a->length : a->length * a->batch;
     const int64_t want = (tokens + fit * lanes - 1) / (fit * lanes);
-    b.run = (int)std::min<int64_t>(std::max<int64_t>((want + 7) / 8 * 8, 8), 1 << 20);
+    b.run = (int)std::min<int64_t>(std::max<int64_t>((want + 3) / 4 * 4, 8), 1 << 20);
     if (!packed) {  // equal shares of every sequence
         const int64_t runs = slots_per_seq(a->length, b.run);
-        b.run = (int)std::max<int64_t>(((a->length + runs - 1) / runs + 7) / 8 * 8, 8);
+        b.run = (int)std::max<int64_t>(((a->length + runs - 1) / runs + 3) / 4 * 4, 8);
     }
     b.slots = slot_total(packed, a->length, a->batch, b.run);
     b.gy = (int)std::max<int64_t>(1, std::min<int64_t>((b.slots + lanes - 1) / lanes, 2 * fit));

@@ -28,7 +28,7 @@ __device__ __forceinline__ void advance(const Stage<NL>& st, int ct, int j, cons
         lds22(st.step + r * K::CW + ct, s);
         lds22(st.su + r * K::CW + ct, su);
         lds_dup4(st.b(r, j), b);
-        decays<MODE>(s, a2, e);
+        decays<MODE, true>(s, a2, e);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll

@@ -139,13 +139,16 @@ __device__ __forceinline__ void load_lanes(const float* p, int lane, float (&v)[
 // kHardware: all on the special-function unit.  kMixed: the first state's on the FMA pipe, for
 // |s a2| <= 126 there; kChecked: the same values without that condition (the warp's choice between
 // the two must not show in a channel's bits).
+// LAST: the polynomials behind the others, whose latency is the longest (the forward is 2 % faster
+// that way, the backward 7 % slower).
 enum Decay { kHardware, kMixed, kChecked };
-template <int MODE>
+template <int MODE, bool LAST = false>
 __device__ __forceinline__ void decays(const float2 (&s)[2], const float2 (&a2)[8], float2 (&e)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
+            const int i = LAST ? 3 - k : k;
             const float2 a = a2[2 * i + p];
             if (i > 0 || MODE == kHardware) e[2 * i + p] = ex2_2(fmul2(s[p], a));
             else if (MODE == kMixed) e[2 * i + p] = exp2_fma2(s[p], a);
