@@ -449,6 +449,18 @@ def test_long_strides_pass_32_bits():
     assert torch.equal(got, want)
 
 
+def test_second_derivatives_are_refused():
+    """The backward's kernels are not differentiable themselves: asking for it raises instead of
+    giving the wrong second derivative."""
+    from visionhope_b200.ssm_core import short_conv
+
+    x = torch.randn(1, 5, 8, device=DEV, requires_grad=True)
+    w = torch.randn(8, 4, device=DEV, requires_grad=True)
+    g = torch.autograd.grad(short_conv(x, w, activation="silu").sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_python_refusals():
     from visionhope_b200 import ssm_core
 

@@ -2,6 +2,7 @@
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _args
@@ -96,6 +97,7 @@ class _ShortConvFunction(torch.autograd.Function):
         return (y, final) if want_final else y
 
     @staticmethod
+    @once_differentiable
     @_lib.on_input_device
     def backward(ctx, dy, dfinal=None):
         if dy is None and dfinal is None:

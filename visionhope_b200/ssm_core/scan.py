@@ -2,6 +2,7 @@
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import _args
@@ -129,6 +130,7 @@ class _SsmScanFunction(torch.autograd.Function):
         return (y, final) if want_final else y
 
     @staticmethod
+    @once_differentiable
     @_lib.on_input_device
     def backward(ctx, dy, dfinal=None):
         if dy is None and dfinal is None:
