@@ -55,8 +55,17 @@ struct Weights {
     float2 w[K][kPairs<V>], b[kPairs<V>];
     __device__ __forceinline__ void load(const ConvParams& p, int c) {
         float v[V * K];
+        const float* src = p.w + (int64_t)c * K;
+        if (V % 4 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
 #pragma unroll
-        for (int i = 0; i < V * K; ++i) v[i] = p.w[(int64_t)c * K + i];
+            for (int i = 0; i < V * K / 4; ++i) {
+                const float4 q = reinterpret_cast<const float4*>(src)[i];
+                v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < V * K; ++i) v[i] = src[i];
+        }
 #pragma unroll
         for (int i = 0; i < kPairs<V>; ++i) {
 #pragma unroll
@@ -148,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
         T* y = static_cast<T*>(p.y) + first_row(p.seqs, seq, s, yr) + c + j0 * ys;
         const T* xj = x + j0 * xs;
         float2 win[K][P];
-        auto step = [&](const Pack<T, V>& in, int t) {
+        auto step = [&](const Pack<T, V>& in) {
             shift(win);
             unpack<T, V>(in, win[K - 1]);
             float2 out[P];
@@ -157,7 +166,8 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
                 const float2 a = wt.at(win, q);
                 out[q] = p.silu ? fmul2(a, sigmoid2(a)) : a;
             }
-            store<T, V>(y + t * ys, out);
+            store<T, V>(y, out);
+            y += ys;
         };
 #pragma unroll
         for (int b = 0; b + 1 < kRing; ++b) {
@@ -174,11 +184,11 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
             cp_async_commit();
             if (t + kBlock <= count) {
 #pragma unroll
-                for (int i = 0; i < kBlock; ++i) step(in[i], t + i);
+                for (int i = 0; i < kBlock; ++i) step(in[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i + 1 < kBlock; ++i)
-                    if (t + i < count) step(in[i], t + i);
+                    if (t + i < count) step(in[i]);
             }
         }
         cp_async_wait<0>();
@@ -290,7 +300,10 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) conv_bwd_kernel(const Co
 #pragma unroll
                         for (int q = 0; q < P; ++q) out[q] = fadd2(out[q], f[q]);
                     }
-                    if (kInner || j >= 0) store<T, V>(dx + j * ys, out);
+                    if (kInner || j >= 0) {
+                        store<T, V>(dx, out);
+                        dx += ys;
+                    }
                     else store<T, V>(di + (j + K - 1) * p.channels, out);
                 }
             };

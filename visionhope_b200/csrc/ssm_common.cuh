@@ -262,7 +262,12 @@ __device__ __forceinline__ float exp2_fma(float s, float a) {
     return fabsf(x) <= 126.f ? y : ex2(x);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.f, 1.f + ex2(-kLog2e * x)); }
+__device__ __forceinline__ float rcp(float x) {  // of a normal number or infinity
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
 // Two of them with one reciprocal, 1 / a = b / (a b): three operations of the special-function unit
 // in place of four.  exp(-x) is held to 2^60, so that a b is finite: below x = -41 the result is
 // 2^-60.
@@ -270,7 +275,7 @@ __device__ __forceinline__ float2 sigmoid2(float2 x) {
     const float2 m = fmul2(x, splat2(-kLog2e));
     constexpr float kMost = 1.152921504606846976e18f;
     const float2 d = fadd2(make_float2(fminf(ex2(m.x), kMost), fminf(ex2(m.y), kMost)), splat2(1.f));
-    const float r = __fdividef(1.f, d.x * d.y);
+    const float r = rcp(d.x * d.y);
     return make_float2(r * d.y, r * d.x);
 }
 
