@@ -1,4 +1,10 @@
 // Selective scan, forward and one-token step (vh_ssm_scan_fwd, vh_ssm_scan_step).
+//
+// The forward is bound by its exponentials and the arithmetic around them, not by memory: two
+// images of 64 x 256 tokens, 384 channels, 16 states, bf16 (12.6 M elements, 103 MB) take 165 us,
+// where the bytes would take 16 and the exponentials alone 45 for each of the two passes over a
+// chain in segments.  The special-function unit is at 56 / 44 %, the FMA pipe at 58 / 53 % and
+// instruction issue at 55 / 57 % in the first / last kernel (69 and about 90 us).
 #include "ssm_scan.cuh"
 
 namespace vh {
@@ -7,7 +13,7 @@ namespace {
 
 constexpr int kWarps = 4;  // warps per CTA: neighbouring channel tiles
 
-constexpr int kAhead = 2;  // groups fetched ahead
+constexpr int kAhead = 2;  // groups fetched ahead (the latency of memory is about two groups' work)
 
 // Shared memory of a warp.
 template <typename T, int NL>
@@ -258,7 +264,9 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
 // One token per stream.  NL = N / 4 lanes share NL channels: a lane loads u, delta and z of its own
 // channel and finishes its y, and holds four states of all NL channels; s and s u of a channel
 // come from its lane, y's sums go back there.  A block keeps its channels' rates over several
-// streams where registers allow.
+// streams where registers allow.  Bound by latency: 256 streams of 2048 channels, 16 states, bf16,
+// take 20 us for 71 MB (3.6 TB/s; the peak's 11 us would need more than the 32 warps of 64 registers
+// an SM holds).  A softplus in every lane and rates read for every stream took 31.
 template <typename T, int NL>
 __global__ void __launch_bounds__(256, NL <= 4 ? 4 : 1) scan_step_kernel(const ScanParams p, const float* state, float* state_out,
                                                         const int32_t* __restrict__ index, int32_t slots) {
@@ -336,10 +344,12 @@ __global__ void __launch_bounds__(256, NL <= 4 ? 4 : 1) scan_step_kernel(const S
 
 bool stride_ok(int64_t v, int m) { return v % m == 0; }
 
-// Warps that a B200 holds of the forward kernel (four CTAs of four an SM).
+// Warps that a B200 holds of the forward kernel (four CTAs of four an SM).  Segments against whole
+// chains of 784 tokens, bf16, by device time: 256 chains 97 against 210 us, 512 168 / 210, 704 222 /
+// 257, 768 235 / 257, 832 261 / 257: whole chains from a third of the warps on.
 int64_t fwd_warps() { return (int64_t)16 * sm_count(); }
 
-int fwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, fwd_warps() / 4, fwd_warps(), kGroup); }
+int fwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, fwd_warps() / 3, fwd_warps(), kGroup); }
 
 template <typename T, int NL>
 int launch_fwd(const ScanParams& p, const Segments& g, cudaStream_t st) {
@@ -430,9 +440,13 @@ int64_t checkpoint_floats(const vh_ssm_scan_args* a) {
 int segment_size(const vh_ssm_scan_args* a, int64_t enough, int64_t warps, int step) {
     const int64_t tiles = tile_count(a), tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
     // The host does not know the lengths of packed sequences: any of them may hold most tokens, so
-    // they are always cut, and twice as fine, because a sequence's last segment is a short one.
+    // they are always cut, and twice as fine, because a sequence's last segment is a short one (17
+    // sequences of 8192 tokens, 1024 channels: 128 us, against 135 as fine and 137 four times as).
+    // With few segments to a chain one wave of warps is badly filled, and two are better (forward of
+    // 512 chains of 784 tokens: 168 against 185 us; of 768: 235 / 289; but of 384: 139 / 133).
     if (a->seq_offsets) warps *= 2;
     else if (a->batch * tiles >= enough) return 0;
+    else if (a->batch * tiles * 5 >= warps) warps *= 2;
     int64_t size = (tokens * tiles + warps - 1) / warps;
     size = std::max<int64_t>((size + step - 1) / step * step, kCheckpoint);
     if (!a->seq_offsets) {
@@ -461,7 +475,8 @@ void place_segments(const vh_ssm_scan_args* a, int size, void* workspace, Segmen
 
 int enter_segments(const ScanParams& p, int states, const Segments& g, const float* first, bool right, cudaStream_t st) {
     // Long chains, of which there are few, are cut into runs; a packed sequence may hold most of the
-    // slots.
+    // slots.  The forward's time with 1 / 4 / 16 runs: 7 segments of 128 chains 29 / 32 / 38 us, 18
+    // of 128 122 / 117 / 121, 74 of 32 63 / 59 / 53, 98 of 24 183 / 173 / 164.
     const int64_t chains = (int64_t)p.seqs.count * p.groups * p.tiles_per_group;
     const int64_t segs = p.seqs.offsets ? std::min<int64_t>(g.slots, 4 * (g.slots / p.seqs.count + 1)) : g.slots / p.seqs.count;
     return with_states(states, [&](auto nl) {

@@ -17,7 +17,12 @@
 // the first of these passes takes all its decays from the special-function unit; the second one's
 // carry the gradient along the whole sequence (see ssm_scan.cuh on the exponentials).  Sums over
 // channels (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias)
-// one per CTA, and small kernels add them in order.
+// one per sequence or segment, and small kernels add them in order.
+//
+// 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 490 us, 375 of them
+// this walk.  It is held by the 8 warps an SM that 255 registers leave: instruction issue is at
+// 39 %, shared memory at 63 %, the special-function unit at 27 %, DRAM at 8 % (243 MB).  Two
+// channels a thread would let 12 warps in, but at 289 M instructions for 186 M: 476 us against 440.
 #include "ssm_scan.cuh"
 
 namespace vh {
@@ -25,7 +30,8 @@ namespace ssm {
 namespace {
 
 constexpr int kGroups = kCheckpoint / kGroup;  // groups in a chunk
-// Warps per CTA (neighbouring channel tiles): what the shared memory of half an SM holds.
+// Warps per CTA (neighbouring channel tiles): two CTAs an SM, in shared memory (fp32 groups take more of
+// it) and registers.
 template <typename T>
 constexpr int kBwdWarps = sizeof(T) == 4 ? 3 : 4;
 
@@ -512,10 +518,14 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
 struct Layout {
     int64_t tokens, rows, bc, a, d, total;  // floats
 };
-// Warps that a B200 holds of the backward kernel (two CTAs of three or four an SM).
+// Warps that a B200 holds of the backward kernel (two CTAs of three or four an SM).  Segments against
+// whole chains of 784 tokens, by device time: bf16, 256 chains 262 against 561 us, 640 602 / 740, 768
+// 709 / 749, 832 748 / 750; fp32, 512 580 / 717, 640 718 / 726, 768 893 / 727: whole chains from two
+// thirds of the warps on.  Four segments a warp even out the last wave: 512 chains 497 us against 533
+// with one and 560 with two, 128 chains of 2048 tokens 319 / 345 / 336; eight gain no more (491, 336).
 int64_t bwd_warps(const vh_ssm_scan_args* a) { return (int64_t)(a->dtype == VH_F32 ? 6 : 8) * sm_count(); }
 
-int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) / 2, 4 * bwd_warps(a), kCheckpoint); }
+int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) * 2 / 3, 4 * bwd_warps(a), kCheckpoint); }
 
 Layout layout_of(const vh_ssm_scan_args* a, int size) {
     Layout l;
