@@ -235,7 +235,7 @@ def test_scan_packed(dtype, reverse, offsets):
 @pytest.mark.parametrize("n,offsets,reverse", [(16, None, False), (16, [0, 5, 700, 700, 2100], True), (8, None, True),
                                                (64, [0, 1100, 1101], False), (4, None, False)])
 def test_scan_long_chains(dtype, n, offsets, reverse):
-    """Few chains of up to 2100 tokens: many warps, and clusters of CTAs, share a chain."""
+    """Few chains of up to 2100 tokens: many warps share a chain."""
     gen = torch.Generator().manual_seed(n)
     lead = (1, 2100) if offsets is None else (offsets[-1],)
     count = 1 if offsets is None else len(offsets) - 1
@@ -246,6 +246,13 @@ def test_scan_many_chains():
     """More than eight chains a multiprocessor: one warp walks each."""
     gen = torch.Generator().manual_seed(1)
     _scan_check(_scan_case(gen, (320, 37), 320, 132, 16, torch.float32), torch.float32, gen)
+
+
+@pytest.mark.parametrize("chains", [480, 640, 800])
+def test_scan_chains_around_the_choices(chains):
+    """Forward and backward in segments, the forward alone, neither."""
+    gen = torch.Generator().manual_seed(chains)
+    _scan_check(_scan_case(gen, (chains, 67), chains, 9, 16, torch.float32), torch.float32, gen)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

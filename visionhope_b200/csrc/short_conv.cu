@@ -3,7 +3,7 @@
 //
 //   c_t = bias + sum_k w_k x_{t-K+1+k},   y_t = c_t or silu(c_t)
 //
-// A thread owns V neighbouring channels (four) and walks runs of tokens with the last K inputs in
+// A thread owns V neighbouring channels (8 bytes of them, or one) and walks runs of tokens with the last K inputs in
 // registers, so each input is read once, plus K - 1 rows of halo per run.  There is no reuse beyond
 // the window and 2 K flops per element, so what counts is bytes in flight and few instructions per
 // element.  A thread therefore fetches its tokens into shared memory of its own two blocks of four
@@ -14,8 +14,8 @@
 //
 // 64 sequences of 3136 tokens, 128 channels, K = 4, silu, bf16: forward 24 us (103 MB, 4.3 TB/s),
 // backward 49 us (154 MB, 3.1 TB/s), its sums over blocks 3.  Instruction issue is at 51 and 45 %,
-// DRAM at 30 %.  16-byte accesses (eight channels a thread, half the threads) took 33 against 31 us,
-// blocks of eight tokens 42 against 39.  24 packed sequences of 16384 tokens, 1024 channels: 20 us
+// DRAM at 30 %.  Accesses of 16 bytes (eight channels a thread, half the threads) took 33 against
+// 31 us, blocks of eight tokens 42 against 39.  24 packed sequences of 16384 tokens, 1024 channels: 20 us
 // (67 MB, 3.4 TB/s).  The step of 256 streams of 2048 channels: 5.3 us, two dependent latencies.
 #include <algorithm>
 #include <type_traits>
@@ -438,14 +438,10 @@ int with_taps(int taps, F&& f) {
         default: return f(std::integral_constant<int, 8>{});
     }
 }
-// V channels at a time: `bytes` (16, 8 or 0, one channel) is what every row's start is a multiple
-// of; MOST bytes an access.
-template <typename T, int MOST, typename F>
-int with_width(int bytes, F&& f) {
-    if constexpr (MOST >= 16) {
-        if (bytes == 16) return f(std::integral_constant<int, 16 / (int)sizeof(T)>{});
-    }
-    if (bytes >= 8) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{});
+// V channels at a time: 8 bytes of them where `wide`, else one.
+template <typename T, typename F>
+int with_width(bool wide, F&& f) {
+    if (wide) return f(std::integral_constant<int, 8 / (int)sizeof(T)>{});
     return f(std::integral_constant<int, 1>{});
 }
 
@@ -466,17 +462,14 @@ int check_conv(const char* what, const vh_short_conv_args* a) {
     return 0;
 }
 
-// The widest access, in bytes, that every row's start and the channel count are multiples of.
-int conv_bytes(const vh_short_conv_args* a, std::initializer_list<const void*> more) {
+// Whether every row's start and the channel count are multiples of 8 bytes.
+bool conv_wide(const vh_short_conv_args* a, std::initializer_list<const void*> more) {
     const int64_t es = (int64_t)dtype_size(a->dtype);
-    for (int bytes : {16, 8}) {
-        bool v = a->channels * es % bytes == 0 && a->x_token_stride * es % bytes == 0 &&
-                 (a->seq_offsets || a->x_batch_stride * es % bytes == 0);
-        for (const void* t : {a->x, a->initial_state}) v = v && (!t || aligned(t, bytes));
-        for (const void* t : more) v = v && (!t || aligned(t, bytes));
-        if (v) return bytes;
-    }
-    return 0;
+    bool v = a->channels * es % 8 == 0 && a->x_token_stride * es % 8 == 0 &&
+             (a->seq_offsets || a->x_batch_stride * es % 8 == 0);
+    for (const void* t : {a->x, a->initial_state}) v = v && (!t || aligned(t, 8));
+    for (const void* t : more) v = v && (!t || aligned(t, 8));
+    return v;
 }
 
 ConvParams conv_params(const vh_short_conv_args* a) {
@@ -531,10 +524,10 @@ extern "C" int vh_short_conv_fwd(const vh_short_conv_args* a, vh_stream_t stream
     clear_error();
     if (int rc = check_conv("vh_short_conv_fwd", a)) return rc;
     ConvParams p = conv_params(a);
-    const int bytes = conv_bytes(a, {a->y, a->final_state});
+    const bool wide = conv_wide(a, {a->y, a->final_state});
     return with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width<T, 8>(bytes, [&](auto width) {
+        return with_width<T>(wide, [&](auto width) {
             constexpr int V = decltype(width)::value;
             const Plan b = plan(a, V, kFwdBlocks);
             p.run = b.run;
@@ -575,14 +568,14 @@ extern "C" int vh_short_conv_bwd(const vh_short_conv_args* a, const void* grad_y
     if (workspace_bytes < vh_short_conv_bwd_workspace_bytes(a) || !aligned(workspace, 4))
         return fail(VH_E_ARG, "vh_short_conv_bwd: workspace too small");
     ConvParams p = conv_params(a);
-    const int bytes = conv_bytes(a, {grad_y, grad_final, grad_x, grad_initial});
+    const bool wide = conv_wide(a, {grad_y, grad_final, grad_x, grad_initial});
     p.dy = grad_y; p.dfinal = grad_final; p.dx = grad_x; p.dinitial = grad_initial;
     p.partial = static_cast<float*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int blocks = 0;
     const int rc = with_dtype(a->dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width<T, 8>(bytes, [&](auto width) {
+        return with_width<T>(wide, [&](auto width) {
             constexpr int V = decltype(width)::value;
             const Plan b = plan(a, V, kBwdBlocks);
             p.run = b.run;
@@ -618,10 +611,10 @@ extern "C" int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t
         return fail(VH_E_ALIGN, "vh_short_conv_step: misaligned pointers");
     if (slots <= 0 || (!slots_index && slots < batch))
         return fail(VH_E_SHAPE, "vh_short_conv_step: %d slots for %d streams", slots, batch);
-    const int bytes = conv_bytes(&a, {state, (const void*)state_out, (const void*)y});
+    const bool wide = conv_wide(&a, {state, (const void*)state_out, (const void*)y});
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        return with_width<T, 8>(bytes, [&](auto width) {
+        return with_width<T>(wide, [&](auto width) {
             constexpr int V = decltype(width)::value;
             const int cgroups = (channels + V - 1) / V;
             const int64_t items = (int64_t)batch * cgroups;
