@@ -1,4 +1,4 @@
-"""The selective state space operators in plain PyTorch, token by token: the checker of
+"""The selective state space operators in plain PyTorch, token by token: the oracle of
 ``visionhope_b200.ssm_core``.  Run it in float64; autograd gives the gradients.
 
 ``offsets`` (a list) splits packed ``[tokens, channels]`` rows into sequences; without it the rows are

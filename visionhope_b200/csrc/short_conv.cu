@@ -3,20 +3,21 @@
 //
 //   c_t = bias + sum_k w_k x_{t-K+1+k},   y_t = c_t or silu(c_t)
 //
-// A thread owns V neighbouring channels (8 bytes of them, or one) and walks runs of tokens with the last K inputs in
-// registers, so each input is read once, plus K - 1 rows of halo per run.  There is no reuse beyond
-// the window and 2 K flops per element, so what counts is bytes in flight and few instructions per
-// element.  A thread therefore fetches its tokens into shared memory of its own two blocks of four
-// ahead (asynchronous copies take no registers; plain loads in one block took 95 us for what now
-// takes 76), and runs are as long as one wave of threads allows, so that weights, halo and the search
-// for the sequence are paid once for many tokens (runs of 8, 16 and 24 tokens: 42, 36 and 35 us
-// against 31 at the time).
+// A thread owns V neighbouring channels (8 bytes of them, or one) and walks runs of tokens with the
+// last K inputs in registers, so each input is read once, plus K - 1 rows of halo per run.  There is
+// no reuse beyond the window and 2 K flops per element, so what counts is bytes in flight and few
+// instructions per element.  A thread therefore fetches its tokens into shared memory of its own two
+// blocks of four ahead (asynchronous copies take no registers; forward and backward of the sizes
+// below took 80 us with them and 95 with plain loads), and runs are as long as one
+// wave of threads allows, so that weights, halo and the search for the sequence are paid once for
+// many tokens (forward with runs of 8, 16 and 24 tokens: 42, 36 and 35 us against 31 at the time).
 //
 // 64 sequences of 3136 tokens, 128 channels, K = 4, silu, bf16: forward 24 us (103 MB, 4.3 TB/s),
-// backward 49 us (154 MB, 3.1 TB/s), its sums over blocks 3.  Instruction issue is at 51 and 45 %,
-// DRAM at 30 %.  Accesses of 16 bytes (eight channels a thread, half the threads) took 33 against
-// 31 us, blocks of eight tokens 42 against 39.  24 packed sequences of 16384 tokens, 1024 channels: 20 us
-// (67 MB, 3.4 TB/s).  The step of 256 streams of 2048 channels: 5.3 us, two dependent latencies.
+// backward 49 us (154 MB, 3.1 TB/s), its sums over blocks 3.  Instruction issue is at 47 and 45 %,
+// DRAM at about 30 %.  Accesses of 16 bytes (eight channels a thread, half the threads) took 33
+// against 31 us, blocks of eight tokens 42 against 39.  24 packed sequences of 16384 tokens, 1024
+// channels: 20 us (67 MB, 3.4 TB/s).  The step of 256 streams of 2048 channels: 5.3 us, two dependent
+// latencies.
 #include <algorithm>
 #include <type_traits>
 

@@ -21,7 +21,7 @@
 //
 // 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 490 us, 375 of them
 // this walk.  It is held by the 8 warps an SM that 255 registers leave: instruction issue is at
-// 39 %, shared memory at 63 %, the special-function unit at 27 %, DRAM at 8 % (243 MB).  Two
+// 39 %, shared memory at 64 %, the special-function unit at 27 %, DRAM at 8 % (243 MB).  Two
 // channels a thread would let 12 warps in, but at 289 M instructions for 186 M: 476 us against 440.
 #include "ssm_scan.cuh"
 
