@@ -475,10 +475,11 @@ int vh_residual_add_bwd(const float* grad_out, const void* branch, int32_t branc
  *
  * Sequences.  With seq_offsets NULL there are `batch` sequences of `length` tokens; element
  * (sequence s, token t, channel c) of a tensor is at base + s * batch_stride + t * token_stride
- * + c (unit channel stride).  With seq_offsets (device, int32 [batch + 1]: 0 first, never
- * decreasing, `length` last) the sequences lie one after another over `length` tokens in all and
- * batch strides are ignored; sequences may be empty.  The offsets are read on the device: values
- * outside [0, length] are clamped, and rows that no sequence covers are not written.
+ * + c (unit channel stride).  With seq_offsets (device, int32 [batch + 1], never decreasing, from
+ * 0 to `length`) the sequences lie one after another over `length` tokens in all and batch strides
+ * are ignored; sequences may be empty.  The offsets are read on the device: values outside
+ * [0, length] are clamped, and rows before the first and from the last one on, which no sequence
+ * covers, get zeros in every output and gradient.
  * reverse != 0 reads each sequence from its last token to its first (states then enter at the
  * last token and leave at the first).  Outputs are contiguous, [tokens, channels].
  * -------------------------------------------------------------------------------------*/

@@ -414,6 +414,50 @@ def test_offsets_out_of_range_are_clamped():
     assert torch.equal(late[43:], a[43:])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [5, 24])
+@pytest.mark.parametrize("op", ["conv", "scan"])
+def test_rows_of_no_sequence_are_zero(op, d, dtype):
+    """A packed buffer longer than its sequences: NaN before and behind them reaches nothing."""
+    from visionhope_b200 import ssm_core
+
+    gen = torch.Generator().manual_seed(d)
+    if op == "conv":
+        base, rows = _conv_case(gen, (54,), 3, d, 4, dtype), ("x",)
+        bars = dict(y=1e-6, final=1e-6, grad=5e-6)
+    else:
+        base, rows = _scan_case(gen, (54,), 3, d, 16, dtype), ("u", "delta", "B", "C", "z")
+        bars = dict(y=5e-6, final=5e-6, grad=2e-5)
+    gy, inside = _rand(gen, 54, d, dtype=dtype), slice(3, 57)
+
+    def padded(t):
+        out = torch.full((70, *t.shape[1:]), float("nan"), dtype=t.dtype)
+        out[inside] = t
+        return out
+
+    ref = _leaves(base, True)
+    dev = _leaves({k: padded(t) if k in rows else t for k, t in base.items()}, False)
+    if op == "conv":
+        y, final = ssm_core.short_conv(dev["x"], dev["weight"], dev["bias"], activation="silu",
+                                       initial_state=dev["initial_state"], return_final_state=True,
+                                       seq_offsets=torch.tensor([3, 10, 10, 57], device=DEV))
+        ey, efinal = oracle.short_conv(ref["x"], ref["weight"], ref["bias"], activation="silu",
+                                       initial_state=ref["initial_state"], offsets=[0, 7, 7, 54])
+    else:
+        y, final = _scan_run(ssm_core, dev, offsets=[3, 10, 10, 57])
+        ey, efinal = _scan_run(oracle, ref, offsets=[0, 7, 7, 54])
+    gf = _rand(gen, *final.shape, dtype=final.dtype)
+    got = torch.autograd.grad([y, final], list(dev.values()), [padded(gy).to(DEV), gf.to(DEV)])
+    exp = torch.autograd.grad([ey, efinal], list(ref.values()), [gy.double(), gf.double()])
+    results = {"y": (y, ey, bars["y"]), "final": (final, efinal, bars["final"])}
+    results.update({"d_" + n: (g, e, bars["grad"]) for n, g, e in zip(dev, got, exp)})
+    for n, (a, e, bar) in results.items():
+        if a.shape[0] == 70:
+            assert (a[:3] == 0).all() and (a[57:] == 0).all(), n
+            a = a[inside]
+        _close(a, e, bar, n)
+
+
 def test_side_stream_and_empty_inputs():
     from visionhope_b200 import ssm_core
 

@@ -140,6 +140,17 @@ struct Ring {
 };
 __device__ __forceinline__ int next_slot(int slot) { return slot + 1 == kRing ? 0 : slot + 1; }
 
+// Zeros in the thread's channels of packed rows of no sequence: every `step`-th row from the `at`-th.
+template <typename T, int V>
+__device__ __forceinline__ void zero_rows(const ConvParams& p, void* out, int c, int64_t at, int64_t step) {
+    if (!p.seqs.offsets) return;
+    const Outside o(p.seqs);
+    float2 zero[kPairs<V>];
+#pragma unroll
+    for (int q = 0; q < kPairs<V>; ++q) zero[q] = make_float2(0.f, 0.f);
+    for (; at < o.count(); at += step) store<T, V>(static_cast<T*>(out) + o.row(at) * p.channels + c, zero);
+}
+
 // A block: `cblock` channel groups by kThreads / cblock runs, over channels and slots.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads, kFwdBlocks)
@@ -208,6 +219,7 @@ __global__ void __launch_bounds__(kThreads, kFwdBlocks)
             for (int k = 1; k < K; ++k) store<T, V>(f + (k - 1) * p.channels, win[k]);
         }
     }
+    zero_rows<T, V>(p, p.y, c, (int64_t)blockIdx.y * lanes + ri, (int64_t)gridDim.y * lanes);
 }
 
 // The backward.  With dc_t = dy_t act'(c_t) (zero outside the sequence):
@@ -347,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, kBwdBlocks) conv_bwd_kernel(const Co
             }
             cp_async_wait<0>();
         }
+        zero_rows<T, V>(p, p.dx, c, (int64_t)blockIdx.y * lanes + ri, (int64_t)gridDim.y * lanes);
     }
     // the block's sums: one value of every thread at a time, added over the runs in order
     __syncthreads();  // the rings are no longer read

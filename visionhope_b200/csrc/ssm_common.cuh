@@ -38,6 +38,35 @@ __device__ __forceinline__ Seq seq_at(const Seqs& q, int s) {
     return {lo, hi - lo};
 }
 
+// Packed rows of no sequence lie before the first offset and from the last one on (buffers may be
+// longer than what they hold).  Outputs and gradients are zero there.
+struct Outside {
+    int64_t first, last;  // rows [first, last) belong to sequences
+    int64_t length;
+    __device__ __forceinline__ explicit Outside(const Seqs& q) : first(0), last(INT64_MAX), length(INT64_MAX) {
+        if (!q.offsets) return;
+        length = q.length;
+        first = seq_at(q, 0).row;
+        const Seq e = seq_at(q, q.count - 1);
+        last = max(first, e.row + e.len);
+    }
+    __device__ __forceinline__ int64_t count() const { return first + length - last; }
+    __device__ __forceinline__ int64_t row(int64_t i) const { return i < first ? i : last + i - first; }
+    __device__ __forceinline__ bool has(int64_t row) const { return row < first || row >= last; }
+};
+// Zeros there in contiguous [rows][width] tensors (null: none); every thread of the grid takes part.
+template <typename T>
+__device__ __forceinline__ void zero_outside(const Seqs& q, int width, void* a, void* b = nullptr, void* c = nullptr) {
+    if (!q.offsets) return;
+    const Outside o(q);
+    const int64_t n = o.count() * width;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t at = o.row(i / width) * width + i % width;
+        for (void* t : {a, b, c})
+            if (t) static_cast<T*>(t)[at] = from_f<T>(0.f);
+    }
+}
+
 // Slots of `step` tokens: sequence s owns the slots from slot_base on, at least one and at least
 // ceil(len / step).  Packed sequences: floor(lo / step) + s, because consecutive starts then
 // differ by floor(hi / step) - floor(lo / step) + 1 >= ceil((hi - lo) / step); the total is at

@@ -454,10 +454,13 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
 }
 
 // db and dc: the channel tiles' partials of each group added in order.  A thread adds four states
-// of one state lane j (j, j + N / 4, ...).
+// of one state lane j (j, j + N / 4, ...).  Rows of no sequence get zeros, in every gradient.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const float4* __restrict__ part, T* __restrict__ db, T* __restrict__ dc,
-                                                     int64_t tokens, int groups, int tiles, int n) {
+__global__ void __launch_bounds__(256) sum_bc_kernel(const BwdParams p, T* __restrict__ db, T* __restrict__ dc, int tiles, int n) {
+    const float4* part = reinterpret_cast<const float4*>(p.part_bc);
+    const int64_t tokens = p.tokens;
+    const int groups = p.f.groups;
+    zero_outside<T>(p.f.seqs, p.f.channels, p.du, p.ddelta, p.dz);
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [token][group][db, dc][state lane]
     const int per = n / 2;
     if (i >= tokens * groups * per) return;
@@ -466,7 +469,8 @@ __global__ void __launch_bounds__(256) sum_bc_kernel(const float4* __restrict__ 
     const int64_t t = tg / groups;
     const int gr = (int)(tg % groups);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < tiles; ++k) {
+    const bool none = Outside(p.f.seqs).has(t);
+    for (int k = 0; k < tiles && !none; ++k) {
         const float4 v = part[((int64_t)(gr * tiles + k) * tokens + t) * per + w];
         sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
     }
@@ -633,8 +637,7 @@ extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, i
         if (outs == 0) return 0;
         const int64_t grid = (outs + 255) / 256;
         if (grid > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many tokens");
-        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(reinterpret_cast<const float4*>(p.part_bc), static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c),
-                                                    l.tokens, f->groups, p.f.tiles_per_group, f->states);
+        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(p, static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c), p.f.tiles_per_group, f->states);
         return launch_status("selective scan backward: b, c");
     });
 }

@@ -124,8 +124,9 @@ def short_conv(x, weight, bias=None, *, activation=None, initial_state=None, ret
     """``y_t = act(bias + sum_k weight[:, k] x_{t - taps + 1 + k})`` per channel and sequence.
 
     x: [B, L, C] (fp32, bf16 or fp16; any batch and token strides), or packed [T, C] with
-    ``seq_offsets`` [B + 1] (int32 or int64 on x's device: 0 first, never decreasing, T last;
-    sequences may be empty; the offsets are not read on the host).  weight: [C, taps], 2 to 8
+    ``seq_offsets`` [B + 1] (int32 or int64 on x's device, never decreasing, from 0 to T; sequences
+    may be empty; rows before the first offset and from the last one on belong to none and give
+    zeros, y's and the gradients'; the offsets are not read on the host).  weight: [C, taps], 2 to 8
     taps.  activation: None or "silu".  initial_state: [B, taps - 1, C] of x's dtype, the inputs
     before each sequence, oldest first (zeros when None).  reverse reads every sequence from its
     last token to its first.  Sums run in fp32 and y, of x's dtype, is rounded once.  Returns y,
