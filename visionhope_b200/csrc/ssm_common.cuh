@@ -54,13 +54,14 @@ struct Outside {
     __device__ __forceinline__ int64_t row(int64_t i) const { return i < first ? i : last + i - first; }
     __device__ __forceinline__ bool has(int64_t row) const { return row < first || row >= last; }
 };
-// Zeros there in contiguous [rows][width] tensors (null: none); every thread of the grid takes part.
+// Zeros there in contiguous [rows][width] tensors (null: none); every thread of `blocks` takes part.
 template <typename T>
-__device__ __forceinline__ void zero_outside(const Seqs& q, int width, void* a, void* b = nullptr, void* c = nullptr) {
+__device__ __forceinline__ void zero_outside(const Seqs& q, int width, int64_t block, int64_t blocks, void* a, void* b = nullptr,
+                                             void* c = nullptr) {
     if (!q.offsets) return;
     const Outside o(q);
     const int64_t n = o.count() * width;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    for (int64_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) {
         const int64_t at = o.row(i / width) * width + i % width;
         for (void* t : {a, b, c})
             if (t) static_cast<T*>(t)[at] = from_f<T>(0.f);

@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t item = (int64_t)blockIdx.x * kWarps + warp;
     if (OWN) launch_dependents();
-    else zero_outside<T>(p.seqs, p.channels, p.y);
+    else zero_outside<T>(p.seqs, p.channels, blockIdx.x, gridDim.x, p.y);
     Unit w;
     if (item >= items || !unit_at(p, g, item, w)) return;
     const int tiles = p.groups * p.tiles_per_group;

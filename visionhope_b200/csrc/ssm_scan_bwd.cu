@@ -19,7 +19,7 @@
 // channels (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias)
 // one per sequence or segment, and small kernels add them in order.
 //
-// 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 490 us, 375 of them
+// 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 488 us, 373 of them
 // this walk.  It is held by the 8 warps an SM that 255 registers leave: instruction issue is at
 // 39 %, shared memory at 64 %, the special-function unit at 27 %, DRAM at 8 % (243 MB).  Two
 // channels a thread would let 12 warps in, but at 289 M instructions for 186 M: 476 us against 440.
@@ -453,18 +453,28 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     }
 }
 
+// The sums that are left, in one launch (14 us of the sizes above, 9 + 13 in two): blocks of da, dD and
+// d delta_bias first (their columns are
+// long), then blocks of db and dc.
+struct Sums {
+    float *da, *dd, *dbias;
+    void *db, *dc;
+    int64_t rows;  // of part_a and part_d
+    int32_t row_blocks;
+};
+
 // db and dc: the channel tiles' partials of each group added in order.  A thread adds four states
 // of one state lane j (j, j + N / 4, ...).  Rows of no sequence get zeros, in every gradient.
-template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const BwdParams p, T* __restrict__ db, T* __restrict__ dc, int tiles, int n) {
+template <typename T, int NL>
+__device__ __forceinline__ void sum_bc_tiles(const BwdParams& p, const Sums& to, int64_t block, int64_t blocks) {
     const float4* part = reinterpret_cast<const float4*>(p.part_bc);
     const int64_t tokens = p.tokens;
-    const int groups = p.f.groups;
-    zero_outside<T>(p.f.seqs, p.f.channels, p.du, p.ddelta, p.dz);
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [token][group][db, dc][state lane]
-    const int per = n / 2;
+    const int groups = p.f.groups, tiles = p.f.tiles_per_group;
+    constexpr int per = 2 * NL;
+    zero_outside<T>(p.f.seqs, p.f.channels, block, blocks, p.du, p.ddelta, p.dz);
+    const int64_t i = block * 256 + threadIdx.x;  // over [token][group][db, dc][state lane]
     if (i >= tokens * groups * per) return;
-    const int w = (int)(i % per), nl = n / 4;
+    const int w = (int)(i % per);
     const int64_t tg = i / per;
     const int64_t t = tg / groups;
     const int gr = (int)(tg % groups);
@@ -474,28 +484,25 @@ __global__ void __launch_bounds__(256) sum_bc_kernel(const BwdParams p, T* __res
         const float4 v = part[((int64_t)(gr * tiles + k) * tokens + t) * per + w];
         sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
     }
-    T* out = (w < nl ? db : dc) + (t * groups + gr) * n + w % nl;
+    T* out = static_cast<T*>(w < NL ? to.db : to.dc) + (t * groups + gr) * 4 * NL + w % NL;
     out[0] = from_f<T>(sum.x);
-    out[nl] = from_f<T>(sum.y);
-    out[2 * nl] = from_f<T>(sum.z);
-    out[3 * nl] = from_f<T>(sum.w);
+    out[NL] = from_f<T>(sum.y);
+    out[2 * NL] = from_f<T>(sum.z);
+    out[3 * NL] = from_f<T>(sum.w);
 }
 
-// da, dD and d delta_bias: the partials' rows added in order, 8 outputs by 32 row lanes per CTA.
+// da, dD and d delta_bias: the partials' rows added in order, 8 outputs by 32 row lanes per block.
 template <int NL>
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ pa, const float* __restrict__ pd, int64_t rows,
-                                                       int tiles, int per_group, int tiles_per_group, float* __restrict__ da,
-                                                       float* __restrict__ dd, float* __restrict__ dbias) {
+__device__ __forceinline__ void sum_rows(const BwdParams& p, const Sums& to, float (&red)[32][9]) {
     constexpr int CW = Tile<NL>::CW, N = 4 * NL;
-    __shared__ float red[32][9];
+    const int tiles_per_group = p.f.tiles_per_group, tiles = p.f.groups * tiles_per_group, per_group = p.f.per_group;
     const int x = threadIdx.x % 8, r = threadIdx.x / 8;
     const int64_t i = (int64_t)blockIdx.x * 8 + x, na = (int64_t)tiles * 512, nd = (int64_t)tiles * CW;
-    if ((int64_t)blockIdx.x * 8 >= na + 2 * nd) return;
-    const float* src = i < na ? pa + i : pd + (i - na);
+    const float* src = i < na ? p.part_a + i : p.part_d + (i - na);
     const int64_t stride = i < na ? na : 2 * nd;
     float sum = 0.f;
     if (i < na + 2 * nd)
-        for (int64_t k = r; k < rows; k += 32) sum += src[k * stride];
+        for (int64_t k = r; k < to.rows; k += 32) sum += src[k * stride];
     red[r][x] = sum;
     __syncthreads();
     for (int o = 16; o > 0; o >>= 1) {
@@ -514,9 +521,17 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
     const int at = (tile % tiles_per_group) * CW + c;
     if (at >= per_group) return;
     const int ch = tile / tiles_per_group * per_group + at;
-    if (i < na) da[(int64_t)ch * N + n] = red[0][x];
-    else if (i < na + nd) { if (dd) dd[ch] = red[0][x]; }
-    else if (dbias) dbias[ch] = red[0][x];
+    if (i < na) to.da[(int64_t)ch * N + n] = red[0][x];
+    else if (i < na + nd) { if (to.dd) to.dd[ch] = red[0][x]; }
+    else if (to.dbias) to.dbias[ch] = red[0][x];
+}
+
+template <typename T, int NL>
+__global__ void __launch_bounds__(256) sums_kernel(const BwdParams p, const Sums to) {
+    __shared__ float red[32][9];
+    wait_for_previous();
+    if ((int)blockIdx.x < to.row_blocks) sum_rows<NL>(p, to, red);
+    else sum_bc_tiles<T, NL>(p, to, (int64_t)blockIdx.x - to.row_blocks, (int64_t)gridDim.x - to.row_blocks);
 }
 
 struct Layout {
@@ -623,21 +638,13 @@ extern "C" int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* a, void* workspace, i
     const int tiles = p.f.groups * p.f.tiles_per_group;
     return with_dtype(f->dtype, [&](auto t) {
         using T = decltype(t);
-        int rc = with_states(f->states, [&](auto nl) {
+        return with_states(f->states, [&](auto nl) {
             constexpr int NL = decltype(nl)::value;
             if (int e = launch_bwd<T, NL>(p, g, st)) return e;
-            const int64_t outs = (int64_t)tiles * (512 + 2 * Tile<NL>::CW);
-            sum_rows_kernel<NL><<<(int)((outs + 7) / 8), 256, 0, st>>>(
-                p.part_a, p.part_d, l.rows, tiles, p.f.per_group, p.f.tiles_per_group, a->grad_a,
-                a->grad_d_skip, a->grad_delta_bias);
-            return launch_status("selective scan backward: parameters");
+            const int64_t row_blocks = ((int64_t)tiles * (512 + 2 * Tile<NL>::CW) + 7) / 8;
+            const int64_t bc_blocks = (l.tokens * f->groups * 2 * NL + 255) / 256;
+            const Sums to{a->grad_a, a->grad_d_skip, a->grad_delta_bias, a->grad_b, a->grad_c, l.rows, (int32_t)row_blocks};
+            return launch_after("selective scan backward: sums", sums_kernel<T, NL>, row_blocks + bc_blocks, 256, 0, st, p, to);
         });
-        if (rc) return rc;
-        const int64_t outs = l.tokens * f->groups * f->states / 2;
-        if (outs == 0) return 0;
-        const int64_t grid = (outs + 255) / 256;
-        if (grid > 0x7fffffff) return fail(VH_E_RANGE, "vh_ssm_scan_bwd: too many tokens");
-        sum_bc_kernel<T><<<(int)grid, 256, 0, st>>>(p, static_cast<T*>(a->grad_b), static_cast<T*>(a->grad_c), p.f.tiles_per_group, f->states);
-        return launch_status("selective scan backward: b, c");
     });
 }
