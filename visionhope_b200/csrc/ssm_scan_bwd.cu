@@ -17,7 +17,7 @@
 // the first of these passes takes all its decays from the special-function unit; the second one's
 // carry the gradient along the whole sequence (see ssm_scan.cuh on the exponentials).  Sums over
 // channels (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias)
-// one per sequence or segment, and small kernels add them in order.
+// one per sequence or segment, and a small kernel adds them in order.
 //
 // 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 488 us, 373 of them
 // this walk.  It is held by the 8 warps an SM that 255 registers leave: instruction issue is at
@@ -453,9 +453,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     }
 }
 
-// The sums that are left, in one launch (14 us of the sizes above, 9 + 13 in two): blocks of da, dD and
-// d delta_bias first (their columns are
-// long), then blocks of db and dc.
+// The sums that are left, in one launch (14 us at the sizes above; two took 9 and 13): blocks of da,
+// dD and d delta_bias first (their columns are long), then blocks of db and dc.
 struct Sums {
     float *da, *dd, *dbias;
     void *db, *dc;
