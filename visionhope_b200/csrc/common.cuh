@@ -103,26 +103,30 @@ __device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
 }
 
 // ---- asynchronous global -> shared copies (LDGSTS) ---------------------------------------
+// Each statement clobbers memory: the compiler then keeps a copy behind the reads of what it
+// overwrites, and the reads of what it brings behind the wait, where no barrier stands between.
 template <int BYTES>
 __device__ __forceinline__ void cp_async(void* smem_dst, const void* gmem_src) {
     static_assert(BYTES == 4 || BYTES == 8 || BYTES == 16, "cp.async size");
     const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst));
     if constexpr (BYTES == 16) {
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(gmem_src));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(gmem_src) : "memory");
     } else {
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(gmem_src),
-                     "n"(BYTES));
+                     "n"(BYTES)
+                     : "memory");
     }
 }
 // 16-byte copy that writes zeros instead when `valid` is false (no bytes are read then).
 __device__ __forceinline__ void cp_async16_zfill(void* smem_dst, const void* gmem_src, bool valid) {
     const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(smem_dst));
     const int n = valid ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(gmem_src), "r"(n));
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(gmem_src), "r"(n)
+                 : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::); }
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N)); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory"); }
 
 // ---- reductions ---------------------------------------------------------------------------
 __device__ __forceinline__ float warp_sum(float v) {
