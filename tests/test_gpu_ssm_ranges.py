@@ -1,0 +1,131 @@
+"""The selective state space operators over the whole range of their inputs: the functions inside
+them where they saturate, the lowest and infinite values that masks are made of.
+
+Bars, from the arithmetic.  A sigmoid is 1 / (1 + 2^(-x log2 e)) by ex2.approx (2^-22) and rcp.approx
+(2^-23); its argument carries the rounding of the product and of the constant, |x| (2^-24 + 2^-25).
+Relative to the value that is REL(x) = |x| 1e-7 + 1e-6 with the products behind it.  Below x = -87 the
+sigmoid is less than fp32's smallest normal number, 1.2e-38, and may be zero: TINY = |x| 1.2e-38 for
+|x| up to 104, past which the true value is smaller still: 2e-36.  A 16-bit
+result has to lie between the two ends of that interval rounded to 16 bits.  silu' = sg (1 + x (1 - sg)) is
+held to REL(x) of the sum of its terms' sizes, sg (1 + |x| (1 - sg)), and for x > 0 to the rounding of
+1 - sg, 2^-23, times x where it is not exactly zero (x < 18).
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda")
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+TINY = 2e-36
+
+
+def _values(dtype):
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    v = [low, -1e30, -1e20, -1e18, -60000.0, -1000.0, -200.0, -104.0, -90.0, -60.0, -42.0, -41.0, -20.0, -5.0, -1.0,
+         -1e-3, 0.0, 1e-3, 1.0, 5.0, 17.0, 20.0, 60.0, 100.0, 1000.0, 60000.0, 1e18, 1e30, high, -float("inf")]
+    return [x for x in v if x == -float("inf") or low <= x <= high]
+
+
+def _table(dtype, d=24):
+    """[sequences, 1, d]: every value beside many others, since neighbouring channels share instructions."""
+    v = _values(dtype)
+    rows = [[v[(b + c * (c + 1) // 2) % len(v)] for c in range(d)] for b in range(len(v))]
+    return torch.tensor(rows, dtype=torch.float64).to(dtype)[:, None]
+
+
+def _rel(x):
+    return x.abs().clamp_max(1e4) * 1e-7 + 1e-6
+
+
+def _check(got, want, bar, dtype):
+    got, want, bar = got.detach().double().cpu(), want.double(), bar.double()
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan)
+    got, want, bar = got[~nan], want[~nan], bar[~nan]
+    low, high = want - bar - TINY, want + bar + TINY
+    if dtype != torch.float32:
+        low, high = low.to(dtype).double(), high.to(dtype).double()
+    off = torch.maximum(low - got, got - high)
+    worst = int(off.argmax())
+    assert float(off[worst]) <= 0, (float(got[worst]), float(want[worst]), float(bar[worst]))
+
+
+def _silu(x):
+    x = x.double()
+    y = x * torch.sigmoid(x)
+    return y, _rel(x) * y.abs()
+
+
+def _silu_slope(x):
+    x = x.double()
+    sg = torch.sigmoid(x)
+    rest = torch.sigmoid(-x)
+    slope = sg + x * sg * rest
+    slope[x == float("-inf")] = float("nan")
+    bar = _rel(x) * sg * (1 + x.abs() * rest) + torch.where((x > 0) & (x < 18), x * 2.0 ** -23, torch.zeros_like(x))
+    bar = bar + torch.where(x >= 17, x.clamp(0, 1e3) * rest, torch.zeros_like(x))  # 1 - sg rounded away
+    return slope, bar
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [24, 7])
+def test_convolution_silu_saturates(dtype, d):
+    """One token through a convolution that passes it on: silu(x), its gradient and its step."""
+    from visionhope_b200.ssm_core import short_conv, short_conv_step
+
+    x = _table(dtype, d)
+    dev = x.to(DEV).requires_grad_()
+    w = torch.tensor([[0.0, 1.0]], device=DEV).expand(d, 2).contiguous()
+    y = short_conv(dev, w, activation="silu")
+    _check(y, *_silu(x), dtype)
+    g = torch.autograd.grad(y, dev, torch.ones_like(y))[0]
+    _check(g, *_silu_slope(x), dtype)
+    state = torch.zeros(x.shape[0], 1, d, dtype=dtype, device=DEV)
+    step = short_conv_step(dev.detach()[:, 0], state, w, activation="silu")
+    _check(step[:, None], *_silu(x), dtype)
+
+
+def _scan_args(x, dtype):
+    """A scan whose state stays zero and whose inner output is u = 1."""
+    b, _, d = x.shape
+    one, none = torch.ones(b, 1, d, dtype=dtype, device=DEV), torch.zeros(b, 1, 16, dtype=dtype, device=DEV)
+    return one, one, -torch.ones(d, 16, device=DEV), none, none, torch.ones(d, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [24, 7])
+def test_scan_gate_saturates(dtype, d):
+    """An inner output of one behind the gate: silu(z), its gradient and the step's."""
+    from visionhope_b200.ssm_core import ssm_scan, ssm_scan_step
+
+    z = _table(dtype, d)
+    dev = z.to(DEV).requires_grad_()
+    u, delta, A, B, C, D = _scan_args(z, dtype)
+    u = u.requires_grad_()
+    y = ssm_scan(u, delta, A, B, C, D, z=dev)
+    _check(y, *_silu(z), dtype)
+    gz, gu = torch.autograd.grad(y, [dev, u], torch.ones_like(y))
+    _check(gz, *_silu_slope(z), dtype)
+    _check(gu, *_silu(z), dtype)
+    state = torch.zeros(z.shape[0], d, 16, device=DEV)
+    step = ssm_scan_step(u.detach()[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], state, D, z=dev.detach()[:, 0])
+    _check(step[:, None], *_silu(z), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [24, 7])
+def test_masked_steps_get_no_gradient(dtype, d):
+    """softplus' derivative at the lowest value and at -inf is zero; at large values it is one."""
+    from visionhope_b200.ssm_core import ssm_scan
+
+    delta = torch.tensor([torch.finfo(dtype).min, -float("inf"), -200.0, -0.5, 0.5, 300.0], dtype=torch.float64).to(dtype)
+    delta = delta[(torch.arange(6)[:, None] + torch.arange(d) * (torch.arange(d) + 1) // 2) % 6][:, None]
+    dev = delta.to(DEV).requires_grad_()
+    u = torch.ones(6, 1, d, dtype=dtype, device=DEV)
+    bc = torch.ones(6, 1, 16, dtype=dtype, device=DEV)
+    y = ssm_scan(u, dev, torch.zeros(d, 16, device=DEV), bc, bc, delta_softplus=True)
+    g = torch.autograd.grad(y, dev, torch.ones_like(y))[0]
+    want = 16 * torch.sigmoid(delta.double())  # y = 16 softplus(delta)
+    _check(g, want, _rel(delta.double().clamp(-104, 104)) * want, dtype)
+    assert (g[delta.to(DEV) < -150] == 0).all()

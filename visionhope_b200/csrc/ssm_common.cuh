@@ -298,15 +298,13 @@ __device__ __forceinline__ float rcp(float x) {  // of a normal number or infini
     return y;
 }
 __device__ __forceinline__ float sigmoid(float x) { return rcp(1.f + ex2(-kLog2e * x)); }
-// Two of them with one reciprocal, 1 / a = b / (a b): three operations of the special-function unit
-// in place of four.  exp(-x) is held to 2^60, so that a b is finite: below x = -41 the result is
-// 2^-60.
+// Each with a reciprocal of its own.  One reciprocal for both, 1 / a = b / (a b), is an operation of the
+// special-function unit less, but a b has to be kept finite (the result then stays above a bound,
+// and times a large negative x grows with it) and a result of 1 comes out as 1 + O(2^-23) by its
+// neighbour, which x (1 - sigmoid(x)) in silu's derivative multiplies by x.
 __device__ __forceinline__ float2 sigmoid2(float2 x) {
-    const float2 m = fmul2(x, splat2(-kLog2e));
-    constexpr float kMost = 1.152921504606846976e18f;
-    const float2 d = fadd2(make_float2(fminf(ex2(m.x), kMost), fminf(ex2(m.y), kMost)), splat2(1.f));
-    const float r = rcp(d.x * d.y);
-    return make_float2(r * d.y, r * d.x);
+    const float2 m = fmul2(x, splat2(-kLog2e)), d = fadd2(make_float2(ex2(m.x), ex2(m.y)), splat2(1.f));
+    return make_float2(rcp(d.x), rcp(d.y));
 }
 
 // log(1 + exp(x)) without cancellation on either side: max(x, 0) + log1p(e), e = exp(-|x|) in
