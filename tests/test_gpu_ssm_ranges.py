@@ -129,3 +129,56 @@ def test_masked_steps_get_no_gradient(dtype, d):
     want = 16 * torch.sigmoid(delta.double())  # y = 16 softplus(delta)
     _check(g, want, _rel(delta.double().clamp(-104, 104)) * want, dtype)
     assert (g[delta.to(DEV) < -150] == 0).all()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_entry_points_pass_states_on_without_tokens(packed):
+    """The C entry points with a length of 0: states and their gradients pass through, parameters get
+    zeros.  (The Python functions answer such calls themselves.)"""
+    import ctypes
+
+    from visionhope_b200 import _lib
+
+    lib = _lib.load()
+    b, d, n, k = 3, 40, 16, 4
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    row = torch.zeros(64, device=DEV)  # stands for rows that are never read
+    off = torch.zeros(b + 1, dtype=torch.int32, device=DEV) if packed else None
+    h0, gf = (torch.randn(b, d, n, generator=gen, device=DEV) for _ in range(2))
+    s0, gs = (torch.randn(b, k - 1, d, generator=gen, device=DEV) for _ in range(2))
+    A, w = -torch.rand(d, n, generator=gen, device=DEV), torch.randn(d, k, generator=gen, device=DEV)
+    stream = _lib.stream_handle(DEV)
+    _lib.ensure_device(row)
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    r = row.data_ptr()
+    final, ck = torch.full_like(h0, 7.0), torch.zeros(b * 2 * 512, device=DEV)
+    a = _lib.VhSsmScanArgs(u=r, delta=r, z=None, b=r, c=r, u_token_stride=d, delta_token_stride=d, b_token_stride=n,
+                           c_token_stride=n, a=ptr(A), initial_state=ptr(h0), y=r, final_state=ptr(final),
+                           checkpoints=ptr(ck), seq_offsets=ptr(off), length=0, dtype=0, batch=b, channels=d, states=n,
+                           groups=1)
+    assert lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)) <= ck.numel() * 4
+    need = lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a))
+    ws = torch.empty(need + 16, dtype=torch.uint8, device=DEV)
+    _lib.check(lib.vh_ssm_scan_fwd(ctypes.byref(a), ptr(ws), need, stream), "vh_ssm_scan_fwd")
+    assert torch.equal(final, h0)
+    gi, ga, gd, gb = torch.full_like(h0, 7.0), torch.full_like(A, 7.0), torch.full((d,), 7.0, device=DEV), torch.full((d,), 7.0, device=DEV)
+    g = _lib.VhSsmScanBwdArgs(fwd=a, grad_y=r, grad_final=ptr(gf), grad_u=r, grad_delta=r, grad_z=None, grad_b=r, grad_c=r,
+                              grad_a=ptr(ga), grad_d_skip=ptr(gd), grad_delta_bias=ptr(gb), grad_initial=ptr(gi))
+    need = lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(g))
+    ws = torch.empty(need + 16, dtype=torch.uint8, device=DEV)
+    _lib.check(lib.vh_ssm_scan_bwd(ctypes.byref(g), ptr(ws), need, stream), "vh_ssm_scan_bwd")
+    assert torch.equal(gi, gf) and not ga.any() and not gd.any() and not gb.any()
+    kept, gw, gi = torch.full_like(s0, 7.0), torch.full_like(w, 7.0), torch.full_like(s0, 7.0)
+    c = _lib.VhShortConvArgs(x=r, x_token_stride=d, weight=ptr(w), initial_state=ptr(s0), y=r, final_state=ptr(kept),
+                             seq_offsets=ptr(off), length=0, dtype=0, activation=1, taps=k, batch=b, channels=d)
+    _lib.check(lib.vh_short_conv_fwd(ctypes.byref(c), stream), "vh_short_conv_fwd")
+    assert torch.equal(kept, s0)
+    need = lib.vh_short_conv_bwd_workspace_bytes(ctypes.byref(c))
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    _lib.check(lib.vh_short_conv_bwd(ctypes.byref(c), r, ptr(gs), r, ptr(gw), None, ptr(gi), ptr(ws), need, stream),
+               "vh_short_conv_bwd")
+    assert torch.equal(gi, gs) and not gw.any()
+    assert not row.any()

@@ -1,0 +1,28 @@
+"""What the selective state space entry points answer without a GPU: sizes and refusals at the edges
+of their arguments' ranges."""
+import ctypes
+
+import pytest
+
+from tests.test_oracle_ssm import _conv_args, _err, _fake, _scan_args
+
+
+def _bwd(lib, p, fwd):
+    return lib.VhSsmScanBwdArgs(fwd=fwd, grad_y=p, grad_final=None, grad_u=p, grad_delta=p, grad_z=p, grad_b=p, grad_c=p,
+                                grad_a=p, grad_d_skip=p, grad_delta_bias=p, grad_initial=None)
+
+
+@pytest.mark.parametrize("states", [4, 16, 64])
+@pytest.mark.parametrize("batch", [1, 2, 5000])
+@pytest.mark.parametrize("packed", [False, True])
+def test_sizes_for_sequences_without_tokens(packed, batch, states):
+    """A length of 0 is allowed: sizes come back, and the host is still there."""
+    from visionhope_b200 import _lib
+
+    lib, (p, keep) = _lib.load(), _fake()
+    a = _scan_args(_lib, p, length=0, batch=batch, states=states, seq_offsets=p if packed else None, checkpoints=p)
+    assert lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a)) >= 0 and _err(lib) == ""
+    assert lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)) >= 0
+    assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(_bwd(_lib, p, a))) > 0 and _err(lib) == ""
+    c = _conv_args(_lib, p, length=0, batch=batch, seq_offsets=p if packed else None)
+    assert lib.vh_short_conv_bwd_workspace_bytes(ctypes.byref(c)) > 0

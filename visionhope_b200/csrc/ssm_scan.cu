@@ -439,6 +439,7 @@ int64_t checkpoint_floats(const vh_ssm_scan_args* a) {
 }
 
 int segment_size(const vh_ssm_scan_args* a, int64_t enough, int64_t warps, int step) {
+    if (a->length == 0) return 0;
     const int64_t tiles = tile_count(a), tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
     // The host does not know the lengths of packed sequences: any of them may hold most tokens, so
     // they are always cut, and twice as fine, because a sequence's last segment is a short one (17
