@@ -26,3 +26,17 @@ def test_sizes_for_sequences_without_tokens(packed, batch, states):
     assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(_bwd(_lib, p, a))) > 0 and _err(lib) == ""
     c = _conv_args(_lib, p, length=0, batch=batch, seq_offsets=p if packed else None)
     assert lib.vh_short_conv_bwd_workspace_bytes(ctypes.byref(c)) > 0
+
+
+@pytest.mark.parametrize("change", [dict(states=12), dict(states=3), dict(states=516), dict(states=1 << 20), dict(states=-16),
+                                    dict(dtype=9), dict(batch=0), dict(groups=3), dict(length=-1), dict(length=1 << 31)])
+def test_sizes_of_unsupported_scans_are_zero(change):
+    """A query with arguments that the operator refuses gives 0, whatever the values."""
+    from visionhope_b200 import _lib
+
+    lib, (p, keep) = _lib.load(), _fake()
+    a = _scan_args(_lib, p, checkpoints=p, **change)
+    assert lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a)) == 0
+    assert lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a)) == 0
+    assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(_bwd(_lib, p, a))) == 0
+    assert lib.vh_ssm_scan_checkpoint_bytes(None) == 0

@@ -374,9 +374,8 @@ int launch_fwd(const ScanParams& p, const Segments& g, cudaStream_t st) {
 
 }  // namespace
 
-int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token) {
+int check_scan_sizes(const char* what, const vh_ssm_scan_args* a, bool one_token) {
     if (!a) return fail(VH_E_ARG, "%s: null argument struct", what);
-    if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->y) return fail(VH_E_ARG, "%s: null pointer argument", what);
     if (!dtype_ok(a->dtype)) return fail(VH_E_DTYPE, "%s: dtype must be VH_F32, VH_BF16 or VH_F16", what);
     if (a->states != 4 && a->states != 8 && a->states != 16 && a->states != 32 && a->states != 64)
         return fail(VH_E_SHAPE, "%s: states must be 4, 8, 16, 32 or 64 (got %d)", what, a->states);
@@ -384,6 +383,16 @@ int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token)
         return fail(VH_E_SHAPE, "%s: batch, channels and groups must be positive", what);
     if (a->channels % a->groups)
         return fail(VH_E_SHAPE, "%s: channels (%d) must be a multiple of groups (%d)", what, a->channels, a->groups);
+    if (one_token) return 0;
+    if (a->length < 0) return fail(VH_E_SHAPE, "%s: negative length", what);
+    if (a->length > 0x7fffffff) return fail(VH_E_RANGE, "%s: at most 2^31 - 1 tokens a sequence", what);
+    return 0;
+}
+
+int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token) {
+    if (!a) return fail(VH_E_ARG, "%s: null argument struct", what);
+    if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->y) return fail(VH_E_ARG, "%s: null pointer argument", what);
+    if (int rc = check_scan_sizes(what, a, one_token)) return rc;
     const size_t es = dtype_size(a->dtype);
     const void* typed[] = {a->u, a->delta, a->z, a->b, a->c, a->y};
     for (const void* t : typed)
@@ -391,11 +400,8 @@ int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token)
     if (!aligned(a->a, 16) || (a->initial_state && !aligned(a->initial_state, 16)) ||
         (a->final_state && !aligned(a->final_state, 16)) || (a->checkpoints && !aligned(a->checkpoints, 16)))
         return fail(VH_E_ALIGN, "%s: a and the states must be 16-byte aligned", what);
-    if (!one_token) {
-        if (a->length < 0) return fail(VH_E_SHAPE, "%s: negative length", what);
-        if (a->length > 0x7fffffff) return fail(VH_E_RANGE, "%s: at most 2^31 - 1 tokens a sequence", what);
-        if (a->seq_offsets && !aligned(a->seq_offsets, 4)) return fail(VH_E_ALIGN, "%s: misaligned offsets", what);
-    }
+    if (!one_token && a->seq_offsets && !aligned(a->seq_offsets, 4))
+        return fail(VH_E_ALIGN, "%s: misaligned offsets", what);
     return 0;
 }
 
@@ -498,9 +504,8 @@ using namespace vh;
 using namespace vh::ssm;
 
 extern "C" int64_t vh_ssm_scan_checkpoint_bytes(const vh_ssm_scan_args* a) {
-    if (!a || a->batch <= 0 || a->length < 0 || a->channels <= 0 || a->groups <= 0 || a->channels % a->groups ||
-        a->states < 4)
-        return 0;
+    clear_error();
+    if (check_scan_sizes("vh_ssm_scan_checkpoint_bytes", a, false)) return 0;
     return checkpoint_floats(a) * 4;
 }
 

@@ -453,6 +453,8 @@ __device__ __forceinline__ void sum_tokens(const float2 (&p)[kPairs<Tile<NL>::CE
 }
 
 // Validates the arguments shared by the entry points; 0 or a status.  `one_token`: the step.
+// The sizes alone are checked by the first, for queries that come before there are pointers.
+int check_scan_sizes(const char* what, const vh_ssm_scan_args* a, bool one_token);
 int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token);
 void fill_scan_params(const vh_ssm_scan_args* a, ScanParams* p);
 int64_t checkpoint_floats(const vh_ssm_scan_args* a);
