@@ -1,0 +1,67 @@
+"""What autograd is told about the selective state space operators: caches that change in place, and
+derivatives that there are none of."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda")
+
+
+def _conv(gen, b=2, L=5, d=8, k=4):
+    x, cache = torch.randn(b, L, d, generator=gen, device=DEV), torch.randn(b, k - 1, d, generator=gen, device=DEV)
+    return x, cache, torch.randn(d, k, generator=gen, device=DEV)
+
+
+def _scan(gen, b=2, L=5, d=8, n=16):
+    u, delta = (torch.randn(b, L, d, generator=gen, device=DEV) for _ in range(2))
+    B, C = (torch.randn(b, L, n, generator=gen, device=DEV) for _ in range(2))
+    return [u, delta, -torch.rand(d, n, generator=gen, device=DEV), B, C], torch.randn(b, d, n, generator=gen, device=DEV)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("op", ["conv", "scan"])
+def test_a_step_on_a_saved_cache_is_noticed(op, apart):
+    """Sequences that started from a cache, then a step that changes it, then the backward: it needs
+    the cache as it was, and raises.  A step into another tensor leaves the cache alone."""
+    from visionhope_b200.ssm_core import short_conv, short_conv_step, ssm_scan, ssm_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    if op == "conv":
+        x, cache, w = _conv(gen)
+        w.requires_grad_()
+        y = short_conv(x, w, initial_state=cache, activation="silu")
+        out = torch.empty_like(cache) if apart else None
+        with torch.no_grad():
+            short_conv_step(x[:, 0], cache, w, state_out=out)
+    else:
+        (u, delta, A, B, C), cache = _scan(gen)
+        w = A.requires_grad_()
+        y = ssm_scan(u, delta, A, B, C, initial_state=cache, delta_softplus=True)
+        out = torch.empty_like(cache) if apart else None
+        with torch.no_grad():
+            ssm_scan_step(u[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], cache, state_out=out)
+    if apart:
+        y.sum().backward()
+        assert torch.isfinite(w.grad).all()
+        assert out._version > 0 and cache._version == 0
+    else:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+@pytest.mark.parametrize("inside", [False, True])
+def test_steps_on_a_cache_of_inference_mode(inside):
+    """Inference tensors have no version to move; steps on them run, in and out of that mode."""
+    from visionhope_b200.ssm_core import short_conv_step, ssm_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    with torch.inference_mode():
+        x, cache, w = _conv(gen)
+        (u, delta, A, B, C), state = _scan(gen)
+    before = cache.clone(), state.clone()
+    with torch.inference_mode(inside):
+        short_conv_step(x[:, 0], cache, w)
+        ssm_scan_step(u[:, 0], delta[:, 0].abs(), A, B[:, 0], C[:, 0], state)
+    assert torch.equal(cache[:, :-1], before[0][:, 1:]) and torch.equal(cache[:, -1], x[:, 0])
+    assert not torch.equal(state, before[1])

@@ -3,6 +3,7 @@
 A step of a small batch takes the GPU a few microseconds, so the host's part counts: the C structs are
 packed in one go (``struct.Struct``) and every check runs on values that are already at hand."""
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _lib
 
@@ -127,6 +128,13 @@ def cache(t, out, tail, batch, slots, dtype, device):
     if slots is None and t.shape[0] < batch:
         raise ValueError(f"the state has {t.shape[0]} slots for {batch} streams")
     return t, out
+
+
+def wrote(t):
+    """Tells autograd that a kernel changed ``t`` in place, as an in-place operation would: a backward
+    that saved it then raises instead of reading the new values."""
+    if not t.is_inference():
+        increment_version(t)
 
 
 def ptr(t):

@@ -166,4 +166,5 @@ def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None,
     _lib.check(_lib.load().vh_short_conv_step(
         x.data_ptr(), x.stride(0), code, weight.data_ptr(), ptr(bias), act, state.data_ptr(), state_out.data_ptr(),
         ptr(slots), state.shape[0], y.data_ptr(), b, d, k, _lib.stream_handle(device)), "vh_short_conv_step")
+    _args.wrote(state_out)
     return y

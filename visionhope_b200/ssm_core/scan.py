@@ -187,4 +187,5 @@ def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, 
         return y
     _lib.check(_lib.load().vh_ssm_scan_step(call.args(y.data_ptr()), state.data_ptr(), state_out.data_ptr(),
                                             ptr(slots), state.shape[0], _lib.stream_handle(device)), "vh_ssm_scan_step")
+    _args.wrote(state_out)
     return y
