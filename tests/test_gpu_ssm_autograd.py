@@ -65,3 +65,75 @@ def test_steps_on_a_cache_of_inference_mode(inside):
         ssm_scan_step(u[:, 0], delta[:, 0].abs(), A, B[:, 0], C[:, 0], state)
     assert torch.equal(cache[:, :-1], before[0][:, 1:]) and torch.equal(cache[:, -1], x[:, 0])
     assert not torch.equal(state, before[1])
+
+
+def test_steps_have_no_backward():
+    """Inputs or parameters that require gradients: the step runs, and a backward through its y raises
+    in place of leaving them out.  A cache that requires gradients is refused and stays as it is."""
+    from visionhope_b200.ssm_core import short_conv_step, ssm_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x, cache, w = _conv(gen)
+    (u, delta, A, B, C), state = _scan(gen)
+    bias = torch.zeros(8, device=DEV)
+    conv = dict(x=x[:, 0], state=cache, weight=w, bias=bias)
+    scan = dict(u=u[:, 0], delta=delta[:, 0].abs(), A=A, B=B[:, 0], C=C[:, 0], state=state, D=bias, z=x[:, 0], delta_bias=bias)
+    for step, args in ((short_conv_step, conv), (ssm_scan_step, scan)):
+        plain = {k: t.clone() for k, t in args.items()}
+        want = step(**plain)
+        assert not want.requires_grad
+        for name in args:
+            given = {k: t.clone() for k, t in args.items()}
+            given[name].requires_grad_()
+            if name == "state":
+                with pytest.raises(RuntimeError, match="cache requires gradients"):
+                    step(**given)
+                assert torch.equal(given["state"], args["state"])
+                out = torch.zeros_like(args["state"])  # read only: as any other input
+                y = step(**given, state_out=out)
+                assert torch.equal(out, plain["state"])
+            else:
+                y = step(**given)
+                assert torch.equal(given["state"], plain["state"])
+            assert torch.equal(y, want)
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                y.sum().backward()
+            given["state"] = args["state"].clone().requires_grad_()
+            with torch.no_grad():
+                y = step(**given)
+            assert not y.requires_grad and torch.equal(given["state"], plain["state"])
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """There is no forward-mode rule: a tangent raises instead of vanishing, under no_grad too (which
+    does not switch forward mode off).  Inputs without one run inside a level as outside."""
+    import torch.autograd.forward_ad as fwd
+
+    from visionhope_b200.ssm_core import short_conv, short_conv_step, ssm_scan, ssm_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x, cache, w = _conv(gen)
+    (u, delta, A, B, C), state = _scan(gen)
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        for run, args in ((short_conv, [x, w, torch.zeros(8, device=DEV)]), (ssm_scan, [u, delta, A, B, C]),
+                              (short_conv_step, [x[:, 0], cache, w]),
+                              (ssm_scan_step, [u[:, 0], delta[:, 0], A, B[:, 0], C[:, 0], state])):
+            run(*args)
+            for i in range(len(args)):
+                dual = list(args)
+                dual[i] = fwd.make_dual(args[i].clone(), torch.ones_like(args[i]))
+                with pytest.raises((NotImplementedError, RuntimeError), match="forward mode|not differentiable"):
+                    run(*dual)
+
+
+def test_function_transforms_are_refused():
+    """torch.func's tangents and batch dimensions do not reach the kernels as plain memory either."""
+    from visionhope_b200.ssm_core import short_conv
+
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x, _, w = _conv(gen)
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(lambda t: short_conv(t, w), (x,), (torch.ones_like(x),))
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.vmap(lambda t: short_conv(t, w))(torch.stack([x, x]))

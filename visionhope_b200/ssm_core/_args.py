@@ -3,6 +3,7 @@
 A step of a small batch takes the GPU a few microseconds, so the host's part counts: the C structs are
 packed in one go (``struct.Struct``) and every check runs on values that are already at hand."""
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from .. import _lib
@@ -135,6 +136,53 @@ def wrote(t):
     that saved it then raises instead of reading the new values."""
     if not t.is_inference():
         increment_version(t)
+
+
+def tracked(tensors):
+    """Whether a derivative by one of the tensors (None among them) is wanted: they require gradients,
+    or carry a forward-mode tangent (which an autograd function without a rule for it refuses)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and _tangent(tensors)
+
+
+def _tangent(tensors):
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+class _NoBackward(torch.autograd.Function):
+    """The identity for a step's y; its backward raises."""
+
+    @staticmethod
+    def forward(ctx, y, name, *tensors):
+        ctx.name = name
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError(f"{ctx.name} is not differentiable: run the tokens as a sequence instead")
+
+
+def step_derivatives(name, tensors, state, state_out):
+    """A step keeps nothing for a backward.  Refuses what could only end in a wrong derivative: tangents,
+    and a cache that is written and takes part in a graph (under ``torch.no_grad()`` it may).  Returns
+    whether others of ``tensors`` (all of them, the states too) require gradients, which
+    :func:`no_backward` then marks y with."""
+    if not tracked(tensors):
+        return False
+    if forward_ad._current_level >= 0 and _tangent(tensors):
+        raise RuntimeError(f"{name} is not differentiable in forward mode")
+    if (state if state_out is None else state_out).requires_grad:
+        raise RuntimeError(f"{name} is not differentiable and its cache requires gradients: call it under torch.no_grad() "
+                           "or detach the cache")
+    return True
+
+
+def no_backward(y, name, tensors):
+    """y of a step some of whose tensors require gradients: a backward through it raises."""
+    return _NoBackward.apply(y, name, *tensors)
 
 
 def ptr(t):

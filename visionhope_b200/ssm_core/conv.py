@@ -111,13 +111,6 @@ class _ShortConvFunction(torch.autograd.Function):
         return dx, _args.grad_like(dw, weight), _args.grad_like(db, bias), di, None, None, None, None
 
 
-def _needs_grad(*tensors):
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
 @_lib.on_input_device
 def short_conv(x, weight, bias=None, *, activation=None, initial_state=None, return_final_state=False,
                seq_offsets=None, reverse=False):
@@ -133,7 +126,7 @@ def short_conv(x, weight, bias=None, *, activation=None, initial_state=None, ret
     or (y, final_state) with ``return_final_state``, the last taps - 1 inputs.  Differentiable in
     x, weight, bias and initial_state, through y and the final state."""
     act = _activation(activation)
-    if torch.is_grad_enabled() and _needs_grad(x, weight, bias, initial_state):
+    if _args.tracked((x, weight, bias, initial_state)):
         return _ShortConvFunction.apply(x, weight, bias, initial_state, act, bool(return_final_state), seq_offsets,
                                         bool(reverse))
     y, final = _Call(x, weight, bias, act, initial_state, seq_offsets, reverse).forward(return_final_state)
@@ -146,8 +139,11 @@ def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None,
     rows move up by one with x as the newest (in place, or into ``state_out``).  slots: int32 or
     int64 [B], each stream's row of the state (row b without it); a stream whose slot lies outside
     the state is skipped and its y is 0; no two streams may name one slot.  Returns y [B, C].  Not
-    differentiable."""
+    differentiable: a backward through y raises, and so does a cache that requires gradients, unless
+    the call is under ``torch.no_grad()``."""
     act = _activation(activation)
+    tensors = x, state, weight, bias, state_out
+    marked = _args.step_derivatives("short_conv_step", tensors, state, state_out)
     _lib.ensure_device(x)
     device, dtype = x.device, x.dtype
     code = _lib.dtype_code(dtype)
@@ -167,4 +163,4 @@ def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None,
         x.data_ptr(), x.stride(0), code, weight.data_ptr(), ptr(bias), act, state.data_ptr(), state_out.data_ptr(),
         ptr(slots), state.shape[0], y.data_ptr(), b, d, k, _lib.stream_handle(device)), "vh_short_conv_step")
     _args.wrote(state_out)
-    return y
+    return _args.no_backward(y, "short_conv_step", tensors) if marked else y

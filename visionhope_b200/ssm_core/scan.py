@@ -7,7 +7,6 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 from . import _args
 from ._args import ptr
-from .conv import _needs_grad
 
 STATES = (4, 8, 16, 32, 64)
 _ARGS = struct.Struct("5Q12q8Qq7i4x")  # vh_ssm_scan_args
@@ -163,7 +162,7 @@ def ssm_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softpl
     final_state) with ``return_final_state``.  Differentiable in every tensor, through y and the
     final state; the sums of the backward run in a fixed order."""
     tensors = (u, delta, A, B, C, D, z, delta_bias, initial_state)
-    if torch.is_grad_enabled() and _needs_grad(*tensors):
+    if _args.tracked(tensors):
         return _SsmScanFunction.apply(*tensors, bool(delta_softplus), bool(return_final_state), seq_offsets,
                                       bool(reverse))
     call = _Call(*tensors[:8], delta_softplus, initial_state, seq_offsets, reverse)
@@ -176,7 +175,9 @@ def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, 
                   state_out=None):
     """One token of ``B`` cached streams: u, delta, z [B, C]; B, C [B, (groups,) states]; state fp32
     [slots, C, states], advanced in place (or into ``state_out``).  slots: as
-    :func:`short_conv_step`.  Returns y [B, C].  Not differentiable."""
+    :func:`short_conv_step`.  Returns y [B, C].  Not differentiable, as :func:`short_conv_step`."""
+    tensors = u, delta, A, B, C, state, D, z, delta_bias, state_out
+    marked = _args.step_derivatives("ssm_scan_step", tensors, state, state_out)
     call = _Call(u, delta, A, B, C, D, z, delta_bias, delta_softplus, None, None, False, one_token=True)
     device = u.device
     b, d, n = call.state_shape
@@ -188,4 +189,4 @@ def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, 
     _lib.check(_lib.load().vh_ssm_scan_step(call.args(y.data_ptr()), state.data_ptr(), state_out.data_ptr(),
                                             ptr(slots), state.shape[0], _lib.stream_handle(device)), "vh_ssm_scan_step")
     _args.wrote(state_out)
-    return y
+    return _args.no_backward(y, "ssm_scan_step", tensors) if marked else y
