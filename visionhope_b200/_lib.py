@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import itertools
 import os
 import threading
 from ctypes import c_float, c_int32, c_int64, c_void_p
@@ -297,11 +296,18 @@ def on_input_device(fn):
     run unchanged."""
     @functools.wraps(fn)
     def call(*args, **kwargs):
-        for value in itertools.chain(args, kwargs.values()):
+        for value in args:
             if isinstance(value, torch.Tensor) and value.is_cuda:
-                if value.device.index != torch.cuda.current_device():
-                    with torch.cuda.device(value.device):
-                        return fn(*args, **kwargs)
                 break
-        return fn(*args, **kwargs)
+        else:
+            for value in kwargs.values():
+                if isinstance(value, torch.Tensor) and value.is_cuda:
+                    break
+            else:
+                return fn(*args, **kwargs)
+        # there is a CUDA tensor, so the current device can be asked for without initialising
+        if value.get_device() == torch._C._cuda_getDevice():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(value.device):
+            return fn(*args, **kwargs)
     return call

@@ -135,7 +135,7 @@ def wrote(t):
     """Tells autograd that a kernel changed ``t`` in place, as an in-place operation would: a backward
     that saved it then raises instead of reading the new values."""
     if not t.is_inference():
-        increment_version(t)
+        increment_version((t,))
 
 
 def tracked(tensors):

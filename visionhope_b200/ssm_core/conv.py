@@ -156,7 +156,7 @@ def short_conv_step(x, state, weight, bias=None, *, activation=None, slots=None,
     bias = _args.fp32(bias, (d,), "bias", device)
     slots = _args.slot_index(slots, b, device)
     state, state_out = _args.cache(state, state_out, (k - 1, d), b, slots, dtype, device)
-    y = torch.empty(shape, dtype=dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if b * d == 0:
         return y
     _lib.check(_lib.load().vh_short_conv_step(

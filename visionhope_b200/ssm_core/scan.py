@@ -183,7 +183,7 @@ def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, 
     b, d, n = call.state_shape
     slots = _args.slot_index(slots, b, device)
     state, state_out = _args.cache(state, state_out, (d, n), b, slots, torch.float32, device)
-    y = torch.empty(u.shape, dtype=u.dtype, device=device)
+    y = torch.empty_like(u, memory_format=torch.contiguous_format)
     if b * d == 0:
         return y
     _lib.check(_lib.load().vh_ssm_scan_step(call.args(y.data_ptr()), state.data_ptr(), state_out.data_ptr(),
