@@ -182,3 +182,18 @@ def test_entry_points_pass_states_on_without_tokens(packed):
                "vh_short_conv_bwd")
     assert torch.equal(gi, gs) and not gw.any()
     assert not row.any()
+
+
+def test_far_offsets_are_clamped():
+    """Offsets of 2^32 + 5 mean the end of the tokens, not token 5."""
+    from visionhope_b200.ssm_core import short_conv, ssm_scan
+
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x, bc = torch.randn(50, 32, generator=gen, device=DEV), torch.randn(50, 16, generator=gen, device=DEV)
+    w, A = torch.randn(32, 4, generator=gen, device=DEV), -torch.rand(32, 16, generator=gen, device=DEV)
+    near = torch.tensor([0, 20, 20, 50], device=DEV)
+    far = torch.tensor([-(1 << 32), 20, 20, (1 << 32) + 5], device=DEV)
+    assert torch.equal(short_conv(x, w, seq_offsets=near), short_conv(x, w, seq_offsets=far))
+    args = x, x, A, bc, bc
+    near, far = (ssm_scan(*args, delta_softplus=True, seq_offsets=o, return_final_state=True) for o in (near, far))
+    assert torch.equal(near[0], far[0]) and torch.equal(near[1], far[1])

@@ -40,3 +40,20 @@ def test_sizes_of_unsupported_scans_are_zero(change):
     assert lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a)) == 0
     assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(_bwd(_lib, p, a))) == 0
     assert lib.vh_ssm_scan_checkpoint_bytes(None) == 0
+
+
+def test_offsets_and_slots_do_not_wrap():
+    """int64 offsets and slots past int32 stay outside the tokens and the cache."""
+    import torch
+
+    from visionhope_b200.ssm_core import _args
+
+    cpu = torch.device("cpu")
+    far = torch.tensor([-(1 << 32), -1, 0, 7, (1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 62])
+    want = torch.tensor([-1, -1, 0, 7] + [(1 << 31) - 1] * 4, dtype=torch.int32)
+    assert torch.equal(_args.offsets_like(far, cpu), want)
+    assert torch.equal(_args.slot_index(far, 8, cpu), want)
+    near = torch.arange(10, dtype=torch.int32)[::2]
+    assert torch.equal(_args.offsets_like(near, cpu), near) and _args.offsets_like(near, cpu).is_contiguous()
+    whole = near.contiguous()
+    assert _args.offsets_like(whole, cpu) is whole

@@ -65,7 +65,7 @@ def state(t, shape, name, dtype, device):
 
 
 def offsets_like(seq_offsets, device):
-    """Sequence offsets as contiguous int32 on ``device``."""
+    """Sequence offsets as contiguous int32 on ``device``; the kernels clamp them to the tokens."""
     if seq_offsets.dim() != 1 or seq_offsets.numel() < 2:
         raise ValueError("seq_offsets must hold at least two offsets, one more than there are sequences")
     if seq_offsets.dtype not in (torch.int32, torch.int64):
@@ -74,7 +74,10 @@ def offsets_like(seq_offsets, device):
         refuse_device("seq_offsets", device, seq_offsets.device)
     if seq_offsets.dtype is torch.int32 and seq_offsets.is_contiguous():
         return seq_offsets
-    return seq_offsets.to(torch.int32).contiguous()
+    if seq_offsets.dtype is torch.int64:
+        # past int32 an offset is outside any tokens, and must not wrap into them
+        seq_offsets = seq_offsets.clamp(-1, 0x7fffffff).to(torch.int32)
+    return seq_offsets.contiguous()
 
 
 def sequences(x, seq_offsets, name):
