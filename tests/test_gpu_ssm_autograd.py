@@ -137,3 +137,28 @@ def test_function_transforms_are_refused():
         torch.func.jvp(lambda t: short_conv(t, w), (x,), (torch.ones_like(x),))
     with pytest.raises((NotImplementedError, RuntimeError)):
         torch.func.vmap(lambda t: short_conv(t, w))(torch.stack([x, x]))
+
+
+@pytest.mark.parametrize("shape", [(2, 5, 0), (2, 0, 8), (0, 5, 8)])
+def test_empty_inputs_get_zero_gradients(shape):
+    """Without channels, tokens or sequences every gradient that has elements is zero (an initial
+    state's is the final one's).  Blocks full of NaN are freed first: gradients left unwritten would
+    show them."""
+    from visionhope_b200.ssm_core import short_conv, ssm_scan
+
+    b, L, d = shape
+    n, k = 16, 4
+    u, delta = (torch.ones(shape, device=DEV, requires_grad=True) for _ in range(2))
+    B, C = (torch.ones(b, L, n, device=DEV, requires_grad=True) for _ in range(2))
+    A, D = torch.ones(d, n, device=DEV, requires_grad=True), torch.ones(d, device=DEV, requires_grad=True)
+    w, h0 = torch.ones(d, k, device=DEV, requires_grad=True), torch.ones(b, d, n, device=DEV, requires_grad=True)
+    x, s0 = torch.ones(shape, device=DEV, requires_grad=True), torch.ones(b, k - 1, d, device=DEV, requires_grad=True)
+    y, h = ssm_scan(u, delta, A, B, C, D, initial_state=h0, return_final_state=True)
+    c, s = short_conv(x, w, initial_state=s0, return_final_state=True)
+    for t in [torch.full((m,), float("nan"), device=DEV) for m in (b * L * n, d * n, d, d * k, b * d * n) for _ in range(8)]:
+        del t
+    scan_in, conv_in = (u, delta, A, B, C, D), (x, w)
+    grads = torch.autograd.grad([y, h], [*scan_in, h0], [torch.ones_like(y), torch.full_like(h, 2.0)])
+    grads = [*grads, *torch.autograd.grad([c, s], [*conv_in, s0], [torch.ones_like(c), torch.full_like(s, 2.0)])]
+    for g, t in zip(grads, [*scan_in, h0, *conv_in, s0]):
+        assert g.shape == t.shape and (g == (2.0 if t is h0 or t is s0 else 0.0)).all()

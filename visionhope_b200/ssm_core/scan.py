@@ -100,8 +100,8 @@ class _Call:
         du, dd, dz, dB, dC = (like(t, dtype) for t in (u, self.delta, self.z, self.B, self.C))
         dA, dD, dbias = (like(t, torch.float32) for t in (self.A, self.D, self.bias))
         di = torch.empty(self.state_shape, dtype=torch.float32, device=dev) if want_initial else None
-        if u.numel() == 0:
-            for t in (dA, dD, dbias):
+        if u.numel() == 0:  # without channels B and C still have elements
+            for t in (dA, dB, dC, dD, dbias):
                 if t is not None:
                     t.zero_()
             if di is not None:
