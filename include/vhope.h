@@ -531,7 +531,8 @@ int vh_short_conv_step(const void* x, int64_t x_batch_stride, int32_t dtype, con
  * delta_bias: fp32 [channels] or NULL; states 4, 8, 16, 32 or 64; initial_state / final_state:
  * fp32 [batch, channels, states] or NULL.  The state is held in fp32 throughout.
  * checkpoints (or NULL): vh_ssm_scan_checkpoint_bytes(args) bytes that receive the state before
- * every 32nd token, which the backward starts from (in an order of the kernels' own). */
+ * every 32nd token, which the backward starts from (in an order of the kernels' own); 16-byte
+ * aligned, as the workspaces. */
 typedef struct {
     const void *u, *delta, *z, *b, *c;
     int64_t u_batch_stride, u_token_stride, delta_batch_stride, delta_token_stride;
@@ -573,7 +574,7 @@ int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* args, void* workspace, int64_t w
  * [batch, groups, states] (the batch strides of args; token strides are not used), state fp32
  * [slots, channels, states].  args gives a, d_skip, delta_bias, delta_softplus, dtype, batch,
  * channels, states, groups and y [batch, channels]; its other fields are not read.  slots_index,
- * slots, state, state_out: as vh_short_conv_step. */
+ * slots, state, state_out: as vh_short_conv_step.  a, state and state_out must be 16-byte aligned. */
 int vh_ssm_scan_step(const vh_ssm_scan_args* args, const float* state, float* state_out, const int32_t* slots_index,
                      int32_t slots, vh_stream_t stream);
 

@@ -197,3 +197,47 @@ def test_far_offsets_are_clamped():
     args = x, x, A, bc, bc
     near, far = (ssm_scan(*args, delta_softplus=True, seq_offsets=o, return_final_state=True) for o in (near, far))
     assert torch.equal(near[0], far[0]) and torch.equal(near[1], far[1])
+
+
+def _shifted(t):
+    """The same values one element past an aligned address."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    view = flat[1:].view(t.shape)
+    view.copy_(t)
+    assert view.data_ptr() % 16
+    return view
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_views_into_larger_buffers(dtype):
+    """Parameters, states, rows and incoming gradients at odd addresses give the same bits.  Only the
+    convolution's sums over tokens (weight, bias) are added in another order where its loads are
+    narrower: 5e-6 of the largest, as against the oracle."""
+    from visionhope_b200.ssm_core import short_conv, short_conv_step, ssm_scan, ssm_scan_step
+
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    b, L, d, n, k = 2, 70, 32, 16, 4
+
+    def normal(*shape, dtype=torch.float32):
+        return torch.randn(*shape, generator=gen, device=DEV).to(dtype)
+
+    scan = [normal(b, L, d, dtype=dtype) for _ in range(2)] + [-normal(d, n).abs()] + [normal(b, L, n, dtype=dtype) for _ in range(2)]
+    scan += [normal(d), normal(b, d, n), normal(d), normal(b, L, d, dtype=dtype)]
+    conv = [normal(b, L, d, dtype=dtype), normal(d, k), normal(d), normal(b, k - 1, d, dtype=dtype)]
+    dy, dh, ds = normal(b, L, d, dtype=dtype), normal(b, d, n), normal(b, k - 1, d, dtype=dtype)
+    results = []
+    for put in (lambda t: t.clone(), _shifted):
+        u, delta, A, B, C, D, h0, bias, z = ts = [put(t).requires_grad_() for t in scan]
+        x, w, wb, s0 = cs = [put(t).requires_grad_() for t in conv]
+        y, h = ssm_scan(u, delta, A, B, C, D, z=z, delta_bias=bias, delta_softplus=True, initial_state=h0, return_final_state=True)
+        c, s = short_conv(x, w, wb, activation="silu", initial_state=s0, return_final_state=True)
+        out = [y, h, c, s, *torch.autograd.grad([y, h], ts, [put(dy), put(dh)]), *torch.autograd.grad([c, s], cs, [put(dy), put(ds)])]
+        with torch.no_grad():
+            out.append(ssm_scan_step(put(u[:, 0]), put(delta[:, 0]), A, put(B[:, 0]), put(C[:, 0]), h0.clone(), D, z=put(z[:, 0]),
+                                     delta_bias=bias, delta_softplus=True))
+            cache = put(s0)
+            out += [short_conv_step(put(x[:, 0]), cache, w, wb, activation="silu"), cache]
+        results.append(out)
+    sums = (4 + len(scan) + 1, 4 + len(scan) + 2)
+    for i, (a, e) in enumerate(zip(*results)):
+        assert float((a - e).abs().max()) <= 5e-6 * float(e.abs().max()) if i in sums else torch.equal(a, e), i

@@ -57,3 +57,31 @@ def test_offsets_and_slots_do_not_wrap():
     assert torch.equal(_args.offsets_like(near, cpu), near) and _args.offsets_like(near, cpu).is_contiguous()
     whole = near.contiguous()
     assert _args.offsets_like(whole, cpu) is whole
+
+
+def test_parameters_and_states_need_four_bytes():
+    """fp32 arrays of the sequence entry points may lie anywhere in a larger buffer; what is moved
+    sixteen bytes at a time (checkpoints, workspaces, the step's rates and states) may not."""
+    from visionhope_b200 import _lib
+
+    lib, (p, keep) = _lib.load(), _fake()
+    names = ("a", "d_skip", "delta_bias", "initial_state", "final_state")
+
+    def scan(**kw):
+        return _scan_args(_lib, p, checkpoints=kw.pop("checkpoints", p), **kw)
+
+    def query(a):
+        lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a))
+        return _err(lib)
+
+    assert query(scan(**{n: p + 4 for n in names})) == ""
+    for n in names:
+        assert "misaligned" in query(scan(**{n: p + 2}))
+    assert "checkpoints" in query(scan(checkpoints=p + 4))
+    a = _bwd(_lib, p, scan(**{n: p + 4 for n in names}))
+    a.grad_final = a.grad_initial = a.grad_a = a.grad_d_skip = a.grad_delta_bias = p + 4
+    assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(a)) > 0 and _err(lib) == ""
+    a.grad_final = p + 2
+    assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(a)) == 0 and "misaligned" in _err(lib)
+    assert lib.vh_ssm_scan_step(ctypes.byref(scan(a=p + 4)), p, p, None, 4, None) == -5
+    assert lib.vh_ssm_scan_step(ctypes.byref(scan()), p + 4, p, None, 4, None) == -5

@@ -397,11 +397,15 @@ int check_scan_args(const char* what, const vh_ssm_scan_args* a, bool one_token)
     const void* typed[] = {a->u, a->delta, a->z, a->b, a->c, a->y};
     for (const void* t : typed)
         if (t && !aligned(t, es)) return fail(VH_E_ALIGN, "%s: misaligned pointers", what);
-    if (!aligned(a->a, 16) || (a->initial_state && !aligned(a->initial_state, 16)) ||
-        (a->final_state && !aligned(a->final_state, 16)) || (a->checkpoints && !aligned(a->checkpoints, 16)))
-        return fail(VH_E_ALIGN, "%s: a and the states must be 16-byte aligned", what);
-    if (!one_token && a->seq_offsets && !aligned(a->seq_offsets, 4))
-        return fail(VH_E_ALIGN, "%s: misaligned offsets", what);
+    if (one_token) {  // it reads its rates four at a time
+        if (!aligned(a->a, 16)) return fail(VH_E_ALIGN, "%s: a must be 16-byte aligned", what);
+        return 0;
+    }
+    for (const void* t : {(const void*)a->a, (const void*)a->d_skip, (const void*)a->delta_bias, (const void*)a->initial_state,
+                          (const void*)a->final_state, (const void*)a->seq_offsets})
+        if (t && !aligned(t, 4)) return fail(VH_E_ALIGN, "%s: misaligned pointers", what);
+    if (a->checkpoints && !aligned(a->checkpoints, 16))
+        return fail(VH_E_ALIGN, "%s: the checkpoints must be 16-byte aligned", what);
     return 0;
 }
 

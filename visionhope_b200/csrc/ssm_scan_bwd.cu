@@ -591,8 +591,9 @@ int check_bwd(const char* what, const vh_ssm_scan_bwd_args* a) {
     const void* typed[] = {a->grad_y, a->grad_u, a->grad_delta, a->grad_z, a->grad_b, a->grad_c};
     for (const void* t : typed)
         if (t && !aligned(t, es)) return fail(VH_E_ALIGN, "%s: misaligned pointers", what);
-    if ((a->grad_final && !aligned(a->grad_final, 16)) || (a->grad_initial && !aligned(a->grad_initial, 16)))
-        return fail(VH_E_ALIGN, "%s: the states must be 16-byte aligned", what);
+    for (const void* t : {(const void*)a->grad_final, (const void*)a->grad_initial, (const void*)a->grad_a,
+                          (const void*)a->grad_d_skip, (const void*)a->grad_delta_bias})
+        if (t && !aligned(t, 4)) return fail(VH_E_ALIGN, "%s: misaligned pointers", what);
     return 0;
 }
 

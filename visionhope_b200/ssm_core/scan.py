@@ -174,9 +174,11 @@ def ssm_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softpl
 def ssm_scan_step(u, delta, A, B, C, state, D=None, *, z=None, delta_bias=None, delta_softplus=False, slots=None,
                   state_out=None):
     """One token of ``B`` cached streams: u, delta, z [B, C]; B, C [B, (groups,) states]; state fp32
-    [slots, C, states], advanced in place (or into ``state_out``).  slots: as
+    [slots, C, states] and 16-byte aligned, advanced in place (or into ``state_out``).  slots: as
     :func:`short_conv_step`.  Returns y [B, C].  Not differentiable, as :func:`short_conv_step`."""
     tensors = u, delta, A, B, C, state, D, z, delta_bias, state_out
+    if A.data_ptr() % 16:  # a view into a larger buffer: the kernel reads four rates at a time
+        A = A.detach().clone()
     marked = _args.step_derivatives("ssm_scan_step", tensors, state, state_out)
     call = _Call(u, delta, A, B, C, D, z, delta_bias, delta_softplus, None, None, False, one_token=True)
     device = u.device
