@@ -241,3 +241,36 @@ def test_views_into_larger_buffers(dtype):
     sums = (4 + len(scan) + 1, 4 + len(scan) + 2)
     for i, (a, e) in enumerate(zip(*results)):
         assert float((a - e).abs().max()) <= 5e-6 * float(e.abs().max()) if i in sums else torch.equal(a, e), i
+
+
+@pytest.mark.parametrize("name", ["B", "C"])
+@pytest.mark.parametrize("n,d", [(16, 32), (8, 64)])
+@pytest.mark.parametrize("L", [1, 2, 3, 4, 5, 7, 33, 130, 131])
+def test_an_infinite_last_token(L, n, d, name):
+    """B or C infinite in one state of the last token: the others' results and whatever does not meet
+    that value stay finite, whether the tokens fill their last group of four or not.  All inputs are
+    positive, so that no sum has infinities of both signs but the steps' gradient.  Finite values to
+    the scan's fp32 bar for gradients, 2e-5 of the largest."""
+    from oracle import ssm as oracle
+    from visionhope_b200 import ssm_core
+
+    gen = torch.Generator().manual_seed(L)
+    ts = dict(u=torch.rand(2, L, d, generator=gen) + 0.1, delta=torch.rand(2, L, d, generator=gen) + 0.1,
+              A=-0.3 - torch.rand(d, n, generator=gen), B=torch.rand(2, L, n, generator=gen) + 0.1,
+              C=torch.rand(2, L, n, generator=gen) + 0.1, D=torch.rand(d, generator=gen) + 0.1,
+              initial_state=torch.rand(2, d, n, generator=gen) + 0.1)
+    ts[name][:, -1, 1] = float("inf")
+    out = []
+    for module, put in ((ssm_core, lambda t: t.to(DEV)), (oracle, lambda t: t.double())):
+        v = {k: put(t).requires_grad_() for k, t in ts.items()}
+        kw = dict(return_final_state=True) if module is ssm_core else {}
+        y, h = module.ssm_scan(v["u"], v["delta"], v["A"], v["B"], v["C"], v["D"], initial_state=v["initial_state"], **kw)
+        out.append({"y": y, "final": h, **dict(zip(v, torch.autograd.grad([y, h], list(v.values()),
+                                                                        [torch.ones_like(y), torch.ones_like(h)])))})
+    for k, e in out[1].items():
+        g, e = out[0][k].detach().double().cpu(), e.detach()
+        assert torch.equal(g.isnan(), e.isnan()) and torch.equal(g.isinf(), e.isinf()), k
+        keep = e.isfinite()
+        if keep.any():
+            assert float((g - e)[keep].abs().max()) <= 2e-5 * float(e[keep].abs().max()), k
+        assert (g[e.isinf()] == e[e.isinf()]).all(), k

@@ -127,6 +127,10 @@ __device__ __forceinline__ void store_lanes(float* p, int lane, const float (&v)
     for (int i = 0; i < 4; ++i)
         reinterpret_cast<float4*>(p)[32 * i + lane] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
 }
+__device__ __forceinline__ void clear_lanes(float* p, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(p)[32 * i + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+}
 __device__ __forceinline__ void load_lanes(const float* p, int lane, float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -200,8 +204,8 @@ __device__ __forceinline__ void sum_parts(const float* rows, int own_c, float2 (
 // A warp's place in its chain: for each sequence the address of the lane's elements in the group
 // at hand, moved from group to group.  A group that the run of tokens ends in reads its last
 // token again in place of the missing ones, and channels past the tile's group read the last
-// ones; both are then staged with the step 0 and s u = 0, which leave every state as it is and
-// add nothing to a sum.
+// ones; both are then staged with the step 0 and s u = 0 (and missing tokens with B = C = 0), which
+// leave every state as it is and add nothing to a sum.
 template <typename T, int NL>
 struct Chain {
     using K = Tile<NL>;
@@ -348,6 +352,8 @@ struct Chain {
                 float* row = st.bc + (at / NL) * Stage<NL>::kRow;
                 float v[4];
                 r.bc[i][lane].get(v);
+                if (count < kGroup && at / (2 * NL) >= count)  // 0 times an infinite value is no 0
+                    v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     row[((n + k) % NL) * 4 + (n + k) / NL] = v[k];

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     // s, s u, B, C and v of the fetched group
     auto stage = [&](int64_t tokens, float2 (&sum)[P]) {
         const int count = (int)min(tokens, (int64_t)kGroup);
-        const bool fast = chn.template stage<OWN, true>(sm.raw.r, count, sm.s, sum, most);
+        const bool fast = chn.template stage<OWN, true>(sm.raw.r, count, sm.s, sum, most) && (OWN || count >= kGroup);
 #pragma unroll
         for (int e = 0; e < TE; ++e) {
             float2 v2[P], z2[P];
@@ -350,6 +350,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
                     }
                     if (gated) put_part<NL>(sm.y + 128 * r, j, ct, acc);
                 }
+                // da takes 0 times the state before a missing token, which may be infinite
+                if (decltype(mode)::value == kChecked)
+                    for (int64_t r = te - t; r < kGroup; ++r) clear_lanes(sm.past[r - 1], lane);
 #pragma unroll
                 for (int r = kGroup - 1; r >= 0; --r) {
                     reload();
