@@ -274,3 +274,30 @@ def test_an_infinite_last_token(L, n, d, name):
         if keep.any():
             assert float((g - e)[keep].abs().max()) <= 2e-5 * float(e[keep].abs().max()), k
         assert (g[e.isinf()] == e[e.isinf()]).all(), k
+
+
+@pytest.mark.parametrize("L", [64, 300, 1100, 2100])
+def test_growing_states_that_are_zero_stay_zero(L):
+    """Rates above zero let a state grow by e^3 a token.  Rows of zeros before the first input (padding),
+    and tokens behind the last one with a gradient, keep states and gradients at zero however many
+    there are.  Finite values to the scan's fp32 bars: 5e-6, gradients 2e-5 of the largest."""
+    from oracle import ssm as oracle
+    from visionhope_b200 import ssm_core
+
+    gen = torch.Generator().manual_seed(L)
+    d, n = 40, 16
+    ts = dict(u=torch.zeros(1, L, d), delta=torch.rand(1, L, d, generator=gen) + 1.5, A=1.0 + torch.rand(d, n, generator=gen),
+              B=torch.randn(1, L, n, generator=gen), C=torch.randn(1, L, n, generator=gen))
+    ts["u"][:, -3:] = torch.randn(1, 3, d, generator=gen)
+    head = torch.zeros(1, L, d)
+    head[:, :3] = torch.randn(1, 3, d, generator=gen)
+    out = []
+    for module, put in ((ssm_core, lambda t: t.to(DEV)), (oracle, lambda t: t.double())):
+        v = {k: put(t).requires_grad_() for k, t in ts.items()}
+        kw = dict(return_final_state=True) if module is ssm_core else {}
+        y, h = module.ssm_scan(*v.values(), **kw)
+        out.append([y, h, *torch.autograd.grad(y, list(v.values()), put(head))])
+    for i, (g, e) in enumerate(zip(*out)):
+        g, e = g.detach().double().cpu(), e.detach()
+        assert float((g - e).abs().max()) <= (5e-6 if i < 2 else 2e-5) * float(e.abs().max()), i
+    assert out[0][0][:, :-3].eq(0).all() and out[0][2][:, 3:].eq(0).all()

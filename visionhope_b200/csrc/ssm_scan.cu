@@ -184,6 +184,12 @@ __global__ void __launch_bounds__(32 * kWarps, 4) scan_fwd_kernel(const ScanPara
     }
 }
 
+// What leaves a segment.  Zero stays zero, although a decay above 1 (a rate or a step against the sign) may
+// be infinite over a whole segment.
+__device__ __forceinline__ float carry(float decay, float state, float own) {
+    return state == 0.f ? own : fmaf(decay, state, own);
+}
+
 // What enters every segment of a chain: a thread holds four states (one of four channels) and one
 // of RUNS runs of segments.  It composes its run, the CTA chains the runs, and it walks its run
 // again.  A CTA has 128 / PARTS of a chain's 128 such fours.
@@ -203,11 +209,11 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
     element<NL>(x, c, n);
     const int ch = tile / p.tiles_per_group * p.per_group + (tile % p.tiles_per_group) * CW + c;
     const int left = p.per_group - ((tile % p.tiles_per_group) * CW + c);
-    float a2[4], carry[4];
+    float a2[4], in[4];  // in: what enters
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         a2[i] = i < left ? to_log2(p.a[(int64_t)(ch + i) * N + n]) : 0.f;
-        carry[i] = first && i < left ? first[((int64_t)s * p.channels + ch + i) * N + n] : 0.f;
+        in[i] = first && i < left ? first[((int64_t)s * p.channels + ch + i) * N + n] : 0.f;
     }
     const Seq seq = seq_at(p.seqs, s);
     const int segs = (int)slots_per_seq(seq.len, g.size), each = (segs + RUNS - 1) / RUNS;
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float d = exp2_fma(sg[i], a2[i]);
-                add[i] = fmaf(d, add[i], own[i]);
+                add[i] = carry(d, add[i], own[i]);
                 dec[i] *= d;
             }
         }
@@ -237,10 +243,10 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
         __syncthreads();
         for (int r = 0; r < run; ++r) {
             const float4 d = s_dec[r][lane], e = s_add[r][lane];
-            carry[0] = fmaf(d.x, carry[0], e.x);
-            carry[1] = fmaf(d.y, carry[1], e.y);
-            carry[2] = fmaf(d.z, carry[2], e.z);
-            carry[3] = fmaf(d.w, carry[3], e.w);
+            in[0] = carry(d.x, in[0], e.x);
+            in[1] = carry(d.y, in[1], e.y);
+            in[2] = carry(d.z, in[2], e.z);
+            in[3] = carry(d.w, in[3], e.w);
         }
     }
     // four segments' loads at a time: the stores between them would hold the loads back
@@ -255,9 +261,9 @@ __global__ void __launch_bounds__(RUNS * 128 / PARTS) enter_segments_kernel(cons
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             if (k + m < k1)
-                *reinterpret_cast<float4*>(state + (k + m) * by * 512) = make_float4(carry[0], carry[1], carry[2], carry[3]);
+                *reinterpret_cast<float4*>(state + (k + m) * by * 512) = make_float4(in[0], in[1], in[2], in[3]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) carry[i] = fmaf(exp2_fma(sg[m][i], a2[i]), carry[i], own[m][i]);
+            for (int i = 0; i < 4; ++i) in[i] = carry(exp2_fma(sg[m][i], a2[i]), in[i], own[m][i]);
         }
     }
 }

@@ -198,23 +198,24 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
     };
 
     if constexpr (OWN) {
-        // sum_t (e_{t0} ... e_t) c_t v_t, in one pass forward
-        float2 prod[8], own[8];
+        // from its last token to its first: own = e_t (c_t v_t + own)
+        float2 own[8];
         float2 sum[P];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { prod[i] = make_float2(1.f, 1.f); own[i] = make_float2(0.f, 0.f); }
+        for (int i = 0; i < 8; ++i) own[i] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < P; ++i) sum[i] = make_float2(0.f, 0.f);
         if (t0 > 0 && t0 < t1) {  // the first segment's own gradient is not needed
-            fetch_at(t0, t1 - t0, true);
-            for (int64_t t = t0; t < t1; t += kGroup) {
+            int64_t t = t0 + (t1 - t0 - 1) / kGroup * kGroup;
+            fetch_at(t, t1 - t, true);
+            for (; t >= t0; t -= kGroup) {
                 cp_async_wait<0>();
                 const bool fast = stage(t1 - t, sum);
                 __syncwarp();
-                if (t + kGroup < t1) fetch_at(t + kGroup, t1 - t - kGroup, true);
+                if (t > t0) fetch_at(t - kGroup, kGroup, true);
                 auto pass = [&](auto mode) {
 #pragma unroll
-                    for (int r = 0; r < kGroup; ++r) {
+                    for (int r = kGroup - 1; r >= 0; --r) {
                         float2 sv[2], vv[2], c[4], e[8];
                         lds22(sm.s.step + r * CW + ct, sv);
                         lds22(sm.v + r * CW + ct, vv);
@@ -223,14 +224,12 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                prod[2 * i + q] = fmul2(prod[2 * i + q], e[2 * i + q]);
-                                own[2 * i + q] = ffma2(prod[2 * i + q], fmul2(c[i], vv[q]), own[2 * i + q]);
-                            }
+                            for (int q = 0; q < 2; ++q)
+                                own[2 * i + q] = fmul2(e[2 * i + q], ffma2(c[i], vv[q], own[2 * i + q]));
                     }
                 };
                 if (fast) pass(std::integral_constant<int, kMixed>{});
-            else pass(std::integral_constant<int, kChecked>{});
+                else pass(std::integral_constant<int, kChecked>{});
                 __syncwarp();
             }
         }
