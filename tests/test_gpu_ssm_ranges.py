@@ -301,3 +301,55 @@ def test_growing_states_that_are_zero_stay_zero(L):
         g, e = g.detach().double().cpu(), e.detach()
         assert float((g - e).abs().max()) <= (5e-6 if i < 2 else 2e-5) * float(e.abs().max()), i
     assert out[0][0][:, :-3].eq(0).all() and out[0][2][:, 3:].eq(0).all()
+
+
+def _segments(L, d, n, dtype, offsets=None):
+    """Segments of the forward, over all chains of one channel tile, as its workspace tells."""
+    import ctypes
+
+    from visionhope_b200 import _lib
+
+    p = 256  # not read by the query
+    a = _lib.VhSsmScanArgs(u=p, delta=p, b=p, c=p, a=p, y=p, seq_offsets=p if offsets else None, length=L,
+                           dtype=_lib.DTYPES[dtype], batch=len(offsets) - 1 if offsets else 2, channels=d, states=n, groups=1)
+    width = 512 // n
+    tiles = -(-d // width)
+    return _lib.load().vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a)) // (4 * (512 + width)) // tiles
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 16), (torch.bfloat16, 16), (torch.float32, 8), (torch.float32, 64),
+                                     (torch.bfloat16, 4)])
+@pytest.mark.parametrize("L", [300, 700, 1024])
+def test_chains_of_nine_to_thirty_two_segments(L, dtype, n, reverse):
+    """States and gradients carried over four runs of segments.  Bars: as every other length's."""
+    from tests.test_gpu_ssm import _scan_case, _scan_check
+
+    assert 9 <= _segments(L, 40, n, dtype) // 2 <= 32
+    gen = torch.Generator().manual_seed(L + n)
+    _scan_check(_scan_case(gen, (2, L), 2, 40, n, dtype), dtype, gen, reverse=reverse)
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("offsets,d", [([0, 3, 690, 700], 40), ([0, 400, 401, 401, 1100, 1300, 2500, 3900, 4000], 1280)])
+def test_packed_chains_over_four_runs(offsets, d, reverse):
+    """Packed sequences of which one has most segments; few chains with up to 32, and more than twice as
+    many chains as multiprocessors.  (The oracle runs on the GPU too: on the CPU it takes a minute.)"""
+    from oracle import ssm as oracle
+    from tests.test_gpu_ssm import _close, _scan_case
+    from visionhope_b200 import ssm_core
+
+    assert _segments(offsets[-1], d, 16, torch.float32, offsets) > 8
+    gen = torch.Generator().manual_seed(d)
+    ts = _scan_case(gen, (offsets[-1],), len(offsets) - 1, d, 16, torch.float32)
+    ts["delta"], ts["delta_bias"] = 0.2 + ts["delta"].abs(), ts["delta_bias"].abs()  # steps as softplus would make them
+    gy, gf = torch.randn(offsets[-1], d, generator=gen).to(DEV), torch.randn(len(offsets) - 1, d, 16, generator=gen).to(DEV)
+    out = []
+    for module, dtype, kw in ((ssm_core, torch.float32, dict(seq_offsets=torch.tensor(offsets, device=DEV), return_final_state=True)),
+                              (oracle, torch.float64, dict(offsets=offsets))):
+        v = {k: t.to(DEV, dtype).requires_grad_() for k, t in ts.items()}
+        y, h = module.ssm_scan(*(v[k] for k in ("u", "delta", "A", "B", "C", "D")), z=v["z"], delta_bias=v["delta_bias"],
+                               initial_state=v["initial_state"], reverse=reverse, **kw)
+        out.append({"y": y, "final": h, **dict(zip(v, torch.autograd.grad([y, h], list(v.values()), [gy.to(dtype), gf.to(dtype)])))})
+    for k, e in out[1].items():
+        _close(out[0][k], e, 5e-6 if k in ("y", "final") else 2e-5, k)
