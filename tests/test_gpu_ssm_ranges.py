@@ -353,3 +353,75 @@ def test_packed_chains_over_four_runs(offsets, d, reverse):
         out.append({"y": y, "final": h, **dict(zip(v, torch.autograd.grad([y, h], list(v.values()), [gy.to(dtype), gf.to(dtype)])))})
     for k, e in out[1].items():
         _close(out[0][k], e, 5e-6 if k in ("y", "final") else 2e-5, k)
+
+
+def _sweep(low, high, count, seed):
+    gen = torch.Generator().manual_seed(seed)
+    even = torch.linspace(low, high, count)
+    near = torch.randn(count, generator=gen) * torch.logspace(-6, 1, count)
+    return torch.cat([even, near.clamp(low, high), torch.rand(count, generator=gen) * (high - low) + low])
+
+
+def _within(got, want, rel):
+    """Relative to each value; below fp32's normal numbers (1.2e-38) a result may be zero."""
+    got, want = got.detach().double().cpu(), want.double()
+    assert torch.isfinite(got).all()
+    off = (got - want).abs() - rel * want.abs() - TINY / 100
+    worst = int(off.argmax())
+    assert float(off.flatten()[worst]) <= 0, (float(got.flatten()[worst]), float(want.flatten()[worst]))
+
+
+def test_softplus_over_its_range():
+    """One token with A = 0, B = u = 1 leaves softplus(delta) in a state that was zero.  e = exp(-|x|) is
+    within 2^-22 (ex2.approx) and, by the constant's rounding of 1.34e-8, |x| 1.34e-8; log1p(e) / e adds
+    3e-8 (the fit) and about four roundings, the sum one: 6e-7 + |x| 1.34e-8."""
+    from visionhope_b200.ssm_core import ssm_scan, ssm_scan_step
+
+    x = torch.cat([_sweep(-120, 120, 4096, 1), torch.tensor([-3e38, -1e4, -104.0, -87.0, 0.0, 88.0, 1e4, 3e38])])
+    d = x.numel()
+    want = torch.logaddexp(x.double(), torch.zeros((), dtype=torch.float64))
+    rel = 6e-7 + x.double().abs().clamp_max(104) * 1.34e-8
+    one, A, bc, state = torch.ones(1, d, device=DEV), torch.zeros(d, 4, device=DEV), torch.ones(1, 4, device=DEV), torch.zeros(1, d, 4, device=DEV)
+    ssm_scan_step(one, x[None].to(DEV), A, bc, bc, state, delta_softplus=True)
+    _, final = ssm_scan(one[None], x[None, None].to(DEV), A, bc[None], bc[None], delta_softplus=True, return_final_state=True)
+    for got in (state, final):
+        for n in range(4):
+            _within(got[0, :, n], want, rel)
+
+
+def test_decays_over_their_range():
+    """One token with u = 0 leaves exp(delta A) in states that were one.  log2(e) A carries its rounding
+    and the constant's, 7.3e-8 of the exponent.  The polynomial (the step; the scan's lowest quarter of
+    the states) adds 2e-7, past an exponent of 126 the hardware's 2^-22 and the argument's rounding; the
+    hardware function (the other states) adds that everywhere: 4e-7 and 1.4e-7 of the exponent."""
+    from visionhope_b200.ssm_core import ssm_scan, ssm_scan_step
+
+    s = _sweep(0.0, 12.0, 2048, 2).abs()
+    d, n = s.numel(), 16
+    gen = torch.Generator().manual_seed(3)
+    A = -torch.rand(d, n, generator=gen) * torch.tensor([0.01, 0.1, 1.0, 11.0]).repeat(d, n // 4)
+    A[::7] *= -0.5  # growing states too
+    x = s.double()[:, None] * A.double()
+    want = torch.exp(x)
+    zero, bc = torch.zeros(1, d, device=DEV), torch.ones(1, n, device=DEV)
+    state = torch.ones(1, d, n, device=DEV)
+    _, final = ssm_scan(zero[None], s[None, None].to(DEV), A.to(DEV), bc[None], bc[None], initial_state=state, return_final_state=True)
+    ssm_scan_step(zero, s[None].to(DEV), A.to(DEV), bc, bc, state)
+    hardware = 4e-7 + x.abs() * 1.4e-7
+    poly = torch.where(x.abs() * 1.4427 < 125, 2e-7 + x.abs() * 7.3e-8, hardware)
+    _within(state[0], want, poly)
+    _within(final[0, :, :n // 4], want[:, :n // 4], poly[:, :n // 4])
+    _within(final[0, :, n // 4:], want[:, n // 4:], hardware[:, n // 4:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_silu_over_its_range(dtype):
+    """Dense values between the saturated ends, through the convolution and its gradient."""
+    from visionhope_b200.ssm_core import short_conv
+
+    x = _sweep(-110, 110, 4096, 4).to(dtype)[:, None, None].expand(-1, 1, 2).contiguous()
+    dev = x.to(DEV).requires_grad_()
+    w = torch.tensor([[0.0, 1.0]], device=DEV).expand(2, 2).contiguous()
+    y = short_conv(dev, w, activation="silu")
+    _check(y, *_silu(x), dtype)
+    _check(torch.autograd.grad(y, dev, torch.ones_like(y))[0], *_silu_slope(x), dtype)
