@@ -106,30 +106,19 @@ __device__ __forceinline__ int64_t first_row(const Seqs& q, const Seq& e, int s,
 }
 __device__ __forceinline__ int64_t row_step(const Seqs& q, const Rows& r) { return q.reverse ? -r.token : r.token; }
 
-// V consecutive channels from c on; channels at or past `end` read as 0.  `vec`: the caller's
-// rule says that V-wide accesses are aligned and never straddle `end`.
-template <int V, typename T>
-__device__ __forceinline__ void load_v(const T* p, int c, int end, bool vec, float (&v)[V]) {
-    if (V > 1 && vec) {
-        if (c < end) {
-            if constexpr (V == 4) {
-                const float4 q = load4(p);
-                v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-            } else {
-                struct alignas(sizeof(T) * V) Pack { T e[V]; };
-                const Pack q = *reinterpret_cast<const Pack*>(p);
-#pragma unroll
-                for (int i = 0; i < V; ++i) v[i] = to_f(q.e[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = 0.f;
-        }
+// Four consecutive values; `vec`: the address is aligned for one access.
+template <typename T>
+__device__ __forceinline__ void load_four(const T* p, bool vec, float (&v)[4]) {
+    if (vec) {
+        const float4 q = load4(p);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = c + i < end ? to_f(p[i]) : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = to_f(p[i]);
     }
 }
+// V consecutive channels from c on, none at or past `end`.  `vec`: the caller's rule says that V-wide
+// accesses are aligned and never straddle `end`.
 template <int V, typename T>
 __device__ __forceinline__ void store_v(T* p, int c, int end, bool vec, const float (&v)[V]) {
     if (V > 1 && vec) {

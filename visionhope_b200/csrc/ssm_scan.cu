@@ -319,8 +319,8 @@ __global__ void __launch_bounds__(256, NL <= 4 ? 4 : 1) scan_step_kernel(const S
             const float si = __shfl_sync(0xffffffffu, st, i, NL), pi = __shfl_sync(0xffffffffu, pu, i, NL);
             const int gi = p.groups == 1 ? 0 : __shfl_sync(0xffffffffu, group, i, NL);
             if (gi != held) {  // a group of lanes may straddle two groups of B and C
-                load_v<4>(pb + gi * p.bg + 4 * j, 0, 4, p.vec_bc, bv);
-                load_v<4>(pc + gi * p.cg + 4 * j, 0, 4, p.vec_bc, cv);
+                load_four(pb + gi * p.bg + 4 * j, p.vec_bc, bv);
+                load_four(pc + gi * p.cg + 4 * j, p.vec_bc, cv);
                 held = gi;
             }
             float av[4];

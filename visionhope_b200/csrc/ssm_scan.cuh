@@ -13,9 +13,9 @@
 //
 // Tokens go in groups of four.  The 4 x 4 CL elements of a group (tokens by channels) spread
 // evenly over the lanes, 16 / NL each: a lane loads its own elements of u, delta and z, applies
-// softplus once, and leaves s and s u in shared memory for the whole warp; y's sums over the
-// state lanes come back scattered in the same way, so that the lane that holds an element's u
-// and z finishes and stores its y.  The next group's loads are issued before a group is computed.
+// softplus once, and leaves s and s u in shared memory for the whole warp.  y's sums over the state
+// lanes go through shared memory too: the lane that holds an element's u and z adds its parts, and
+// finishes and stores its y.  Groups are fetched ahead, two in the forward and one in the backward.
 //
 // Exponentials.  The decays are N exponentials per element, by far the largest part of the work:
 // the special-function unit gives 16 a cycle and SM, one element of 16 states a cycle, when the
@@ -64,7 +64,7 @@ struct ScanParams {
 };
 
 // Which elements of a group a lane owns: tokens t0 .. t0 + TE - 1, channels c0 .. c0 + CE - 1 of
-// the warp's tile (the layout reduce_scatter leaves over the state lanes).
+// the warp's tile: of the 4 x 4 (tokens by channels) of a channel lane, state lane j has the j-th part.
 template <int NL>
 struct LaneElems {
     int t0, c0;

@@ -237,221 +237,221 @@ __global__ void __launch_bounds__(32 * kBwdWarps<T>, OWN ? 4 : 2) scan_bwd_kerne
         store_lanes(seg.state + unit * 512, lane, v16);
         sum_tokens<NL>(sum, lane, own_c, seg.sigma + unit * CW);
     } else {
-    if (seg.state) {
-        wait_for_previous();
-        load_lanes(seg.state + unit * 512, lane, v16);
-    } else if (dfinal) {
-        load_block<NL>(dfinal, c0, cend, j, v16);
-    } else {
+        if (seg.state) {
+            wait_for_previous();
+            load_lanes(seg.state + unit * 512, lane, v16);
+        } else if (dfinal) {
+            load_block<NL>(dfinal, c0, cend, j, v16);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v16[i] = 0.f;
-    }
-    pair_up(v16, g);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) da[i] = make_float2(0.f, 0.f);
-
-    T* du = static_cast<T*>(bp.du) + y0;
-    T* dd = static_cast<T*>(bp.ddelta) + y0;
-    T* dz = bp.dz ? static_cast<T*>(bp.dz) + y0 : nullptr;
-    const Rows tr{p.seqs.length, 1};
-    float* pbc = bp.part_bc + ((int64_t)tile * bp.tokens + first_row(p.seqs, seq, s, tr)) * 2 * N;
-    const int64_t ps = row_step(p.seqs, tr) * 2 * N;
-    const float* ck = p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512;
-    float2 skip[P], dskip[P], dbias[P], unused[P];
-    chn.load_params(p.d_skip, skip);
-#pragma unroll
-    for (int i = 0; i < P; ++i) dskip[i] = dbias[i] = unused[i] = make_float2(0.f, 0.f);
-
-    const int64_t first = t0 / kCheckpoint, last = (t1 + kCheckpoint - 1) / kCheckpoint;
-    if (t0 < t1) {  // the last chunk's first group
-        const int64_t tc = (last - 1) * kCheckpoint;
-        fetch_at(tc, t1 - tc, t1 - tc <= kGroup);
-    }
-    for (int64_t ch = last - 1; ch >= first && t0 < t1; --ch) {
-        const int64_t tc = ch * kCheckpoint;
-        const int64_t te = min(t1, tc + kCheckpoint);
-        const int groups = (int)((te - tc + kGroup - 1) / kGroup);
-        float2 h[8];
-        load_lanes(ck + ch * tiles * 512, lane, v16);
-        pair_up(v16, h);
-        // forward over all groups but the last, whose state is not needed beyond its start
-        {
-            for (int gi = 0; gi < groups; ++gi) {
-                pair_down(h, v16);
-                store_lanes(sm.h[gi], lane, v16);
-                if (gi + 1 == groups) break;
-                cp_async_wait<0>();
-                chn.template stage<false, false>(sm.raw.r, kGroup, sm.s, unused);
-                __syncwarp();
-                const int64_t next = tc + (gi + 1) * kGroup;  // of the last group all, for the way back
-                fetch_at(next, te - next, gi + 2 == groups);
-#pragma unroll
-                for (int r = 0; r < kGroup; ++r) {
-                    float2 sv[2], pv[2], b[4], e[8];
-                    lds22(sm.s.step + r * CW + ct, sv);
-                    lds22(sm.s.su + r * CW + ct, pv);
-                    lds_dup4(sm.s.b(r, j), b);
-                    decays<kHardware>(sv, a2, e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) h[2 * i + q] = ffma2(e[2 * i + q], h[2 * i + q], fmul2(pv[q], b[i]));
-                }
-                __syncwarp();
-            }
+            for (int i = 0; i < 16; ++i) v16[i] = 0.f;
         }
-        for (int gi = groups - 1; gi >= 0; --gi) {
-            const int64_t t = tc + gi * kGroup;
-            cp_async_wait<0>();
-            const bool fast = stage(te - t, unused);
-            Pack<T, CE> nu[TE], nd[TE], nz[TE], ndy[TE];
+        pair_up(v16, g);
 #pragma unroll
-            for (int x = 0; x < TE; ++x) {
-                nu[x] = sm.raw.r.u[x][lane];
-                nd[x] = sm.raw.r.d[x][lane];
-                ndy[x] = sm.raw.dy[x][lane];
-                if (gated) nz[x] = sm.raw.r.z[x][lane];
-            }
-            __syncwarp();
-            if (gi > 0) fetch_at(t - kGroup, kGroup, true);
-            else if (ch > first) fetch_at(tc - kCheckpoint, kGroup, false);
-            auto pass = [&](auto mode) {
-                float2 e[kGroup][8];
-                float dcs[kGroup][4];
-                load_lanes(sm.h[gi], lane, v16);
-                pair_up(v16, h);
+        for (int i = 0; i < 8; ++i) da[i] = make_float2(0.f, 0.f);
+
+        T* du = static_cast<T*>(bp.du) + y0;
+        T* dd = static_cast<T*>(bp.ddelta) + y0;
+        T* dz = bp.dz ? static_cast<T*>(bp.dz) + y0 : nullptr;
+        const Rows tr{p.seqs.length, 1};
+        float* pbc = bp.part_bc + ((int64_t)tile * bp.tokens + first_row(p.seqs, seq, s, tr)) * 2 * N;
+        const int64_t ps = row_step(p.seqs, tr) * 2 * N;
+        const float* ck = p.checkpoints + (slot_base(p.seqs, s, seq.row, kCheckpoint) * tiles + tile) * 512;
+        float2 skip[P], dskip[P], dbias[P], unused[P];
+        chn.load_params(p.d_skip, skip);
 #pragma unroll
-                for (int r = 0; r < kGroup; ++r) {
-                    reload();
-                    float2 sv[2], pv[2], vv[2], b[4], c[4], acc[2], dc[4];
-                    lds22(sm.s.step + r * CW + ct, sv);
-                    lds22(sm.s.su + r * CW + ct, pv);
-                    lds22(sm.v + r * CW + ct, vv);
-                    lds_dup4(sm.s.b(r, j), b);
-                    lds_dup4(sm.s.c(r, j), c);
-                    decays<decltype(mode)::value>(sv, a2, e[r]);
-                    acc[0] = acc[1] = make_float2(0.f, 0.f);
-                    if (r > 0) {
-                        pair_down(h, v16);
-                        store_lanes(sm.past[r - 1], lane, v16);
+        for (int i = 0; i < P; ++i) dskip[i] = dbias[i] = unused[i] = make_float2(0.f, 0.f);
+
+        const int64_t first = t0 / kCheckpoint, last = (t1 + kCheckpoint - 1) / kCheckpoint;
+        if (t0 < t1) {  // the last chunk's first group
+            const int64_t tc = (last - 1) * kCheckpoint;
+            fetch_at(tc, t1 - tc, t1 - tc <= kGroup);
+        }
+        for (int64_t ch = last - 1; ch >= first && t0 < t1; --ch) {
+            const int64_t tc = ch * kCheckpoint;
+            const int64_t te = min(t1, tc + kCheckpoint);
+            const int groups = (int)((te - tc + kGroup - 1) / kGroup);
+            float2 h[8];
+            load_lanes(ck + ch * tiles * 512, lane, v16);
+            pair_up(v16, h);
+            // forward over all groups but the last, whose state is not needed beyond its start
+            {
+                for (int gi = 0; gi < groups; ++gi) {
+                    pair_down(h, v16);
+                    store_lanes(sm.h[gi], lane, v16);
+                    if (gi + 1 == groups) break;
+                    cp_async_wait<0>();
+                    chn.template stage<false, false>(sm.raw.r, kGroup, sm.s, unused);
+                    __syncwarp();
+                    const int64_t next = tc + (gi + 1) * kGroup;  // of the last group all, for the way back
+                    fetch_at(next, te - next, gi + 2 == groups);
+#pragma unroll
+                    for (int r = 0; r < kGroup; ++r) {
+                        float2 sv[2], pv[2], b[4], e[8];
+                        lds22(sm.s.step + r * CW + ct, sv);
+                        lds22(sm.s.su + r * CW + ct, pv);
+                        lds_dup4(sm.s.b(r, j), b);
+                        decays<kHardware>(sv, a2, e);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) h[2 * i + q] = ffma2(e[2 * i + q], h[2 * i + q], fmul2(pv[q], b[i]));
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        dc[i] = make_float2(0.f, 0.f);
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            float2& hh = h[2 * i + q];
-                            hh = ffma2(e[r][2 * i + q], hh, fmul2(pv[q], b[i]));
-                            acc[q] = ffma2(c[i], hh, acc[q]);
-                            dc[i] = ffma2(vv[q], hh, dc[i]);
-                        }
-                        dcs[r][i] = dc[i].x + dc[i].y;
-                    }
-                    if (gated) put_part<NL>(sm.y + 128 * r, j, ct, acc);
+                    __syncwarp();
                 }
-                // da takes 0 times the state before a missing token, which may be infinite
-                if (decltype(mode)::value == kChecked)
-                    for (int64_t r = te - t; r < kGroup; ++r) clear_lanes(sm.past[r - 1], lane);
+            }
+            for (int gi = groups - 1; gi >= 0; --gi) {
+                const int64_t t = tc + gi * kGroup;
+                cp_async_wait<0>();
+                const bool fast = stage(te - t, unused);
+                Pack<T, CE> nu[TE], nd[TE], nz[TE], ndy[TE];
 #pragma unroll
-                for (int r = kGroup - 1; r >= 0; --r) {
-                    reload();
-                    float2 sv[2], pv[2], vv[2], b[4], c[4], dsum[2], gsum[2], db[4];
-                    float dbs[4];
-                    lds22(sm.s.step + r * CW + ct, sv);
-                    lds22(sm.s.su + r * CW + ct, pv);
-                    lds22(sm.v + r * CW + ct, vv);
-                    lds_dup4(sm.s.b(r, j), b);
-                    lds_dup4(sm.s.c(r, j), c);
-                    dsum[0] = dsum[1] = gsum[0] = gsum[1] = make_float2(0.f, 0.f);
-                    load_lanes(r > 0 ? sm.past[r - 1] : sm.h[gi], lane, v16);
+                for (int x = 0; x < TE; ++x) {
+                    nu[x] = sm.raw.r.u[x][lane];
+                    nd[x] = sm.raw.r.d[x][lane];
+                    ndy[x] = sm.raw.dy[x][lane];
+                    if (gated) nz[x] = sm.raw.r.z[x][lane];
+                }
+                __syncwarp();
+                if (gi > 0) fetch_at(t - kGroup, kGroup, true);
+                else if (ch > first) fetch_at(tc - kCheckpoint, kGroup, false);
+                auto pass = [&](auto mode) {
+                    float2 e[kGroup][8];
+                    float dcs[kGroup][4];
+                    load_lanes(sm.h[gi], lane, v16);
                     pair_up(v16, h);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        db[i] = make_float2(0.f, 0.f);
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const int k = 2 * i + q;
-                            g[k] = ffma2(c[i], vv[q], g[k]);
-                            gsum[q] = ffma2(b[i], g[k], gsum[q]);
-                            db[i] = ffma2(pv[q], g[k], db[i]);
-                            g[k] = fmul2(g[k], e[r][k]);
-                            const float2 w = fmul2(g[k], h[k]);
-                            da[k] = ffma2(sv[q], w, da[k]);
-                            dsum[q] = ffma2(a2[k], w, dsum[q]);
+                    for (int r = 0; r < kGroup; ++r) {
+                        reload();
+                        float2 sv[2], pv[2], vv[2], b[4], c[4], acc[2], dc[4];
+                        lds22(sm.s.step + r * CW + ct, sv);
+                        lds22(sm.s.su + r * CW + ct, pv);
+                        lds22(sm.v + r * CW + ct, vv);
+                        lds_dup4(sm.s.b(r, j), b);
+                        lds_dup4(sm.s.c(r, j), c);
+                        decays<decltype(mode)::value>(sv, a2, e[r]);
+                        acc[0] = acc[1] = make_float2(0.f, 0.f);
+                        if (r > 0) {
+                            pair_down(h, v16);
+                            store_lanes(sm.past[r - 1], lane, v16);
                         }
-                        dbs[i] = db[i].x + db[i].y;
-                    }
-                    __syncwarp();  // every lane has read the state that the sums replace
-                    float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
-                    put_part<NL>(sums, j, ct, dsum);
-                    put_part<NL>(sums + 128, j, ct, gsum);
-                    put_bc<NL>(sums + 256, j, lane % CL, dbs, dcs[r]);
-                }
-            };
-            if (fast) pass(std::integral_constant<int, kMixed>{});
-            else pass(std::integral_constant<int, kChecked>{});
-            __syncwarp();
-            auto sums_of = [&](int r) { return r > 0 ? sm.past[r - 1] : sm.h[gi]; };
-            sum_bc<NL>([&](int r) { return sums_of(r) + 256; }, lane, te - t, pbc + t * ps, ps);
 #pragma unroll
-            for (int x = 0; x < TE; ++x) {
-                const int r = own_t + x;
-                const int64_t row = t + r;
-                float2 yo[P], dso[P], gbo[P], st2[P], du2[P], dd2[P], dz2[P], u2[P], r2[P], v2[P], z2[P];
-                float f[CE];
-                unpack<T, CE>(nu[x], u2);
-                unpack<T, CE>(nd[x], r2);
-                unpack<T, CE>(ndy[x], v2);
-                const float* sums = sums_of(r);
-                sum_parts<NL>(sums, own_c, dso);
-                sum_parts<NL>(sums + 128, own_c, gbo);
-                lds_v<CE>(sm.s.step + r * CW + own_c, f);
-                to_pairs<CE>(f, st2);
-                if (gated) {
-                    sum_parts<NL>(sm.y + 128 * r, own_c, yo);
-                    unpack<T, CE>(nz[x], z2);
+                        for (int i = 0; i < 4; ++i) {
+                            dc[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                float2& hh = h[2 * i + q];
+                                hh = ffma2(e[r][2 * i + q], hh, fmul2(pv[q], b[i]));
+                                acc[q] = ffma2(c[i], hh, acc[q]);
+                                dc[i] = ffma2(vv[q], hh, dc[i]);
+                            }
+                            dcs[r][i] = dc[i].x + dc[i].y;
+                        }
+                        if (gated) put_part<NL>(sm.y + 128 * r, j, ct, acc);
+                    }
+                    // da takes 0 times the state before a missing token, which may be infinite
+                    if (decltype(mode)::value == kChecked)
+                        for (int64_t r = te - t; r < kGroup; ++r) clear_lanes(sm.past[r - 1], lane);
+#pragma unroll
+                    for (int r = kGroup - 1; r >= 0; --r) {
+                        reload();
+                        float2 sv[2], pv[2], vv[2], b[4], c[4], dsum[2], gsum[2], db[4];
+                        float dbs[4];
+                        lds22(sm.s.step + r * CW + ct, sv);
+                        lds22(sm.s.su + r * CW + ct, pv);
+                        lds22(sm.v + r * CW + ct, vv);
+                        lds_dup4(sm.s.b(r, j), b);
+                        lds_dup4(sm.s.c(r, j), c);
+                        dsum[0] = dsum[1] = gsum[0] = gsum[1] = make_float2(0.f, 0.f);
+                        load_lanes(r > 0 ? sm.past[r - 1] : sm.h[gi], lane, v16);
+                        pair_up(v16, h);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            db[i] = make_float2(0.f, 0.f);
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int k = 2 * i + q;
+                                g[k] = ffma2(c[i], vv[q], g[k]);
+                                gsum[q] = ffma2(b[i], g[k], gsum[q]);
+                                db[i] = ffma2(pv[q], g[k], db[i]);
+                                g[k] = fmul2(g[k], e[r][k]);
+                                const float2 w = fmul2(g[k], h[k]);
+                                da[k] = ffma2(sv[q], w, da[k]);
+                                dsum[q] = ffma2(a2[k], w, dsum[q]);
+                            }
+                            dbs[i] = db[i].x + db[i].y;
+                        }
+                        __syncwarp();  // every lane has read the state that the sums replace
+                        float* sums = r > 0 ? sm.past[r - 1] : sm.h[gi];
+                        put_part<NL>(sums, j, ct, dsum);
+                        put_part<NL>(sums + 128, j, ct, gsum);
+                        put_bc<NL>(sums + 256, j, lane % CL, dbs, dcs[r]);
+                    }
+                };
+                if (fast) pass(std::integral_constant<int, kMixed>{});
+                else pass(std::integral_constant<int, kChecked>{});
+                __syncwarp();
+                auto sums_of = [&](int r) { return r > 0 ? sm.past[r - 1] : sm.h[gi]; };
+                sum_bc<NL>([&](int r) { return sums_of(r) + 256; }, lane, te - t, pbc + t * ps, ps);
+#pragma unroll
+                for (int x = 0; x < TE; ++x) {
+                    const int r = own_t + x;
+                    const int64_t row = t + r;
+                    float2 yo[P], dso[P], gbo[P], st2[P], du2[P], dd2[P], dz2[P], u2[P], r2[P], v2[P], z2[P];
+                    float f[CE];
+                    unpack<T, CE>(nu[x], u2);
+                    unpack<T, CE>(nd[x], r2);
+                    unpack<T, CE>(ndy[x], v2);
+                    const float* sums = sums_of(r);
+                    sum_parts<NL>(sums, own_c, dso);
+                    sum_parts<NL>(sums + 128, own_c, gbo);
+                    lds_v<CE>(sm.s.step + r * CW + own_c, f);
+                    to_pairs<CE>(f, st2);
+                    if (gated) {
+                        sum_parts<NL>(sm.y + 128 * r, own_c, yo);
+                        unpack<T, CE>(nz[x], z2);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            // silu'(z) = sg (1 + z (1 - sg))
+                            const float2 sg = sigmoid2(z2[i]), one = splat2(1.f);
+                            const float2 slope = fmul2(sg, ffma2(z2[i], fsub2(one, sg), one));
+                            dz2[i] = fmul2(fmul2(v2[i], ffma2(skip[i], u2[i], yo[i])), slope);
+                            v2[i] = fmul2(v2[i], fmul2(z2[i], sg));
+                        }
+                    }
 #pragma unroll
                     for (int i = 0; i < P; ++i) {
-                        // silu'(z) = sg (1 + z (1 - sg))
-                        const float2 sg = sigmoid2(z2[i]), one = splat2(1.f);
-                        const float2 slope = fmul2(sg, ffma2(z2[i], fsub2(one, sg), one));
-                        dz2[i] = fmul2(fmul2(v2[i], ffma2(skip[i], u2[i], yo[i])), slope);
-                        v2[i] = fmul2(v2[i], fmul2(z2[i], sg));
+                        du2[i] = ffma2(st2[i], gbo[i], fmul2(skip[i], v2[i]));
+                        dd2[i] = ffma2(u2[i], gbo[i], fmul2(splat2(kLn2), dso[i]));
+                        if (p.softplus) dd2[i] = fmul2(dd2[i], sigmoid2(fadd2(r2[i], chn.bias[i])));
+                    }
+                    if (row < te) {
+                        const int64_t off = row * ys;
+                        float duo[CE], ddo[CE], dzo[CE];
+                        from_pairs<CE>(du2, duo);
+                        from_pairs<CE>(dd2, ddo);
+                        from_pairs<CE>(dz2, dzo);
+#pragma unroll
+                        for (int i = 0; i < P; ++i) {
+                            dskip[i] = ffma2(v2[i], u2[i], dskip[i]);
+                            dbias[i] = fadd2(dbias[i], dd2[i]);
+                        }
+                        store_v<CE>(du + off, ec, cend, bp.vec, duo);
+                        store_v<CE>(dd + off, ec, cend, bp.vec, ddo);
+                        if (dz) store_v<CE>(dz + off, ec, cend, bp.vec, dzo);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    du2[i] = ffma2(st2[i], gbo[i], fmul2(skip[i], v2[i]));
-                    dd2[i] = ffma2(u2[i], gbo[i], fmul2(splat2(kLn2), dso[i]));
-                    if (p.softplus) dd2[i] = fmul2(dd2[i], sigmoid2(fadd2(r2[i], chn.bias[i])));
-                }
-                if (row < te) {
-                    const int64_t off = row * ys;
-                    float duo[CE], ddo[CE], dzo[CE];
-                    from_pairs<CE>(du2, duo);
-                    from_pairs<CE>(dd2, ddo);
-                    from_pairs<CE>(dz2, dzo);
-#pragma unroll
-                    for (int i = 0; i < P; ++i) {
-                        dskip[i] = ffma2(v2[i], u2[i], dskip[i]);
-                        dbias[i] = fadd2(dbias[i], dd2[i]);
-                    }
-                    store_v<CE>(du + off, ec, cend, bp.vec, duo);
-                    store_v<CE>(dd + off, ec, cend, bp.vec, ddo);
-                    if (dz) store_v<CE>(dz + off, ec, cend, bp.vec, dzo);
-                }
+                __syncwarp();
             }
-            __syncwarp();
         }
-    }
-    if (bp.dinitial && t0 == 0) {
-        pair_down(g, v16);
-        store_block<NL>(bp.dinitial + (int64_t)s * p.channels * N, c0, cend, j, v16);
-    }
-    pair_down(da, v16);
-    store_lanes(bp.part_a + unit * 512, lane, v16);
-    sum_tokens<NL>(dskip, lane, own_c, bp.part_d + (w.slot * 2 * tiles + tile) * CW);
-    sum_tokens<NL>(dbias, lane, own_c, bp.part_d + ((w.slot * 2 + 1) * tiles + tile) * CW);
+        if (bp.dinitial && t0 == 0) {
+            pair_down(g, v16);
+            store_block<NL>(bp.dinitial + (int64_t)s * p.channels * N, c0, cend, j, v16);
+        }
+        pair_down(da, v16);
+        store_lanes(bp.part_a + unit * 512, lane, v16);
+        sum_tokens<NL>(dskip, lane, own_c, bp.part_d + (w.slot * 2 * tiles + tile) * CW);
+        sum_tokens<NL>(dbias, lane, own_c, bp.part_d + ((w.slot * 2 + 1) * tiles + tile) * CW);
     }
 }
 
