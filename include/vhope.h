@@ -567,6 +567,11 @@ typedef struct {
     float *grad_a, *grad_d_skip, *grad_delta_bias, *grad_initial;
 } vh_ssm_scan_bwd_args;
 
+/* Per element of u (token by channel) the checkpoints take states / 8 bytes and the backward's workspace
+ * states^2 / 64 (4 bytes at 16 states, 64 bytes at 64: a partial sum of grad_b and grad_c for every
+ * token and tile of 512 / states channels).  Chains in segments add up to 20 MB (forward) and 40 MB
+ * (backward).  Packed sequences add per sequence and tile up to 3 KB in the forward, 6 KB in the
+ * backward and 2 KB of checkpoints.  Sizes depend on the current device's multiprocessors. */
 int64_t vh_ssm_scan_bwd_workspace_bytes(const vh_ssm_scan_bwd_args* args);
 int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
 

@@ -85,3 +85,22 @@ def test_parameters_and_states_need_four_bytes():
     assert lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(a)) == 0 and "misaligned" in _err(lib)
     assert lib.vh_ssm_scan_step(ctypes.byref(scan(a=p + 4)), p, p, None, 4, None) == -5
     assert lib.vh_ssm_scan_step(ctypes.byref(scan()), p + 4, p, None, 4, None) == -5
+
+
+@pytest.mark.parametrize("states", [4, 8, 16, 32, 64])
+@pytest.mark.parametrize("batch,length,channels,packed", [(64, 3136, 1024, False), (2, 16384, 384, False), (8, 196, 512, False),
+                                                          (1000, 20000, 512, True), (17, 8192, 1024, True)])
+def test_memory_is_as_documented(batch, length, channels, packed, states):
+    """Checkpoints and workspaces per element, plus what segments and packed sequences add."""
+    from visionhope_b200 import _lib
+
+    lib, (p, keep) = _lib.load(), _fake()
+    a = _scan_args(_lib, p, batch=batch, length=length, channels=channels, states=states, seq_offsets=p if packed else None,
+                   checkpoints=p)
+    elements = channels * length * (1 if packed else batch)
+    per = batch * -(-channels * states // 512) if packed else 0  # sequences by tiles
+    fwd, ck = lib.vh_ssm_scan_fwd_workspace_bytes(ctypes.byref(a)), lib.vh_ssm_scan_checkpoint_bytes(ctypes.byref(a))
+    bwd = lib.vh_ssm_scan_bwd_workspace_bytes(ctypes.byref(_bwd(_lib, p, a)))
+    assert 0 <= fwd <= (20 << 20) + 3072 * per
+    assert elements * states // 8 <= ck + 2048 * per <= elements * states // 8 * 1.2 + 4096 * per
+    assert 0 <= bwd - elements * states ** 2 // 64 <= (40 << 20) + 6144 * per

@@ -12,9 +12,10 @@
 // wave of threads allows, so that weights, halo and the search for the sequence are paid once for
 // many tokens (forward with runs of 8, 16 and 24 tokens: 42, 36 and 35 us against 31 at the time).
 //
-// 64 sequences of 3136 tokens, 128 channels, K = 4, silu, bf16: forward 24 us (103 MB, 4.3 TB/s),
-// backward 49 us (154 MB, 3.1 TB/s), its sums over blocks 3.  Instruction issue is at 47 and 45 %,
-// DRAM at about 30 %.  Accesses of 16 bytes (eight channels a thread, half the threads) took 33
+// 64 sequences of 3136 tokens, 128 channels, K = 4, silu, bf16: forward 24 us (103 MB, 4.2 TB/s),
+// backward 48 us (154 MB, 3.2 TB/s), its sums over blocks 3.  No unit is at its limit: instruction issue
+// at 42 %, the special-function unit at 57 and 27 %, DRAM at about 30 %, with 20 and 15 warps an SM
+// waiting for memory.  Accesses of 16 bytes (eight channels a thread, half the threads) took 33
 // against 31 us, blocks of eight tokens 42 against 39.  24 packed sequences of 16384 tokens, 1024
 // channels: 20 us (67 MB, 3.4 TB/s).  The step of 256 streams of 2048 channels: 5.3 us, two dependent
 // latencies.

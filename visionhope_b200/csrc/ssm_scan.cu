@@ -3,8 +3,9 @@
 // The forward is bound by its exponentials and the arithmetic around them, not by memory: two
 // images of 64 x 256 tokens, 384 channels, 16 states, bf16 (12.6 M elements, 103 MB) take 165 us,
 // where the bytes would take 16 and the exponentials alone 45 for each of the two passes over a
-// chain in segments.  The special-function unit is at 56 / 44 %, the FMA pipe at 58 / 53 % and
-// instruction issue at 55 / 57 % in the first / last kernel (69 and about 90 us).
+// chain in segments.  The special-function unit is at 56 / 46 %, the FMA pipe at 57 / 52 % and
+// instruction issue at 55 / 56 % in the first / last kernel (70 and about 90 us): their 105 M warp
+// instructions alone would take 94 us at four a cycle and SM.
 #include "ssm_scan.cuh"
 
 namespace vh {
@@ -352,8 +353,8 @@ __global__ void __launch_bounds__(256, NL <= 4 ? 4 : 1) scan_step_kernel(const S
 bool stride_ok(int64_t v, int m) { return v % m == 0; }
 
 // Warps that a B200 holds of the forward kernel (four CTAs of four an SM).  Segments against whole
-// chains of 784 tokens, bf16, by device time: 256 chains 97 against 210 us, 512 168 / 210, 704 222 /
-// 257, 768 235 / 257, 832 261 / 257: whole chains from a third of the warps on.
+// chains of 784 tokens, bf16, by device time: 256 chains 99 against 211 us, 512 168 / 211, 704 223 /
+// 256, 768 236 / 256, 832 262 / 257: whole chains from a third of the warps on.
 int64_t fwd_warps() { return (int64_t)16 * sm_count(); }
 
 int fwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, fwd_warps() / 3, fwd_warps(), kGroup); }
@@ -459,9 +460,9 @@ int segment_size(const vh_ssm_scan_args* a, int64_t enough, int64_t warps, int s
     const int64_t tiles = tile_count(a), tokens = a->seq_offsets ? a->length : (int64_t)a->batch * a->length;
     // The host does not know the lengths of packed sequences: any of them may hold most tokens, so
     // they are always cut, and twice as fine, because a sequence's last segment is a short one (17
-    // sequences of 8192 tokens, 1024 channels: 128 us, against 135 as fine and 137 four times as).
+    // sequences of 8192 tokens, 1024 channels: 132 us, against 134 as fine and 141 four times as).
     // With few segments to a chain one wave of warps is badly filled, and two are better (forward of
-    // 512 chains of 784 tokens: 168 against 185 us; of 768: 235 / 289; but of 384: 139 / 133).
+    // 512 chains of 784 tokens: 169 against 185 us; of 768: 235 / 291; but of 384: 140 / 132).
     if (a->seq_offsets) warps *= 2;
     else if (a->batch * tiles >= enough) return 0;
     else if (a->batch * tiles * 5 >= warps) warps *= 2;
@@ -493,8 +494,8 @@ void place_segments(const vh_ssm_scan_args* a, int size, void* workspace, Segmen
 
 int enter_segments(const ScanParams& p, int states, const Segments& g, const float* first, bool right, cudaStream_t st) {
     // Long chains, of which there are few, are cut into runs; a packed sequence may hold most of the
-    // slots.  The forward's time with 1 / 4 / 16 runs: 7 segments of 128 chains 29 / 32 / 38 us, 18
-    // of 128 122 / 117 / 121, 74 of 32 63 / 59 / 53, 98 of 24 183 / 173 / 164.
+    // slots.  The forward's time with 1 / 4 / 16 runs: 7 segments of 128 chains 29 / 33 / 39 us, 18
+    // of 128 122 / 117 / 122, 74 of 32 62 / 59 / 54, 98 of 24 183 / 172 / 164.
     const int64_t chains = (int64_t)p.seqs.count * p.groups * p.tiles_per_group;
     const int64_t segs = p.seqs.offsets ? std::min<int64_t>(g.slots, 4 * (g.slots / p.seqs.count + 1)) : g.slots / p.seqs.count;
     return with_states(states, [&](auto nl) {

@@ -19,9 +19,10 @@
 // channels (db, dc) leave one partial per channel tile, sums over tokens (da, dD, d delta_bias)
 // one per sequence or segment, and a small kernel adds them in order.
 //
-// 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 488 us, 373 of them
-// this walk.  It is held by the 8 warps an SM that 255 registers leave: instruction issue is at
-// 39 %, shared memory at 64 %, the special-function unit at 27 %, DRAM at 8 % (243 MB).  Two
+// 64 sequences of 784 tokens, 256 channels, 16 states, bf16 (12.8 M elements): 479 us, 377 of them
+// this walk.  It is held by the 8 warps an SM that 255 registers and 27 KB of shared memory a warp
+// leave: instruction issue is at 39 %, shared memory at 64 %, the special-function unit at 28 %, DRAM at
+// 8 % (242 MB).  Two
 // channels a thread would let 12 warps in, but at 289 M instructions for 186 M: 476 us against 440.
 #include "ssm_scan.cuh"
 
@@ -539,10 +540,11 @@ struct Layout {
     int64_t tokens, rows, bc, a, d, total;  // floats
 };
 // Warps that a B200 holds of the backward kernel (two CTAs of three or four an SM).  Segments against
-// whole chains of 784 tokens, by device time: bf16, 256 chains 262 against 561 us, 640 602 / 740, 768
-// 709 / 749, 832 748 / 750; fp32, 512 580 / 717, 640 718 / 726, 768 893 / 727: whole chains from two
-// thirds of the warps on.  Four segments a warp even out the last wave: 512 chains 497 us against 533
-// with one and 560 with two, 128 chains of 2048 tokens 319 / 345 / 336; eight gain no more (491, 336).
+// whole chains of 784 tokens, by device time: bf16, 256 chains 251 against 567 us, 640 581 / 743, 768
+// 707 / 750, 832 727 / 752; fp32, 512 573 / 724, 640 711 / 732, 768 846 / 735: whole chains from two
+// thirds of the warps on (fp32's limit; bf16 would bear a few more segments).  Four segments a warp even
+// out the last wave: 512 chains 480 us against 540 with one and 477 with two, 128 chains of 2048 tokens
+// 308 / 332 / 324; eight 468 and 320.
 int64_t bwd_warps(const vh_ssm_scan_args* a) { return (int64_t)(a->dtype == VH_F32 ? 6 : 8) * sm_count(); }
 
 int bwd_segment_size(const vh_ssm_scan_args* a) { return segment_size(a, bwd_warps(a) * 2 / 3, 4 * bwd_warps(a), kCheckpoint); }

@@ -117,7 +117,8 @@ class _Call:
 
 
 class _SsmScanFunction(torch.autograd.Function):
-    """Saves the inputs and the state before every 32nd token (2 bytes per element at 16 states)."""
+    """Saves the inputs and the state before every 32nd token (states / 8 bytes per element of u); the
+    backward's workspace takes states^2 / 64 bytes per element."""
 
     @staticmethod
     def forward(ctx, u, delta, A, B, C, D, z, delta_bias, initial, softplus, want_final, offsets, reverse):
@@ -160,7 +161,9 @@ def ssm_scan(u, delta, A, B, C, D=None, *, z=None, delta_bias=None, delta_softpl
     [B, C, states] (zeros when None).  reverse reads every sequence from its last token to its
     first.  The state is fp32 throughout; y, of u's dtype, is rounded once.  Returns y, or (y,
     final_state) with ``return_final_state``.  Differentiable in every tensor, through y and the
-    final state; the sums of the backward run in a fixed order."""
+    final state; the sums of the backward run in a fixed order.  Steps times A are meant to be at most 0,
+    so that states decay: where they grow, a state other than zero may overflow sooner than token by
+    token, because long chains are computed in segments."""
     tensors = (u, delta, A, B, C, D, z, delta_bias, initial_state)
     if _args.tracked(tensors):
         return _SsmScanFunction.apply(*tensors, bool(delta_softplus), bool(return_final_state), seq_offsets,
