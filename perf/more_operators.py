@@ -75,8 +75,8 @@ def draw(rng):
         return dict(op=op, type=kind, batch=batch, slots=batch + rng.randrange(0, 64), heads=rng.randrange(1, 17), key=key,
                     value=value)
     if op == "linear":
-        key, value = rng.choice([(16, 16), (32, 32), (64, 64), (64, 64), (64, 128), (128, 128), (128, 128), (128, 256),
-                                 (48, 72), (100, 60)])
+        key, value = rng.choice([(16, 16), (32, 32), (64, 64), (64, 64), (64, 128), (128, 128), (128, 128), (48, 72),
+                                 (100, 60)])
         ragged = rng.random() < 0.4
         while True:
             batch, length, heads = _spread(rng, 1, 64), _spread(rng, 16, 16384), _spread(rng, 1, 16)
