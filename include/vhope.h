@@ -583,6 +583,52 @@ int vh_ssm_scan_bwd(const vh_ssm_scan_bwd_args* args, void* workspace, int64_t w
 int vh_ssm_scan_step(const vh_ssm_scan_args* args, const float* state, float* state_out, const int32_t* slots_index,
                      int32_t slots, vh_stream_t stream);
 
+/* Linear attention with a decay for each head (no counterpart in the reference).  Per sequence and
+ * head h, with lambda = exp(log_decay[h]) and a state S of [key_dim, value_dim] (initial_state, zeros
+ * if NULL, before the first token):
+ *     S_t = lambda S_{t-1} + k_t v_t^T,      o_t = scale q_t^T S_t
+ * q, k: [tokens, heads, key_dim], v: [tokens, heads, value_dim] of dtype, unit stride last, any batch,
+ * token and head strides (in elements); o: dtype, contiguous [tokens, heads, value_dim]; log_decay:
+ * fp32 [heads], at most 0; initial_state / final_state: fp32 [batch, heads, key_dim, value_dim] or
+ * NULL.  key_dim and value_dim 1 to 128.  Sequences, seq_offsets and reverse: as above.  The state is
+ * fp32 throughout.  workspace: vh_linear_attention_fwd_workspace_bytes(args) bytes, 16-byte aligned
+ * (its size depends on the current device's multiprocessors; sizes, dtype and whether seq_offsets is
+ * NULL are all that the query reads). */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    const float *log_decay, *initial_state;
+    void* o;
+    float* final_state;
+    const int32_t* seq_offsets;
+    int64_t length;
+    float scale;
+    int32_t dtype, batch, heads, key_dim, value_dim, reverse;
+} vh_linear_attention_args;
+
+int64_t vh_linear_attention_fwd_workspace_bytes(const vh_linear_attention_args* args);
+int vh_linear_attention_fwd(const vh_linear_attention_args* args, void* workspace, int64_t workspace_bytes,
+                            vh_stream_t stream);
+
+/* Its backward.  args: the forward's (o and final_state are not read).  grad_o: dtype, contiguous
+ * [tokens, heads, value_dim]; grad_final: fp32 [batch, heads, key_dim, value_dim] or NULL.  Writes
+ * grad_q, grad_k (dtype, contiguous [tokens, heads, key_dim]), grad_v (dtype, contiguous [tokens,
+ * heads, value_dim]) and grad_initial (fp32, as grad_final, or NULL).  The decays are constants: they
+ * get no gradient.  Nothing is saved by the forward; sums run in a fixed order. */
+int64_t vh_linear_attention_bwd_workspace_bytes(const vh_linear_attention_args* args);
+int vh_linear_attention_bwd(const vh_linear_attention_args* args, const void* grad_o, const float* grad_final, void* grad_q,
+                            void* grad_k, void* grad_v, float* grad_initial, void* workspace, int64_t workspace_bytes,
+                            vh_stream_t stream);
+
+/* One token of `batch` cached streams: q, k [batch, heads, key_dim], v [batch, heads, value_dim] (the
+ * batch and head strides of args; token strides are not used), o contiguous [batch, heads, value_dim],
+ * state fp32 [slots, heads, key_dim, value_dim].  args gives log_decay, scale and the sizes; its other
+ * fields are not read.  slots_index, slots, state, state_out: as vh_short_conv_step. */
+int vh_linear_attention_step(const vh_linear_attention_args* args, const float* state, float* state_out,
+                             const int32_t* slots_index, int32_t slots, vh_stream_t stream);
+
 /* Measurement helper (no reference counterpart): launches `blocks` x 256 threads, each
  * running 32 * iters dependent-free FMAs; out needs blocks * 256 floats.  bench.py times it
  * to measure the device's FP32 (non-tensor) FMA peak. */

@@ -99,6 +99,14 @@ class VhSsmScanBwdArgs(ctypes.Structure):
                                            "grad_c", "grad_a", "grad_d_skip", "grad_delta_bias", "grad_initial")])
 
 
+class VhLinearAttentionArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v")]
+                + [(f"{n}_{s}_stride", c_int64) for n in ("q", "k", "v") for s in ("batch", "token", "head")]
+                + [(n, c_void_p) for n in ("log_decay", "initial_state", "o", "final_state", "seq_offsets")]
+                + [("length", c_int64), ("scale", c_float)]
+                + [(n, c_int32) for n in ("dtype", "batch", "heads", "key_dim", "value_dim", "reverse")])
+
+
 _lib = None
 _lock = threading.Lock()
 _inited = set()
@@ -224,6 +232,18 @@ def load() -> ctypes.CDLL:
             lib.vh_ssm_scan_bwd.argtypes = [scan_bwd, c_void_p, c_int64, c_void_p]
             lib.vh_ssm_scan_step.restype = c_int32
             lib.vh_ssm_scan_step.argtypes = [scan, c_void_p, c_void_p, c_void_p, c_int32, c_void_p]
+            # linear attention with a decay for each head
+            linear = c_void_p
+            for name in ("fwd", "bwd"):
+                query = getattr(lib, f"vh_linear_attention_{name}_workspace_bytes")
+                query.restype = c_int64
+                query.argtypes = [linear]
+            lib.vh_linear_attention_fwd.restype = c_int32
+            lib.vh_linear_attention_fwd.argtypes = [linear, c_void_p, c_int64, c_void_p]
+            lib.vh_linear_attention_bwd.restype = c_int32
+            lib.vh_linear_attention_bwd.argtypes = [linear] + [c_void_p] * 7 + [c_int64, c_void_p]
+            lib.vh_linear_attention_step.restype = c_int32
+            lib.vh_linear_attention_step.argtypes = [linear, c_void_p, c_void_p, c_void_p, c_int32, c_void_p]
             _lib = lib
     return _lib
 

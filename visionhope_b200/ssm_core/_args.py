@@ -117,7 +117,7 @@ def cache(t, out, tail, batch, slots, dtype, device):
     """The step's state and where its successor goes (in place when ``out`` is None): both
     contiguous [slots, *tail] of ``dtype``, large enough for ``batch`` when there is no index."""
     for name, s in (("state", t),) if out is None else (("state", t), ("state_out", out)):
-        if s.dim() != 3 or s.shape[1:] != tail:
+        if s.dim() != len(tail) + 1 or s.shape[1:] != tail:
             raise ValueError(f"{name} must have shape [slots, {', '.join(map(str, tail))}], got {tuple(s.shape)}")
         if s.dtype is not dtype:
             refuse_dtype(name, dtype, s.dtype)
