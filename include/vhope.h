@@ -629,6 +629,36 @@ int vh_linear_attention_bwd(const vh_linear_attention_args* args, const void* gr
 int vh_linear_attention_step(const vh_linear_attention_args* args, const float* state, float* state_out,
                              const int32_t* slots_index, int32_t slots, vh_stream_t stream);
 
+/* Group norm over channels-last data with an activation and a gate (no counterpart in the reference).
+ * Each of `samples` has `pixels` rows of `channels`, and statistics over the channels / groups channels
+ * of a group at all its pixels (pixels 1: every row by itself):
+ *     pre = (x - mean) / sqrt(var + eps) * weight + bias,      y = act(pre) * silu(gate)
+ * x, gate (or NULL: no gate): dtype, unit channel stride, any sample and pixel strides (in elements);
+ * y: dtype, contiguous; weight, bias: fp32 [channels] or NULL (1, 0); activation: 0 none, 1 silu, 2
+ * gelu (by the error function); mean, rstd: fp32 [samples, groups], written for the backward, or both
+ * NULL.  workspace: vh_group_norm_fwd_workspace_bytes(args) bytes, 4-byte aligned (the query reads sizes
+ * and dtype alone; its answer depends on the current device's multiprocessors). */
+typedef struct {
+    const void *x, *gate;
+    int64_t x_sample_stride, x_pixel_stride, gate_sample_stride, gate_pixel_stride;
+    const float *weight, *bias;
+    void* y;
+    float *mean, *rstd;
+    int64_t samples, pixels;
+    float eps;
+    int32_t dtype, channels, groups, activation;
+} vh_group_norm_args;
+
+int64_t vh_group_norm_fwd_workspace_bytes(const vh_group_norm_args* args);
+int vh_group_norm_fwd(const vh_group_norm_args* args, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
+
+/* Its backward.  args: the forward's, with the mean and rstd it wrote (y is not read).  grad_y: dtype,
+ * contiguous.  Writes grad_x and, if not NULL, grad_gate (dtype, contiguous), grad_weight and grad_bias
+ * (fp32 [channels]).  Sums run in a fixed order. */
+int64_t vh_group_norm_bwd_workspace_bytes(const vh_group_norm_args* args);
+int vh_group_norm_bwd(const vh_group_norm_args* args, const void* grad_y, void* grad_x, void* grad_gate, float* grad_weight,
+                      float* grad_bias, void* workspace, int64_t workspace_bytes, vh_stream_t stream);
+
 /* Measurement helper (no reference counterpart): launches `blocks` x 256 threads, each
  * running 32 * iters dependent-free FMAs; out needs blocks * 256 floats.  bench.py times it
  * to measure the device's FP32 (non-tensor) FMA peak. */

@@ -107,6 +107,14 @@ class VhLinearAttentionArgs(ctypes.Structure):
                 + [(n, c_int32) for n in ("dtype", "batch", "heads", "key_dim", "value_dim", "reverse")])
 
 
+class VhGroupNormArgs(ctypes.Structure):
+    _fields_ = ([(n, c_void_p) for n in ("x", "gate")]
+                + [(f"{n}_{s}_stride", c_int64) for n in ("x", "gate") for s in ("sample", "pixel")]
+                + [(n, c_void_p) for n in ("weight", "bias", "y", "mean", "rstd")]
+                + [("samples", c_int64), ("pixels", c_int64), ("eps", c_float)]
+                + [(n, c_int32) for n in ("dtype", "channels", "groups", "activation")])
+
+
 _lib = None
 _lock = threading.Lock()
 _inited = set()
@@ -244,6 +252,16 @@ def load() -> ctypes.CDLL:
             lib.vh_linear_attention_bwd.argtypes = [linear] + [c_void_p] * 7 + [c_int64, c_void_p]
             lib.vh_linear_attention_step.restype = c_int32
             lib.vh_linear_attention_step.argtypes = [linear, c_void_p, c_void_p, c_void_p, c_int32, c_void_p]
+            # group norm with an activation and a gate
+            norm = c_void_p
+            for name in ("fwd", "bwd"):
+                query = getattr(lib, f"vh_group_norm_{name}_workspace_bytes")
+                query.restype = c_int64
+                query.argtypes = [norm]
+            lib.vh_group_norm_fwd.restype = c_int32
+            lib.vh_group_norm_fwd.argtypes = [norm, c_void_p, c_int64, c_void_p]
+            lib.vh_group_norm_bwd.restype = c_int32
+            lib.vh_group_norm_bwd.argtypes = [norm] + [c_void_p] * 6 + [c_int64, c_void_p]
             _lib = lib
     return _lib
 
