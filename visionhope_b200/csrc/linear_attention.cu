@@ -54,6 +54,33 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// c += the products of planes of one k-step.  The matrix unit truncates its sums (a bias of up to 2^-23 of
+// the sum for each instruction), so where several planes make up a value, or a sum lives on from chunk to
+// chunk, a k-step is summed from zero, its small products first, and added to c by a rounded addition.
+template <int NA, int NB, int KEEP>
+__device__ __forceinline__ void product(float (&c0)[4], float (&c1)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][4]) {
+    if constexpr (NA == 1 && NB == 1) {
+        mma(c0, a[0], b[0][0], b[0][1]);
+        mma(c1, a[0], b[0][2], b[0][3]);
+    } else {
+        float d0[4] = {}, d1[4] = {};
+#pragma unroll
+        for (int sum = KEEP - 1; sum >= 0; --sum)
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int j = sum - i;
+                if (j < 0 || j >= NB) continue;
+                mma(d0, a[i], b[j][0], b[j][1]);
+                mma(d1, a[i], b[j][2], b[j][3]);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c0[i] += d0[i];
+            c1[i] += d1[i];
+        }
+    }
+}
+
 // ---- shared memory ------------------------------------------------------------------------------
 // Rows are 16 bytes longer than they hold, so that the eight rows of a matrix load lie in different
 // banks.
@@ -252,17 +279,13 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
             // q S_0 and the scores q k^T, up to the diagonal
             auto from_state = [&](int kk, const uint32_t (&qa)[NP][4]) {
 #pragma unroll
-                for (int np = 0; np < 4; ++np)
+                for (int np = 0; np < 4; ++np) {
+                    uint32_t b[NP][4];
 #pragma unroll
-                    for (int pb = 0; pb < NP; ++pb) {
-                        uint32_t b[4];
-                        ldsm4t(b, state + pb * L::kS + (kk * 16 + (lane & 15)) * VP + np * 16 + (lane >> 4) * 8);
-#pragma unroll
-                        for (int pa = 0; pa + pb < NP; ++pa) {
-                            mma(o[2 * np], qa[pa], b[0], b[1]);
-                            mma(o[2 * np + 1], qa[pa], b[2], b[3]);
-                        }
-                    }
+                    for (int pb = 0; pb < NP; ++pb)
+                        ldsm4t(b[pb], state + pb * L::kS + (kk * 16 + (lane & 15)) * VP + np * 16 + (lane >> 4) * 8);
+                    product<NP, NP, NP>(o[2 * np], o[2 * np + 1], qa, b);
+                }
             };
             auto load_q = [&](int kk, uint32_t (&qa)[NP][4]) {
 #pragma unroll
@@ -277,16 +300,11 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
 #pragma unroll
                 for (int np = 0; np < 4; ++np) {
                     if (np > warp) continue;
+                    uint32_t b[NP][4];
 #pragma unroll
-                    for (int pb = 0; pb < NP; ++pb) {
-                        uint32_t b[4];
-                        ldsm4(b, kt + pb * L::kQ + (np * 16 + (lane & 7) + (lane >> 4) * 8) * P + kk * 16 + ((lane >> 3) & 1) * 8);
-#pragma unroll
-                        for (int pa = 0; pa + pb < NP; ++pa) {
-                            mma(sc[2 * np], qa[pa], b[0], b[1]);
-                            mma(sc[2 * np + 1], qa[pa], b[2], b[3]);
-                        }
-                    }
+                    for (int pb = 0; pb < NP; ++pb)
+                        ldsm4(b[pb], kt + pb * L::kQ + (np * 16 + (lane & 7) + (lane >> 4) * 8) * P + kk * 16 + ((lane >> 3) & 1) * 8);
+                    product<NP, NP, NP>(sc[2 * np], sc[2 * np + 1], qa, b);
                 }
             }
             const int i0 = row0 + g, i1 = i0 + 8;
@@ -323,17 +341,13 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
                     }
                 }
 #pragma unroll
-                for (int nq = 0; nq < 4; ++nq)
+                for (int nq = 0; nq < 4; ++nq) {
+                    uint32_t b[NP][4];
 #pragma unroll
-                    for (int pb = 0; pb < NP; ++pb) {
-                        uint32_t b[4];
-                        ldsm4t(b, vt + pb * L::kV + (np * 16 + (lane & 15)) * VP + nq * 16 + (lane >> 4) * 8);
-#pragma unroll
-                        for (int pl = 0; pl + pb < NP; ++pl) {
-                            mma(o[2 * nq], pa_[np][pl], b[0], b[1]);
-                            mma(o[2 * nq + 1], pa_[np][pl], b[2], b[3]);
-                        }
-                    }
+                    for (int pb = 0; pb < NP; ++pb)
+                        ldsm4t(b[pb], vt + pb * L::kV + (np * 16 + (lane & 15)) * VP + nq * 16 + (lane >> 4) * 8);
+                    product<NP, NP, NP>(o[2 * nq], o[2 * nq + 1], pa_[np], b);
+                }
             }
             // A value that is not finite must not reach the rows before it: 0 times it is NaN in the
             // product above.  Such chunks are rare; their rows are summed again, term by term.
@@ -461,17 +475,13 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
                         for (int pl = 0; pl < 3; ++pl) a[pl][i] = w3[pl];
                     }
 #pragma unroll
-                    for (int np = 0; np < 4; ++np)
+                    for (int np = 0; np < 4; ++np) {
+                        uint32_t b[NP][4];
 #pragma unroll
-                        for (int pb = 0; pb < NP; ++pb) {
-                            uint32_t b[4];
-                            ldsm4t(b, vt + pb * L::kV + (kk * 16 + (lane & 15)) * VP + np * 16 + (lane >> 4) * 8);
-#pragma unroll
-                            for (int pl = 0; pl + pb < 3; ++pl) {
-                                mma(s[mt][2 * np], a[pl], b[0], b[1]);
-                                mma(s[mt][2 * np + 1], a[pl], b[2], b[3]);
-                            }
-                        }
+                        for (int pb = 0; pb < NP; ++pb)
+                            ldsm4t(b[pb], vt + pb * L::kV + (kk * 16 + (lane & 15)) * VP + np * 16 + (lane >> 4) * 8);
+                        product<3, NP, 3>(s[mt][2 * np], s[mt][2 * np + 1], a, b);
+                    }
                 }
             }
         }
