@@ -90,7 +90,7 @@ def test_sequences(dtype, shape, reverse):
         want = recurrence(q, k, v, g, scale, initial, reverse, do, dfinal)
         aq, ak, av, ai, ado, adf = absolute(q, k, v, initial, do, dfinal)
         size = recurrence(aq, ak, av, g, scale, ai, reverse, ado, adf)
-        leaves = [t.detach().clone().requires_grad_() if t is not None else None for t in (q, k, v, initial)]
+        leaves = [t.detach().requires_grad_() if t is not None else None for t in (q, k, v, initial)]  # strides as they are
         plain, final = linear_attention(q, k, v, g, initial_state=initial, return_final_state=True, reverse=reverse)
         near(plain, want[0], size[0], dtype, chunks)
         near(final, want[1], size[1], dtype, chunks, operand=2 ** -15 if dtype == torch.float16 else 2 ** -22)
@@ -102,6 +102,38 @@ def test_sequences(dtype, shape, reverse):
         for x, w, s in zip(got, want[2:], size[2:]):
             exact = x.dtype == torch.float32 and dtype != torch.float32
             near(x, w, s, dtype, chunks, operand=2 ** -15 if exact else None)
+
+
+ALIGNED = [(1, 128, 1, 64, 64), (2, 129, 3, 64, 64), (1, 200, 2, 128, 128), (2, 255, 2, 64, 128), (1, 384, 2, 128, 64), (3, 777, 2, 64, 64),
+           (1, 300, 2, 72, 104), (2, 640, 1, 16, 8), (1, 5000, 2, 128, 128), (1, 4099, 1, 64, 64), (40, 257, 4, 64, 64), (2, 100, 2, 64, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", ALIGNED)
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("with_states", [False, True])
+def test_aligned_rows(dtype, shape, reverse, with_states):
+    """As above from rows that start on 16 bytes, where wide copies and tiles are taken."""
+    b, n, h, dk, dv = shape
+    rows = normal(1, b, n, h * (2 * dk + dv), dtype=dtype)
+    q, k, v = rows.split((h * dk, h * dk, h * dv), dim=-1)
+    q, k, v = q.view(b, n, h, dk), k.view(b, n, h, dk), v.view(b, n, h, dv)
+    g, scale, chunks = decays(h), dk ** -0.5, n // 64 + 2
+    initial = normal(2, b, h, dk, dv) if with_states else None
+    do = normal(3, b, n, h, dv, dtype=dtype)
+    dfinal = normal(4, b, h, dk, dv) if with_states else None
+    want = recurrence(q, k, v, g, scale, initial, reverse, do, dfinal)
+    size = recurrence(*absolute(q, k, v), g, scale, *absolute(initial), reverse, *absolute(do, dfinal))
+    leaves = [t.detach().requires_grad_() if t is not None else None for t in (q, k, v, initial)]
+    got = linear_attention(*leaves[:3], g, initial_state=leaves[3], return_final_state=with_states, reverse=reverse)
+    o = got[0] if with_states else got
+    near(o, want[0], size[0], dtype, chunks)
+    if with_states:
+        near(got[1], want[1], size[1], dtype, chunks, operand=2 ** -15 if dtype == torch.float16 else 2 ** -22)
+    live = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad([o, got[1]] if with_states else [o], live, [do, dfinal] if with_states else [do])
+    for x, w, s in zip(grads, want[2:], size[2:]):
+        near(x, w, s, dtype, chunks, operand=2 ** -15 if x.dtype == torch.float32 and dtype != torch.float32 else None)
 
 
 def test_default_scale_and_no_state():
@@ -313,6 +345,13 @@ def test_streams_and_graphs():
         s = state.clone()
         assert torch.equal(o3, linear_attention_step(fresh[0][:, 0].detach(), fresh[1][:, 0].detach(), fresh[2][:, 0].detach(), g, s))
         assert torch.equal(s2, s)
+
+
+def test_no_wait_gave_up():
+    """After everything above, none of the tensor-core kernels' bounded waits has run out."""
+    from visionhope_b200 import _lib
+
+    assert _lib.load().vh_tc_status(0) == 0
 
 
 @pytest.mark.parametrize("shape", [(0, 5, 2, 64, 64), (2, 0, 2, 64, 64), (2, 5, 0, 64, 64)])

@@ -135,33 +135,6 @@ __device__ __forceinline__ void load_tile(uint16_t* dst, const T* src, int64_t s
     }
 }
 
-// One unit of work: which tokens of which sequence.
-struct Unit {
-    int s;
-    Seq e;
-    int64_t slot, t0, t1;
-    bool live;
-};
-__device__ __forceinline__ Unit unit_at(const Params& p, int64_t index) {
-    Unit u;
-    u.slot = index;
-    if (p.segment == 0) {
-        u.s = (int)index;
-        u.e = ssm::seq_at(p.seqs, u.s);
-        u.t0 = 0;
-        u.t1 = u.e.len;
-        u.live = true;
-        return u;
-    }
-    u.s = ssm::seq_of_slot(p.seqs, index, p.segment);
-    u.e = ssm::seq_at(p.seqs, u.s);
-    const int64_t j = index - ssm::slot_base(p.seqs, u.s, u.e.row, p.segment);
-    u.t0 = j * p.segment;
-    u.t1 = min(u.e.len, u.t0 + p.segment);
-    u.live = j >= 0 && (u.t0 < u.e.len || j == 0);
-    return u;
-}
-
 // A chain, or a segment of one: a CTA walks its chunks, the state in the accumulators of its four
 // warps (each a quarter of the key rows by 64 value columns) and, for the outputs, as a bf16 operand
 // in shared memory.  OUT false computes only what the segment adds to the state.
@@ -706,11 +679,6 @@ int segment_size(int64_t length, int batch, bool packed, int heads, int dv) {
     return size < length ? (int)size : 0;
 }
 
-int64_t segment_bytes(int64_t length, int batch, bool packed, int heads, int dk, int dv, int size) {
-    if (size == 0) return 0;
-    return ssm::slot_total(packed, length, batch, size) * heads * dk * dv * (int64_t)sizeof(float);
-}
-
 template <typename T, int DK, bool OUT>
 int launch_chunks(const Params& p, int64_t units, cudaStream_t st) {
     using L = Layout<T, DK, OUT>;
@@ -721,36 +689,39 @@ int launch_chunks(const Params& p, int64_t units, cudaStream_t st) {
     return launch_status(OUT ? "linear attention" : "linear attention: segment states");
 }
 
-// One pass of the operator over prepared parameters; `states` holds segment_bytes() if there are segments.
+// One pass of the operator over prepared parameters; `states` holds pass_bytes().
 int run(Params p, int dtype, void* states, cudaStream_t st) {
     const bool packed = p.seqs.offsets != nullptr;
+    p.vec_o = vec_of(p.o, {0, (int64_t)p.heads * p.dv}, p.dv, p.dv, dtype, true);
+    int rc = 0;
+    if (dtype == VH_BF16 && tc_run(p, states, st, &rc)) return rc;
     p.segment = segment_size(p.seqs.length, p.seqs.count, packed, p.heads, p.dv);
     p.states = static_cast<float*>(states);
-    p.vec_o = vec_of(p.o, {0, (int64_t)p.heads * p.dv}, p.dv, p.dv, dtype, true);
     const int64_t units = p.segment ? ssm::slot_total(packed, p.seqs.length, p.seqs.count, p.segment) : p.seqs.count;
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         const bool narrow = p.dk <= 64;
         if (p.segment) {
             if (int rc = narrow ? launch_chunks<T, 64, false>(p, units, st) : launch_chunks<T, 128, false>(p, units, st)) return rc;
-            const int64_t states_n = (int64_t)p.dk * p.dv;
-            enter_kernel<<<dim3(p.seqs.count, p.heads, (unsigned)((states_n + 255) / 256)), 256, 0, st>>>(p);
-            if (int rc = launch_status("linear attention: entering states")) return rc;
+            if (int rc = enter_segments(p, st)) return rc;
         }
         return narrow ? launch_chunks<T, 64, true>(p, units, st) : launch_chunks<T, 128, true>(p, units, st);
     });
 }
 
-int64_t fwd_bytes(const vh_linear_attention_args* a) {
+// The states of a pass's segments, in whichever form it runs.
+int64_t pass_bytes(const vh_linear_attention_args* a, int dk, int dv) {
     const bool packed = a->seq_offsets != nullptr;
-    return segment_bytes(a->length, a->batch, packed, a->heads, a->key_dim, a->value_dim,
-                         segment_size(a->length, a->batch, packed, a->heads, a->value_dim));
+    int64_t most = 0;
+    for (int size : {segment_size(a->length, a->batch, packed, a->heads, dv),
+                     a->dtype == VH_BF16 ? tc_segment_size(a->length, a->batch, packed, a->heads, dk, dv) : 0})
+        if (size) most = std::max(most, ssm::slot_total(packed, a->length, a->batch, size) * a->heads * dk * dv * (int64_t)sizeof(float));
+    return most;
 }
-// dq and dk have the key dim as their value columns
+int64_t fwd_bytes(const vh_linear_attention_args* a) { return pass_bytes(a, a->key_dim, a->value_dim); }
+// the passes for dq and dk have the two dims the other way round
 int64_t bwd_bytes(const vh_linear_attention_args* a) {
-    const bool packed = a->seq_offsets != nullptr;
-    return std::max(fwd_bytes(a), segment_bytes(a->length, a->batch, packed, a->heads, a->key_dim, a->value_dim,
-                                                segment_size(a->length, a->batch, packed, a->heads, a->key_dim)));
+    return std::max(fwd_bytes(a), pass_bytes(a, a->value_dim, a->key_dim));
 }
 
 int check_workspace(const char* what, const void* ws, int64_t have, int64_t need) {
@@ -761,6 +732,13 @@ int check_workspace(const char* what, const void* ws, int64_t have, int64_t need
 }
 
 }  // namespace
+
+int enter_segments(const Params& p, cudaStream_t st) {
+    const int64_t states = (int64_t)p.dk * p.dv;
+    enter_kernel<<<dim3(p.seqs.count, p.heads, (unsigned)((states + 255) / 256)), 256, 0, st>>>(p);
+    return launch_status("linear attention: entering states");
+}
+
 }  // namespace lin
 }  // namespace vh
 

@@ -56,5 +56,41 @@ __device__ __forceinline__ float decay_power(float log_decay, int64_t n) {
     return expf(g * (float)n);
 }
 
+// One unit of work: which tokens of which sequence.
+struct Unit {
+    int s;
+    Seq e;
+    int64_t slot, t0, t1;
+    bool live;
+};
+__device__ __forceinline__ Unit unit_at(const Params& p, int64_t index) {
+    Unit u;
+    u.slot = index;
+    if (p.segment == 0) {
+        u.s = (int)index;
+        u.e = ssm::seq_at(p.seqs, u.s);
+        u.t0 = 0;
+        u.t1 = u.e.len;
+        u.live = true;
+        return u;
+    }
+    u.s = ssm::seq_of_slot(p.seqs, index, p.segment);
+    u.e = ssm::seq_at(p.seqs, u.s);
+    const int64_t j = index - ssm::slot_base(p.seqs, u.s, u.e.row, p.segment);
+    u.t0 = j * p.segment;
+    u.t1 = min(u.e.len, u.t0 + p.segment);
+    u.live = j >= 0 && (u.t0 < u.e.len || j == 0);
+    return u;
+}
+
+// From what each segment adds to the state before each of them (linear_attention.cu).
+int enter_segments(const Params& p, cudaStream_t st);
+
+// The tcgen05 form (linear_attention_tc.cu).  tc_run does nothing and returns false where it does not
+// apply; `states` holds the states of its segments.
+int tc_segment_size(int64_t length, int batch, bool packed, int heads, int dk, int dv);
+bool tc_run(Params p, void* states, cudaStream_t st, int* rc);
+unsigned tc_status(bool reset);
+
 }  // namespace lin
 }  // namespace vh

@@ -692,6 +692,12 @@ int run_tc_sequence(const ScanParams& p, cudaStream_t st) {
 
 }  // namespace vh
 
+namespace vh {
+namespace lin {
+unsigned tc_status(bool reset);  // linear_attention_tc.cu
+}
+}  // namespace vh
+
 extern "C" int vh_tc_status(int32_t reset) {
     unsigned int v = 0;
     if (cudaMemcpyFromSymbol(&v, vh::tc::g_tc_status, sizeof(v)) != cudaSuccess) return -1;
@@ -699,5 +705,5 @@ extern "C" int vh_tc_status(int32_t reset) {
         const unsigned int z = 0;
         cudaMemcpyToSymbol(vh::tc::g_tc_status, &z, sizeof(z));
     }
-    return (int)v;
+    return (int)(v | vh::lin::tc_status(reset != 0));
 }
