@@ -489,26 +489,25 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
 // the segments of its sequence.
 __global__ void __launch_bounds__(256) enter_kernel(Params p) {
     const int s = blockIdx.x, h = blockIdx.y;
-    const int64_t states = (int64_t)p.dk * p.dv;
-    const int64_t i = (int64_t)blockIdx.z * 256 + threadIdx.x;
+    const int states = p.dk * p.dv, i = blockIdx.z * 256 + threadIdx.x;
     const Seq e = ssm::seq_at(p.seqs, s);
     if (i >= states || e.len <= p.segment) return;
     const int64_t base = ssm::slot_base(p.seqs, s, e.row, p.segment);
     const float g = p.log_decay[h];
-    const int64_t a = i / p.dv, b = i % p.dv;
+    const int a = i / p.dv, b = i - a * p.dv;
     float run = p.initial ? p.initial[((int64_t)s * p.heads + h) * states + a * p.init_a + b * p.init_b] : 0.f;
     const float step = decay_power(g, p.segment);
     float w = p.entry ? decay_power(g, p.segment - 1) : step;
     float* at = p.states + (base * p.heads + h) * states + i;
-    const int64_t stride = p.heads * states;
+    const int64_t stride = (int64_t)p.heads * states;
     const int64_t segs = (e.len + p.segment - 1) / p.segment;
     int64_t j = 0;
-    for (; j + 4 < segs; j += 4) {  // loads ahead of the chain; the last segment adds to nobody's start
-        float own[4];
+    for (; j + 8 < segs; j += 8) {  // loads ahead of the chain; the last segment adds to nobody's start
+        float own[8];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) own[x] = at[(j + x) * stride];
+        for (int x = 0; x < 8; ++x) own[x] = at[(j + x) * stride];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < 8; ++x) {
             at[(j + x) * stride] = run;
             run = run * w + own[x];
             w = step;

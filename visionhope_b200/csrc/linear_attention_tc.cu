@@ -1,6 +1,6 @@
 // Linear attention on tcgen05: bf16 rows whose addresses TMA takes, in chunks of 128 tokens.
 //
-// A CTA of 256 threads walks the chunks of one chain or segment (one head).  Per chunk, with the fp32
+// A CTA walks the chunks of one chain or segment (one head).  Per chunk, with the fp32
 // state S in registers and its bf16 rounding in shared memory:
 //     scores = Q K^T, O2 = Q S             -> TMEM   (operands as TMA brought them)
 //     P = scores * lambda^(i-j), bf16      TMEM -> TMEM
@@ -30,14 +30,14 @@ namespace lin {
 namespace {
 
 constexpr int kT = 128;         // tokens a chunk
-constexpr int kThreads = 256;
+constexpr int kCompute = 256;   // threads at the tiles
 constexpr int kTileBytes = kT * 128;  // 128 rows of 64 bf16, 128-byte swizzle
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 __device__ unsigned int g_status;  // non-zero once a bounded wait gave up
 
 struct Maps {
-    CUtensorMap q, k, v;
+    CUtensorMap q, k, v, o;
 };
 
 // ---- instructions that only this kernel uses ------------------------------------------------------
@@ -48,6 +48,9 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
+// The operand `bytes` further on.  Descriptors come from one by additions of constants: a product that waits
+// for its descriptor's arithmetic takes twice its 64 cycles to issue.
+__device__ __forceinline__ uint64_t ahead(uint64_t d, uint32_t bytes) { return d + (bytes >> 4); }
 constexpr uint32_t kMajorA = 1u << 15, kMajorB = 1u << 16;  // outer axis contiguous
 
 // D (+)= A B with A in TMEM (32-bit columns of two consecutive contraction elements).
@@ -76,178 +79,435 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// A tile from shared memory (rows of 64 columns in the same swizzle) to global memory.
+__device__ __forceinline__ void tma_store_4d(const void* map, const void* src, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(tcu::smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- shared memory ------------------------------------------------------------------------------
-// Two stages of tiles [K | V | Q], each of blocks of 64 columns; then the state's operand, which is also
-// where the third plane of K~ goes.  The second plane goes where Q was, or, without Q, behind.
-template <int DK, int DV, int KP, bool OUT>
+// Two stages of tiles [V | K | Q], each of blocks of 64 columns; then the state's operand, which is also
+// where the third plane of K~ goes (the second goes where Q was).  A chunk's outputs leave from the end of
+// its stage: what lies before them is loaded for the chunk after next at once, the rest when they have left.
+template <int DK, int DV, int KP>
 struct Smem {
-    static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64), kQ = OUT ? kK : 0;
-    static constexpr int kStage = kK + kV + kQ;
-    static constexpr int kState = OUT ? (KP == 3 && kK > DK * DV * 2 ? kK : DK * DV * 2) : kK * (KP - 1);
+    static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64);
+    static constexpr int kKeys = kV, kQueries = kV + kK, kStage = kV + 2 * kK, kOut = kStage - kV;
+    static constexpr bool kKeysEarly = kOut >= kQueries;
+    static constexpr int kState = KP == 3 && kK > DK * DV * 2 ? kK : DK * DV * 2;
     static constexpr int kPower = 2 * kStage + kState;             // lambda^n, n = 0..128, and times kv_scale
-    static constexpr int kBars = kPower + 2 * 132 * 4;             // 5 barriers, TMEM base, a flag
-    static constexpr int kBytes = kBars + 64;
-    static constexpr int kLaunch = kBytes + 1024;                  // the tiles start on 1024 bytes
+    static constexpr int kWeights = kPower + 2 * 132 * 4;          // of a score: by column, and on the diagonal
+    static constexpr int kBars = kWeights + (32 + 64) * 4;         // 5 barriers, TMEM base, a flag
+    static constexpr int kLaunch = kBars + 64 + 1024;              // the tiles start on 1024 bytes
+    static_assert(kLaunch <= 232448, "shared memory of an SM");
+};
+// Without outputs: three stages of tiles [V | K] where they fit, and the planes of K~ behind the first.
+template <int DK, int DV, int KP>
+struct StatesSmem {
+    static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64);
+    static constexpr int kStage = kK + kV, kPlanes = (KP - 1) * kK;
+    static constexpr int kStages = 3 * kStage + kPlanes + 2048 <= (DK + DV == 128 ? 114 : 226) * 1024 ? 3 : 2;
+    static constexpr int kPower = kStages * kStage + kPlanes;
+    static constexpr int kBars = kPower + 132 * 4;                 // a barrier a stage, the product's, TMEM base, a flag
+    static constexpr int kLaunch = kBars + 64 + 1024;
     static_assert(kLaunch <= 232448, "shared memory of an SM");
 };
 
-template <int DK, int DV, int KP, bool OUT>
-__global__ void __launch_bounds__(kThreads, DK + DV == 128 ? 2 : 1) tc_kernel(const __grid_constant__ Params p,
-                                                                             const __grid_constant__ Maps maps) {
-    using S = Smem<DK, DV, KP, OUT>;
-    constexpr int kCols = DV == 64 ? 256 : 512;
-    constexpr uint32_t cScore = 0, cO1 = 128, cO2 = 128 + DV, cU = DV == 64 ? 64 : 384;
-    constexpr int NC = DK == 128 ? DV / 2 : DV / 4;  // state columns a thread
+// What both kernels know of their unit.
+template <int DK, int DV>
+struct Chain {
+    static constexpr int NC = DK == 128 ? DV / 2 : DV / 4;  // state columns a thread
+    const Params& p;
+    const Unit& u;
+    int a, b0;  // this thread's part of the state: key row a, NC value columns from b0 on
+
+    __device__ __forceinline__ Chain(const Params& params, const Unit& unit) : p(params), u(unit) {
+        const int quad = threadIdx.x >> 5 & 3, half = threadIdx.x >> 7, lane = threadIdx.x & 31;
+        a = DK == 128 ? quad * 32 + lane : (quad & 1) * 32 + lane;
+        b0 = DK == 128 ? half * NC : (half * 2 + (quad >> 1)) * NC;
+    }
+    __device__ __forceinline__ int chunks() const { return (int)((u.t1 - u.t0 + kT - 1) / kT); }
+    __device__ __forceinline__ int tokens(int c) const { return (int)min((int64_t)kT, u.t1 - u.t0 - (int64_t)c * kT); }
+    // a chunk's first row in memory, counted from the sequence's
+    __device__ __forceinline__ int64_t first_row(int c) const {
+        const int64_t t = u.t0 + (int64_t)c * kT;
+        return p.seqs.reverse ? u.e.len - t - tokens(c) : t;
+    }
+    __device__ __forceinline__ int row_at(int c) const { return (int)(first_row(c) + (p.seqs.offsets ? u.e.row : 0)); }
+    __device__ __forceinline__ int batch_at() const { return p.seqs.offsets ? 0 : u.s; }
+
+    // The state from global memory: element (a, b) at from[a fa + b fb].  Through shared memory (`tile`, rows
+    // of DV + 4), because a thread's columns are far from its neighbour's.  Ends with everybody done reading.
+    template <typename Sync>
+    __device__ __forceinline__ void load_state(float (&s)[NC], const float* from, int64_t fa, int64_t fb, float* tile, Sync sync) const {
+        const bool across = fb == 1;
+        const int inner = across ? p.dv : p.dk, outer = across ? p.dk : p.dv;
+        for (int i = threadIdx.x; i < inner * outer; i += kCompute) {
+            const int o = i / inner, x = i - o * inner;
+            const int ra = across ? o : x, cb = across ? x : o;
+            tile[ra * (DV + 4) + cb] = from[ra * fa + cb * fb];
+        }
+        sync();
+#pragma unroll
+        for (int i = 0; i < NC; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(tile + a * (DV + 4) + b0 + i);
+            const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i + e] = a < p.dk && b0 + i + e < p.dv ? f[e] : 0.f;
+        }
+        sync();
+    }
+    template <typename Sync>
+    __device__ __forceinline__ void store_state(const float (&s)[NC], float* to, float scale, float* tile, Sync sync) const {
+        sync();
+#pragma unroll
+        for (int i = 0; i < NC; i += 4)
+            *reinterpret_cast<float4*>(tile + a * (DV + 4) + b0 + i) =
+                make_float4(s[i] * scale, s[i + 1] * scale, s[i + 2] * scale, s[i + 3] * scale);
+        sync();
+        for (int i = threadIdx.x; i < p.dk * p.dv; i += kCompute) {
+            const int r = i / p.dv, c = i - r * p.dv;
+            to[i] = tile[r * (DV + 4) + c];
+        }
+    }
+    // S = w S + U
+    __device__ __forceinline__ void update(float (&s)[NC], uint32_t at, float w) const {
+#pragma unroll
+        for (int i0 = 0; i0 < NC; i0 += 16) {
+            float x[16];
+            tcu::tmem_ld16(at + b0 + i0, x);
+            tcu::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i0 + i] = fmaf(s[i0 + i], w, x[i]);
+        }
+    }
+};
+
+// Planes of the weighted keys of n tokens, the first in place; rows past the sequence become zeros.
+template <int DK, int KP>
+__device__ __forceinline__ void weigh_keys(uint8_t* kt, uint8_t* plane1, uint8_t* plane2, const float* weight, int n, bool reverse) {
+#pragma unroll 2
+    for (int i = threadIdx.x; i < kT * DK / 8; i += kCompute) {
+        const int j = i / 8 % kT;
+        uint4 x = *reinterpret_cast<const uint4*>(kt + i * 16);
+        if (j >= n) x = make_uint4(0, 0, 0, 0);
+        const float2 w = splat2(weight[j < n ? (reverse ? j : n - 1 - j) : 0]);
+        const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+        uint32_t out[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float2 v = fmul2(make_float2(__uint_as_float(words[e] << 16), __uint_as_float(words[e] & 0xffff0000u)), w);
+#pragma unroll
+            for (int pl = 0; pl < KP; ++pl) {
+                const uint32_t b = ssm::join(v.x, v.y, __nv_bfloat16{});
+                out[pl][e] = b;
+                if (pl + 1 < KP) v = fsub2(v, make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)));
+            }
+        }
+        *reinterpret_cast<uint4*>(kt + i * 16) = make_uint4(out[0][0], out[0][1], out[0][2], out[0][3]);
+        *reinterpret_cast<uint4*>(plane1 + i * 16) = make_uint4(out[1][0], out[1][1], out[1][2], out[1][3]);
+        if constexpr (KP == 3) *reinterpret_cast<uint4*>(plane2 + i * 16) = make_uint4(out[2][0], out[2][1], out[2][2], out[2][3]);
+    }
+    tcu::fence_proxy_async_smem();
+}
+
+// Rows past the sequence are another's: their products with zeros must be zeros.
+template <int DV>
+__device__ __forceinline__ void clear_values(uint8_t* vt, int n) {
+    for (int i = threadIdx.x; i < (kT - n) * (DV / 8); i += kCompute) {
+        const int r = n + i / (DV / 8), ch = i % (DV / 8);
+        *reinterpret_cast<uint4*>(vt + (ch / 8) * kTileBytes + r * 128 + (ch % 8) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    tcu::fence_proxy_async_smem();
+}
+
+// U = K~^T V over n tokens, the smallest plane first.  64 keys: a lead of 0 puts them into both halves of
+// the 128 rows, so that all four warps of a column half have a share of the state.
+template <int DK, int DV, int KP>
+__device__ __forceinline__ void issue_update(uint32_t d, uint32_t kt, uint32_t plane1, uint32_t plane2, uint32_t vt, int n) {
+    constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorA | kMajorB, lead = DK == 128 ? kTileBytes : 0;
+    const uint64_t dv = desc(vt, kTileBytes);
+#pragma unroll
+    for (int pl = KP - 1; pl >= 0; --pl) {
+        const uint64_t dk = desc(pl == 0 ? kt : pl == 1 ? plane1 : plane2, lead);
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk)
+            if (kk * 16 < n) tcu::mma_bf16(d, ahead(dk, kk * 2048), ahead(dv, kk * 2048), id, pl < KP - 1 || kk > 0);
+    }
+}
+
+struct Waits {
+    uint64_t* bars;
+    volatile uint32_t* dead;
+    __device__ __forceinline__ void operator()(int bar, uint32_t parity) const {
+        if (!tcu::mbar_wait(&bars[bar], parity, *dead ? 1000 : kWaitNs)) {
+            *dead = 1;
+            atomicOr(&g_status, 1u);
+        }
+    }
+};
+template <int N>
+__device__ __forceinline__ void bar_sync(int id) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
+}
+
+// ---- chunks with outputs ------------------------------------------------------------------------
+// Eight warps work on the tiles.  A thread that issues products waits for the matrix unit to take them
+// (about as long as they run), so another warp does that; it leaves its registers to the others (a group
+// of four warps, three of which do nothing, as registers move by groups).  With keys and values of at most
+// 64 two CTAs share an SM, and there one of the eight issues: the warp whose scores are all masked.
+template <int DK, int DV>
+constexpr bool kApart = DK + DV != 128;
+template <int DK, int DV>
+constexpr int kBlock = kApart<DK, DV> ? kCompute + 128 : kCompute;
+
+template <int DK, int DV, int KP>
+__global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_kernel(const __grid_constant__ Params p,
+                                                                                 const __grid_constant__ Maps maps) {
+    using S = Smem<DK, DV, KP>;
+    constexpr bool APART = kApart<DK, DV>;
+    // Where two CTAs share TMEM, the update takes the half of the scores that P leaves free; otherwise it has
+    // columns of its own, and runs before P V while P is made.
+    constexpr int kCols = APART ? 512 : 256, kSync = APART ? kCompute + 32 : kCompute;
+    constexpr uint32_t cScore = 0, cO1 = 128, cO2 = 128 + DV, cU = APART ? 128 + 2 * DV : 64;
+    constexpr int NC = Chain<DK, DV>::NC;
+    enum { kScores = 2, kPV = 3, kUpdate = 4 };  // barriers after the two stages'
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + (1024 - (tcu::smem_u32(raw) & 1023)) % 1024;
     uint8_t* state = smem + 2 * S::kStage;
     float* power = reinterpret_cast<float*>(smem + S::kPower);
     float* powk = power + 132;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);  // tiles 0, tiles 1, scores, PV, U
+    float* column = reinterpret_cast<float*>(smem + S::kWeights);  // lambda^(31-i), reversed lambda^i
+    float* diagonal = column + 32;                                 // [31 + x]: lambda^x, reversed lambda^-x; 0 where masked
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 5);
-    volatile uint32_t* dead = tmem_at + 1;
+    const Waits wait{bars, tmem_at + 1};
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3, half = warp >> 2;
     const int h = blockIdx.y;
-    Unit u = unit_at(p, blockIdx.x);
-    if constexpr (OUT)
-        ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, (int64_t)blockIdx.x * gridDim.y + h, (int64_t)gridDim.x * gridDim.y, p.o);
-    if (!u.live || (!OUT && u.t1 >= u.e.len)) return;
+    const Unit u = unit_at(p, blockIdx.x);
+    ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, (int64_t)blockIdx.x * gridDim.y + h, (int64_t)gridDim.x * gridDim.y, p.o);
+    if (!u.live) return;
+    const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
-    const int chunks = (int)((u.t1 - u.t0 + kT - 1) / kT);
+    const int chunks = chain.chunks();
     const float log_decay = p.log_decay[h];
     if (tid <= kT) {
         const float w = decay_power(log_decay, tid);
         power[tid] = w;
         powk[tid] = w * p.kv_scale;
     }
+    if (tid >= 128 && tid < 192) {
+        const int i = tid - 128, x = reverse ? 31 - i : i - 31;
+        diagonal[i] = x >= 0 ? decay_power(log_decay, x) * p.kv_scale : 0.f;
+        if (i < 32) column[i] = decay_power(log_decay, reverse ? i : 31 - i) * p.kv_scale;
+    }
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < 5; ++i) tcu::mbar_init(&bars[i], 1);
         tcu::fence_barrier_init();
-        *dead = 0;
+        tmem_at[1] = 0;
     }
     if (warp == 0) tcu::tmem_alloc(tmem_at, kCols);
 
-    // this thread's part of the state: key row a, NC value columns from b0 on
-    const int a = DK == 128 ? quad * 32 + lane : (quad & 1) * 32 + lane;
-    const int b0 = DK == 128 ? half * NC : (half * 2 + (quad >> 1)) * NC;
-    float s[NC];
     const int64_t states = (int64_t)p.dk * p.dv;
-    const float* from = nullptr;
+    const float* from;
     int64_t fa = p.dv, fb = 1;
-    if (OUT) {
-        if (u.t0 == 0) {
-            from = p.initial ? p.initial + ((int64_t)u.s * p.heads + h) * states : nullptr;
-            fa = p.init_a;
-            fb = p.init_b;
-        } else {
-            from = p.states + (u.slot * p.heads + h) * states;
-        }
+    if (u.t0 == 0) {
+        from = p.initial ? p.initial + ((int64_t)u.s * p.heads + h) * states : nullptr;
+        fa = p.init_a;
+        fb = p.init_b;
+    } else {
+        from = p.states + (u.slot * p.heads + h) * states;
     }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) s[i] = from && a < p.dk && b0 + i < p.dv ? from[a * fa + (b0 + i) * fb] : 0.f;
     bool has_state = from != nullptr;
-    // rows of 64 value columns, one a key: the contraction runs over keys
-    auto put_state = [&] {
-#pragma unroll
-        for (int i = 0; i < NC; i += 8) {
-            const int b = b0 + i;
-            uint4 w;
-            w.x = ssm::join(s[i], s[i + 1], __nv_bfloat16{});
-            w.y = ssm::join(s[i + 2], s[i + 3], __nv_bfloat16{});
-            w.z = ssm::join(s[i + 4], s[i + 5], __nv_bfloat16{});
-            w.w = ssm::join(s[i + 6], s[i + 7], __nv_bfloat16{});
-            *reinterpret_cast<uint4*>(state + (b / 64) * (DK * 128) + a * 128 + (((b % 64) / 8) ^ (a & 7)) * 16) = w;
-        }
-        tcu::fence_proxy_async_smem();
-    };
-    if (OUT && has_state) put_state();
-    tcu::tc_fence_before_sync();
-    __syncthreads();
-    tcu::tc_fence_after_sync();
-    const uint32_t tmem = *tmem_at, tmem_lane = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t base = tcu::smem_u32(smem), state_addr = tcu::smem_u32(state);
+    // is the state after a chunk wanted
+    auto updates = [&](int c) { return c + 1 < chunks || (p.final_state && u.t1 >= u.e.len); };
 
-    auto wait = [&](int bar, uint32_t parity) {
-        if (!tcu::mbar_wait(&bars[bar], parity, *dead ? 1000 : kWaitNs)) {
-            *dead = 1;
-            atomicOr(&g_status, 1u);
-        }
-    };
-    auto tokens = [&](int c) { return (int)min((int64_t)kT, u.t1 - u.t0 - (int64_t)c * kT); };
-    // the chunk's first row in memory, counted from the sequence's
-    auto first_row = [&](int c) {
-        const int64_t t = u.t0 + (int64_t)c * kT;
-        return reverse ? u.e.len - t - tokens(c) : t;
-    };
-    auto load_tiles = [&](int c) {  // thread 0
+    // the tiles of chunk c: what the outputs of chunk c - 2 do not lie on, and the rest
+    auto load_tiles = [&](int c, bool early) {
         uint8_t* at = smem + (c & 1) * S::kStage;
         uint64_t* bar = &bars[c & 1];
-        tcu::mbar_arrive_expect_tx(bar, S::kStage);
-        const int row = (int)(first_row(c) + (p.seqs.offsets ? u.e.row : 0)), b = p.seqs.offsets ? 0 : u.s;
+        if (early) tcu::mbar_arrive_expect_tx(bar, S::kStage);
+        const int row = chain.row_at(c), b = chain.batch_at();
 #pragma unroll
-        for (int i = 0; i < DK / 64; ++i) tcu::tma_load_4d(at + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
+        for (int i = 0; i < DV / 64; ++i)
+            if (early) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, i * 64, h, row, b);
 #pragma unroll
-        for (int i = 0; i < DV / 64; ++i) tcu::tma_load_4d(at + S::kK + i * kTileBytes, &maps.v, bar, i * 64, h, row, b);
-        if constexpr (OUT) {
-#pragma unroll
-            for (int i = 0; i < DK / 64; ++i) tcu::tma_load_4d(at + S::kK + S::kV + i * kTileBytes, &maps.q, bar, i * 64, h, row, b);
+        for (int i = 0; i < DK / 64; ++i) {
+            if (early == S::kKeysEarly) tcu::tma_load_4d(at + S::kKeys + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
+            if (!early) tcu::tma_load_4d(at + S::kQueries + i * kTileBytes, &maps.q, bar, i * 64, h, row, b);
         }
     };
-    // scores and q S of chunk c (thread 0)
-    auto first_products = [&](int c) {
-        const uint32_t kt = base + (c & 1) * S::kStage, qt = kt + S::kK + S::kV;
+    auto store_tiles = [&](int c) {  // a full chunk's outputs
+        const int row = chain.row_at(c), b = chain.batch_at();
+#pragma unroll
+        for (int i = 0; i < DV / 64; ++i)
+            if (i * 64 < p.dv) tma_store_4d(&maps.o, smem + (c & 1) * S::kStage + S::kOut + i * kTileBytes, i * 64, h, row, b);
+    };
+    const uint32_t base = tcu::smem_u32(smem), state_addr = base + 2 * S::kStage;
+    uint32_t tmem = 0;
+    // The issuer's part, between the workers' steps.
+    auto issue_first = [&](int c, bool with_state) {  // scores and q S
+        const uint32_t kt = base + (c & 1) * S::kStage + S::kKeys, qt = kt + S::kK;
         wait(c & 1, (c >> 1) & 1);
         tcu::tc_fence_after_sync();
         constexpr uint32_t id = tcu::idesc_bf16_f32(128, 128), id_state = tcu::idesc_bf16_f32(128, DV) | kMajorB;
+        const uint64_t dq = desc(qt, 16), dk = desc(kt, 16), ds = desc(state_addr, DK * 128);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             const uint32_t at = (kk / 4) * kTileBytes + (kk % 4) * 32;
-            tcu::mma_bf16(tmem + cScore, desc(qt + at, 16), desc(kt + at, 16), id, kk > 0);
+            tcu::mma_bf16(tmem + cScore, ahead(dq, at), ahead(dk, at), id, kk > 0);
         }
-        if (has_state) {
+        if (with_state) {
 #pragma unroll
             for (int kk = 0; kk < DK / 16; ++kk) {
                 const uint32_t at = (kk / 4) * kTileBytes + (kk % 4) * 32;
-                tcu::mma_bf16(tmem + cO2, desc(qt + at, 16), desc(state_addr + kk * 2048, DK * 128), id_state, kk > 0);
+                tcu::mma_bf16(tmem + cO2, ahead(dq, at), ahead(ds, kk * 2048), id_state, kk > 0);
             }
         }
-        tcu::mma_commit(&bars[2]);
+        tcu::mma_commit(&bars[kScores]);
     };
+    auto issue_start = [&] {
+        for (int c = 0; c < min(chunks, 2); ++c) {
+            load_tiles(c, true);
+            load_tiles(c, false);
+        }
+        if (chunks > 0) issue_first(0, has_state);
+    };
+    auto issue_next = [&](int c) {  // after chunk c
+        if (c + 1 < chunks) issue_first(c + 1, true);
+        if (c + 2 < chunks) load_tiles(c + 2, true);
+    };
+    auto load_rest = [&](int c) {  // of chunk c + 1, once the outputs of c - 1 have left
+        if (c == 0) return;
+        stores_read();
+        if (c + 1 < chunks) load_tiles(c + 1, false);
+    };
+    auto issue_pv = [&](int c) {
+        const uint32_t vt = base + (c & 1) * S::kStage;
+        tcu::tc_fence_after_sync();
+        constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorB;
+        const int n = chain.tokens(c);
+        const uint64_t dv = desc(vt, kTileBytes);
+#pragma unroll
+        for (int kk = 0; kk < kT / 16; ++kk)
+            if (kk * 16 < n) mma_ts(tmem + cO1, tmem + cScore + kk * 8, ahead(dv, kk * 2048), id, kk > 0);
+        tcu::mma_commit(&bars[kPV]);
+    };
+    auto issue_u = [&](int c) {
+        const uint32_t vt = base + (c & 1) * S::kStage;
+        tcu::tc_fence_after_sync();
+        issue_update<DK, DV, KP>(tmem + cU, vt + S::kKeys, vt + S::kQueries, state_addr, vt, chain.tokens(c));
+        tcu::mma_commit(&bars[kUpdate]);
+    };
+    // every step ends with the writes to shared memory fenced and the TMEM accesses ordered
+    auto sync = [&] {
+        tcu::tc_fence_before_sync();
+        bar_sync<kSync>(1);
+        tcu::tc_fence_after_sync();
+    };
+    auto sync_workers = [&] { bar_sync<kCompute>(2); };
 
-    if (tid == 0) {
-        if (chunks > 0) load_tiles(0);
-        if (chunks > 1) load_tiles(1);
-        if (OUT && chunks > 0) first_products(0);
-    }
-
-    for (int c = 0; c < chunks; ++c) {
-        const int n = tokens(c);
-        const int entry = p.entry && u.t0 == 0 && c == 0;
-        uint8_t* stage = smem + (c & 1) * S::kStage;
-        uint8_t *kt = stage, *vt = stage + S::kK, *qt = vt + S::kV;
-        uint8_t* plane1 = OUT ? qt : state;
-        uint8_t* plane2 = OUT ? state : state + S::kK;
-        const uint32_t vt_addr = tcu::smem_u32(vt);
-        const bool more = c + 1 < chunks;
-        // the state after the last chunk of a sequence is only wanted where it is handed out
-        const bool update = !OUT || more || (p.final_state && u.t1 >= u.e.len);
-        wait(c & 1, (c >> 1) & 1);
-        if (n < kT) {  // rows of another sequence: their products with zeros must be zeros
-            for (int i = tid; i < (kT - n) * (DV / 8); i += kThreads) {
-                const int r = n + i / (DV / 8), ch = i % (DV / 8);
-                *reinterpret_cast<uint4*>(vt + (ch / 8) * kTileBytes + r * 128 + (ch % 8) * 16) = make_uint4(0, 0, 0, 0);
+    if (APART && warp >= kCompute / 32) {
+        if constexpr (APART) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+        if (warp == kCompute / 32) {
+            const bool issuer = lane == 0;
+            bar_sync<kSync>(1);  // barriers, TMEM and the state are there
+            tcu::tc_fence_after_sync();
+            tmem = *tmem_at;
+            if (issuer) issue_start();
+            for (int c = 0; c < chunks; ++c) {
+                if (updates(c)) {
+                    __syncwarp();
+                    sync();  // keys weighed
+                    if (issuer) issue_u(c);
+                }
+                __syncwarp();
+                sync();  // scores read
+                if (issuer && c > 0) store_tiles(c - 1);
+                __syncwarp();
+                sync();  // P written
+                if (issuer) {
+                    issue_pv(c);
+                    load_rest(c);
+                }
+                __syncwarp();
+                sync();  // outputs read, state written
+                if (issuer) issue_next(c);
+            }
+            if (chunks > 0) {
+                __syncwarp();
+                sync();  // the last outputs are in their tiles
+                if (issuer) {
+                    if (chain.tokens(chunks - 1) == kT) store_tiles(chunks - 1);
+                    stores_read();
+                }
+            }
+        }
+    } else {
+        if constexpr (APART) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const bool issuer = !APART && tid == (reverse ? 96 : 128);
+        float s[NC];
+        // rows of 64 value columns, one a key: the contraction runs over keys
+        auto put_state = [&] {
+#pragma unroll
+            for (int i = 0; i < NC; i += 8) {
+                const int b = chain.b0 + i, a = chain.a;
+                uint4 w;
+                w.x = ssm::join(s[i], s[i + 1], __nv_bfloat16{});
+                w.y = ssm::join(s[i + 2], s[i + 3], __nv_bfloat16{});
+                w.z = ssm::join(s[i + 4], s[i + 5], __nv_bfloat16{});
+                w.w = ssm::join(s[i + 6], s[i + 7], __nv_bfloat16{});
+                *reinterpret_cast<uint4*>(state + (b / 64) * (DK * 128) + a * 128 + (((b % 64) / 8) ^ (a & 7)) * 16) = w;
             }
             tcu::fence_proxy_async_smem();
+        };
+        float* scratch = reinterpret_cast<float*>(smem);  // before the first tiles and after the last
+        if (from) {
+            chain.load_state(s, from, fa, fb, scratch, sync_workers);
+            put_state();
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[i] = 0.f;
         }
-        const int row = quad * 32 + lane;           // of the scores and outputs
-        const int pos = reverse ? n - 1 - row : row;
-        if constexpr (OUT) {
-            wait(2, c & 1);
+        tcu::fence_proxy_async_smem();
+        sync();
+        tmem = *tmem_at;
+        const uint32_t tmem_lane = tmem + ((uint32_t)(quad * 32) << 16);
+        if (issuer) issue_start();
+        const int row = quad * 32 + lane;  // of the scores and outputs
+        for (int c = 0; c < chunks; ++c) {
+            const int n = chain.tokens(c);
+            const int entry = p.entry && u.t0 == 0 && c == 0;
+            uint8_t* vt = smem + (c & 1) * S::kStage;
+            uint8_t *kt = vt + S::kKeys, *qt = vt + S::kQueries;
+            const bool update = updates(c);
+            const int pos = reverse ? n - 1 - row : row;
+            wait(c & 1, (c >> 1) & 1);
+            if (n < kT) clear_values<DV>(vt, n);
+            wait(kScores, c & 1);
             tcu::tc_fence_after_sync();
+            auto weigh = [&] {
+                weigh_keys<DK, KP>(kt, qt, state, powk, n, reverse);
+                sync();
+                if (issuer) {
+                    issue_u(c);
+                    load_rest(c);
+                }
+            };
+            auto renew = [&] {
+                wait(kUpdate, c & 1);
+                tcu::tc_fence_after_sync();
+                chain.update(s, tmem_lane + cU, power[n - entry]);
+                if (c + 1 < chunks) put_state();
+            };
+            if (APART && update) weigh();
             // P: columns 64 half .. + 63 of this row, two blocks of 32
             uint32_t pw[2][16];
 #pragma unroll
@@ -261,99 +521,49 @@ __global__ void __launch_bounds__(kThreads, DK + DV == 128 ? 2 : 1) tc_kernel(co
                 uint32_t x[32];
                 ld32(tmem_lane + cScore + j0, x);
                 tcu::tmem_wait_ld();
-                if (cb == quad || n < kT) {
-                    const int d0 = reverse ? j0 - row : row - j0;
+                // columns of this block that exist: reversed, the ones past the sequence are not masked
+                uint32_t on = reverse && n - j0 < 32 ? (1u << (n - j0)) - 1 : 0xffffffffu;
+                if (cb == quad) {
+                    on &= reverse ? 0xffffffffu << lane : 0xffffffffu >> (31 - lane);
+                    const float* w = diagonal + 31 + lane;
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        float v[2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int d = reverse ? d0 + i + e : d0 - i - e;
-                            const bool on = d >= 0 && j0 + i + e < n;
-                            v[e] = on ? __uint_as_float(x[i + e]) * powk[on ? d : 0] : 0.f;
-                        }
-                        pw[blk][i / 2] = ssm::join(v[0], v[1], __nv_bfloat16{});
+                        const float2 v = fmul2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(w[-i], w[-i - 1]));
+                        pw[blk][i / 2] = ssm::join(v.x, v.y, __nv_bfloat16{});
                     }
                 } else {
                     // lambda^|i-j| = (from the row to the block's near edge) (within the block)
-                    const float wr = power[reverse ? j0 - row : row - j0 - 31];
-                    const float2 wr2 = splat2(wr);
+                    const float2 wr = splat2(power[reverse ? j0 - row : row - j0 - 31]);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 wc = reverse ? make_float2(powk[i], powk[i + 1]) : make_float2(powk[31 - i], powk[30 - i]);
-                        const float2 v = fmul2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), fmul2(wr2, wc));
-                        pw[blk][i / 2] = ssm::join(v.x, v.y, __nv_bfloat16{});
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 wc = *reinterpret_cast<const float4*>(column + i);
+                        const float2 v0 = fmul2(fmul2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(wc.x, wc.y)), wr);
+                        const float2 v1 = fmul2(fmul2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), make_float2(wc.z, wc.w)), wr);
+                        pw[blk][i / 2] = ssm::join(v0.x, v0.y, __nv_bfloat16{});
+                        pw[blk][i / 2 + 1] = ssm::join(v1.x, v1.y, __nv_bfloat16{});
                     }
+                }
+                // what is masked is cleared, not multiplied by zero: it may not be finite
+                if (cb == quad || on != 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2)
+                        pw[blk][i / 2] &= (on >> i & 1 ? 0xffffu : 0u) | (on >> (i + 1) & 1 ? 0xffff0000u : 0u);
                 }
             }
             // P takes the place of the scores' first half, which others may still be reading
-            tcu::tc_fence_before_sync();
-            __syncthreads();
-            tcu::tc_fence_after_sync();
+            sync();
+            if (issuer && c > 0) store_tiles(c - 1);
             st16(tmem_lane + cScore + half * 32, pw[0]);
             st16(tmem_lane + cScore + half * 32 + 16, pw[1]);
             wait_st();
-            tcu::tc_fence_before_sync();
-            __syncthreads();
-            if (tid == 0) {
-                tcu::tc_fence_after_sync();
-                constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorB;
-                const int steps = (n + 15) / 16;
-                for (int kk = 0; kk < steps; ++kk)
-                    mma_ts(tmem + cO1, tmem + cScore + kk * 8, desc(vt_addr + kk * 2048, kTileBytes), id, kk > 0);
-                tcu::mma_commit(&bars[3]);
+            sync();
+            if (issuer) issue_pv(c);
+            if (update) {
+                if (APART) renew(); else weigh();
             }
-        }
-        if (update) {
-            // planes of the weighted keys; rows past the sequence become zeros
-#pragma unroll 2
-            for (int i = tid; i < kT * DK / 8; i += kThreads) {
-                const int j = i / 8 % kT;
-                const float w = j < n ? powk[reverse ? j : n - 1 - j] : 0.f;
-                const uint4 x = *reinterpret_cast<const uint4*>(kt + i * 16);
-                const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-                uint32_t out[3][4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float lo = __uint_as_float(words[e] << 16) * w, hi = __uint_as_float(words[e] & 0xffff0000u) * w;
-                    if (j >= n) lo = hi = 0.f;
-#pragma unroll
-                    for (int pl = 0; pl < KP; ++pl) {
-                        const uint32_t b = ssm::join(lo, hi, __nv_bfloat16{});
-                        out[pl][e] = b;
-                        lo -= __uint_as_float(b << 16);
-                        hi -= __uint_as_float(b & 0xffff0000u);
-                    }
-                }
-                *reinterpret_cast<uint4*>(kt + i * 16) = make_uint4(out[0][0], out[0][1], out[0][2], out[0][3]);
-                *reinterpret_cast<uint4*>(plane1 + i * 16) = make_uint4(out[1][0], out[1][1], out[1][2], out[1][3]);
-                if constexpr (KP == 3)
-                    *reinterpret_cast<uint4*>(plane2 + i * 16) = make_uint4(out[2][0], out[2][1], out[2][2], out[2][3]);
-            }
-            tcu::fence_proxy_async_smem();
-            tcu::tc_fence_before_sync();
-            __syncthreads();
-            if (tid == 0) {
-                tcu::tc_fence_after_sync();
-                // 64 keys: a lead of 0 puts them into both halves of the 128 rows
-                constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorA | kMajorB, lead = DK == 128 ? kTileBytes : 0;
-                const int steps = (n + 15) / 16;
-                bool sum = false;
-#pragma unroll
-                for (int pl = KP - 1; pl >= 0; --pl) {
-                    const uint32_t at = tcu::smem_u32(pl == 0 ? kt : pl == 1 ? plane1 : plane2);
-                    for (int kk = 0; kk < steps; ++kk) {
-                        tcu::mma_bf16(tmem + cU, desc(at + kk * 2048, lead), desc(vt_addr + kk * 2048, kTileBytes), id, sum);
-                        sum = true;
-                    }
-                }
-                tcu::mma_commit(&bars[4]);
-            }
-        }
-        // this row's outputs, DV / 2 columns
-        uint32_t out[DV / 4];
-        if constexpr (OUT) {
-            wait(3, c & 1);
+            // this row's outputs, DV / 2 columns
+            uint32_t out[DV / 4];
+            wait(kPV, c & 1);
             tcu::tc_fence_after_sync();
             const float wi = row < n ? power[pos + 1 - entry] : 0.f;
 #pragma unroll
@@ -363,37 +573,36 @@ __global__ void __launch_bounds__(kThreads, DK + DV == 128 ? 2 : 1) tc_kernel(co
                 ld32(tmem_lane + cO1 + c0, x);
                 if (has_state) ld32(tmem_lane + cO2 + c0, y);
                 tcu::tmem_wait_ld();
-                bool odd = false;
+                float2 zero = splat2(0.f);  // NaN once a value is not finite
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    float v = __uint_as_float(x[i]);
-                    odd |= !(fabsf(v) <= 3.4028234e38f);
-                    if (has_state) v = fmaf(__uint_as_float(y[i]), wi, v);
-                    x[i] = __float_as_uint(v);
+                for (int i = 0; i < 32; i += 2) {
+                    float2 v = make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    zero = ffma2(v, splat2(0.f), zero);
+                    if (has_state) v = ffma2(make_float2(__uint_as_float(y[i]), __uint_as_float(y[i + 1])), splat2(wi), v);
+                    x[i] = __float_as_uint(v.x);
+                    x[i + 1] = __float_as_uint(v.y);
                 }
                 // A value that is not finite must not reach the rows before it: 0 times it is NaN in the
                 // product.  Such chunks are rare; their rows are summed again, term by term.
-                if (__any_sync(0xffffffffu, odd)) {
+                if (__any_sync(0xffffffffu, !(zero.x + zero.y == 0.f))) {
                     float sum[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) sum[i] = has_state ? __uint_as_float(y[i]) * wi : 0.f;
-                    for (int j0 = 0; j0 < n; j0 += 32) {
-                        float pr[16];
-                        tcu::tmem_ld16(tmem_lane + cScore + j0 / 2, pr);
+#pragma unroll 1
+                    for (int j = 0; j < n; ++j) {
+                        float pr[2];
+                        tcu::tmem_ld2(tmem_lane + cScore + j / 4 * 2, pr);
                         tcu::tmem_wait_ld();
+                        const uint32_t w = __float_as_uint(j & 2 ? pr[1] : pr[0]);
+                        const float pv = __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+                        if (reverse ? j >= row : j <= row) {
 #pragma unroll
-                        for (int jj = 0; jj < 32; ++jj) {
-                            const int j = j0 + jj;
-                            const uint32_t w = __float_as_uint(pr[jj / 2]);
-                            const float pv = __uint_as_float(jj & 1 ? w & 0xffff0000u : w << 16);
-                            if (j < n && (reverse ? j >= row : j <= row)) {
+                            for (int i = 0; i < 32; i += 8) {
+                                const int cc = c0 + i;
+                                float b[8];
+                                load8(reinterpret_cast<const __nv_bfloat16*>(vt + (cc / 64) * kTileBytes + j * 128 + (((cc % 64) / 8) ^ (j & 7)) * 16), b);
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
-                                    const int cc = c0 + i;
-                                    const uint16_t b = *reinterpret_cast<const uint16_t*>(
-                                        vt + (cc / 64) * kTileBytes + j * 128 + (((cc % 64) / 8) ^ (j & 7)) * 16 + (cc % 8) * 2);
-                                    sum[i] = fmaf(pv, __uint_as_float((uint32_t)b << 16), sum[i]);
-                                }
+                                for (int e = 0; e < 8; ++e) sum[i + e] = fmaf(pv, b[e], sum[i + e]);
                             }
                         }
                         __syncwarp();
@@ -406,68 +615,128 @@ __global__ void __launch_bounds__(kThreads, DK + DV == 128 ? 2 : 1) tc_kernel(co
                     out[blk * 16 + i] = ssm::join(__uint_as_float(x[2 * i]) * p.out_scale, __uint_as_float(x[2 * i + 1]) * p.out_scale,
                                                   __nv_bfloat16{});
             }
-        }
-        if (update) {
-            wait(4, c & 1);
-            tcu::tc_fence_after_sync();
-            const float w = power[n - entry];
-#pragma unroll
-            for (int i0 = 0; i0 < NC; i0 += 16) {
-                float x[16];
-                tcu::tmem_ld16(tmem_lane + cU + b0 + i0, x);
-                tcu::tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i0 + i] = fmaf(s[i0 + i], w, x[i]);
-            }
-            has_state = true;
-            if (OUT && more) put_state();
-        }
-        tcu::tc_fence_before_sync();
-        __syncthreads();
-        if (OUT && more && tid == 0) {
-            tcu::tc_fence_after_sync();
-            first_products(c + 1);
-        }
-        if constexpr (OUT) {
-            // the rows of o through shared memory (where K was), 16 bytes in eight places by row
+            if (!APART && update) renew();
+            has_state |= update;
+            sync();
+            if (issuer) issue_next(c);
+            // the rows of o at the end of the stage, in the swizzle of their tiles; they leave during the next chunk
 #pragma unroll
             for (int i = 0; i < DV / 16; ++i) {
                 const int ch = half * (DV / 16) + i;
-                *reinterpret_cast<uint4*>(kt + (ch / 8) * kTileBytes + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
+                *reinterpret_cast<uint4*>(vt + S::kOut + (ch / 8) * kTileBytes + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
                     make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
             }
-            __syncthreads();
-            const int64_t step = (int64_t)p.heads * p.dv;
-            __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.e.row + first_row(c)) * step + (int64_t)h * p.dv;
-            for (int i = tid; i < n * (DV / 8); i += kThreads) {
-                const int r = i / (DV / 8), ch = i % (DV / 8);
-                if (ch * 8 >= p.dv) continue;
-                const uint4 v = *reinterpret_cast<const uint4*>(kt + (ch / 8) * kTileBytes + r * 128 + ((ch % 8) ^ (r & 7)) * 16);
-                *reinterpret_cast<uint4*>(to + r * step + ch * 8) = v;
-            }
             tcu::fence_proxy_async_smem();
-            __syncthreads();
         }
-        if (tid == 0 && c + 2 < chunks) {
-            tcu::fence_proxy_async_smem();
-            load_tiles(c + 2);
+        if (chunks > 0) {
+            sync();
+            const int c = chunks - 1, n = chain.tokens(c);
+            if (n < kT) {  // rows past these are another sequence's
+                const uint8_t* from_tile = smem + (c & 1) * S::kStage + S::kOut;
+                const int64_t step = (int64_t)p.heads * p.dv;
+                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.e.row + chain.first_row(c)) * step + (int64_t)h * p.dv;
+                for (int i = tid; i < n * (DV / 8); i += kCompute) {
+                    const int r = i / (DV / 8), ch = i % (DV / 8);
+                    if (ch * 8 >= p.dv) continue;
+                    const uint4 v = *reinterpret_cast<const uint4*>(from_tile + (ch / 8) * kTileBytes + r * 128 + ((ch % 8) ^ (r & 7)) * 16);
+                    *reinterpret_cast<uint4*>(to + r * step + ch * 8) = v;
+                }
+            }
+            if (issuer) {
+                if (n == kT) store_tiles(c);
+                stores_read();
+            }
+        }
+        if (p.final_state && u.t1 >= u.e.len) {
+            // the stage that the last outputs do not lie in
+            float* tile = reinterpret_cast<float*>(smem + (chunks & 1) * S::kStage);
+            const float last = p.exit_decay && u.e.len > 0 ? decay_power(log_decay, 1) : 1.f;
+            chain.store_state(s, p.final_state + ((int64_t)u.s * p.heads + h) * states, last, tile, sync_workers);
         }
     }
+    tcu::tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 0) tcu::tmem_dealloc(*tmem_at, kCols);
+}
 
-    float* to = nullptr;
-    float last = 1.f;
-    if constexpr (OUT) {
-        if (p.final_state && u.t1 >= u.e.len) {
-            to = p.final_state + ((int64_t)u.s * p.heads + h) * states;
-            if (p.exit_decay && u.e.len > 0) last = decay_power(log_decay, 1);
+// ---- what a segment adds to the state -------------------------------------------------------------
+template <int DK, int DV, int KP>
+__global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_states_kernel(const __grid_constant__ Params p,
+                                                                                       const __grid_constant__ Maps maps) {
+    using S = StatesSmem<DK, DV, KP>;
+    constexpr int kCols = DV, NC = Chain<DK, DV>::NC;
+    constexpr int kUpdate = S::kStages;
+    extern __shared__ uint8_t raw[];
+    uint8_t* smem = raw + (1024 - (tcu::smem_u32(raw) & 1023)) % 1024;
+    float* powk = reinterpret_cast<float*>(smem + S::kPower);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + S::kStages + 1);
+    const Waits wait{bars, tmem_at + 1};
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3;
+    const int h = blockIdx.y;
+    const Unit u = unit_at(p, blockIdx.x);
+    if (!u.live || u.t1 >= u.e.len) return;  // the state after a sequence's last segment is nobody's start
+    const Chain<DK, DV> chain(p, u);
+    const bool reverse = p.seqs.reverse;
+    const int chunks = chain.chunks();
+    const float log_decay = p.log_decay[h];
+    if (tid <= kT) powk[tid] = decay_power(log_decay, tid) * p.kv_scale;
+    const float decay = decay_power(log_decay, kT);  // all chunks of these segments are full
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 0; i <= S::kStages; ++i) tcu::mbar_init(&bars[i], 1);
+        tcu::fence_barrier_init();
+        tmem_at[1] = 0;
+    }
+    if (warp == 0) tcu::tmem_alloc(tmem_at, kCols);
+    auto sync = [&] {
+        tcu::tc_fence_before_sync();
+        __syncthreads();
+        tcu::tc_fence_after_sync();
+    };
+    sync();
+    const uint32_t tmem = *tmem_at;
+    uint8_t* planes = smem + S::kStages * S::kStage;
+    auto load_tiles = [&](int c) {
+        uint8_t* at = smem + c % S::kStages * S::kStage;
+        uint64_t* bar = &bars[c % S::kStages];
+        tcu::mbar_arrive_expect_tx(bar, S::kStage);
+        const int row = chain.row_at(c), b = chain.batch_at();
+#pragma unroll
+        for (int i = 0; i < DV / 64; ++i) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, i * 64, h, row, b);
+#pragma unroll
+        for (int i = 0; i < DK / 64; ++i) tcu::tma_load_4d(at + S::kV + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
+    };
+    if (warp == kCompute / 32) {
+        const uint32_t first = tcu::smem_u32(smem), pl = tcu::smem_u32(planes);
+        if (lane == 0)
+            for (int c = 0; c < min(chunks, S::kStages); ++c) load_tiles(c);
+        for (int c = 0; c < chunks; ++c) {
+            __syncwarp();
+            sync();  // keys of chunk c weighed, product c - 1 read
+            if (lane == 0) {
+                const uint32_t vt = first + c % S::kStages * S::kStage;
+                issue_update<DK, DV, KP>(tmem, vt + S::kV, pl, pl + S::kK, vt, kT);
+                tcu::mma_commit(&bars[kUpdate]);
+                if (c > 0 && c - 1 + S::kStages < chunks) load_tiles(c - 1 + S::kStages);
+            }
         }
     } else {
-        to = p.states + (u.slot * p.heads + h) * states;
-    }
-    if (to && a < p.dk) {
+        float s[NC];
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-            if (b0 + i < p.dv) to[(int64_t)a * p.dv + b0 + i] = s[i] * last;
+        for (int i = 0; i < NC; ++i) s[i] = 0.f;
+        for (int c = 0; c < chunks; ++c) {
+            uint8_t* kt = smem + c % S::kStages * S::kStage + S::kV;
+            wait(c % S::kStages, c / S::kStages & 1);
+            weigh_keys<DK, KP>(kt, planes, planes + S::kK, powk, kT, reverse);
+            sync();
+            wait(kUpdate, c & 1);
+            tcu::tc_fence_after_sync();
+            chain.update(s, tmem + ((uint32_t)(quad * 32) << 16), decay);
+        }
+        const int64_t states = (int64_t)p.dk * p.dv;
+        chain.store_state(s, p.states + (u.slot * p.heads + h) * states, 1.f, reinterpret_cast<float*>(smem),
+                          [&] { bar_sync<kCompute>(2); });
     }
     tcu::tc_fence_before_sync();
     __syncthreads();
@@ -506,22 +775,28 @@ bool encode(CUtensorMap* m, const Heads& t, const Params& p, int dim) {
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DK, int DV, int KP, bool OUT>
-int launch(const Params& p, const Maps& m, int64_t units, cudaStream_t st) {
-    using L = Smem<DK, DV, KP, OUT>;
-    const void* fn = reinterpret_cast<const void*>(&tc_kernel<DK, DV, KP, OUT>);
-    if (!ensure_smem_attr(fn, L::kLaunch)) return fail(VH_E_DEVICE, "linear attention: shared memory");
-    tc_kernel<DK, DV, KP, OUT><<<dim3((unsigned)units, p.heads), kThreads, L::kLaunch, st>>>(p, m);
-    return launch_status(OUT ? "linear attention" : "linear attention: segment states");
+template <int DK, int DV, int KP>
+int launch(const Params& p, const Maps& m, int64_t units, bool outputs, cudaStream_t st) {
+    const size_t smem = outputs ? Smem<DK, DV, KP>::kLaunch : StatesSmem<DK, DV, KP>::kLaunch;
+    const void* fn = outputs ? reinterpret_cast<const void*>(&tc_kernel<DK, DV, KP>)
+                             : reinterpret_cast<const void*>(&tc_states_kernel<DK, DV, KP>);
+    if (!ensure_smem_attr(fn, smem)) return fail(VH_E_DEVICE, "linear attention: shared memory");
+    const dim3 grid((unsigned)units, p.heads);
+    if (outputs) tc_kernel<DK, DV, KP><<<grid, kBlock<DK, DV>, smem, st>>>(p, m);
+    else tc_states_kernel<DK, DV, KP><<<grid, kCompute + 32, smem, st>>>(p, m);
+    return launch_status(outputs ? "linear attention" : "linear attention: segment states");
 }
 
 template <int DK, int DV>
 int run_dims(const Params& p, const Maps& m, int64_t units, bool exact, cudaStream_t st) {
+    auto one = [&](bool outputs) {
+        return exact ? launch<DK, DV, 3>(p, m, units, outputs, st) : launch<DK, DV, 2>(p, m, units, outputs, st);
+    };
     if (p.segment) {
-        if (int rc = exact ? launch<DK, DV, 3, false>(p, m, units, st) : launch<DK, DV, 2, false>(p, m, units, st)) return rc;
+        if (int rc = one(false)) return rc;
         if (int rc = enter_segments(p, st)) return rc;
     }
-    return exact ? launch<DK, DV, 3, true>(p, m, units, st) : launch<DK, DV, 2, true>(p, m, units, st);
+    return one(true);
 }
 
 }  // namespace
@@ -545,7 +820,9 @@ int tc_segment_size(int64_t length, int batch, bool packed, int heads, int dk, i
 bool tc_run(Params p, void* states, cudaStream_t st, int* rc) {
     if (p.q.vec != 8 || p.k.vec != 8 || p.v.vec != 8 || p.vec_o != 8 || p.seqs.length < kT || !encoder()) return false;
     Maps m;
-    if (!encode(&m.q, p.q, p, p.dk) || !encode(&m.k, p.k, p, p.dk) || !encode(&m.v, p.v, p, p.dv)) return false;
+    const int64_t row = (int64_t)p.heads * p.dv;
+    const Heads o{p.o, {p.seqs.length * row, row}, p.dv, 8};
+    if (!encode(&m.q, p.q, p, p.dk) || !encode(&m.k, p.k, p, p.dk) || !encode(&m.v, p.v, p, p.dv) || !encode(&m.o, o, p, p.dv)) return false;
     const bool packed = p.seqs.offsets != nullptr, exact = p.final_state != nullptr;
     p.segment = tc_segment_size(p.seqs.length, p.seqs.count, packed, p.heads, p.dk, p.dv);
     p.states = static_cast<float*>(states);
