@@ -485,41 +485,34 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
             }
 }
 
-// From what each segment adds to the state before each of them, in place: a thread per element walks
-// the segments of its sequence.
+// From what each segment adds to the state before each of them, in place: a thread per element walks the
+// segments of its sequence, 16 loads ahead (one pass over memory, bound by its latency; four elements a thread
+// took 5.7 us instead of 3.7 for 32 segments of 8 chains of 64 x 64).
+constexpr int kEnterAhead = 16;
 __global__ void __launch_bounds__(256) enter_kernel(Params p) {
     const int s = blockIdx.x, h = blockIdx.y;
     const int states = p.dk * p.dv, i = blockIdx.z * 256 + threadIdx.x;
     const Seq e = ssm::seq_at(p.seqs, s);
     if (i >= states || e.len <= p.segment) return;
     const int64_t base = ssm::slot_base(p.seqs, s, e.row, p.segment);
-    const float g = p.log_decay[h];
+    const float g = p.log_decay[h], step = decay_power(g, p.segment);
     const int a = i / p.dv, b = i - a * p.dv;
     float run = p.initial ? p.initial[((int64_t)s * p.heads + h) * states + a * p.init_a + b * p.init_b] : 0.f;
-    const float step = decay_power(g, p.segment);
     float w = p.entry ? decay_power(g, p.segment - 1) : step;
     float* at = p.states + (base * p.heads + h) * states + i;
-    const int64_t stride = (int64_t)p.heads * states;
-    const int64_t segs = (e.len + p.segment - 1) / p.segment;
-    int64_t j = 0;
-    for (; j + 8 < segs; j += 8) {  // loads ahead of the chain; the last segment adds to nobody's start
-        float own[8];
+    const int64_t stride = (int64_t)p.heads * states, segs = (e.len + p.segment - 1) / p.segment;
+    for (int64_t j = 0; j < segs; j += kEnterAhead) {
+        float own[kEnterAhead];  // the last segment adds to nobody's start
 #pragma unroll
-        for (int x = 0; x < 8; ++x) own[x] = at[(j + x) * stride];
+        for (int x = 0; x < kEnterAhead; ++x) own[x] = j + x + 1 < segs ? at[(j + x) * stride] : 0.f;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
+        for (int x = 0; x < kEnterAhead; ++x) {
+            if (j + x >= segs) break;
             at[(j + x) * stride] = run;
             run = run * w + own[x];
             w = step;
         }
     }
-    for (; j + 1 < segs; ++j) {
-        const float own = at[j * stride];
-        at[j * stride] = run;
-        run = run * w + own;
-        w = step;
-    }
-    at[j * stride] = run;
 }
 
 // ---- one token ----------------------------------------------------------------------------------

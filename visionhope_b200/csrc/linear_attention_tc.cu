@@ -92,27 +92,31 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 
 // ---- shared memory ------------------------------------------------------------------------------
 // Two stages of tiles [V | K | Q], each of blocks of 64 columns; then the state's operand, which is also
-// where the third plane of K~ goes (the second goes where Q was).  A chunk's outputs leave from the end of
-// its stage: what lies before them is loaded for the chunk after next at once, the rest when they have left.
+// where the third plane of K~ goes (the second goes where Q was).  A chunk's outputs leave from where its V
+// was: Q and K of the chunk after next, which its scores wait for, are loaded at once, and V when they have left.
 template <int DK, int DV, int KP>
 struct Smem {
     static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64);
-    static constexpr int kKeys = kV, kQueries = kV + kK, kStage = kV + 2 * kK, kOut = kStage - kV;
-    static constexpr bool kKeysEarly = kOut >= kQueries;
+    static constexpr int kKeys = kV, kQueries = kV + kK, kStage = kV + 2 * kK;
     static constexpr int kState = KP == 3 && kK > DK * DV * 2 ? kK : DK * DV * 2;
     static constexpr int kPower = 2 * kStage + kState;             // lambda^n, n = 0..128, and times kv_scale
     static constexpr int kWeights = kPower + 2 * 132 * 4;          // of a score: by column, and on the diagonal
-    static constexpr int kBars = kWeights + (32 + 64) * 4;         // 5 barriers, TMEM base, a flag
+    static constexpr int kBars = kWeights + (32 + 64) * 4;         // 7 barriers, TMEM base, a flag
     static constexpr int kLaunch = kBars + 64 + 1024;              // the tiles start on 1024 bytes
     static_assert(kLaunch <= 232448, "shared memory of an SM");
 };
-// Without outputs: three stages of tiles [V | K] where they fit, and the planes of K~ behind the first.
+// Without outputs: tiles [V | K], and the planes of K~ behind the first.  Where two CTAs share an SM, two stages
+// and planes for two chunks, so that the keys of one are weighed while the other's product runs (64 x 256
+// tokens of two images 14.6 us, against 19.8 in three stages); else three stages (two for three planes of
+// 128 keys and values), as two leave too little time to load 64 KB (62 against 89 us for half of 4 x 8192
+// tokens of 16 heads of 128).
 template <int DK, int DV, int KP>
 struct StatesSmem {
     static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64);
     static constexpr int kStage = kK + kV, kPlanes = (KP - 1) * kK;
-    static constexpr int kStages = 3 * kStage + kPlanes + 2048 <= (DK + DV == 128 ? 114 : 226) * 1024 ? 3 : 2;
-    static constexpr int kPower = kStages * kStage + kPlanes;
+    static constexpr int kBuffers = DK + DV == 128 ? 2 : 1;
+    static constexpr int kStages = kBuffers == 1 && 3 * kStage + kPlanes + 2048 <= 226 * 1024 ? 3 : 2;
+    static constexpr int kPower = kStages * kStage + kBuffers * kPlanes;
     static constexpr int kBars = kPower + 132 * 4;                 // a barrier a stage, the product's, TMEM base, a flag
     static constexpr int kLaunch = kBars + 64 + 1024;
     static_assert(kLaunch <= 232448, "shared memory of an SM");
@@ -124,10 +128,13 @@ struct Chain {
     static constexpr int NC = DK == 128 ? DV / 2 : DV / 4;  // state columns a thread
     const Params& p;
     const Unit& u;
-    int a, b0;  // this thread's part of the state: key row a, NC value columns from b0 on
+    int col0, cols;  // the value columns of this CTA
+    int a, b0;       // this thread's part of the state: key row a, NC of these columns from b0 on
 
     __device__ __forceinline__ Chain(const Params& params, const Unit& unit) : p(params), u(unit) {
         const int quad = threadIdx.x >> 5 & 3, half = threadIdx.x >> 7, lane = threadIdx.x & 31;
+        col0 = blockIdx.z * DV;
+        cols = min(DV, p.dv - col0);
         a = DK == 128 ? quad * 32 + lane : (quad & 1) * 32 + lane;
         b0 = DK == 128 ? half * NC : (half * 2 + (quad >> 1)) * NC;
     }
@@ -146,7 +153,8 @@ struct Chain {
     template <typename Sync>
     __device__ __forceinline__ void load_state(float (&s)[NC], const float* from, int64_t fa, int64_t fb, float* tile, Sync sync) const {
         const bool across = fb == 1;
-        const int inner = across ? p.dv : p.dk, outer = across ? p.dk : p.dv;
+        const int inner = across ? cols : p.dk, outer = across ? p.dk : cols;
+        from += col0 * fb;
         for (int i = threadIdx.x; i < inner * outer; i += kCompute) {
             const int o = i / inner, x = i - o * inner;
             const int ra = across ? o : x, cb = across ? x : o;
@@ -158,7 +166,7 @@ struct Chain {
             const float4 v = *reinterpret_cast<const float4*>(tile + a * (DV + 4) + b0 + i);
             const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i + e] = a < p.dk && b0 + i + e < p.dv ? f[e] : 0.f;
+            for (int e = 0; e < 4; ++e) s[i + e] = a < p.dk && b0 + i + e < cols ? f[e] : 0.f;
         }
         sync();
     }
@@ -170,9 +178,9 @@ struct Chain {
             *reinterpret_cast<float4*>(tile + a * (DV + 4) + b0 + i) =
                 make_float4(s[i] * scale, s[i + 1] * scale, s[i + 2] * scale, s[i + 3] * scale);
         sync();
-        for (int i = threadIdx.x; i < p.dk * p.dv; i += kCompute) {
-            const int r = i / p.dv, c = i - r * p.dv;
-            to[i] = tile[r * (DV + 4) + c];
+        for (int i = threadIdx.x; i < p.dk * cols; i += kCompute) {
+            const int r = i / cols, c = i - r * cols;
+            to[r * p.dv + col0 + c] = tile[r * (DV + 4) + c];
         }
     }
     // S = w S + U
@@ -276,7 +284,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     constexpr int kCols = APART ? 512 : 256, kSync = APART ? kCompute + 32 : kCompute;
     constexpr uint32_t cScore = 0, cO1 = 128, cO2 = 128 + DV, cU = APART ? 128 + 2 * DV : 64;
     constexpr int NC = Chain<DK, DV>::NC;
-    enum { kScores = 2, kPV = 3, kUpdate = 4 };  // barriers after the two stages'
+    enum { kValues = 2, kScores = 4, kPV = 5, kUpdate = 6 };  // barriers; 0 and 1: Q and K of the two stages
     extern __shared__ uint8_t raw[];
     uint8_t* smem = raw + (1024 - (tcu::smem_u32(raw) & 1023)) % 1024;
     uint8_t* state = smem + 2 * S::kStage;
@@ -285,13 +293,14 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     float* column = reinterpret_cast<float*>(smem + S::kWeights);  // lambda^(31-i), reversed lambda^i
     float* diagonal = column + 32;                                 // [31 + x]: lambda^x, reversed lambda^-x; 0 where masked
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 5);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 7);
     const Waits wait{bars, tmem_at + 1};
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3, half = warp >> 2;
     const int h = blockIdx.y;
     const Unit u = unit_at(p, blockIdx.x);
-    ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, (int64_t)blockIdx.x * gridDim.y + h, (int64_t)gridDim.x * gridDim.y, p.o);
+    ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, ((int64_t)blockIdx.x * gridDim.y + h) * gridDim.z + blockIdx.z,
+                                     (int64_t)gridDim.x * gridDim.y * gridDim.z, p.o);
     if (!u.live) return;
     const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
@@ -309,7 +318,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     }
     if (tid == 0) {
 #pragma unroll
-        for (int i = 0; i < 5; ++i) tcu::mbar_init(&bars[i], 1);
+        for (int i = 0; i < 7; ++i) tcu::mbar_init(&bars[i], 1);
         tcu::fence_barrier_init();
         tmem_at[1] = 0;
     }
@@ -329,26 +338,31 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     // is the state after a chunk wanted
     auto updates = [&](int c) { return c + 1 < chunks || (p.final_state && u.t1 >= u.e.len); };
 
-    // the tiles of chunk c: what the outputs of chunk c - 2 do not lie on, and the rest
-    auto load_tiles = [&](int c, bool early) {
+    auto load_keys = [&](int c) {  // and queries
         uint8_t* at = smem + (c & 1) * S::kStage;
         uint64_t* bar = &bars[c & 1];
-        if (early) tcu::mbar_arrive_expect_tx(bar, S::kStage);
+        tcu::mbar_arrive_expect_tx(bar, 2 * S::kK);
         const int row = chain.row_at(c), b = chain.batch_at();
 #pragma unroll
-        for (int i = 0; i < DV / 64; ++i)
-            if (early) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, i * 64, h, row, b);
-#pragma unroll
         for (int i = 0; i < DK / 64; ++i) {
-            if (early == S::kKeysEarly) tcu::tma_load_4d(at + S::kKeys + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
-            if (!early) tcu::tma_load_4d(at + S::kQueries + i * kTileBytes, &maps.q, bar, i * 64, h, row, b);
+            tcu::tma_load_4d(at + S::kKeys + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
+            tcu::tma_load_4d(at + S::kQueries + i * kTileBytes, &maps.q, bar, i * 64, h, row, b);
         }
     };
+    auto load_values = [&](int c) {
+        uint8_t* at = smem + (c & 1) * S::kStage;
+        uint64_t* bar = &bars[kValues + (c & 1)];
+        tcu::mbar_arrive_expect_tx(bar, S::kV);
+        const int row = chain.row_at(c), b = chain.batch_at();
+#pragma unroll
+        for (int i = 0; i < DV / 64; ++i) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, chain.col0 + i * 64, h, row, b);
+    };
+    auto wait_values = [&](int c) { wait(kValues + (c & 1), (c >> 1) & 1); };
     auto store_tiles = [&](int c) {  // a full chunk's outputs
         const int row = chain.row_at(c), b = chain.batch_at();
 #pragma unroll
         for (int i = 0; i < DV / 64; ++i)
-            if (i * 64 < p.dv) tma_store_4d(&maps.o, smem + (c & 1) * S::kStage + S::kOut + i * kTileBytes, i * 64, h, row, b);
+            if (i * 64 < chain.cols) tma_store_4d(&maps.o, smem + (c & 1) * S::kStage + i * kTileBytes, chain.col0 + i * 64, h, row, b);
     };
     const uint32_t base = tcu::smem_u32(smem), state_addr = base + 2 * S::kStage;
     uint32_t tmem = 0;
@@ -375,22 +389,23 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     };
     auto issue_start = [&] {
         for (int c = 0; c < min(chunks, 2); ++c) {
-            load_tiles(c, true);
-            load_tiles(c, false);
+            load_keys(c);
+            load_values(c);
         }
         if (chunks > 0) issue_first(0, has_state);
     };
     auto issue_next = [&](int c) {  // after chunk c
         if (c + 1 < chunks) issue_first(c + 1, true);
-        if (c + 2 < chunks) load_tiles(c + 2, true);
+        if (c + 2 < chunks) load_keys(c + 2);
     };
-    auto load_rest = [&](int c) {  // of chunk c + 1, once the outputs of c - 1 have left
+    auto load_rest = [&](int c) {  // the values of chunk c + 1, once the outputs of c - 1 have left
         if (c == 0) return;
         stores_read();
-        if (c + 1 < chunks) load_tiles(c + 1, false);
+        if (c + 1 < chunks) load_values(c + 1);
     };
     auto issue_pv = [&](int c) {
         const uint32_t vt = base + (c & 1) * S::kStage;
+        wait_values(c);
         tcu::tc_fence_after_sync();
         constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorB;
         const int n = chain.tokens(c);
@@ -402,6 +417,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     };
     auto issue_u = [&](int c) {
         const uint32_t vt = base + (c & 1) * S::kStage;
+        wait_values(c);
         tcu::tc_fence_after_sync();
         issue_update<DK, DV, KP>(tmem + cU, vt + S::kKeys, vt + S::kQueries, state_addr, vt, chain.tokens(c));
         tcu::mma_commit(&bars[kUpdate]);
@@ -490,7 +506,10 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             const bool update = updates(c);
             const int pos = reverse ? n - 1 - row : row;
             wait(c & 1, (c >> 1) & 1);
-            if (n < kT) clear_values<DV>(vt, n);
+            if (n < kT) {
+                wait_values(c);
+                clear_values<DV>(vt, n);
+            }
             wait(kScores, c & 1);
             tcu::tc_fence_after_sync();
             auto weigh = [&] {
@@ -563,6 +582,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             }
             // this row's outputs, DV / 2 columns
             uint32_t out[DV / 4];
+            wait_values(c);
             wait(kPV, c & 1);
             tcu::tc_fence_after_sync();
             const float wi = row < n ? power[pos + 1 - entry] : 0.f;
@@ -619,11 +639,11 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             has_state |= update;
             sync();
             if (issuer) issue_next(c);
-            // the rows of o at the end of the stage, in the swizzle of their tiles; they leave during the next chunk
+            // the rows of o where V was, in the swizzle of its tiles; they leave during the next chunk
 #pragma unroll
             for (int i = 0; i < DV / 16; ++i) {
                 const int ch = half * (DV / 16) + i;
-                *reinterpret_cast<uint4*>(vt + S::kOut + (ch / 8) * kTileBytes + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
+                *reinterpret_cast<uint4*>(vt + (ch / 8) * kTileBytes + row * 128 + ((ch % 8) ^ (row & 7)) * 16) =
                     make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
             }
             tcu::fence_proxy_async_smem();
@@ -632,12 +652,12 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             sync();
             const int c = chunks - 1, n = chain.tokens(c);
             if (n < kT) {  // rows past these are another sequence's
-                const uint8_t* from_tile = smem + (c & 1) * S::kStage + S::kOut;
+                const uint8_t* from_tile = smem + (c & 1) * S::kStage;
                 const int64_t step = (int64_t)p.heads * p.dv;
-                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.e.row + chain.first_row(c)) * step + (int64_t)h * p.dv;
+                __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.o) + (u.e.row + chain.first_row(c)) * step + (int64_t)h * p.dv + chain.col0;
                 for (int i = tid; i < n * (DV / 8); i += kCompute) {
                     const int r = i / (DV / 8), ch = i % (DV / 8);
-                    if (ch * 8 >= p.dv) continue;
+                    if (ch * 8 >= chain.cols) continue;
                     const uint4 v = *reinterpret_cast<const uint4*>(from_tile + (ch / 8) * kTileBytes + r * 128 + ((ch % 8) ^ (r & 7)) * 16);
                     *reinterpret_cast<uint4*>(to + r * step + ch * 8) = v;
                 }
@@ -696,26 +716,25 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
     };
     sync();
     const uint32_t tmem = *tmem_at;
-    uint8_t* planes = smem + S::kStages * S::kStage;
+    auto planes_of = [&](int c) { return smem + S::kStages * S::kStage + (c % S::kBuffers) * S::kPlanes; };
     auto load_tiles = [&](int c) {
         uint8_t* at = smem + c % S::kStages * S::kStage;
         uint64_t* bar = &bars[c % S::kStages];
         tcu::mbar_arrive_expect_tx(bar, S::kStage);
         const int row = chain.row_at(c), b = chain.batch_at();
 #pragma unroll
-        for (int i = 0; i < DV / 64; ++i) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, i * 64, h, row, b);
+        for (int i = 0; i < DV / 64; ++i) tcu::tma_load_4d(at + i * kTileBytes, &maps.v, bar, chain.col0 + i * 64, h, row, b);
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) tcu::tma_load_4d(at + S::kV + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
     };
     if (warp == kCompute / 32) {
-        const uint32_t first = tcu::smem_u32(smem), pl = tcu::smem_u32(planes);
         if (lane == 0)
             for (int c = 0; c < min(chunks, S::kStages); ++c) load_tiles(c);
         for (int c = 0; c < chunks; ++c) {
             __syncwarp();
             sync();  // keys of chunk c weighed, product c - 1 read
             if (lane == 0) {
-                const uint32_t vt = first + c % S::kStages * S::kStage;
+                const uint32_t vt = tcu::smem_u32(smem) + c % S::kStages * S::kStage, pl = tcu::smem_u32(planes_of(c));
                 issue_update<DK, DV, KP>(tmem, vt + S::kV, pl, pl + S::kK, vt, kT);
                 tcu::mma_commit(&bars[kUpdate]);
                 if (c > 0 && c - 1 + S::kStages < chunks) load_tiles(c - 1 + S::kStages);
@@ -725,14 +744,19 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
         float s[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) s[i] = 0.f;
-        for (int c = 0; c < chunks; ++c) {
-            uint8_t* kt = smem + c % S::kStages * S::kStage + S::kV;
+        auto weigh = [&](int c) {
+            uint8_t *kt = smem + c % S::kStages * S::kStage + S::kV, *pl = planes_of(c);
             wait(c % S::kStages, c / S::kStages & 1);
-            weigh_keys<DK, KP>(kt, planes, planes + S::kK, powk, kT, reverse);
+            weigh_keys<DK, KP>(kt, pl, pl + S::kK, powk, kT, reverse);
+        };
+        weigh(0);
+        for (int c = 0; c < chunks; ++c) {
             sync();
+            if (S::kBuffers == 2 && c + 1 < chunks) weigh(c + 1);
             wait(kUpdate, c & 1);
             tcu::tc_fence_after_sync();
             chain.update(s, tmem + ((uint32_t)(quad * 32) << 16), decay);
+            if (S::kBuffers == 1 && c + 1 < chunks) weigh(c + 1);
         }
         const int64_t states = (int64_t)p.dk * p.dv;
         chain.store_state(s, p.states + (u.slot * p.heads + h) * states, 1.f, reinterpret_cast<float*>(smem),
@@ -781,7 +805,7 @@ int launch(const Params& p, const Maps& m, int64_t units, bool outputs, cudaStre
     const void* fn = outputs ? reinterpret_cast<const void*>(&tc_kernel<DK, DV, KP>)
                              : reinterpret_cast<const void*>(&tc_states_kernel<DK, DV, KP>);
     if (!ensure_smem_attr(fn, smem)) return fail(VH_E_DEVICE, "linear attention: shared memory");
-    const dim3 grid((unsigned)units, p.heads);
+    const dim3 grid((unsigned)units, p.heads, (p.dv + DV - 1) / DV);
     if (outputs) tc_kernel<DK, DV, KP><<<grid, kBlock<DK, DV>, smem, st>>>(p, m);
     else tc_states_kernel<DK, DV, KP><<<grid, kCompute + 32, smem, st>>>(p, m);
     return launch_status(outputs ? "linear attention" : "linear attention: segment states");
@@ -801,15 +825,20 @@ int run_dims(const Params& p, const Maps& m, int64_t units, bool exact, cudaStre
 
 }  // namespace
 
-// CTAs fill the card once: one an SM, two where keys and values are at most 64.  Chains that are fewer
+// The value columns a CTA takes: 64 where that makes up for chains that are fewer than the SMs (scores and
+// weighted keys are then computed twice), else all.
+static bool narrow_values(int64_t chains, int dv) { return dv <= 64 || 2 * chains <= sm_count(); }
+
+// CTAs fill the card once: one an SM, two where keys and columns are at most 64.  Chains that are fewer
 // than half of them are cut; packed sequences always are, as the host does not know their lengths.
 int tc_segment_size(int64_t length, int batch, bool packed, int heads, int dk, int dv) {
-    const int64_t ctas = (int64_t)sm_count() * (dk <= 64 && dv <= 64 ? 2 : 1), chains = (int64_t)batch * heads;
+    const bool narrow = narrow_values((int64_t)batch * heads, dv);
+    const int64_t ctas = (int64_t)sm_count() * (dk <= 64 && narrow ? 2 : 1), rows = heads * (narrow ? (dv + 63) / 64 : 1);
     int64_t size;
     if (packed) {
-        size = (length * heads + ctas - 1) / ctas;
+        size = (length * rows + ctas - 1) / ctas;
     } else {
-        const int64_t segs = ctas / chains;
+        const int64_t segs = ctas / (batch * rows);
         if (segs < 2) return 0;
         size = (length + segs - 1) / segs;
     }
@@ -827,8 +856,9 @@ bool tc_run(Params p, void* states, cudaStream_t st, int* rc) {
     p.segment = tc_segment_size(p.seqs.length, p.seqs.count, packed, p.heads, p.dk, p.dv);
     p.states = static_cast<float*>(states);
     const int64_t units = p.segment ? ssm::slot_total(packed, p.seqs.length, p.seqs.count, p.segment) : p.seqs.count;
-    if (p.dk <= 64) *rc = p.dv <= 64 ? run_dims<64, 64>(p, m, units, exact, st) : run_dims<64, 128>(p, m, units, exact, st);
-    else *rc = p.dv <= 64 ? run_dims<128, 64>(p, m, units, exact, st) : run_dims<128, 128>(p, m, units, exact, st);
+    const bool narrow = narrow_values((int64_t)p.seqs.count * p.heads, p.dv);
+    if (p.dk <= 64) *rc = narrow ? run_dims<64, 64>(p, m, units, exact, st) : run_dims<64, 128>(p, m, units, exact, st);
+    else *rc = narrow ? run_dims<128, 64>(p, m, units, exact, st) : run_dims<128, 128>(p, m, units, exact, st);
     return true;
 }
 
