@@ -43,85 +43,122 @@ struct Norm {
     int channels, groups, per, act;
 };
 
+// ---- V consecutive values, as pairs for the packed arithmetic --------------------------------------
+template <int V>
+constexpr int kP = ssm::kPairs<V>;
+
+template <int V, typename T>
+__device__ __forceinline__ void unpack(const ssm::Pack<T, V>& q, float2 (&v)[kP<V>]) {
+    ssm::unpack<T, V>(q, v);
+}
+template <int V, typename T>
+__device__ __forceinline__ void get(const T* p, float2 (&v)[kP<V>]) {
+    ssm::unpack<T, V>(*reinterpret_cast<const ssm::Pack<T, V>*>(p), v);
+}
+template <int V, typename T>
+__device__ __forceinline__ void put(T* p, const float2 (&v)[kP<V>]) {
+    float f[V];
+    ssm::from_pairs<V>(v, f);
+    ssm::Pack<T, V> q;
+    q.set(f);
+    *reinterpret_cast<ssm::Pack<T, V>*>(p) = q;
+}
+template <int V>
+__device__ __forceinline__ void set_pair(float2 (&v)[kP<V>], int i, float f) {
+    if (V == 1) v[0] = splat2(f);
+    else if (i % 2) v[i / 2].y = f;
+    else v[i / 2].x = f;
+}
+// The sum of V values.
+template <int V>
+__device__ __forceinline__ float total(const float2 (&v)[kP<V>]) {
+    if constexpr (V == 1) return v[0].x;
+    float2 s = v[0];
+#pragma unroll
+    for (int i = 1; i < kP<V>; ++i) s = fadd2(s, v[i]);
+    return s.x + s.y;
+}
+
 // ---- activations --------------------------------------------------------------------------------
 // Phi(x) and its density.  16-bit outputs take the approximation of gelu2 (absolute error 7.5e-8).
 template <typename T>
-__device__ __forceinline__ void normal_cdf(float x, float* cdf, float* density) {
+__device__ __forceinline__ void normal_cdf(float2 x, float2* cdf, float2* density) {
     constexpr float kDensity = 0.3989422804014327f;
     if constexpr (sizeof(T) == 4) {
-        *cdf = 0.5f * erfcf(-0.70710678118654752f * x);
-        *density = kDensity * expf(-0.5f * x * x);
+        *cdf = make_float2(0.5f * erfcf(-0.70710678118654752f * x.x), 0.5f * erfcf(-0.70710678118654752f * x.y));
+        *density = make_float2(kDensity * expf(-0.5f * x.x * x.x), kDensity * expf(-0.5f * x.y * x.y));
     } else {
-        const float ax = fabsf(x), t = rcp_approx(fmaf(ax, 0.3275911f * 0.70710678118654752f, 1.f));
-        const float e = ex2_approx(x * x * (-0.5f * 1.4426950408889634f));
-        float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-        q = fmaf(q, t, 0.5f * 1.421413741f);
-        q = fmaf(q, t, 0.5f * -0.284496736f);
-        q = fmaf(q, t, 0.5f * 0.254829592f) * t * e;
-        *cdf = x >= 0.f ? 1.f - q : (x < 0.f ? q : x);
-        *density = kDensity * e;
+        const float2 ax = make_float2(fabsf(x.x), fabsf(x.y));
+        const float2 d = ffma2(ax, splat2(0.3275911f * 0.70710678118654752f), splat2(1.f));
+        const float2 t = make_float2(rcp_approx(d.x), rcp_approx(d.y));
+        const float2 arg = fmul2(fmul2(x, x), splat2(-0.5f * 1.4426950408889634f));
+        const float2 e = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+        float2 q = ffma2(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
+        q = ffma2(q, t, splat2(0.5f * 1.421413741f));
+        q = ffma2(q, t, splat2(0.5f * -0.284496736f));
+        q = ffma2(q, t, splat2(0.5f * 0.254829592f));
+        q = fmul2(fmul2(q, t), e);
+        const float2 r = fsub2(splat2(1.f), q);
+        *cdf = make_float2(x.x >= 0.f ? r.x : (x.x < 0.f ? q.x : x.x), x.y >= 0.f ? r.y : (x.y < 0.f ? q.y : x.y));
+        *density = fmul2(e, splat2(kDensity));
     }
 }
 
-// act(pre) in place of pre, and act'(pre) in `slope` if SLOPE.
-template <typename T, bool SLOPE, int V>
-__device__ __forceinline__ void activate(int act, float (&pre)[V], float (&slope)[V]) {
+// x sigmoid(x), and its derivative s + x s (1 - s).
+__device__ __forceinline__ float2 silu2(float2 x, float2* slope) {
+    const float2 s = ssm::sigmoid2(x), y = fmul2(x, s);
+    *slope = ffma2(y, fsub2(splat2(1.f), s), s);
+    return y;
+}
+__device__ __forceinline__ float2 silu2(float2 x) { return fmul2(x, ssm::sigmoid2(x)); }
+
+// act(pre) in place of pre.
+template <typename T, int V>
+__device__ __forceinline__ void activate(int act, float2 (&pre)[kP<V>]) {
     if (act == 1) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float x = pre[i], s = ssm::sigmoid(x);
-            pre[i] = x * s;
-            if (SLOPE) slope[i] = s * fmaf(x, 1.f - s, 1.f);
+        for (int i = 0; i < kP<V>; ++i) pre[i] = silu2(pre[i]);
+    } else if (act == 2) {
+#pragma unroll
+        for (int i = 0; i < kP<V>; ++i) {
+            float2 cdf, density;
+            normal_cdf<T>(pre[i], &cdf, &density);
+            pre[i] = fmul2(pre[i], cdf);
+        }
+    }
+}
+// d act'(pre) in place of d; act(pre) in place of pre if WANT.
+template <typename T, bool WANT, int V>
+__device__ __forceinline__ void through(int act, float2 (&pre)[kP<V>], float2 (&d)[kP<V>]) {
+    if (act == 1) {
+#pragma unroll
+        for (int i = 0; i < kP<V>; ++i) {
+            float2 slope;
+            const float2 y = silu2(pre[i], &slope);
+            d[i] = fmul2(d[i], slope);
+            if (WANT) pre[i] = y;
         }
     } else if (act == 2) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float x = pre[i];
-            float cdf, density;
-            normal_cdf<T>(x, &cdf, &density);
-            pre[i] = x * cdf;
-            if (SLOPE) slope[i] = fmaf(x, density, cdf);
+        for (int i = 0; i < kP<V>; ++i) {
+            float2 cdf, density;
+            normal_cdf<T>(pre[i], &cdf, &density);
+            d[i] = fmul2(d[i], ffma2(pre[i], density, cdf));
+            if (WANT) pre[i] = fmul2(pre[i], cdf);
         }
-    } else if (SLOPE) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) slope[i] = 1.f;
     }
 }
 
-// ---- V consecutive values -----------------------------------------------------------------------
-template <int V, typename T>
-__device__ __forceinline__ void get(const T* p, float (&v)[V]) {
-    if constexpr (V == 8) {
-        load8(p, v);
-    } else if constexpr (V == 4) {
-        const float4 f = load4(p);
-        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = to_f(p[i]);
-    }
-}
-template <int V, typename T>
-__device__ __forceinline__ void put(T* p, const float (&v)[V]) {
-    if constexpr (V == 8) {
-        store8(p, v);
-    } else if constexpr (V == 4) {
-        store4(p, make_float4(v[0], v[1], v[2], v[3]));
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) p[i] = from_f<T>(v[i]);
-    }
-}
-
+// ---- channels -----------------------------------------------------------------------------------
 // Parameters and statistics of V channels from c on.
 template <int V>
 struct Channel {
-    float w[V], b[V], mean[V], rstd[V];
+    float2 w[kP<V>], b[kP<V>], mean[kP<V>], rstd[kP<V>];
     __device__ __forceinline__ void params(const Norm& p, int c) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            w[i] = p.weight ? p.weight[c + i] : 1.f;
-            b[i] = p.bias ? p.bias[c + i] : 0.f;
+            set_pair<V>(w, i, p.weight ? p.weight[c + i] : 1.f);
+            set_pair<V>(b, i, p.bias ? p.bias[c + i] : 0.f);
         }
     }
     // `m`, `r`: of the groups from the one of channel c0 on
@@ -129,51 +166,69 @@ struct Channel {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const int g = (c + i - c0) / per;
-            mean[i] = m[g];
-            rstd[i] = r[g];
+            set_pair<V>(mean, i, m[g]);
+            set_pair<V>(rstd, i, r[g]);
+        }
+    }
+    __device__ __forceinline__ void stats(float m, float r) {
+#pragma unroll
+        for (int i = 0; i < kP<V>; ++i) {
+            mean[i] = splat2(m);
+            rstd[i] = splat2(r);
         }
     }
 };
 
 // y of V values.
 template <typename T, int V>
-__device__ __forceinline__ void forward(const Norm& p, const Channel<V>& k, float (&x)[V], const T* gate, T* y) {
-    float unused[V];
+__device__ __forceinline__ void forward(const Norm& p, const Channel<V>& k, float2 (&x)[kP<V>], bool gated, const ssm::Pack<T, V>& gate, T* y) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = fmaf((x[i] - k.mean[i]) * k.rstd[i], k.w[i], k.b[i]);
-    activate<T, false, V>(p.act, x, unused);
-    if (gate) {
-        float z[V];
-        get<V>(gate, z);
+    for (int i = 0; i < kP<V>; ++i) x[i] = ffma2(fmul2(fsub2(x[i], k.mean[i]), k.rstd[i]), k.w[i], k.b[i]);
+    activate<T, V>(p.act, x);
+    if (gated) {
+        float2 z[kP<V>];
+        unpack<V>(gate, z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) x[i] *= z[i] * ssm::sigmoid(z[i]);
+        for (int i = 0; i < kP<V>; ++i) x[i] = fmul2(x[i], silu2(z[i]));
     }
     put<V>(y, x);
 }
 
 // x^ in place of x and dn in place of dy; the gate's gradient if `dgate`.
 template <typename T, int V>
-__device__ __forceinline__ void backward(const Norm& p, const Channel<V>& k, float (&x)[V], float (&dy)[V], const T* gate, T* dgate) {
-    float pre[V], slope[V];
+__device__ __forceinline__ void backward(const Norm& p, const Channel<V>& k, float2 (&x)[kP<V>], float2 (&dy)[kP<V>], bool gated,
+                                         const ssm::Pack<T, V>& gate, T* dgate) {
+    float2 pre[kP<V>];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        x[i] = (x[i] - k.mean[i]) * k.rstd[i];
-        pre[i] = fmaf(x[i], k.w[i], k.b[i]);
+    for (int i = 0; i < kP<V>; ++i) {
+        x[i] = fmul2(fsub2(x[i], k.mean[i]), k.rstd[i]);
+        pre[i] = ffma2(x[i], k.w[i], k.b[i]);
     }
-    activate<T, true, V>(p.act, pre, slope);
-    if (gate) {
-        float z[V], dz[V];
-        get<V>(gate, z);
+    if (gated) {
+        float2 z[kP<V>], dz[kP<V>];
+        unpack<V>(gate, z);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float s = ssm::sigmoid(z[i]);
-            dz[i] = dy[i] * pre[i] * (s * fmaf(z[i], 1.f - s, 1.f));
-            dy[i] *= z[i] * s;
+        for (int i = 0; i < kP<V>; ++i) {
+            const float2 g = silu2(z[i], &z[i]);
+            dz[i] = fmul2(dy[i], z[i]);
+            dy[i] = fmul2(dy[i], g);
         }
-        if (dgate) put<V>(dgate, dz);
-    }
+        through<T, true, V>(p.act, pre, dy);
+        if (dgate) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) dy[i] *= slope[i];
+            for (int i = 0; i < kP<V>; ++i) dz[i] = fmul2(dz[i], pre[i]);
+            put<V>(dgate, dz);
+        }
+    } else {
+        through<T, false, V>(p.act, pre, dy);
+    }
+}
+// rstd (w dn - a - x^ b) from x^ and dn, with a and b times rstd already.
+template <int V>
+__device__ __forceinline__ void input_gradient(const Channel<V>& k, const float2 (&x)[kP<V>], float2 (&d)[kP<V>], const float2 (&ra)[kP<V>],
+                                               const float2 (&rb)[kP<V>]) {
+#pragma unroll
+    for (int i = 0; i < kP<V>; ++i) d[i] = fsub2(fsub2(fmul2(fmul2(k.rstd[i], k.w[i]), d[i]), ra[i]), fmul2(x[i], rb[i]));
 }
 
 __device__ __forceinline__ float rstd_of(float m2, float count, float eps) { return 1.f / sqrtf(m2 / count + eps); }
@@ -191,47 +246,74 @@ __device__ __forceinline__ float lanes_sum(float v) {
 
 template <typename T, int V, int SW, int NV, bool BACK>
 __global__ void __launch_bounds__(kThreads) rows_kernel(Norm p, int gb) {
+    constexpr int P = kP<V>;
+    using Pack = ssm::Pack<T, V>;
     const int lane = threadIdx.x % SW, unit = threadIdx.x / SW, phases = kThreads / (gb * SW);
     const int g = blockIdx.y * gb + unit % gb, phase = unit / gb;
-    const bool live = phase < phases && g < p.groups;
+    const bool live = phase < phases && g < p.groups, gated = p.gate != nullptr;
     const int c0 = live ? g * p.per : 0;
     Channel<V> k[NV];
     bool has[NV];
-    float aw[NV][V], ab[NV][V];
+    float2 aw[NV][P], ab[NV][P];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int c = (lane + j * SW) * V;
         has[j] = live && c < p.per;
         k[j].params(p, has[j] ? c0 + c : 0);
 #pragma unroll
-        for (int i = 0; i < V; ++i) aw[j][i] = ab[j][i] = 0.f;
+        for (int i = 0; i < P; ++i) aw[j][i] = ab[j][i] = splat2(0.f);
     }
     const float count = (float)p.per;
-    if (live) {
-        for (int64_t r = (int64_t)blockIdx.x * phases + phase; r < p.samples; r += (int64_t)gridDim.x * phases) {
-            const T* x = static_cast<const T*>(p.x) + r * p.xs + c0 + lane * V;
-            const T* z = p.gate ? static_cast<const T*>(p.gate) + r * p.gs + c0 + lane * V : nullptr;
-            const int64_t at = r * p.channels + c0 + lane * V;
-            float v[NV][V];
+    // a row's values, fetched while the one before is worked on
+    struct Row {
+        Pack x[NV], z[NV], d[NV];
+        float mean, rstd;
+    };
+    auto fetch = [&](Row& q, int64_t r) {
+        const T* x = static_cast<const T*>(p.x) + r * p.xs + c0 + lane * V;
+        const T* z = static_cast<const T*>(p.gate) + r * p.gs + c0 + lane * V;
+        const T* d = static_cast<const T*>(p.dy) + r * p.channels + c0 + lane * V;
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                if (has[j]) get<V>(x + j * SW * V, v[j]);
+        for (int j = 0; j < NV; ++j) {
+            if (has[j]) {
+                q.x[j] = *reinterpret_cast<const Pack*>(x + j * SW * V);
+                if (gated) q.z[j] = *reinterpret_cast<const Pack*>(z + j * SW * V);
+                if (BACK) q.d[j] = *reinterpret_cast<const Pack*>(d + j * SW * V);
             }
+        }
+        if (BACK) {
+            q.mean = p.mean[r * p.groups + g];
+            q.rstd = p.rstd[r * p.groups + g];
+        }
+    };
+    const int64_t step = (int64_t)gridDim.x * phases;
+    int64_t r = (int64_t)blockIdx.x * phases + phase;
+    if (live && r < p.samples) {
+        Row next;
+        fetch(next, r);
+        for (; r < p.samples; r += step) {
+            const Row q = next;
+            if (r + step < p.samples) fetch(next, r + step);
+            const int64_t at = r * p.channels + c0 + lane * V;
+            float2 v[NV][P];
+#pragma unroll
+            for (int j = 0; j < NV; ++j) unpack<V>(q.x[j], v[j]);
             if constexpr (!BACK) {
                 float s = 0.f;
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) s += has[j] ? v[j][i] : 0.f;
+                for (int j = 0; j < NV; ++j) s += has[j] ? total<V>(v[j]) : 0.f;
                 const float mean = lanes_sum<SW>(s) / count;
                 s = 0.f;
 #pragma unroll
-                for (int j = 0; j < NV; ++j)
+                for (int j = 0; j < NV; ++j) {
+                    float2 d[P];
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float d = v[j][i] - mean;
-                        s += has[j] ? d * d : 0.f;
+                    for (int i = 0; i < P; ++i) {
+                        d[i] = fsub2(v[j][i], splat2(mean));
+                        d[i] = fmul2(d[i], d[i]);
                     }
+                    s += has[j] ? total<V>(d) : 0.f;
+                }
                 const float rstd = rstd_of(lanes_sum<SW>(s), count, p.eps);
                 if (p.mean && lane == 0) {
                     p.mean[r * p.groups + g] = mean;
@@ -240,50 +322,46 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(Norm p, int gb) {
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
                     if (has[j]) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            k[j].mean[i] = mean;
-                            k[j].rstd[i] = rstd;
-                        }
-                        forward<T, V>(p, k[j], v[j], z ? z + j * SW * V : nullptr, static_cast<T*>(p.y) + at + j * SW * V);
+                        k[j].stats(mean, rstd);
+                        forward<T, V>(p, k[j], v[j], gated, q.z[j], static_cast<T*>(p.y) + at + j * SW * V);
                     }
             } else {
-                const float mean = p.mean[r * p.groups + g], rstd = p.rstd[r * p.groups + g];
-                float d[NV][V], s1 = 0.f, s2 = 0.f;
+                float2 d[NV][P];
+                float s1 = 0.f, s2 = 0.f;
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
                     if (has[j]) {
-                        get<V>(static_cast<const T*>(p.dy) + at + j * SW * V, d[j]);
+                        unpack<V>(q.d[j], d[j]);
+                        k[j].stats(q.mean, q.rstd);
+                        backward<T, V>(p, k[j], v[j], d[j], gated, q.z[j], p.dgate ? static_cast<T*>(p.dgate) + at + j * SW * V : nullptr);
+                        float2 a[P], b[P];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            k[j].mean[i] = mean;
-                            k[j].rstd[i] = rstd;
+                        for (int i = 0; i < P; ++i) {
+                            ab[j][i] = fadd2(ab[j][i], d[j][i]);
+                            aw[j][i] = ffma2(d[j][i], v[j][i], aw[j][i]);
+                            a[i] = fmul2(d[j][i], k[j].w[i]);
+                            b[i] = fmul2(a[i], v[j][i]);
                         }
-                        backward<T, V>(p, k[j], v[j], d[j], z ? z + j * SW * V : nullptr,
-                                       p.dgate ? static_cast<T*>(p.dgate) + at + j * SW * V : nullptr);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            ab[j][i] += d[j][i];
-                            aw[j][i] = fmaf(d[j][i], v[j][i], aw[j][i]);
-                            d[j][i] *= k[j].w[i];
-                            s1 += d[j][i];
-                            s2 = fmaf(d[j][i], v[j][i], s2);
-                        }
+                        s1 += total<V>(a);
+                        s2 += total<V>(b);
                     }
-                s1 = lanes_sum<SW>(s1) / count;
-                s2 = lanes_sum<SW>(s2) / count;
+                const float2 ra = splat2(lanes_sum<SW>(s1) / count * q.rstd), rb = splat2(lanes_sum<SW>(s2) / count * q.rstd);
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
                     if (has[j]) {
+                        float2 a[P], b[P];
 #pragma unroll
-                        for (int i = 0; i < V; ++i) d[j][i] = rstd * (d[j][i] - s1 - v[j][i] * s2);
+                        for (int i = 0; i < P; ++i) {
+                            a[i] = ra;
+                            b[i] = rb;
+                        }
+                        input_gradient<V>(k[j], v[j], d[j], a, b);
                         put<V>(static_cast<T*>(p.dx) + at + j * SW * V, d[j]);
                     }
             }
         }
     }
     if constexpr (BACK) {
-        if (!p.part) return;
         // the row phases in order, each thread's channels
         extern __shared__ float red[];
         float* out = p.part + (int64_t)blockIdx.x * 2 * p.channels;
@@ -294,10 +372,13 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(Norm p, int gb) {
                 for (int j = 0; j < NV; ++j)
                     if (has[j]) {
                         const int c = (lane + j * SW) * V, at = (unit % gb) * p.per + c;
+                        float fb[V], fw[V];
+                        ssm::from_pairs<V>(ab[j], fb);
+                        ssm::from_pairs<V>(aw[j], fw);
 #pragma unroll
                         for (int i = 0; i < V; ++i) {
-                            const float b = (ph ? red[2 * (at + i)] : 0.f) + ab[j][i];
-                            const float w = (ph ? red[2 * (at + i) + 1] : 0.f) + aw[j][i];
+                            const float b = (ph ? red[2 * (at + i)] : 0.f) + fb[i];
+                            const float w = (ph ? red[2 * (at + i) + 1] : 0.f) + fw[i];
                             if (ph + 1 < phases) {
                                 red[2 * (at + i)] = b;
                                 red[2 * (at + i) + 1] = w;
@@ -332,49 +413,106 @@ __global__ void __launch_bounds__(1024) params_kernel(const float* __restrict__ 
 
 // ---- pixels over a block ------------------------------------------------------------------------
 // A block's threads over w channels: qn = w / V vectors side by side, kThreads / qn pixel phases.
-// f(c, r) is called for the first channel of a vector and every pixel of this thread's phase;
-// before(c) and after() around the pixels of each vector.
-template <int V, typename B, typename F, typename A>
-__device__ __forceinline__ void each(int w, int rows, B&& before, F&& f, A&& after) {
+// fetch(c, r) reads what work(c, r, .) takes for the vector at channel c of pixel r; U pixels are fetched
+// before the first is worked on, as loads do not pass the stores of another pixel.  before(c) and
+// after(...) stand around the pixels of each vector.
+template <int V, int U, typename B, typename L, typename F, typename A>
+__device__ __forceinline__ void each(int w, int rows, B&& before, L&& fetch, F&& work, A&& after) {
     const int q = w / V;
     for (int q0 = 0; q0 < q; q0 += kThreads) {
         const int qn = min(q - q0, kThreads), phases = kThreads / qn;
         const int qi = threadIdx.x % qn, ph = threadIdx.x / qn;
-        if (ph < phases) {
+        {  // threads past the last phase have a vector and no pixel
             const int c = (q0 + qi) * V;
             before(c);
-            for (int r = ph; r < rows; r += phases) f(c, r);
+            int r = ph < phases ? ph : rows;
+            for (; r + (U - 1) * phases < rows; r += U * phases) {
+                decltype(fetch(c, r)) raw[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = fetch(c, r + u * phases);
+#pragma unroll
+                for (int u = 0; u < U; ++u) work(c, r + u * phases, raw[u]);
+            }
+            for (; r < rows; r += phases) work(c, r, fetch(c, r));
         }
         after(q0, qn, phases, qi, ph);
     }
 }
 
-// Adds the V values of each thread over the pixel phases, into out[0..w), in a fixed order: first runs
-// of phases side by side, then the runs.
+// Adds V pairs of values of each thread over the pixel phases, into outa and outb [0..w), in a fixed order:
+// the lanes of a warp with the same vector, then the warps; or, where the vectors are no power of two up to
+// 32, runs of phases side by side, then the runs.  `red`: kThreads * V floats.
 template <int V>
-__device__ __forceinline__ void add_phases(const float (&v)[V], int q0, int qn, int phases, int qi, int ph, float* red, float* out) {
+__device__ __forceinline__ void add_phases(const float2 (&pa)[kP<V>], const float2 (&pb)[kP<V>], int q0, int qn, int phases, int qi, int ph,
+                                           float* red, float* outa, float* outb) {
     const int n = qn * V;
-    __syncthreads();
-    if (ph < phases) {
+    float v[2][V];
+    ssm::from_pairs<V>(pa, v[0]);
+    ssm::from_pairs<V>(pb, v[1]);
+    if (qn <= 8 && (qn & (qn - 1)) == 0) {
+        for (int o = qn; o < 32; o *= 2)
 #pragma unroll
-        for (int i = 0; i < V; ++i) red[ph * n + qi * V + i] = v[i];
+            for (int i = 0; i < V; ++i) {
+                v[0][i] += __shfl_xor_sync(0xffffffffu, v[0][i], o);
+                v[1][i] += __shfl_xor_sync(0xffffffffu, v[1][i], o);
+            }
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;  // 2 n <= kThreads / 32 * V * 2: red holds all warps
+        __syncthreads();
+        if (lane < qn) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                red[warp * 2 * n + lane * V + i] = v[0][i];
+                red[warp * 2 * n + n + lane * V + i] = v[1][i];
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * n; c += kThreads) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < kThreads / 32; ++k) s += red[k * 2 * n + c];
+            (c < n ? outa : outb)[q0 * V + (c < n ? c : c - n)] = s;
+        }
+        __syncthreads();
+        return;
+    }
+    for (int which = 0; which < 2; ++which) {
+        float* out = which ? outb : outa;
+        __syncthreads();
+        if (ph < phases) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) red[ph * n + qi * V + i] = which ? v[1][i] : v[0][i];
+        }
+        __syncthreads();
+        const int runs = max(1, min(phases, kThreads / n)), len = (phases + runs - 1) / runs;
+        float s = 0.f;
+        if (runs > 1) {
+            const int c = threadIdx.x % n, run = threadIdx.x / n;
+            if (run < runs)
+                for (int k = run * len; k < min(phases, (run + 1) * len); ++k) s += red[k * n + c];
+            __syncthreads();
+            if (run < runs) red[run * n + c] = s;
+            __syncthreads();
+        }
+        const int left = runs > 1 ? runs : phases;
+        for (int c = threadIdx.x; c < n; c += kThreads) {
+            s = 0.f;
+            for (int k = 0; k < left; ++k) s += red[k * n + c];
+            out[q0 * V + c] = s;
+        }
     }
     __syncthreads();
-    const int runs = max(1, min(phases, kThreads / n)), len = (phases + runs - 1) / runs;
-    float s = 0.f;
-    if (runs > 1) {
-        const int c = threadIdx.x % n, run = threadIdx.x / n;
-        if (run < runs)
-            for (int k = run * len; k < min(phases, (run + 1) * len); ++k) s += red[k * n + c];
-        __syncthreads();
-        if (run < runs) red[run * n + c] = s;
-        __syncthreads();
-    }
-    const int left = runs > 1 ? runs : phases;
-    for (int c = threadIdx.x; c < n; c += kThreads) {
-        s = 0.f;
-        for (int k = 0; k < left; ++k) s += red[k * n + c];
-        out[q0 * V + c] = s;
+}
+
+// Of values seen as differences to a pivot (`sum`, `square` over `rows` pixels): each channel's mean and sum of
+// squares around it, in place.
+template <typename Pivot>
+__device__ __forceinline__ void center(float* sum, float* square, int w, int rows, Pivot&& pivot) {
+    const float inv = rows ? 1.f / (float)rows : 0.f;
+    for (int c = threadIdx.x; c < w; c += kThreads) {
+        const float m = sum[c] * inv;
+        const float q = square[c] - sum[c] * m;
+        square[c] = q < 0.f ? 0.f : q;  // NaN stays
+        sum[c] = rows ? pivot(c) + m : 0.f;
     }
     __syncthreads();
 }
@@ -387,6 +525,26 @@ __device__ __forceinline__ void add_groups(const float* channel, int w, int per,
         for (int c = lane; c < per; c += 32) s += channel[g * per + c];
         s = warp_sum(s);
         if (lane == 0) out[g] = s;
+    }
+    __syncthreads();
+}
+
+// A group's mean and squares from its channels', each over `rows` pixels: a warp a group.
+__device__ __forceinline__ void join_groups(const float* mean, const float* square, int w, int per, int rows, float* gmean, float* gsquare) {
+    const int lane = threadIdx.x & 31;
+    for (int g = threadIdx.x >> 5; g < w / per; g += kThreads / 32) {
+        float s = 0.f, q = 0.f;
+        for (int c = lane; c < per; c += 32) s += mean[g * per + c];
+        const float mu = warp_sum(s) / (float)per;
+        for (int c = lane; c < per; c += 32) {
+            const float d = mean[g * per + c] - mu;
+            q += fmaf((float)rows * d, d, square[g * per + c]);
+        }
+        q = warp_sum(q);
+        if (lane == 0) {
+            gmean[g] = mu;
+            gsquare[g] = q;
+        }
     }
     __syncthreads();
 }
@@ -407,6 +565,14 @@ __device__ __forceinline__ float ld_cluster(const float* local, uint32_t rank) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
     return v;
+}
+
+// Pixels are cut into `parts` slices of one length, the last ones shorter or empty.
+__host__ __device__ __forceinline__ int slice_len(int64_t pixels, int parts) { return (int)((pixels + parts - 1) / parts); }
+__device__ __forceinline__ int slice_rows(int64_t pixels, int part, int parts) {
+    const int len = slice_len(pixels, parts);
+    const int64_t left = pixels - (int64_t)part * len;
+    return (int)(left < 0 ? 0 : left < len ? left : len);
 }
 
 // A slab of w channels of a slice of pixels into shared memory, [rows][w].
@@ -436,9 +602,9 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
     float *ca = head, *cb = ca + width, *red = cb + width, *ga = red + kThreads * V, *gb = ga + width / per,
           *mean = gb + width / per, *rstd = mean + width / per;
     T* xs = reinterpret_cast<T*>(head + head_floats(width, per, V));
-    const int64_t s0 = p.pixels * rank / cluster;
-    const int rows = (int)(p.pixels * (rank + 1) / cluster - s0);
-    T* ds = xs + (int64_t)((p.pixels + cluster - 1) / cluster) * width;
+    const int len = slice_len(p.pixels, cluster), rows = slice_rows(p.pixels, rank, cluster);
+    const int64_t s0 = (int64_t)rank * len;
+    T* ds = xs + len * width;
 
     load_slab<T, V>(xs, static_cast<const T*>(p.x) + n * p.xs + s0 * p.xp + c0, p.xp, rows, w);
     const int64_t at = (n * p.pixels + s0) * p.channels + c0;  // in contiguous tensors
@@ -449,54 +615,61 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
     __syncthreads();
 
     Channel<V> k;
+    constexpr int P = kP<V>;
+    using Pack = ssm::Pack<T, V>;
+    const bool gated = gate != nullptr;
+    auto gate_at = [&](int c, int r) {
+        Pack z = {};
+        if (gated) z = *reinterpret_cast<const Pack*>(gate + r * p.gp + c);
+        return z;
+    };
+    struct Two {
+        Pack a, b;
+    };
+    struct Three {
+        Pack a, b, c;
+    };
+    auto three = [&](int c, int r) {
+        return Three{*reinterpret_cast<const Pack*>(xs + r * w + c), *reinterpret_cast<const Pack*>(ds + r * w + c), gate_at(c, r)};
+    };
     if constexpr (!BACK) {
-        // the slice's mean, then its squares around it
-        float acc[V];
-        auto zero = [&] {
+        // sums of differences to the slice's first pixel, a channel
+        float2 sum[P], square[P], first[P];
+        each<V, 1>(w, rows,
+                   [&](int c) {
+                       get<V>(xs + c, first);
 #pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = 0.f;
-        };
-        zero();
-        each<V>(w, rows, [&](int) {},
-                [&](int c, int r) {
-                    float v[V];
-                    get<V>(xs + (int64_t)r * w + c, v);
+                       for (int i = 0; i < P; ++i) sum[i] = square[i] = splat2(0.f);
+                   },
+                   [&](int c, int r) { return *reinterpret_cast<const Pack*>(xs + r * w + c); },
+                   [&](int, int, const Pack& q) {
+                       float2 v[P];
+                       unpack<V>(q, v);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) acc[i] += v[i];
-                },
-                [&](int q0, int qn, int phases, int qi, int ph) { add_phases<V>(acc, q0, qn, phases, qi, ph, red, ca); zero(); });
-        add_groups(ca, w, per, ga);
-        const float count = (float)rows * per;
-        for (int g = threadIdx.x; g < groups; g += kThreads) ga[g] = rows ? ga[g] / count : 0.f;
-        __syncthreads();
-        each<V>(w, rows,
-                [&](int c) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) k.mean[i] = ga[(c + i) / per];
-                },
-                [&](int c, int r) {
-                    float v[V];
-                    get<V>(xs + (int64_t)r * w + c, v);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float d = v[i] - k.mean[i];
-                        acc[i] = fmaf(d, d, acc[i]);
-                    }
-                },
-                [&](int q0, int qn, int phases, int qi, int ph) { add_phases<V>(acc, q0, qn, phases, qi, ph, red, cb); zero(); });
-        add_groups(cb, w, per, gb);
+                       for (int i = 0; i < P; ++i) {
+                           v[i] = fsub2(v[i], first[i]);
+                           sum[i] = fadd2(sum[i], v[i]);
+                           square[i] = ffma2(v[i], v[i], square[i]);
+                       }
+                   },
+                   [&](int q0, int qn, int phases, int qi, int ph) { add_phases<V>(sum, square, q0, qn, phases, qi, ph, red, ca, cb); });
+        center(ca, cb, w, rows, [&](int c) { return to_f(xs[c]); });
+        join_groups(ca, cb, w, per, rows, ga, gb);
         if (cluster > 1) cluster_sync();
         const float m = (float)p.pixels * per;
         for (int g = threadIdx.x; g < groups; g += kThreads) {
-            float mu = 0.f, m2 = 0.f;
-            for (int j = 0; j < cluster; ++j) {
-                const float nk = (float)(p.pixels * (j + 1) / cluster - p.pixels * j / cluster) * per;
-                mu = fmaf(nk / m, cluster > 1 ? ld_cluster(ga + g, j) : ga[g], mu);
+            float part[kMaxCluster], more[kMaxCluster], mu = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) {
+                part[j] = j < cluster ? (cluster > 1 ? ld_cluster(ga + g, j) : ga[g]) : 0.f;
+                more[j] = j < cluster ? (cluster > 1 ? ld_cluster(gb + g, j) : gb[g]) : 0.f;
             }
-            for (int j = 0; j < cluster; ++j) {
-                const float nk = (float)(p.pixels * (j + 1) / cluster - p.pixels * j / cluster) * per;
-                const float d = (cluster > 1 ? ld_cluster(ga + g, j) : ga[g]) - mu;
-                m2 += fmaf(nk * d, d, cluster > 1 ? ld_cluster(gb + g, j) : gb[g]);
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) mu = fmaf((float)slice_rows(p.pixels, j, cluster) * per / m, part[j], mu);
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) {
+                const float d = part[j] - mu;
+                if (j < cluster) m2 += fmaf((float)slice_rows(p.pixels, j, cluster) * per * d, d, more[j]);
             }
             mean[g] = mu;
             rstd[g] = rstd_of(m2, m, p.eps);
@@ -506,17 +679,18 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
             }
         }
         __syncthreads();
-        each<V>(w, rows,
-                [&](int c) {
-                    k.params(p, c0 + c);
-                    k.stats(mean, rstd, per, c, 0);
-                },
-                [&](int c, int r) {
-                    float v[V];
-                    get<V>(xs + (int64_t)r * w + c, v);
-                    forward<T, V>(p, k, v, gate ? gate + r * p.gp + c : nullptr, static_cast<T*>(p.y) + at + (int64_t)r * p.channels + c);
-                },
-                [&](int, int, int, int, int) {});
+        each<V, 2>(w, rows,
+                   [&](int c) {
+                       k.params(p, c0 + c);
+                       k.stats(mean, rstd, per, c, 0);
+                   },
+                   [&](int c, int r) { return Two{*reinterpret_cast<const Pack*>(xs + r * w + c), gate_at(c, r)}; },
+                   [&](int c, int r, const Two& q) {
+                       float2 v[P];
+                       unpack<V>(q.a, v);
+                       forward<T, V>(p, k, v, gated, q.b, static_cast<T*>(p.y) + at + (int64_t)r * p.channels + c);
+                   },
+                   [&](int, int, int, int, int) {});
         if (cluster > 1) cluster_sync();  // nobody leaves while its sums may still be read
     } else {
         for (int g = threadIdx.x; g < groups; g += kThreads) {
@@ -524,42 +698,45 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
             rstd[g] = p.rstd[n * p.groups + c0 / per + g];
         }
         __syncthreads();
-        float sb[V], sw[V];
-        auto zero = [&] {
-#pragma unroll
-            for (int i = 0; i < V; ++i) sb[i] = sw[i] = 0.f;
-        };
+        float2 sb[P], sw[P];
         auto before = [&](int c) {
             k.params(p, c0 + c);
             k.stats(mean, rstd, per, c, 0);
         };
-        zero();
-        each<V>(w, rows, before,
-                [&](int c, int r) {
-                    float v[V], d[V];
-                    get<V>(xs + (int64_t)r * w + c, v);
-                    get<V>(ds + (int64_t)r * w + c, d);
-                    backward<T, V>(p, k, v, d, gate ? gate + r * p.gp + c : nullptr, nullptr);
+        each<V, 1>(w, rows,
+                   [&](int c) {
+                       before(c);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        sb[i] += d[i];
-                        sw[i] = fmaf(d[i], v[i], sw[i]);
-                    }
-                },
-                [&](int q0, int qn, int phases, int qi, int ph) {
-                    add_phases<V>(sb, q0, qn, phases, qi, ph, red, ca);
-                    add_phases<V>(sw, q0, qn, phases, qi, ph, red, cb);
-                    zero();
-                });
+                       for (int i = 0; i < P; ++i) sb[i] = sw[i] = splat2(0.f);
+                   },
+                   three,
+                   [&](int c, int r, const Three& q) {
+                       float2 v[P], d[P];
+                       unpack<V>(q.a, v);
+                       unpack<V>(q.b, d);
+                       backward<T, V>(p, k, v, d, gated, q.c, static_cast<T*>(nullptr));
+#pragma unroll
+                       for (int i = 0; i < P; ++i) {
+                           sb[i] = fadd2(sb[i], d[i]);
+                           sw[i] = ffma2(d[i], v[i], sw[i]);
+                       }
+                   },
+                   [&](int q0, int qn, int phases, int qi, int ph) { add_phases<V>(sb, sw, q0, qn, phases, qi, ph, red, ca, cb); });
         if (cluster > 1) cluster_sync();
         // all slices' sums a channel (into the scratch, as others still read ca and cb), then a group's
         float *ta = red, *tb = red + w;
         const bool fits = 2 * w <= kThreads * V;
         for (int c = threadIdx.x; c < w; c += kThreads) {
-            float b = 0.f, s = 0.f;
-            for (int j = 0; j < cluster; ++j) {
-                b += cluster > 1 ? ld_cluster(ca + c, j) : ca[c];
-                s += cluster > 1 ? ld_cluster(cb + c, j) : cb[c];
+            float fb[kMaxCluster], fw[kMaxCluster], b = 0.f, s = 0.f;
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) {
+                fb[j] = j < cluster ? (cluster > 1 ? ld_cluster(ca + c, j) : ca[c]) : 0.f;
+                fw[j] = j < cluster ? (cluster > 1 ? ld_cluster(cb + c, j) : cb[c]) : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < kMaxCluster; ++j) {
+                b += fb[j];
+                s += fw[j];
             }
             if (rank == 0) {
                 p.part[n * 2 * p.channels + c0 + c] = b;
@@ -578,21 +755,28 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
         add_groups(fits ? ta : ca, w, per, ga);
         add_groups(fits ? tb : cb, w, per, gb);
         const float m = (float)p.pixels * per;
-        each<V>(w, rows, before,
-                [&](int c, int r) {
-                    float v[V], d[V];
-                    get<V>(xs + (int64_t)r * w + c, v);
-                    get<V>(ds + (int64_t)r * w + c, d);
-                    const int64_t to = at + (int64_t)r * p.channels + c;
-                    backward<T, V>(p, k, v, d, gate ? gate + r * p.gp + c : nullptr, p.dgate ? static_cast<T*>(p.dgate) + to : nullptr);
+        float2 ra[P], rb[P];
+        each<V, 1>(w, rows,
+                   [&](int c) {
+                       before(c);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int g = (c + i) / per;
-                        d[i] = k.rstd[i] * (k.w[i] * d[i] - ga[g] / m - v[i] * (gb[g] / m));
-                    }
-                    put<V>(static_cast<T*>(p.dx) + to, d);
-                },
-                [&](int, int, int, int, int) {});
+                       for (int i = 0; i < V; ++i) {
+                           const int g = (c + i) / per;
+                           set_pair<V>(ra, i, ga[g] / m * rstd[g]);
+                           set_pair<V>(rb, i, gb[g] / m * rstd[g]);
+                       }
+                   },
+                   three,
+                   [&](int c, int r, const Three& q) {
+                       float2 v[P], d[P];
+                       unpack<V>(q.a, v);
+                       unpack<V>(q.b, d);
+                       const int64_t to = at + (int64_t)r * p.channels + c;
+                       backward<T, V>(p, k, v, d, gated, q.c, p.dgate ? static_cast<T*>(p.dgate) + to : nullptr);
+                       input_gradient<V>(k, v, d, ra, rb);
+                       put<V>(static_cast<T*>(p.dx) + to, d);
+                   },
+                   [&](int, int, int, int, int) {});
         if (cluster > 1) cluster_sync();
     }
 }
@@ -604,75 +788,67 @@ __global__ void __launch_bounds__(kThreads) part_kernel(Norm p, int splits, int 
     extern __shared__ __align__(16) float head[];
     float *red = head, *ca = red + kThreads * V, *cb = ca + width;
     const int split = blockIdx.x, c0 = blockIdx.y * width, w = min(width, p.channels - c0);
-    const int64_t s0 = p.pixels * split / splits;
-    const int rows = (int)(p.pixels * (split + 1) / splits - s0);
+    const int rows = slice_rows(p.pixels, split, splits);
+    const int64_t s0 = (int64_t)split * slice_len(p.pixels, splits);
     for (int64_t n = blockIdx.z; n < p.samples; n += gridDim.z) {
         const T* x = static_cast<const T*>(p.x) + n * p.xs + s0 * p.xp + c0;
         const int64_t at = (n * p.pixels + s0) * p.channels + c0;
         const T* gate = p.gate ? static_cast<const T*>(p.gate) + n * p.gs + s0 * p.gp + c0 : nullptr;
-        float sa[V], sq[V], first[V];
-        Channel<V> k;
-        int mine = 0;
-        auto zero = [&] {
-#pragma unroll
-            for (int i = 0; i < V; ++i) sa[i] = sq[i] = first[i] = 0.f;
-            mine = 0;
+        constexpr int P = kP<V>;
+        using Pack = ssm::Pack<T, V>;
+        struct Raw {
+            Pack x, d, z;
         };
-        zero();
-        each<V>(w, rows,
-                [&](int c) {
-                    if constexpr (BACK) {
-                        const int g0 = (c0 + c) / p.per;
-                        k.params(p, c0 + c);
-                        k.stats(p.mean + n * p.groups + g0, p.rstd + n * p.groups + g0, p.per, c0 + c, g0 * p.per);
+        float2 sa[P], sq[P], first[P];
+        Channel<V> k;
+        each<V, BACK ? 2 : 4>(
+            w, rows,
+            [&](int c) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) sa[i] = sq[i] = first[i] = splat2(0.f);
+                if constexpr (BACK) {
+                    const int g0 = (c0 + c) / p.per;
+                    k.params(p, c0 + c);
+                    k.stats(p.mean + n * p.groups + g0, p.rstd + n * p.groups + g0, p.per, c0 + c, g0 * p.per);
+                } else if (rows > 0) {
+                    get<V>(x + c, first);
+                }
+            },
+            [&](int c, int r) {
+                Raw q = {};
+                q.x = *reinterpret_cast<const Pack*>(x + r * p.xp + c);
+                if constexpr (BACK) {
+                    q.d = *reinterpret_cast<const Pack*>(static_cast<const T*>(p.dy) + at + (int64_t)r * p.channels + c);
+                    if (gate) q.z = *reinterpret_cast<const Pack*>(gate + r * p.gp + c);
+                }
+                return q;
+            },
+            [&](int, int, const Raw& q) {
+                float2 v[P];
+                unpack<V>(q.x, v);
+                if constexpr (BACK) {
+                    float2 d[P];
+                    unpack<V>(q.d, d);
+                    backward<T, V>(p, k, v, d, gate != nullptr, q.z, static_cast<T*>(nullptr));
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        sa[i] = fadd2(sa[i], d[i]);
+                        sq[i] = ffma2(d[i], v[i], sq[i]);
                     }
-                },
-                [&](int c, int r) {
-                    float v[V];
-                    get<V>(x + r * p.xp + c, v);
-                    if constexpr (BACK) {
-                        float d[V];
-                        get<V>(static_cast<const T*>(p.dy) + at + (int64_t)r * p.channels + c, d);
-                        backward<T, V>(p, k, v, d, gate ? gate + r * p.gp + c : nullptr, nullptr);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            sa[i] += d[i];
-                            sq[i] = fmaf(d[i], v[i], sq[i]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            if (mine == 0) first[i] = v[i];
-                            const float d = v[i] - first[i];
-                            sa[i] += d;
-                            sq[i] = fmaf(d, d, sq[i]);
-                        }
-                        ++mine;
+                    for (int i = 0; i < P; ++i) {
+                        v[i] = fsub2(v[i], first[i]);
+                        sa[i] = fadd2(sa[i], v[i]);
+                        sq[i] = ffma2(v[i], v[i], sq[i]);
                     }
-                },
-                [&](int q0, int qn, int phases, int qi, int ph) {
-                    if constexpr (!BACK) {
-                        // the slice's mean a channel, then this thread's squares around it
-                        float sum[V];
-#pragma unroll
-                        for (int i = 0; i < V; ++i) sum[i] = fmaf((float)mine, first[i], sa[i]);
-                        add_phases<V>(sum, q0, qn, phases, qi, ph, red, ca);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const float mu = rows && ph < phases ? ca[(q0 + qi) * V + i] / (float)rows : 0.f;
-                            const float own = mine ? sa[i] / (float)mine : 0.f, d = first[i] + own - mu;
-                            sq[i] = mine ? fmaf((float)mine * d, d, fmaxf(sq[i] - sa[i] * own, 0.f)) : 0.f;
-                        }
-                        add_phases<V>(sq, q0, qn, phases, qi, ph, red, cb);
-                    } else {
-                        add_phases<V>(sa, q0, qn, phases, qi, ph, red, ca);
-                        add_phases<V>(sq, q0, qn, phases, qi, ph, red, cb);
-                    }
-                    zero();
-                });
+                }
+            },
+            [&](int q0, int qn, int phases, int qi, int ph) { add_phases<V>(sa, sq, q0, qn, phases, qi, ph, red, ca, cb); });
+        if (!BACK) center(ca, cb, w, rows, [&](int c) { return to_f(x[c]); });
         float* out = p.part + ((n * splits + split) * 2) * p.channels + c0;
         for (int c = threadIdx.x; c < w; c += kThreads) {
-            out[c] = BACK || rows == 0 ? ca[c] : ca[c] / (float)rows;
+            out[c] = ca[c];
             out[p.channels + c] = cb[c];
         }
         __syncthreads();
@@ -697,7 +873,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Norm p, int splits) {
         return v;
     };
     const float m = (float)p.pixels * p.per;
-    auto rows = [&](int s) { return (float)(p.pixels * (s + 1) / splits - p.pixels * s / splits); };
+    const int len = slice_len(p.pixels, splits);
+    auto rows = [&](int s) { return (float)max((int64_t)0, min((int64_t)len, p.pixels - (int64_t)s * len)); };
     float mu = 0.f;
     for (int i = threadIdx.x; i < total; i += kThreads) {
         const int s = i / p.per;
@@ -733,8 +910,8 @@ template <typename T, int V, bool BACK>
 __global__ void __launch_bounds__(kThreads) apply_kernel(Norm p, int splits, int width, const float* sums) {
     extern __shared__ __align__(16) float head[];
     const int split = blockIdx.x, c0 = blockIdx.y * width, w = min(width, p.channels - c0);
-    const int64_t s0 = p.pixels * split / splits;
-    const int rows = (int)(p.pixels * (split + 1) / splits - s0);
+    const int rows = slice_rows(p.pixels, split, splits);
+    const int64_t s0 = (int64_t)split * slice_len(p.pixels, splits);
     const float m = (float)p.pixels * p.per;
     for (int64_t n = blockIdx.z; n < p.samples; n += gridDim.z) {
         const T* x = static_cast<const T*>(p.x) + n * p.xs + s0 * p.xp + c0;
@@ -763,38 +940,51 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Norm p, int splits, int
             }
             __syncthreads();
         }
+        constexpr int P = kP<V>;
+        using Pack = ssm::Pack<T, V>;
+        struct Raw {
+            Pack x, d, z;
+        };
         Channel<V> k;
-        float ma[V], mb[V];
-        each<V>(w, rows,
-                [&](int c) {
-                    const int gc = (c0 + c) / p.per;
-                    k.params(p, c0 + c);
-                    k.stats(p.mean + n * p.groups + gc, p.rstd + n * p.groups + gc, p.per, c0 + c, gc * p.per);
-                    if constexpr (BACK) {
+        float2 ra[P], rb[P];
+        each<V, BACK ? 2 : 4>(
+            w, rows,
+            [&](int c) {
+                const int gc = (c0 + c) / p.per;
+                k.params(p, c0 + c);
+                k.stats(p.mean + n * p.groups + gc, p.rstd + n * p.groups + gc, p.per, c0 + c, gc * p.per);
+                if constexpr (BACK) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            ma[i] = ga[(c0 + c + i) / p.per - g0];
-                            mb[i] = gb[(c0 + c + i) / p.per - g0];
-                        }
+                    for (int i = 0; i < V; ++i) {
+                        const int g = (c0 + c + i) / p.per;
+                        const float rstd = p.rstd[n * p.groups + g];
+                        set_pair<V>(ra, i, ga[g - g0] * rstd);
+                        set_pair<V>(rb, i, gb[g - g0] * rstd);
                     }
-                },
-                [&](int c, int r) {
-                    float v[V];
-                    get<V>(x + r * p.xp + c, v);
-                    const T* z = gate ? gate + r * p.gp + c : nullptr;
-                    const int64_t to = at + (int64_t)r * p.channels + c;
-                    if constexpr (BACK) {
-                        float d[V];
-                        get<V>(static_cast<const T*>(p.dy) + to, d);
-                        backward<T, V>(p, k, v, d, z, p.dgate ? static_cast<T*>(p.dgate) + to : nullptr);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) d[i] = k.rstd[i] * (k.w[i] * d[i] - ma[i] - v[i] * mb[i]);
-                        put<V>(static_cast<T*>(p.dx) + to, d);
-                    } else {
-                        forward<T, V>(p, k, v, z, static_cast<T*>(p.y) + to);
-                    }
-                },
-                [&](int, int, int, int, int) {});
+                }
+            },
+            [&](int c, int r) {
+                Raw q = {};
+                q.x = *reinterpret_cast<const Pack*>(x + r * p.xp + c);
+                if (gate) q.z = *reinterpret_cast<const Pack*>(gate + r * p.gp + c);
+                if constexpr (BACK) q.d = *reinterpret_cast<const Pack*>(static_cast<const T*>(p.dy) + at + (int64_t)r * p.channels + c);
+                return q;
+            },
+            [&](int c, int r, const Raw& q) {
+                float2 v[P];
+                unpack<V>(q.x, v);
+                const int64_t to = at + (int64_t)r * p.channels + c;
+                if constexpr (BACK) {
+                    float2 d[P];
+                    unpack<V>(q.d, d);
+                    backward<T, V>(p, k, v, d, gate != nullptr, q.z, p.dgate ? static_cast<T*>(p.dgate) + to : nullptr);
+                    input_gradient<V>(k, v, d, ra, rb);
+                    put<V>(static_cast<T*>(p.dx) + to, d);
+                } else {
+                    forward<T, V>(p, k, v, gate != nullptr, q.z, static_cast<T*>(p.y) + to);
+                }
+            },
+            [&](int, int, int, int, int) {});
     }
 }
 
