@@ -150,6 +150,20 @@ __device__ __forceinline__ void through(int act, float2 (&pre)[kP<V>], float2 (&
 }
 
 // ---- channels -----------------------------------------------------------------------------------
+// f(i, g) for V channels from c on, i = 0..V-1, with g the group of channel c + i: one division for all of them
+// (a thread has some fifty values, and one division a channel were a third of its instructions).
+template <int V, typename F>
+__device__ __forceinline__ void with_groups(int c, int per, F&& f) {
+    int g = c / per, left = per - (c - g * per);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        f(i, g);
+        if (--left == 0) {
+            ++g;
+            left = per;
+        }
+    }
+}
 // Parameters and statistics of V channels from c on.
 template <int V>
 struct Channel {
@@ -163,12 +177,10 @@ struct Channel {
     }
     // `m`, `r`: of the groups from the one of channel c0 on
     __device__ __forceinline__ void stats(const float* m, const float* r, int per, int c, int c0) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int g = (c + i - c0) / per;
+        with_groups<V>(c - c0, per, [&](int i, int g) {
             set_pair<V>(mean, i, m[g]);
             set_pair<V>(rstd, i, r[g]);
-        }
+        });
     }
     __device__ __forceinline__ void stats(float m, float r) {
 #pragma unroll
@@ -755,16 +767,19 @@ __global__ void __launch_bounds__(kThreads) resident_kernel(Norm p, int width, i
         add_groups(fits ? ta : ca, w, per, ga);
         add_groups(fits ? tb : cb, w, per, gb);
         const float m = (float)p.pixels * per;
+        for (int g = threadIdx.x; g < groups; g += kThreads) {
+            ga[g] = ga[g] / m * rstd[g];
+            gb[g] = gb[g] / m * rstd[g];
+        }
+        __syncthreads();
         float2 ra[P], rb[P];
         each<V, 1>(w, rows,
                    [&](int c) {
                        before(c);
-#pragma unroll
-                       for (int i = 0; i < V; ++i) {
-                           const int g = (c + i) / per;
-                           set_pair<V>(ra, i, ga[g] / m * rstd[g]);
-                           set_pair<V>(rb, i, gb[g] / m * rstd[g]);
-                       }
+                       with_groups<V>(c, per, [&](int i, int g) {
+                           set_pair<V>(ra, i, ga[g]);
+                           set_pair<V>(rb, i, gb[g]);
+                       });
                    },
                    three,
                    [&](int c, int r, const Three& q) {
@@ -934,8 +949,9 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Norm p, int splits, int
                 a = warp_sum(a);
                 b = warp_sum(b);
                 if (lane == 0) {
-                    ga[g - g0] = a / m;
-                    gb[g - g0] = b / m;
+                    const float rstd = p.rstd[n * p.groups + g] / m;
+                    ga[g - g0] = a * rstd;
+                    gb[g - g0] = b * rstd;
                 }
             }
             __syncthreads();
@@ -954,13 +970,10 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(Norm p, int splits, int
                 k.params(p, c0 + c);
                 k.stats(p.mean + n * p.groups + gc, p.rstd + n * p.groups + gc, p.per, c0 + c, gc * p.per);
                 if constexpr (BACK) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const int g = (c0 + c + i) / p.per;
-                        const float rstd = p.rstd[n * p.groups + g];
-                        set_pair<V>(ra, i, ga[g - g0] * rstd);
-                        set_pair<V>(rb, i, gb[g - g0] * rstd);
-                    }
+                    with_groups<V>(c0 + c, p.per, [&](int i, int g) {
+                        set_pair<V>(ra, i, ga[g - g0]);
+                        set_pair<V>(rb, i, gb[g - g0]);
+                    });
                 }
             },
             [&](int c, int r) {
