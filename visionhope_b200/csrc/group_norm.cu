@@ -26,7 +26,8 @@ namespace vh {
 namespace gn {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // of a block; half as many as 256 pay half as often for a channel's parameters
+constexpr int kJoinThreads = 256;
 constexpr int kMaxCluster = 8;
 
 struct Norm {
@@ -461,7 +462,7 @@ __device__ __forceinline__ void add_phases(const float2 (&pa)[kP<V>], const floa
     float v[2][V];
     ssm::from_pairs<V>(pa, v[0]);
     ssm::from_pairs<V>(pb, v[1]);
-    if (qn <= 8 && (qn & (qn - 1)) == 0) {
+    if (qn <= 4 && (qn & (qn - 1)) == 0) {
         for (int o = qn; o < 32; o *= 2)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -871,8 +872,8 @@ __global__ void __launch_bounds__(kThreads) part_kernel(Norm p, int splits, int 
 }
 
 // Joins the slices' means and squares of a group: a block per sample and group.
-__global__ void __launch_bounds__(kThreads) join_kernel(Norm p, int splits) {
-    __shared__ float red[kThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Norm p, int splits) {
+    __shared__ float red[kJoinThreads / 32];
     const int g = blockIdx.x;
     const int64_t n = blockIdx.y + (int64_t)blockIdx.z * gridDim.y;
     if (n >= p.samples) return;
@@ -884,20 +885,20 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Norm p, int splits) {
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
         __syncthreads();
         v = 0.f;
-        for (int i = 0; i < kThreads / 32; ++i) v += red[i];
+        for (int i = 0; i < kJoinThreads / 32; ++i) v += red[i];
         return v;
     };
     const float m = (float)p.pixels * p.per;
     const int len = slice_len(p.pixels, splits);
     auto rows = [&](int s) { return (float)max((int64_t)0, min((int64_t)len, p.pixels - (int64_t)s * len)); };
     float mu = 0.f;
-    for (int i = threadIdx.x; i < total; i += kThreads) {
+    for (int i = threadIdx.x; i < total; i += kJoinThreads) {
         const int s = i / p.per;
         mu = fmaf(rows(s) / m, part[(int64_t)s * 2 * p.channels + i % p.per], mu);
     }
     mu = block_sum(mu);
     float m2 = 0.f;
-    for (int i = threadIdx.x; i < total; i += kThreads) {
+    for (int i = threadIdx.x; i < total; i += kJoinThreads) {
         const int s = i / p.per;
         const float* at = part + (int64_t)s * 2 * p.channels + i % p.per;
         const float d = at[0] - mu;
@@ -911,8 +912,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(Norm p, int splits) {
 }
 
 // Sums the slices of a sample, in order: [samples][splits][2 channels] -> [samples][2 channels].
-__global__ void __launch_bounds__(kThreads) fold_kernel(const float* __restrict__ part, int splits, int64_t samples, int n, float* out) {
-    const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) fold_kernel(const float* __restrict__ part, int splits, int64_t samples, int n, float* out) {
+    const int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x;
     if (i >= samples * n) return;
     const float* at = part + i / n * splits * n + i % n;
     float s = 0.f;
@@ -1191,10 +1192,10 @@ int run_split(Norm p, const Plan& q, float* ws, cudaStream_t st) {
     part_kernel<T, V, BACK><<<grid, kThreads, smem, st>>>(p, q.splits, q.width);
     if (int rc = launch_status("group norm: slices")) return rc;
     if (!BACK) {
-        join_kernel<<<dim3(p.groups, nz, (unsigned)((p.samples + nz - 1) / nz)), kThreads, 0, st>>>(p, q.splits);
+        join_kernel<<<dim3(p.groups, nz, (unsigned)((p.samples + nz - 1) / nz)), kJoinThreads, 0, st>>>(p, q.splits);
         if (int rc = launch_status("group norm: statistics")) return rc;
     } else {
-        fold_kernel<<<(unsigned)((p.samples * row + kThreads - 1) / kThreads), kThreads, 0, st>>>(ws, q.splits, p.samples, (int)row, after);
+        fold_kernel<<<(unsigned)((p.samples * row + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, st>>>(ws, q.splits, p.samples, (int)row, after);
         if (int rc = launch_status("group norm: sums")) return rc;
     }
     const size_t more = BACK ? (size_t)2 * (q.width / p.per + 2) * sizeof(float) : 0;

@@ -23,36 +23,38 @@ _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 
 
 class _Call:
-    """One call's checked arguments; ``args`` packs them with the output pointers.  x and gate:
-    [samples, pixels, channels], unit stride last."""
+    """One call's checked arguments; ``args`` packs them with the output pointers.  x and gate: [samples,
+    channels] (``pixels`` 1, unit stride last) or contiguous [samples, pixels, channels]."""
 
-    __slots__ = ("x", "gate", "weight", "bias", "stats_shape", "head", "tail")
+    __slots__ = ("x", "gate", "weight", "bias", "samples", "groups", "head", "tail")
 
     def __init__(self, x, gate, weight, bias, groups, eps, activation):
-        n, p, c = x.shape
-        device = x.device
-        self.x, self.gate = x, gate
+        shape, device, xs = x.shape, x.device, x.stride()
+        n, c = shape[0], shape[-1]
+        self.x, self.gate, self.samples, self.groups = x, gate, n, groups
         self.weight = weight = _args.fp32(weight, (c,), "weight", device)
         self.bias = bias = _args.fp32(bias, (c,), "bias", device)
-        self.stats_shape = n, groups
-        xs, gs = x.stride(), (0, 0) if gate is None else gate.stride()
-        self.head = (x.data_ptr(), ptr(gate), xs[0], xs[1], gs[0], gs[1], ptr(weight), ptr(bias))
-        self.tail = n, p, eps, _lib.dtype_code(x.dtype), c, groups, activation
+        gs = (0, 0) if gate is None else gate.stride()
+        self.head = (x.data_ptr(), ptr(gate), xs[0], xs[-2], gs[0], gs[-2], ptr(weight), ptr(bias))
+        self.tail = n, shape[1] if len(shape) == 3 else 1, eps, _lib.DTYPES[x.dtype], c, groups, activation
 
     def args(self, y=0, mean=None, rstd=None):
         return _ARGS.pack(*self.head, y, ptr(mean), ptr(rstd), *self.tail)
 
     def forward(self, want_stats):
         x = self.x
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        mean, rstd = (torch.empty(self.stats_shape, dtype=torch.float32, device=x.device) if want_stats else None for _ in range(2))
+        dev = x.device
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        mean = rstd = None
+        if want_stats:
+            mean, rstd = torch.empty((2, self.samples, self.groups), dtype=torch.float32, device=dev)
         if y.numel() == 0:
             return y, mean, rstd
         lib = _lib.load()
         args = self.args(y.data_ptr(), mean, rstd)
         nbytes = lib.vh_group_norm_fwd_workspace_bytes(args)
-        ws = _args.workspace(nbytes, x.device) if nbytes else None
-        _lib.check(lib.vh_group_norm_fwd(args, ptr(ws), nbytes, _lib.stream_handle(x.device)), "vh_group_norm_fwd")
+        ws = _args.workspace(nbytes, dev) if nbytes else None
+        _lib.check(lib.vh_group_norm_fwd(args, ptr(ws), nbytes, _lib.stream_handle(dev)), "vh_group_norm_fwd")
         return y, mean, rstd
 
     def backward(self, dy, mean, rstd, want_gate):
@@ -95,21 +97,14 @@ class _GroupNormFunction(torch.autograd.Function):
         return (*(_args.grad_like(g, t) for g, t in zip(grads, inputs)), None, None, None)
 
 
-def _check(x, channels, groups, weight, bias, activation, gate):
+def _check(x, channels, groups, activation, gate):
     _lib.ensure_device(x)
-    _lib.dtype_code(x.dtype)
+    if x.dtype not in _lib.DTYPES:
+        _lib.dtype_code(x.dtype)
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation must be None, 'silu' or 'gelu', got {activation!r}")
     if groups < 1 or channels % groups:
         raise ValueError(f"groups must be a divisor of {channels}, got {groups}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            if t.shape != (channels,):
-                _args.refuse_shape(name, (channels,), t.shape)
-            if t.device != x.device:
-                _args.refuse_device(name, x.device, t.device)
-            if not t.is_floating_point():
-                raise TypeError(f"{name} must be a floating-point tensor, got {t.dtype}")
     if gate is not None:
         if gate.shape != x.shape:
             _args.refuse_shape("gate", x.shape, gate.shape)
@@ -117,6 +112,21 @@ def _check(x, channels, groups, weight, bias, activation, gate):
             raise TypeError(f"gate must be {x.dtype} as x, got {gate.dtype}")
         if gate.device != x.device:
             _args.refuse_device("gate", x.device, gate.device)
+
+
+def _flat(t):
+    """[..., C] as [rows, C] with unit stride last: a view where the strides allow it."""
+    c = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(t.numel() // c if c else 0, c)
+    return t if t.stride(-1) == 1 or c == 1 else t.contiguous()
+
+
+def _pixels(t):
+    """[B, C, H, W] as contiguous [B, H * W, C]: a view of a channels-last tensor."""
+    t = t.contiguous(memory_format=torch.channels_last).permute(0, 2, 3, 1)
+    # a single row of pixels or channel lets a tensor count as channels-last with any strides
+    return (t if t.is_contiguous() else t.contiguous()).flatten(1, 2)
 
 
 def _run(x, gate, weight, bias, groups, eps, activation):
@@ -136,17 +146,9 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, *, activation=None, 
     every tensor; the sums of the backward run in a fixed order."""
     if x.dim() != 4:
         raise ValueError(f"x must be [batch, channels, height, width], got {tuple(x.shape)}")
-    _check(x, x.shape[1], groups, weight, bias, activation, gate)
     b, c, h, w = x.shape
-
-    def rows(t):
-        if t is None:
-            return None
-        t = t.contiguous(memory_format=torch.channels_last).permute(0, 2, 3, 1)
-        # a single pixel row or channel lets a tensor count as channels-last with any strides
-        return (t if t.is_contiguous() else t.contiguous()).view(b, h * w, c)
-
-    y = _run(rows(x), rows(gate), weight, bias, groups, eps, activation)
+    _check(x, c, groups, activation, gate)
+    y = _run(_pixels(x), None if gate is None else _pixels(gate), weight, bias, groups, eps, activation)
     return y.view(b, h, w, c).permute(0, 3, 1, 2)
 
 
@@ -156,18 +158,9 @@ def group_norm_rows(x, groups, weight=None, bias=None, eps=1e-5, *, activation=N
     groups channels of a group.  x and gate may be parts of wider rows (unit stride last)."""
     if x.dim() < 1:
         raise ValueError("x must be [..., channels]")
-    c = x.shape[-1]
-    _check(x, c, groups, weight, bias, activation, gate)
-
-    def rows(t):
-        if t is None:
-            return None
-        t = t.reshape(t.numel() // c, c) if c else t.reshape(0, c)
-        if t.stride(-1) != 1 and c > 1:
-            t = t.contiguous()
-        return t.unsqueeze(1)
-
-    return _run(rows(x), rows(gate), weight, bias, groups, eps, activation).view(x.shape)
+    _check(x, x.shape[-1], groups, activation, gate)
+    y = _run(_flat(x), None if gate is None else _flat(gate), weight, bias, groups, eps, activation)
+    return y if y.shape == x.shape else y.view(x.shape)
 
 
 class GroupNorm(nn.Module):
