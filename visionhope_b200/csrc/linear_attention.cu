@@ -48,7 +48,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
                  : "memory");
 }
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -110,28 +110,44 @@ __device__ __forceinline__ void load_tile(uint16_t* dst, const T* src, int64_t s
             return;
         }
     }
-#pragma unroll 4
-    for (int i = threadIdx.x; i < kChunk * (W / 4); i += kThreads) {
-        const int r = i / (W / 4), c = i % (W / 4) * 4;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < n) {
-            const T* p = src + r * step + c;
-            if (vec >= 4) {
-                if (c < dim) {
-                    const float4 f = load4(p);
-                    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (c + e < dim) v[e] = to_f(p[e]);
-            }
-        }
+    auto put = [&](int r, int c, const float (&v)[4]) {
         uint32_t lo[NP], hi[NP];
         split2<NP>(v[0], v[1], lo);
         split2<NP>(v[2], v[3], hi);
 #pragma unroll
         for (int pl = 0; pl < NP; ++pl) *reinterpret_cast<uint2*>(dst + pl * PLANE + r * PITCH + c) = make_uint2(lo[pl], hi[pl]);
+    };
+    if (vec >= 4) {
+        // several loads before the first is split; the places that do not exist read the tile's first
+        constexpr int kAhead = 8;
+#pragma unroll 1
+        for (int i0 = threadIdx.x; i0 < kChunk * (W / 4); i0 += kAhead * kThreads) {
+            float4 f[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + k * kThreads, r = i / (W / 4), c = i % (W / 4) * 4;
+                f[k] = load4(r < n && c < dim ? src + r * step + c : src);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = i0 + k * kThreads, r = i / (W / 4), c = i % (W / 4) * 4;
+                const bool live = r < n && c < dim;
+                const float v[4] = {live ? f[k].x : 0.f, live ? f[k].y : 0.f, live ? f[k].z : 0.f, live ? f[k].w : 0.f};
+                put(r, c, v);
+            }
+        }
+        return;
+    }
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kChunk * (W / 4); i += kThreads) {
+        const int r = i / (W / 4), c = i % (W / 4) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (r < n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < dim) v[e] = to_f(src[r * step + c + e]);
+        }
+        put(r, c, v);
     }
 }
 
@@ -154,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) chunk_kernel(Params p) {
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t2 = (lane & 3) * 2;
     const int h = blockIdx.y, col0 = blockIdx.z * kTile, cols = min(kTile, p.dv - col0);
-    const Unit u = unit_at(p, blockIdx.x);
+    const Unit u = block_unit(p, reinterpret_cast<int*>(power + kChunk + 1));
     if constexpr (OUT) {
         const int64_t block = ((int64_t)blockIdx.x * gridDim.y + h) * gridDim.z + blockIdx.z;
         ssm::zero_outside<T>(p.seqs, p.heads * p.dv, block, (int64_t)gridDim.x * gridDim.y * gridDim.z, p.o);
@@ -500,18 +516,31 @@ __global__ void __launch_bounds__(256) enter_kernel(Params p) {
     float run = p.initial ? p.initial[((int64_t)s * p.heads + h) * states + a * p.init_a + b * p.init_b] : 0.f;
     float w = p.entry ? decay_power(g, p.segment - 1) : step;
     float* at = p.states + (base * p.heads + h) * states + i;
-    const int64_t stride = (int64_t)p.heads * states, segs = (e.len + p.segment - 1) / p.segment;
-    for (int64_t j = 0; j < segs; j += kEnterAhead) {
-        float own[kEnterAhead];  // the last segment adds to nobody's start
+    const int64_t stride = (int64_t)p.heads * states;
+    const int segs = (int)((e.len + p.segment - 1) / p.segment);
+    float own[kEnterAhead];
+    int j = 0;
+    for (; j + kEnterAhead < segs; j += kEnterAhead) {
 #pragma unroll
-        for (int x = 0; x < kEnterAhead; ++x) own[x] = j + x + 1 < segs ? at[(j + x) * stride] : 0.f;
+        for (int x = 0; x < kEnterAhead; ++x) own[x] = at[(j + x) * stride];
 #pragma unroll
         for (int x = 0; x < kEnterAhead; ++x) {
-            if (j + x >= segs) break;
             at[(j + x) * stride] = run;
             run = run * w + own[x];
             w = step;
         }
+    }
+#pragma unroll
+    for (int x = 0; x < kEnterAhead; ++x) {  // the last segment adds to nobody's start
+        if (j + x + 1 >= segs) break;
+        own[x] = at[(j + x) * stride];
+    }
+#pragma unroll
+    for (int x = 0; x < kEnterAhead; ++x) {
+        if (j + x >= segs) break;
+        at[(j + x) * stride] = run;
+        if (j + x + 1 < segs) run = run * w + own[x];
+        w = step;
     }
 }
 
@@ -660,14 +689,15 @@ Params base_params(const vh_linear_attention_args* a) {
 }
 
 // Tokens a segment, 0 for whole chains.  A CTA takes one segment of one head and 64 value columns, and
-// two CTAs fit an SM: fewer chains than that many are cut so that they fill the card once.  Packed
-// sequences are always cut, as the host does not know their lengths.
+// two CTAs fit an SM: fewer chains than half as many are cut so that they fill the card once, into at least
+// two chunks each (three sequences of 785 tokens, 5 heads of 48 and 72 in fp32, training: 255 us, with four
+// chunks 434, with one 246).  Packed sequences are always cut, as the host does not know their lengths.
 int segment_size(int64_t length, int batch, bool packed, int heads, int dv) {
     const int64_t ctas = 2 * (int64_t)sm_count(), lanes = (int64_t)heads * ((dv + kTile - 1) / kTile);
-    if (!packed && batch * lanes >= ctas) return 0;
+    if (!packed && 2 * batch * lanes > ctas) return 0;
     const int64_t tokens = packed ? length : (int64_t)batch * length;
     int64_t size = (tokens * lanes + ctas - 1) / ctas;
-    size = std::max<int64_t>((size + kChunk - 1) / kChunk * kChunk, 4 * kChunk);
+    size = std::max<int64_t>((size + kChunk - 1) / kChunk * kChunk, 2 * kChunk);
     return size < length ? (int)size : 0;
 }
 

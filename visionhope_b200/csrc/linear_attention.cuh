@@ -48,6 +48,7 @@ struct Params {
     // chains in segments: the state before segment j of a sequence in `states` (0: whole chains)
     int32_t segment;
     float* states;                    // [slots, heads, dk, dv]
+    int32_t join;                     // `states` holds what each segment adds: a start is the sum of those before it
 };
 
 // exp(log_decay) to the n-th.  A decay of 0 (log_decay -inf) leaves the power 0 at 1.
@@ -63,20 +64,37 @@ struct Unit {
     int64_t slot, t0, t1;
     bool live;
 };
-__device__ __forceinline__ Unit unit_at(const Params& p, int64_t index) {
+// Of block column blockIdx.x; every thread takes part.  `found`: a word of shared memory.  Whose segment it is in packed sequences, the last
+// sequence whose slots start at or before this one, is looked up by all threads at once: a binary search is
+// five to ten loads one after another, and as long as a chunk.
+__device__ __forceinline__ Unit block_unit(const Params& p, int* found) {
     Unit u;
-    u.slot = index;
+    u.slot = blockIdx.x;
     if (p.segment == 0) {
-        u.s = (int)index;
-        u.e = ssm::seq_at(p.seqs, u.s);
+        u.s = (int)u.slot;
+    } else if (!p.seqs.offsets) {
+        u.s = (int)(u.slot / ssm::slots_per_seq(p.seqs.length, p.segment));
+    } else {
+        if (threadIdx.x == 0) *found = 0;
+        __syncthreads();
+        int mine = 0;
+        for (int s = threadIdx.x; s < p.seqs.count; s += blockDim.x) {
+            int64_t row = p.seqs.offsets[s];
+            row = row < 0 ? 0 : (row > p.seqs.length ? p.seqs.length : row);
+            if (row / p.segment + s <= u.slot) mine = s;
+        }
+        if (mine > 0) atomicMax(found, mine);
+        __syncthreads();
+        u.s = *found;
+    }
+    u.e = ssm::seq_at(p.seqs, u.s);
+    if (p.segment == 0) {
         u.t0 = 0;
         u.t1 = u.e.len;
         u.live = true;
         return u;
     }
-    u.s = ssm::seq_of_slot(p.seqs, index, p.segment);
-    u.e = ssm::seq_at(p.seqs, u.s);
-    const int64_t j = index - ssm::slot_base(p.seqs, u.s, u.e.row, p.segment);
+    const int64_t j = u.slot - ssm::slot_base(p.seqs, u.s, u.e.row, p.segment);
     u.t0 = j * p.segment;
     u.t1 = min(u.e.len, u.t0 + p.segment);
     u.live = j >= 0 && (u.t0 < u.e.len || j == 0);

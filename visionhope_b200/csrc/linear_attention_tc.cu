@@ -148,17 +148,36 @@ struct Chain {
     __device__ __forceinline__ int row_at(int c) const { return (int)(first_row(c) + (p.seqs.offsets ? u.e.row : 0)); }
     __device__ __forceinline__ int batch_at() const { return p.seqs.offsets ? 0 : u.s; }
 
-    // The state from global memory: element (a, b) at from[a fa + b fb].  Through shared memory (`tile`, rows
-    // of DV + 4), because a thread's columns are far from its neighbour's.  Ends with everybody done reading.
+    // The state from global memory, through shared memory (`tile`, rows of DV + 4), because a thread's columns
+    // are far from its neighbour's.  `initial`: element (a, b) at a init_a + b init_b, or null; `adds`: what
+    // `before` segments ahead of this one add, `stride` apart, or null, or (before 0) the state itself.  Ends
+    // with everybody done reading.
     template <typename Sync>
-    __device__ __forceinline__ void load_state(float (&s)[NC], const float* from, int64_t fa, int64_t fb, float* tile, Sync sync) const {
-        const bool across = fb == 1;
-        const int inner = across ? cols : p.dk, outer = across ? p.dk : cols;
-        from += col0 * fb;
-        for (int i = threadIdx.x; i < inner * outer; i += kCompute) {
-            const int o = i / inner, x = i - o * inner;
-            const int ra = across ? o : x, cb = across ? x : o;
-            tile[ra * (DV + 4) + cb] = from[ra * fa + cb * fb];
+    __device__ __forceinline__ void load_state(float (&s)[NC], const float* initial, const float* adds, int before, int64_t stride,
+                                               float log_decay, float* tile, Sync sync) const {
+        const float step = decay_power(log_decay, p.segment), first = decay_power(log_decay, p.segment - (p.entry ? 1 : 0));
+        const bool across = !initial || p.init_b == 1;
+        const int inner = across ? cols : p.dk, total = p.dk * cols;
+        constexpr int kAhead = 8;
+#pragma unroll 1
+        for (int i0 = threadIdx.x; i0 < total; i0 += kAhead * kCompute) {
+            float run[kAhead];
+            int at[kAhead], to[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = min(i0 + k * kCompute, total - 1), o = i / inner, x = i - o * inner;
+                const int ra = across ? o : x, cb = across ? x : o;
+                to[k] = ra * (DV + 4) + cb;
+                at[k] = ra * p.dv + col0 + cb;
+                run[k] = initial ? initial[ra * p.init_a + (col0 + cb) * p.init_b] : adds && before == 0 ? adds[at[k]] : 0.f;
+            }
+            for (int j = 0; j < before; ++j) {
+                const float w = j == 0 ? first : step;
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) run[k] = run[k] * w + adds[j * stride + at[k]];
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) tile[to[k]] = run[k];
         }
         sync();
 #pragma unroll
@@ -298,10 +317,15 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3, half = warp >> 2;
     const int h = blockIdx.y;
-    const Unit u = unit_at(p, blockIdx.x);
-    ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, ((int64_t)blockIdx.x * gridDim.y + h) * gridDim.z + blockIdx.z,
-                                     (int64_t)gridDim.x * gridDim.y * gridDim.z, p.o);
-    if (!u.live) return;
+    const Unit u = block_unit(p, reinterpret_cast<int*>(power + 131));
+    auto zero_outside = [&] {
+        ssm::zero_outside<__nv_bfloat16>(p.seqs, p.heads * p.dv, ((int64_t)blockIdx.x * gridDim.y + h) * gridDim.z + blockIdx.z,
+                                         (int64_t)gridDim.x * gridDim.y * gridDim.z, p.o);
+    };
+    if (!u.live) {
+        zero_outside();
+        return;
+    }
     const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
     const int chunks = chain.chunks();
@@ -325,16 +349,15 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     if (warp == 0) tcu::tmem_alloc(tmem_at, kCols);
 
     const int64_t states = (int64_t)p.dk * p.dv;
-    const float* from;
-    int64_t fa = p.dv, fb = 1;
-    if (u.t0 == 0) {
-        from = p.initial ? p.initial + ((int64_t)u.s * p.heads + h) * states : nullptr;
-        fa = p.init_a;
-        fb = p.init_b;
-    } else {
-        from = p.states + (u.slot * p.heads + h) * states;
+    // where the state before the first chunk comes from
+    const float *initial = nullptr, *adds = nullptr;
+    int before = 0;
+    if (u.t0 == 0 || p.join) initial = p.initial ? p.initial + ((int64_t)u.s * p.heads + h) * states : nullptr;
+    if (u.t0 > 0) {
+        before = p.join ? (int)(u.t0 / p.segment) : 0;
+        adds = p.states + ((u.slot - before) * p.heads + h) * states;
     }
-    bool has_state = from != nullptr;
+    bool has_state = initial || adds;
     // is the state after a chunk wanted
     auto updates = [&](int c) { return c + 1 < chunks || (p.final_state && u.t1 >= u.e.len); };
 
@@ -485,8 +508,8 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             tcu::fence_proxy_async_smem();
         };
         float* scratch = reinterpret_cast<float*>(smem);  // before the first tiles and after the last
-        if (from) {
-            chain.load_state(s, from, fa, fb, scratch, sync_workers);
+        if (has_state) {
+            chain.load_state(s, initial, adds, before, p.heads * states, log_decay, scratch, sync_workers);
             put_state();
         } else {
 #pragma unroll
@@ -677,6 +700,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     tcu::tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tcu::tmem_dealloc(*tmem_at, kCols);
+    zero_outside();
 }
 
 // ---- what a segment adds to the state -------------------------------------------------------------
@@ -694,7 +718,7 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
     const Waits wait{bars, tmem_at + 1};
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3;
     const int h = blockIdx.y;
-    const Unit u = unit_at(p, blockIdx.x);
+    const Unit u = block_unit(p, reinterpret_cast<int*>(powk + 131));
     if (!u.live || u.t1 >= u.e.len) return;  // the state after a sequence's last segment is nobody's start
     const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
@@ -818,7 +842,8 @@ int run_dims(const Params& p, const Maps& m, int64_t units, bool exact, cudaStre
     };
     if (p.segment) {
         if (int rc = one(false)) return rc;
-        if (int rc = enter_segments(p, st)) return rc;
+        if (!p.join)
+            if (int rc = enter_segments(p, st)) return rc;
     }
     return one(true);
 }
@@ -855,6 +880,9 @@ bool tc_run(Params p, void* states, cudaStream_t st, int* rc) {
     const bool packed = p.seqs.offsets != nullptr, exact = p.final_state != nullptr;
     p.segment = tc_segment_size(p.seqs.length, p.seqs.count, packed, p.heads, p.dk, p.dv);
     p.states = static_cast<float*>(states);
+    // Sequences of a few segments add up their starts themselves, which saves a launch; long ones would read
+    // the square of their number.
+    p.join = p.segment && p.seqs.length <= 24 * (int64_t)p.segment;
     const int64_t units = p.segment ? ssm::slot_total(packed, p.seqs.length, p.seqs.count, p.segment) : p.seqs.count;
     const bool narrow = narrow_values((int64_t)p.seqs.count * p.heads, p.dv);
     if (p.dk <= 64) *rc = narrow ? run_dims<64, 64>(p, m, units, exact, st) : run_dims<64, 128>(p, m, units, exact, st);
