@@ -93,12 +93,12 @@ def test_refused_workspaces_states_and_gradients():
                                                  (5000, 20000, True), (1, (1 << 31) - 1, False)])
 @pytest.mark.parametrize("heads,dk,dv", [(1, 1, 1), (4, 64, 64), (16, 128, 128), (3, 64, 128)])
 def test_workspace_is_as_documented(batch, length, packed, heads, dk, dv):
-    """At most one fp32 state for every 256 tokens of a head, and one more a sequence."""
+    """At most one fp32 state for every 128 tokens of a head, and two more a sequence."""
     from visionhope_b200 import _lib
 
     lib = _lib.load()
     a, p, keep = _args(batch=batch, length=length, heads=heads, key_dim=dk, value_dim=dv, seq_offsets=(lambda p: p) if packed else None)
     tokens = length * (1 if packed else batch)
-    most = (tokens // 256 + 2 * batch) * heads * dk * dv * 4
+    most = (tokens // 128 + 2 * batch) * heads * dk * dv * 4
     for f in (lib.vh_linear_attention_fwd_workspace_bytes, lib.vh_linear_attention_bwd_workspace_bytes):
         assert 0 <= f(ctypes.byref(a)) <= most and _err() == ""
