@@ -24,7 +24,7 @@ _ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 
 class _Call:
     """One call's checked arguments; ``args`` packs them with the output pointers.  x and gate: [samples,
-    channels] (``pixels`` 1, unit stride last) or contiguous [samples, pixels, channels]."""
+    channels] (unit stride last) or contiguous [samples, pixels, channels]."""
 
     __slots__ = ("x", "gate", "weight", "bias", "samples", "groups", "head", "tail")
 
@@ -61,7 +61,8 @@ class _Call:
         x, dev = self.x, self.x.device
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
         dgate = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_gate else None
-        dw, db = (None if t is None else torch.empty(t.shape, dtype=torch.float32, device=dev) for t in (self.weight, self.bias))
+        both = torch.empty((2, x.shape[-1]), dtype=torch.float32, device=dev)
+        dw, db = None if self.weight is None else both[0], None if self.bias is None else both[1]
         if dx.numel() == 0:
             for t in (dw, db):
                 if t is not None:
@@ -74,27 +75,6 @@ class _Call:
         _lib.check(lib.vh_group_norm_bwd(args, dy.data_ptr(), dx.data_ptr(), ptr(dgate), ptr(dw), ptr(db), ws.data_ptr(), nbytes,
                                          _lib.stream_handle(dev)), "vh_group_norm_bwd")
         return dx, dgate, dw, db
-
-
-class _GroupNormFunction(torch.autograd.Function):
-    """Saves its inputs and each group's mean and 1 / standard deviation."""
-
-    @staticmethod
-    def forward(ctx, x, gate, weight, bias, groups, eps, activation):
-        y, mean, rstd = _Call(x, gate, weight, bias, groups, eps, activation).forward(True)
-        ctx.save_for_backward(x, gate, weight, bias, mean, rstd)
-        ctx.options = groups, eps, activation
-        return y
-
-    @staticmethod
-    @once_differentiable
-    @_lib.on_input_device
-    def backward(ctx, dy):
-        *inputs, mean, rstd = ctx.saved_tensors
-        x, gate, weight, bias = inputs
-        call = _Call(x, gate, weight, bias, *ctx.options)
-        grads = call.backward(_args.grad_rows(dy), mean, rstd, gate is not None and ctx.needs_input_grad[1])
-        return (*(_args.grad_like(g, t) for g, t in zip(grads, inputs)), None, None, None)
 
 
 def _check(x, channels, groups, activation, gate):
@@ -129,12 +109,46 @@ def _pixels(t):
     return (t if t.is_contiguous() else t.contiguous()).flatten(1, 2)
 
 
-def _run(x, gate, weight, bias, groups, eps, activation):
+def _shaped(t, like):
+    """[rows, C] or [B, H * W, C] in the shape of the call's x, an image channels-last."""
+    if t is None or t.shape == like.shape:
+        return t
+    if t.dim() == 2:
+        return t.view(like.shape)
+    b, c, h, w = like.shape
+    return t.view(b, h, w, c).permute(0, 3, 1, 2)
+
+
+class _GroupNormFunction(torch.autograd.Function):
+    """Saves its inputs and each group's mean and 1 / standard deviation.  Takes x as the caller has it: views
+    outside would be nodes of the graph, some 10 us of host time each."""
+
+    @staticmethod
+    def forward(ctx, x, gate, weight, bias, layout, groups, eps, activation):
+        y, mean, rstd = _Call(layout(x), None if gate is None else layout(gate), weight, bias, groups, eps, activation).forward(True)
+        ctx.save_for_backward(x, gate, weight, bias, mean, rstd)
+        ctx.options = groups, eps, activation
+        ctx.layout = layout
+        return _shaped(y, x)
+
+    @staticmethod
+    @once_differentiable
+    @_lib.on_input_device
+    def backward(ctx, dy):
+        x, gate, weight, bias, mean, rstd = ctx.saved_tensors
+        layout = ctx.layout
+        call = _Call(layout(x), None if gate is None else layout(gate), weight, bias, *ctx.options)
+        dx, dgate, dw, db = call.backward(_args.grad_rows(layout(dy)), mean, rstd, gate is not None and ctx.needs_input_grad[1])
+        return (_shaped(dx, x), None if dgate is None else _shaped(dgate, gate), _args.grad_like(dw, weight),
+                _args.grad_like(db, bias), None, None, None, None)
+
+
+def _run(x, gate, weight, bias, layout, groups, eps, activation):
     options = int(groups), float(eps), _ACTIVATIONS[activation]
-    tensors = x, gate, weight, bias
-    if _args.tracked(tensors):
-        return _GroupNormFunction.apply(*tensors, *options)
-    return _Call(*tensors, *options).forward(False)[0]
+    if _args.tracked((x, gate, weight, bias)):
+        return _GroupNormFunction.apply(x, gate, weight, bias, layout, *options)
+    call = _Call(layout(x), None if gate is None else layout(gate), weight, bias, *options)
+    return _shaped(call.forward(False)[0], x)
 
 
 @_lib.on_input_device
@@ -146,10 +160,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, *, activation=None, 
     every tensor; the sums of the backward run in a fixed order."""
     if x.dim() != 4:
         raise ValueError(f"x must be [batch, channels, height, width], got {tuple(x.shape)}")
-    b, c, h, w = x.shape
-    _check(x, c, groups, activation, gate)
-    y = _run(_pixels(x), None if gate is None else _pixels(gate), weight, bias, groups, eps, activation)
-    return y.view(b, h, w, c).permute(0, 3, 1, 2)
+    _check(x, x.shape[1], groups, activation, gate)
+    return _run(x, gate, weight, bias, _pixels, groups, eps, activation)
 
 
 @_lib.on_input_device
@@ -159,8 +171,7 @@ def group_norm_rows(x, groups, weight=None, bias=None, eps=1e-5, *, activation=N
     if x.dim() < 1:
         raise ValueError("x must be [..., channels]")
     _check(x, x.shape[-1], groups, activation, gate)
-    y = _run(_flat(x), None if gate is None else _flat(gate), weight, bias, groups, eps, activation)
-    return y if y.shape == x.shape else y.view(x.shape)
+    return _run(x, gate, weight, bias, _flat, groups, eps, activation)
 
 
 class GroupNorm(nn.Module):
