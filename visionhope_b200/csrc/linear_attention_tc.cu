@@ -79,6 +79,19 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// One thread of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+// A value that all lanes have, in a form that the compiler knows to be one: what products are issued with then
+// stays in uniform registers.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 // A tile from shared memory (rows of 64 columns in the same swizzle) to global memory.
 __device__ __forceinline__ void tma_store_4d(const void* map, const void* src, int c0, int c1, int c2, int c3) {
     asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
@@ -99,7 +112,9 @@ struct Smem {
     static constexpr int kK = kTileBytes * (DK / 64), kV = kTileBytes * (DV / 64);
     static constexpr int kKeys = kV, kQueries = kV + kK, kStage = kV + 2 * kK;
     static constexpr int kState = KP == 3 && kK > DK * DV * 2 ? kK : DK * DV * 2;
-    static constexpr int kPower = 2 * kStage + kState;             // lambda^n, n = 0..128, and times kv_scale
+    static constexpr bool kAhead = DK == 128 && DV == 64 && KP == 2;  // see tc_kernel
+    static constexpr int kPlane = 2 * kStage + kState;             // the second plane, where it does not take Q's place
+    static constexpr int kPower = kPlane + (kAhead ? kK : 0);      // lambda^n, n = 0..128, and times kv_scale
     static constexpr int kWeights = kPower + 2 * 132 * 4;          // of a score: by column, and on the diagonal
     static constexpr int kBars = kWeights + (32 + 64) * 4;         // 7 barriers, TMEM base, a flag
     static constexpr int kLaunch = kBars + 64 + 1024;              // the tiles start on 1024 bytes
@@ -258,13 +273,19 @@ __device__ __forceinline__ void clear_values(uint8_t* vt, int n) {
 template <int DK, int DV, int KP>
 __device__ __forceinline__ void issue_update(uint32_t d, uint32_t kt, uint32_t plane1, uint32_t plane2, uint32_t vt, int n) {
     constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorA | kMajorB, lead = DK == 128 ? kTileBytes : 0;
-    const uint64_t dv = desc(vt, kTileBytes);
+    const uint64_t dv = desc(vt, kTileBytes), dk[3] = {desc(kt, lead), desc(plane1, lead), desc(plane2, lead)};
+    if (n > kT - 16) {
 #pragma unroll
-    for (int pl = KP - 1; pl >= 0; --pl) {
-        const uint64_t dk = desc(pl == 0 ? kt : pl == 1 ? plane1 : plane2, lead);
+        for (int pl = KP - 1; pl >= 0; --pl)
 #pragma unroll
-        for (int kk = 0; kk < kT / 16; ++kk)
-            if (kk * 16 < n) tcu::mma_bf16(d, ahead(dk, kk * 2048), ahead(dv, kk * 2048), id, pl < KP - 1 || kk > 0);
+            for (int kk = 0; kk < kT / 16; ++kk)
+                tcu::mma_bf16(d, ahead(dk[pl], kk * 2048), ahead(dv, kk * 2048), id, pl < KP - 1 || kk > 0);
+    } else {
+#pragma unroll
+        for (int pl = KP - 1; pl >= 0; --pl)
+#pragma unroll 1
+            for (int kk = 0; kk * 16 < n; ++kk)
+                tcu::mma_bf16(d, ahead(dk[pl], kk * 2048), ahead(dv, kk * 2048), id, pl < KP - 1 || kk > 0);
     }
 }
 
@@ -300,8 +321,13 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     constexpr bool APART = kApart<DK, DV>;
     // Where two CTAs share TMEM, the update takes the half of the scores that P leaves free; otherwise it has
     // columns of its own, and runs before P V while P is made.
+    // With 128 keys, 64 columns and two planes there is room, in TMEM and in shared memory, for the scores of two
+    // chunks, a P of its own and a second plane that leaves Q alone: the next chunk's scores then follow P V.
+    constexpr bool AHEAD = S::kAhead;
     constexpr int kCols = APART ? 512 : 256, kSync = APART ? kCompute + 32 : kCompute;
-    constexpr uint32_t cScore = 0, cO1 = 128, cO2 = 128 + DV, cU = APART ? 128 + 2 * DV : 64;
+    constexpr uint32_t kScoreCols = AHEAD ? 256 : 128;
+    constexpr uint32_t cO1 = kScoreCols, cO2 = cO1 + DV, cU = APART ? cO2 + DV : 64, cP = AHEAD ? cU + DV : 0;
+    auto scores_at = [](int c) { return AHEAD ? (uint32_t)(c & 1) * 128 : 0u; };
     constexpr int NC = Chain<DK, DV>::NC;
     enum { kValues = 2, kScores = 4, kPV = 5, kUpdate = 6 };  // barriers; 0 and 1: Q and K of the two stages
     extern __shared__ uint8_t raw[];
@@ -390,35 +416,44 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     const uint32_t base = tcu::smem_u32(smem), state_addr = base + 2 * S::kStage;
     uint32_t tmem = 0;
     // The issuer's part, between the workers' steps.
-    auto issue_first = [&](int c, bool with_state) {  // scores and q S
+    auto issue_scores = [&](int c) {
         const uint32_t kt = base + (c & 1) * S::kStage + S::kKeys, qt = kt + S::kK;
         wait(c & 1, (c >> 1) & 1);
         tcu::tc_fence_after_sync();
-        constexpr uint32_t id = tcu::idesc_bf16_f32(128, 128), id_state = tcu::idesc_bf16_f32(128, DV) | kMajorB;
-        const uint64_t dq = desc(qt, 16), dk = desc(kt, 16), ds = desc(state_addr, DK * 128);
+        constexpr uint32_t id = tcu::idesc_bf16_f32(128, 128);
+        const uint64_t dq = desc(qt, 16), dk = desc(kt, 16);
 #pragma unroll
         for (int kk = 0; kk < DK / 16; ++kk) {
             const uint32_t at = (kk / 4) * kTileBytes + (kk % 4) * 32;
-            tcu::mma_bf16(tmem + cScore, ahead(dq, at), ahead(dk, at), id, kk > 0);
+            tcu::mma_bf16(tmem + scores_at(c), ahead(dq, at), ahead(dk, at), id, kk > 0);
         }
-        if (with_state) {
+    };
+    auto issue_state = [&](int c) {  // q S
+        const uint32_t qt = base + (c & 1) * S::kStage + S::kQueries;
+        constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorB;
+        const uint64_t dq = desc(qt, 16), ds = desc(state_addr, DK * 128);
 #pragma unroll
-            for (int kk = 0; kk < DK / 16; ++kk) {
-                const uint32_t at = (kk / 4) * kTileBytes + (kk % 4) * 32;
-                tcu::mma_bf16(tmem + cO2, ahead(dq, at), ahead(ds, kk * 2048), id_state, kk > 0);
-            }
-        }
-        tcu::mma_commit(&bars[kScores]);
+        for (int kk = 0; kk < DK / 16; ++kk)
+            tcu::mma_bf16(tmem + cO2, ahead(dq, (kk / 4) * kTileBytes + (kk % 4) * 32), ahead(ds, kk * 2048), id, kk > 0);
     };
     auto issue_start = [&] {
         for (int c = 0; c < min(chunks, 2); ++c) {
             load_keys(c);
             load_values(c);
         }
-        if (chunks > 0) issue_first(0, has_state);
+        if (chunks > 0) {
+            issue_scores(0);
+            if (AHEAD) tcu::mma_commit(&bars[kScores]);
+            if (has_state) issue_state(0);
+            if (!AHEAD) tcu::mma_commit(&bars[kScores]);
+        }
     };
     auto issue_next = [&](int c) {  // after chunk c
-        if (c + 1 < chunks) issue_first(c + 1, true);
+        if (c + 1 < chunks) {
+            if (!AHEAD) issue_scores(c + 1);
+            issue_state(c + 1);
+            if (!AHEAD) tcu::mma_commit(&bars[kScores]);
+        }
         if (c + 2 < chunks) load_keys(c + 2);
     };
     auto load_rest = [&](int c) {  // the values of chunk c + 1, once the outputs of c - 1 have left
@@ -426,23 +461,30 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
         stores_read();
         if (c + 1 < chunks) load_values(c + 1);
     };
-    auto issue_pv = [&](int c) {
+    auto issue_pv = [&](int c, int n) {
         const uint32_t vt = base + (c & 1) * S::kStage;
         wait_values(c);
         tcu::tc_fence_after_sync();
         constexpr uint32_t id = tcu::idesc_bf16_f32(128, DV) | kMajorB;
-        const int n = chain.tokens(c);
         const uint64_t dv = desc(vt, kTileBytes);
+        if (n > kT - 16) {
 #pragma unroll
-        for (int kk = 0; kk < kT / 16; ++kk)
-            if (kk * 16 < n) mma_ts(tmem + cO1, tmem + cScore + kk * 8, ahead(dv, kk * 2048), id, kk > 0);
-        tcu::mma_commit(&bars[kPV]);
+            for (int kk = 0; kk < kT / 16; ++kk) mma_ts(tmem + cO1, tmem + cP + kk * 8, ahead(dv, kk * 2048), id, kk > 0);
+        } else {
+#pragma unroll 1
+            for (int kk = 0; kk * 16 < n; ++kk) mma_ts(tmem + cO1, tmem + cP + kk * 8, ahead(dv, kk * 2048), id, kk > 0);
+        }
+        tcu::mma_commit(&bars[kPV]);  // and of q S before it
+        if (AHEAD && c + 1 < chunks) {
+            issue_scores(c + 1);
+            tcu::mma_commit(&bars[kScores]);
+        }
     };
-    auto issue_u = [&](int c) {
+    auto issue_u = [&](int c, int n) {
         const uint32_t vt = base + (c & 1) * S::kStage;
         wait_values(c);
         tcu::tc_fence_after_sync();
-        issue_update<DK, DV, KP>(tmem + cU, vt + S::kKeys, vt + S::kQueries, state_addr, vt, chain.tokens(c));
+        issue_update<DK, DV, KP>(tmem + cU, vt + S::kKeys, AHEAD ? base + S::kPlane : vt + S::kQueries, state_addr, vt, n);
         tcu::mma_commit(&bars[kUpdate]);
     };
     // every step ends with the writes to shared memory fenced and the TMEM accesses ordered
@@ -456,38 +498,49 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     if (APART && warp >= kCompute / 32) {
         if constexpr (APART) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         if (warp == kCompute / 32) {
-            const bool issuer = lane == 0;
             bar_sync<kSync>(1);  // barriers, TMEM and the state are there
             tcu::tc_fence_after_sync();
-            tmem = *tmem_at;
-            if (issuer) issue_start();
-            for (int c = 0; c < chunks; ++c) {
+            tmem = uniform(*tmem_at);
+            const int count = (int)uniform((uint32_t)chunks), last = (int)uniform((uint32_t)(chunks > 0 ? chain.tokens(chunks - 1) : 0));
+            if (elect()) issue_start();
+            for (int c = 0; c < count; ++c) {
+                const int n = c + 1 < count ? kT : last;
+                bool stored = c == 0;
                 if (updates(c)) {
                     __syncwarp();
                     sync();  // keys weighed
-                    if (issuer) issue_u(c);
+                    if (elect()) {
+                        issue_u(c, n);
+                        if (AHEAD && !stored) store_tiles(c - 1);
+                    }
+                    stored |= AHEAD;
+                }
+                if (!AHEAD) {
+                    __syncwarp();
+                    sync();  // scores read
+                    if (elect() && !stored) store_tiles(c - 1);
+                    stored = true;
                 }
                 __syncwarp();
-                sync();  // scores read
-                if (issuer && c > 0) store_tiles(c - 1);
-                __syncwarp();
                 sync();  // P written
-                if (issuer) {
-                    issue_pv(c);
+                if (elect()) {
+                    if (!stored) store_tiles(c - 1);
+                    issue_pv(c, n);
                     load_rest(c);
                 }
                 __syncwarp();
                 sync();  // outputs read, state written
-                if (issuer) issue_next(c);
+                if (elect()) issue_next(c);
             }
-            if (chunks > 0) {
+            if (count > 0) {
                 __syncwarp();
                 sync();  // the last outputs are in their tiles
-                if (issuer) {
-                    if (chain.tokens(chunks - 1) == kT) store_tiles(chunks - 1);
+                if (elect()) {
+                    if (last == kT) store_tiles(count - 1);
                     stores_read();
                 }
             }
+            __syncwarp();
         }
     } else {
         if constexpr (APART) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -536,10 +589,10 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             wait(kScores, c & 1);
             tcu::tc_fence_after_sync();
             auto weigh = [&] {
-                weigh_keys<DK, KP>(kt, qt, state, powk, n, reverse);
+                weigh_keys<DK, KP>(kt, AHEAD ? smem + S::kPlane : qt, state, powk, n, reverse);
                 sync();
                 if (issuer) {
-                    issue_u(c);
+                    issue_u(c, n);
                     load_rest(c);
                 }
             };
@@ -561,7 +614,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
                     continue;
                 }
                 uint32_t x[32];
-                ld32(tmem_lane + cScore + j0, x);
+                ld32(tmem_lane + scores_at(c) + j0, x);
                 tcu::tmem_wait_ld();
                 // columns of this block that exist: reversed, the ones past the sequence are not masked
                 uint32_t on = reverse && n - j0 < 32 ? (1u << (n - j0)) - 1 : 0xffffffffu;
@@ -592,14 +645,15 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
                         pw[blk][i / 2] &= (on >> i & 1 ? 0xffffu : 0u) | (on >> (i + 1) & 1 ? 0xffff0000u : 0u);
                 }
             }
-            // P takes the place of the scores' first half, which others may still be reading
-            sync();
-            if (issuer && c > 0) store_tiles(c - 1);
-            st16(tmem_lane + cScore + half * 32, pw[0]);
-            st16(tmem_lane + cScore + half * 32 + 16, pw[1]);
+            if (!AHEAD) {  // P takes the place of the scores' first half, which others may still be reading
+                sync();
+                if (issuer && c > 0) store_tiles(c - 1);
+            }
+            st16(tmem_lane + cP + half * 32, pw[0]);
+            st16(tmem_lane + cP + half * 32 + 16, pw[1]);
             wait_st();
             sync();
-            if (issuer) issue_pv(c);
+            if (issuer) issue_pv(c, n);
             if (update) {
                 if (APART) renew(); else weigh();
             }
@@ -634,7 +688,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
 #pragma unroll 1
                     for (int j = 0; j < n; ++j) {
                         float pr[2];
-                        tcu::tmem_ld2(tmem_lane + cScore + j / 4 * 2, pr);
+                        tcu::tmem_ld2(tmem_lane + cP + j / 4 * 2, pr);
                         tcu::tmem_wait_ld();
                         const uint32_t w = __float_as_uint(j & 2 ? pr[1] : pr[0]);
                         const float pv = __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
