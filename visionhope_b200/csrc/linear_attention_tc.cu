@@ -354,7 +354,9 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     }
     const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
-    const int chunks = chain.chunks();
+    const int chunks = (int)uniform((uint32_t)chain.chunks());
+    const int last_tokens = (int)uniform((uint32_t)(chunks > 0 ? chain.tokens(chunks - 1) : 0));
+    auto tokens = [&](int c) { return c + 1 < chunks ? kT : last_tokens; };  // every chunk but a sequence's last is full
     const float log_decay = p.log_decay[h];
     if (tid <= kT) {
         const float w = decay_power(log_decay, tid);
@@ -495,16 +497,15 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     };
     auto sync_workers = [&] { bar_sync<kCompute>(2); };
 
-    if (APART && warp >= kCompute / 32) {
+    if (APART && uniform((uint32_t)warp) >= kCompute / 32) {
         if constexpr (APART) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        if (warp == kCompute / 32) {
+        if (uniform((uint32_t)warp) == kCompute / 32) {
             bar_sync<kSync>(1);  // barriers, TMEM and the state are there
             tcu::tc_fence_after_sync();
             tmem = uniform(*tmem_at);
-            const int count = (int)uniform((uint32_t)chunks), last = (int)uniform((uint32_t)(chunks > 0 ? chain.tokens(chunks - 1) : 0));
             if (elect()) issue_start();
-            for (int c = 0; c < count; ++c) {
-                const int n = c + 1 < count ? kT : last;
+            for (int c = 0; c < chunks; ++c) {
+                const int n = tokens(c);
                 bool stored = c == 0;
                 if (updates(c)) {
                     __syncwarp();
@@ -532,11 +533,11 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
                 sync();  // outputs read, state written
                 if (elect()) issue_next(c);
             }
-            if (count > 0) {
+            if (chunks > 0) {
                 __syncwarp();
                 sync();  // the last outputs are in their tiles
                 if (elect()) {
-                    if (last == kT) store_tiles(count - 1);
+                    if (last_tokens == kT) store_tiles(chunks - 1);
                     stores_read();
                 }
             }
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
         }
     } else {
         if constexpr (APART) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-        const bool issuer = !APART && tid == (reverse ? 96 : 128);
+        const bool issues = !APART && uniform((uint32_t)warp) == (reverse ? 3u : 4u);  // then one thread of the warp does
         float s[NC];
         // rows of 64 value columns, one a key: the contraction runs over keys
         auto put_state = [&] {
@@ -570,12 +571,12 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
         }
         tcu::fence_proxy_async_smem();
         sync();
-        tmem = *tmem_at;
+        tmem = uniform(*tmem_at);
         const uint32_t tmem_lane = tmem + ((uint32_t)(quad * 32) << 16);
-        if (issuer) issue_start();
+        if (issues && elect()) issue_start();
         const int row = quad * 32 + lane;  // of the scores and outputs
         for (int c = 0; c < chunks; ++c) {
-            const int n = chain.tokens(c);
+            const int n = tokens(c);
             const int entry = p.entry && u.t0 == 0 && c == 0;
             uint8_t* vt = smem + (c & 1) * S::kStage;
             uint8_t *kt = vt + S::kKeys, *qt = vt + S::kQueries;
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             auto weigh = [&] {
                 weigh_keys<DK, KP>(kt, AHEAD ? smem + S::kPlane : qt, state, powk, n, reverse);
                 sync();
-                if (issuer) {
+                if (issues && elect()) {
                     issue_u(c, n);
                     load_rest(c);
                 }
@@ -647,13 +648,13 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             }
             if (!AHEAD) {  // P takes the place of the scores' first half, which others may still be reading
                 sync();
-                if (issuer && c > 0) store_tiles(c - 1);
+                if (c > 0 && issues && elect()) store_tiles(c - 1);
             }
             st16(tmem_lane + cP + half * 32, pw[0]);
             st16(tmem_lane + cP + half * 32 + 16, pw[1]);
             wait_st();
             sync();
-            if (issuer) issue_pv(c, n);
+            if (issues && elect()) issue_pv(c, n);
             if (update) {
                 if (APART) renew(); else weigh();
             }
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             if (!APART && update) renew();
             has_state |= update;
             sync();
-            if (issuer) issue_next(c);
+            if (issues && elect()) issue_next(c);
             // the rows of o where V was, in the swizzle of its tiles; they leave during the next chunk
 #pragma unroll
             for (int i = 0; i < DV / 16; ++i) {
@@ -727,7 +728,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
         }
         if (chunks > 0) {
             sync();
-            const int c = chunks - 1, n = chain.tokens(c);
+            const int c = chunks - 1, n = last_tokens;
             if (n < kT) {  // rows past these are another sequence's
                 const uint8_t* from_tile = smem + (c & 1) * S::kStage;
                 const int64_t step = (int64_t)p.heads * p.dv;
@@ -739,7 +740,8 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
                     *reinterpret_cast<uint4*>(to + r * step + ch * 8) = v;
                 }
             }
-            if (issuer) {
+            __syncwarp();
+            if (issues && elect()) {
                 if (n == kT) store_tiles(c);
                 stores_read();
             }
@@ -770,13 +772,13 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + S::kStages + 1);
     const Waits wait{bars, tmem_at + 1};
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, quad = warp & 3;
+    const int tid = threadIdx.x, warp = tid >> 5, quad = warp & 3;
     const int h = blockIdx.y;
     const Unit u = block_unit(p, reinterpret_cast<int*>(powk + 131));
     if (!u.live || u.t1 >= u.e.len) return;  // the state after a sequence's last segment is nobody's start
     const Chain<DK, DV> chain(p, u);
     const bool reverse = p.seqs.reverse;
-    const int chunks = chain.chunks();
+    const int chunks = (int)uniform((uint32_t)chain.chunks());
     const float log_decay = p.log_decay[h];
     if (tid <= kT) powk[tid] = decay_power(log_decay, tid) * p.kv_scale;
     const float decay = decay_power(log_decay, kT);  // all chunks of these segments are full
@@ -793,7 +795,7 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
         tcu::tc_fence_after_sync();
     };
     sync();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = uniform(*tmem_at);
     auto planes_of = [&](int c) { return smem + S::kStages * S::kStage + (c % S::kBuffers) * S::kPlanes; };
     auto load_tiles = [&](int c) {
         uint8_t* at = smem + c % S::kStages * S::kStage;
@@ -805,13 +807,13 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
 #pragma unroll
         for (int i = 0; i < DK / 64; ++i) tcu::tma_load_4d(at + S::kV + i * kTileBytes, &maps.k, bar, i * 64, h, row, b);
     };
-    if (warp == kCompute / 32) {
-        if (lane == 0)
+    if (uniform((uint32_t)warp) == kCompute / 32) {
+        if (elect())
             for (int c = 0; c < min(chunks, S::kStages); ++c) load_tiles(c);
         for (int c = 0; c < chunks; ++c) {
             __syncwarp();
             sync();  // keys of chunk c weighed, product c - 1 read
-            if (lane == 0) {
+            if (elect()) {
                 const uint32_t vt = tcu::smem_u32(smem) + c % S::kStages * S::kStage, pl = tcu::smem_u32(planes_of(c));
                 issue_update<DK, DV, KP>(tmem, vt + S::kV, pl, pl + S::kK, vt, kT);
                 tcu::mma_commit(&bars[kUpdate]);
