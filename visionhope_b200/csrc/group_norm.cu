@@ -12,8 +12,12 @@
 //   resident  a slab of whole groups in the shared memory of a cluster of 1 to 8 CTAs, each a slice of
 //             the pixels: x is read once
 //   split     larger ones: partial sums a slice, one kernel that joins them, a second pass over x
-// The variance comes from differences to a mean (registers, shared memory) or to the first value of
-// each channel that a thread sees (split), joined by Chan's formula, so that a large mean costs nothing.
+// The variance comes from differences to the mean (rows) or to a channel's first value in the slice, joined by
+// Chan's formula, so that a large mean costs nothing.
+//
+// Measured (bf16, forward + backward): 50176 gated rows of 256 channels 23 + 28 us, 3.3 and 4.5 TB/s; 64 maps of
+// 56 x 56 x 128 with SiLU 41 + 70 us (resident), 2.5 and 2.2 TB/s; two maps of 128 x 512 x 128 with GELU 36 us
+// (split, forward).  Issue slots are 38 to 48 % busy, with 14 to 20 warps an SM: latency between the passes.
 #include <algorithm>
 
 #include "abi_util.h"

@@ -155,6 +155,10 @@ __device__ __forceinline__ void load_tile(uint16_t* dst, const T* src, int64_t s
 // warps (each a quarter of the key rows by 64 value columns) and, for the outputs, as a bf16 operand
 // in shared memory.  OUT false computes only what the segment adds to the state.
 //
+// Four warps, because a chunk of 64 rows gives each of them 16 whole rows of scores, which then never leave its
+// registers; 64 value columns, so that a state of 128 keys fits the accumulators.  Bound by latency (three
+// sequences of 785 tokens, 5 heads of 48 and 72 in fp32, forward and backward: 192 us, tensor pipe 15 %).
+//
 // The state itself is fp32 throughout: a key's weight lambda^{n-1-j} is multiplied in fp32 and the
 // product enters as three planes, so nothing of it is rounded.  As an operand of the outputs the
 // state is rounded to NP planes, and so are the weighted scores: for bf16 inputs that is one rounding
@@ -556,9 +560,9 @@ struct StepParams {
     int32_t slots, batch, heads, dk, dv;
 };
 
-// A CTA per (stream, head, 64 or 128 value columns): the state is read and written once, four columns
-// a thread (V = 4) over key rows that the row groups share; the sums over key rows meet in shared
-// memory.  Bound by the state's bytes (8 per element).
+// A CTA per (stream, head): the state is read and written once, four columns a thread (V = 4) over key rows that
+// the row groups share; the sums over key rows meet in shared memory.  Bound by the state's bytes (8 per
+// element): 256 streams of 16 heads of 128 x 128 in 91 us, 5.9 TB/s.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) step_kernel(StepParams p) {
     __shared__ float ks[kMaxDim], qs[kMaxDim];
