@@ -304,6 +304,13 @@ struct Waits {
         }
     }
 };
+// After a wait gave up: no more copies are started, and those in flight get a millisecond to land.
+__device__ __forceinline__ void settle(const Waits& wait) {
+    if (!*wait.dead) return;
+    const uint64_t t0 = tcu::globaltimer_ns();
+    while (tcu::globaltimer_ns() - t0 < 1000000) {
+    }
+}
 template <int N>
 __device__ __forceinline__ void bar_sync(int id) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory");
@@ -395,6 +402,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
     auto updates = [&](int c) { return c + 1 < chunks || (p.final_state && u.t1 >= u.e.len); };
 
     auto load_keys = [&](int c) {  // and queries
+        if (*wait.dead) return;
         uint8_t* at = smem + (c & 1) * S::kStage;
         uint64_t* bar = &bars[c & 1];
         tcu::mbar_arrive_expect_tx(bar, 2 * S::kK);
@@ -406,6 +414,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
         }
     };
     auto load_values = [&](int c) {
+        if (*wait.dead) return;
         uint8_t* at = smem + (c & 1) * S::kStage;
         uint64_t* bar = &bars[kValues + (c & 1)];
         tcu::mbar_arrive_expect_tx(bar, S::kV);
@@ -758,6 +767,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             chain.store_state(s, p.final_state + ((int64_t)u.s * p.heads + h) * states, last, tile, sync_workers);
         }
     }
+    settle(wait);
     tcu::tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tcu::tmem_dealloc(*tmem_at, kCols);
@@ -803,6 +813,7 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
     const uint32_t tmem = uniform(*tmem_at);
     auto planes_of = [&](int c) { return smem + S::kStages * S::kStage + (c % S::kBuffers) * S::kPlanes; };
     auto load_tiles = [&](int c) {
+        if (*wait.dead) return;
         uint8_t* at = smem + c % S::kStages * S::kStage;
         uint64_t* bar = &bars[c % S::kStages];
         tcu::mbar_arrive_expect_tx(bar, S::kStage);
@@ -847,6 +858,7 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
         chain.store_state(s, p.states + (u.slot * p.heads + h) * states, 1.f, reinterpret_cast<float*>(smem),
                           [&] { bar_sync<kCompute>(2); });
     }
+    settle(wait);
     tcu::tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tcu::tmem_dealloc(tmem, kCols);
