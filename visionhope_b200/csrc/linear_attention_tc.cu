@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(kBlock<DK, DV>, kApart<DK, DV> ? 1 : 2) tc_ker
             chain.store_state(s, p.final_state + ((int64_t)u.s * p.heads + h) * states, last, tile, sync_workers);
         }
     }
-    settle(wait);
+    if (tid == 0) settle(wait);  // warps without work have not waited for the flag to be set up
     tcu::tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tcu::tmem_dealloc(*tmem_at, kCols);
@@ -858,7 +858,7 @@ __global__ void __launch_bounds__(kCompute + 32, DK + DV == 128 ? 2 : 1) tc_stat
         chain.store_state(s, p.states + (u.slot * p.heads + h) * states, 1.f, reinterpret_cast<float*>(smem),
                           [&] { bar_sync<kCompute>(2); });
     }
-    settle(wait);
+    if (tid == 0) settle(wait);
     tcu::tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tcu::tmem_dealloc(tmem, kCols);
