@@ -157,7 +157,7 @@ __device__ __forceinline__ void load_tile(uint16_t* dst, const T* src, int64_t s
 //
 // Four warps, because a chunk of 64 rows gives each of them 16 whole rows of scores, which then never leave its
 // registers; 64 value columns, so that a state of 128 keys fits the accumulators.  Bound by latency (three
-// sequences of 785 tokens, 5 heads of 48 and 72 in fp32, forward and backward: 192 us, tensor pipe 15 %).
+// sequences of 785 tokens, 5 heads of 48 and 72 in fp32, forward and backward: 186 us, tensor pipe 15 %).
 //
 // The state itself is fp32 throughout: a key's weight lambda^{n-1-j} is multiplied in fp32 and the
 // product enters as three planes, so nothing of it is rounded.  As an operand of the outputs the

@@ -15,8 +15,8 @@
 //
 // A token and head of 128 keys and values takes 1 KB of memory (0.16 ns) and, with two planes, 2.2 times the
 // recurrence's operations (0.12 ns at the tensor cores' rate); a CTA's steps depend on one another, which bounds
-// it.  4 x 8192 tokens of 16 heads of 128: 178 us, 3.0 TB/s, tensor pipe 25 %; warp-level matrix instructions took
-// 825.  64 x 784 tokens of 4 heads of 64, forward and backward: 129 us (577).
+// it.  4 x 8192 tokens of 16 heads of 128: 184 us, 2.9 TB/s, tensor pipe 25 %; warp-level matrix instructions took
+// 825.  64 x 784 tokens of 4 heads of 64, forward and backward: 135 us (577).
 //
 // Reversed sequences keep their rows in memory order and turn the mask and the weights around: local row
 // r has position n-1-r.
