@@ -164,3 +164,23 @@ def test_step_takes_one_state_per_stream_in_any_order():
     c = state.clone()
     linear_attention_step(q, k, v, g, c, slots=torch.tensor([-1, 5, -1], device="cuda"))
     assert torch.equal(c, state)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 3000, 1, 64, 64), (1, 20000, 2, 64, 64), (1, 2500, 2, 128, 128)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_values_that_are_not_finite_in_segments(dtype, shape, reverse):
+    """Where a sequence is cut into segments, tokens before an infinite value keep their bits outside its chunk."""
+    b, n, h, dk, dv = shape
+    q, k, v = (normal(i, b, n, h, d, dtype=dtype) for i, d in enumerate((dk, dk, dv)))
+    g, at = decays(h), 1700
+    clean = linear_attention(q, k, v, g, reverse=reverse)
+    v[0, at, 0, 3] = float("inf")
+    o = linear_attention(q, k, v, g, reverse=reverse)
+    before = slice(at + 129, n) if reverse else slice(0, at - 128)
+    after = slice(0, at + 1) if reverse else slice(at, n)
+    assert torch.equal(o[:, before], clean[:, before]) and torch.equal(o[:, :, 1:], clean[:, :, 1:])
+    others = torch.arange(dv, device="cuda") != 3
+    chunk = slice(at + 1, at + 129) if reverse else slice(at - 128, at)
+    near(o[:, chunk], clean[:, chunk].double(), clean[:, chunk].double().abs() + 30, dtype, 4, operand=2 ** -8 if dtype != torch.float32 else None)
+    assert torch.isfinite(o[:, after, 0][..., others]).all() and not torch.isfinite(o[0, at, 0, 3])
